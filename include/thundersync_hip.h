@@ -500,6 +500,106 @@ int ts_matmul_exact_ws(const void* a, int64_t a_m, int64_t a_k, const void* b, i
                        int64_t workspace_bytes, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Distillation from a teacher's top logits through the head
+ *
+ * Row n brings `top` slots (ids[n, k], teacher[n, k]); a negative id or a
+ * logit of -inf is an absent slot.  With p the softmax of the present slots'
+ * teacher / T (slots of one token added together) and q the softmax over the
+ * vocabulary of hidden[n] . weight^T / T:
+ *   loss[n] = sum_k p_k (log p_k - log q_k),  dlogits = grad / T (q - p).
+ * A row without a present slot has loss 0 and dlogits 0; an id of vocab or
+ * more makes its row's loss NaN and takes no part in dlogits.
+ * The slots' tokens, probabilities and logits (slot_id, slot_p, slot_z) are
+ * [rows, pitch] with top <= pitch <= 1024; state is [rows].
+ * No counterpart in the reference, whose distillation scores sampled tokens
+ * (opd/objectives.py:607-611).
+ * ------------------------------------------------------------------------ */
+
+/* slot_id (-1: no entry), slot_p (fp64 for dtype TS_F64, otherwise fp32) and
+ * state (0: no present slot, 1, 2: an id past the vocabulary) of the teacher's
+ * [rows, top] ids (dense) and logits (row stride ld_teacher). */
+int ts_distill_teacher(const int64_t* ids, const void* teacher, int64_t ld_teacher, int teacher_dtype, int64_t rows,
+                       int64_t top, int64_t vocab, double temperature, int32_t* slot_id, void* slot_p,
+                       int64_t pitch, int32_t* state, int dtype, void* stream);
+
+/* Workspace bytes ts_distill_fwd needs. */
+int64_t ts_distill_fwd_workspace(int64_t rows, int64_t vocab);
+
+/* bf16 or fp16: loss, lse (of the logits over T, natural log) and slot_z (the
+ * logits at the slots, not over T), all fp32.  hidden and weight as for
+ * ts_logprob_fwd. */
+int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
+                   int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
+                   float* slot_z, int64_t pitch, int64_t top, const int32_t* state, float* loss, float* lse,
+                   void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* bf16 or fp16: dlogits [rows, ld_dlogits >= vocab rounded up to 8] in the
+ * element type, each rounded once from fp32; columns past the vocabulary are
+ * written as zero.  Inputs as ts_distill_fwd took and gave them. */
+int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
+                       int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
+                       const float* slot_z, int64_t pitch, int64_t top, const int32_t* state, const float* lse,
+                       const float* grad, void* dlogits, int64_t ld_dlogits, int dtype, void* stream);
+
+/* The parts of the fp32 and fp64 path, around ts_logprob_fwd_exact and
+ * ts_logprob_dlogits_exact on rows divided by T: slot_z = hidden . weight[slot_id]
+ * (any dtype), loss from slot_z and lse (both over T), the slots' entries of
+ * dlogits = grad_scale grad (exp(logit_scale slot_z - lse) - slot_p), and
+ * out = scale hidden with zeros in the rows whose state is 0. */
+int ts_distill_scores(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight,
+                      const int32_t* slot_id, int64_t pitch, int64_t rows, int64_t top, int64_t dim, void* slot_z,
+                      int dtype, void* stream);
+int ts_distill_loss(const int32_t* slot_id, const void* slot_p, const void* slot_z, int64_t pitch, int64_t top,
+                    const int32_t* state, const void* lse, int64_t rows, void* loss, int dtype, void* stream);
+int ts_distill_slots(const int32_t* slot_id, const void* slot_p, const void* slot_z, int64_t pitch, int64_t top,
+                     const void* lse, const void* grad, int64_t rows, double logit_scale, double grad_scale,
+                     void* dlogits, int64_t ld_dlogits, int dtype, void* stream);
+int ts_distill_rows(const void* hidden, int64_t ld_hidden, const int32_t* state, int64_t rows, int64_t dim,
+                    double scale, void* out, int64_t ld_out, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Embedding (fp32, fp16 or bf16)
+ * ------------------------------------------------------------------------ */
+
+/* out [n, dim] (dense) = scale weight[ids]; an id outside [0, vocab) gives a
+ * row of NaN.  No counterpart in the reference (torch.nn.Embedding). */
+int ts_embedding_fwd(const int64_t* ids, int64_t n, const void* weight, int64_t ld_weight, int64_t vocab, int64_t dim,
+                     float scale, void* out, int dtype, void* stream);
+
+/* Workspace bytes ts_embedding_bwd needs. */
+int64_t ts_embedding_bwd_workspace(int64_t n, int64_t dim);
+
+/* grad_weight [vocab, dim] (dense, 16-byte aligned) = scale times the sum of
+ * grad_out's rows (row stride ld_grad, 0 for one row for all) by id, in fp32 in
+ * token order and rounded once: the same bytes on every call.  Ids outside the
+ * vocabulary and the id `padding` (-1: none) take no part; rows no id names are
+ * zero.  n and vocab below 2^31 - 1. */
+int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_t ld_grad, int64_t vocab, int64_t dim,
+                     int64_t padding, float scale, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                     int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Sampling (fp32, fp16 or bf16 logits)
+ * ------------------------------------------------------------------------ */
+
+/* One token per row of logits [rows, vocab] from uniform[rows] (TS_F32 or
+ * TS_F64, in [0, 1)) and the logprob of the token in the distribution it was
+ * drawn from.  Weights are w = exp((logit - max) / temperature), their order is
+ * by falling logit, equal ones by index.  Kept are the first top_k (0: all), of
+ * those the ones whose predecessors weigh less than top_p times all of those
+ * (1 or more: all), of those the ones with w >= min_p; the first is always
+ * kept.  The token is the first in index order whose running sum of kept
+ * weights exceeds uniform times their total.  A temperature of 0 draws the
+ * first maximum.  A row with a NaN or without a logit above -inf gets token -1
+ * and logprob NaN.  Each option is one value for all rows, or where its pointer
+ * is not null one per row.  vocab at most 2^21.  No counterpart in the reference
+ * (its rollouts sample inside vLLM, rollout/engine.py). */
+int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, const void* uniform,
+              int uniform_dtype, const float* temperature, double temperature_all, const int32_t* top_k,
+              int64_t top_k_all, const float* top_p, double top_p_all, const float* min_p, double min_p_all,
+              int64_t* tokens, float* logprobs, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
  * Merged-weight LoRA linear (bf16 or fp16 operands, fp32 accumulation)
  *
  * The caller has merged the adapters into the weight (W_eff = W + s B A,

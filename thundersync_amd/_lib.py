@@ -35,6 +35,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ts_hip_version": (ctypes.c_char_p, []),
     "ts_hip_last_error": (ctypes.c_char_p, []),
@@ -76,6 +77,26 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, ctypes.c_float, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64,
          _INT, _P],
     ),
+    "ts_distill_teacher": (
+        _INT, [_P, _P, _I64, _INT, _I64, _I64, _I64, _D, _P, _P, _I64, _P, _INT, _P]),
+    "ts_distill_fwd_workspace": (_I64, [_I64, _I64]),
+    "ts_distill_fwd": (
+        _INT,
+        [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _INT, _P],
+    ),
+    "ts_distill_scores": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _INT, _P]),
+    "ts_distill_loss": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _I64, _P, _INT, _P]),
+    "ts_distill_dlogits": (
+        _INT,
+        [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _INT, _P],
+    ),
+    "ts_distill_slots": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _I64, _D, _D, _P, _I64, _INT, _P]),
+    "ts_distill_rows": (_INT, [_P, _I64, _P, _I64, _I64, _D, _P, _I64, _INT, _P]),
+    "ts_embedding_fwd": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _F, _P, _INT, _P]),
+    "ts_embedding_bwd_workspace": (_I64, [_I64, _I64]),
+    "ts_embedding_bwd": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _I64, _INT, _P]),
+    "ts_sample": (
+        _INT, [_P, _I64, _I64, _I64, _P, _INT, _P, _D, _P, _I64, _P, _D, _P, _D, _P, _P, _INT, _P]),
     "ts_adjoint_reduce": (_INT, [ctypes.POINTER(_P), _INT, _P, _P, _I64, _INT, _P]),
     "ts_ledger_add": (_INT, [_P, _P, _I64, _INT, _INT, _P]),
     "ts_forest_build": (_INT, [_I64, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P]),

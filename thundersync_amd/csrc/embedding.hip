@@ -1,0 +1,442 @@
+// Embedding lookup with a scale, and the table's gradient by sorted tokens, for gfx950.
+//
+//   out[n] = scale W[ids[n]]        dW[v] = scale sum over n with ids[n] = v of dout[n]
+//
+// Lookup: bandwidth-bound, 16 bytes a lane.  Gradient: the tokens' positions are sorted by
+// id (stable, so equal ids keep the token order), and chunks of kChunk sorted positions add
+// up their rows of dout in fp32; an id whose positions end inside the chunk is written once,
+// one that a chunk border cuts leaves fp32 partial rows that join_kernel adds in chunk
+// order.  No atomics on values: the same bits every time.  Rows of the table that no token
+// names are zeros.  Bound by the write of the [V, D] gradient where tokens are few.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.h"
+#include "timing.h"
+#include "../../include/thundersync_hip.h"
+
+namespace ts {
+namespace embed {
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 32;      // sorted positions per work-group of the reduction
+constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
+constexpr int kRounds = 8, kWaves = kThreads / 64, kSortTile = kThreads * kRounds;
+
+template <typename T> constexpr int kVec = 16 / sizeof(T);
+
+// VEC elements as fp32, and back with one rounding
+template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float (&x)[VEC]) {
+  if constexpr (VEC == 1) {
+    x[0] = to_f(*p);
+  } else if constexpr (sizeof(T) == 2) {
+    load8(p, x);
+  } else {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i];
+  }
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
+  if constexpr (VEC == 1) *p = from_f<T>(x[0]);
+  else if constexpr (sizeof(T) == 2) store8(p, x);
+  else *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+}
+
+// ---------------------------------------------------------------------------
+// lookup; a token id outside [0, vocab) gives a row of NaN
+// ---------------------------------------------------------------------------
+template <typename T, int VEC>
+__global__ __launch_bounds__(kThreads) void lookup_kernel(const int64_t* __restrict__ ids, int64_t n,
+                                                          const T* __restrict__ w, int64_t ldw, int64_t vocab, int dim,
+                                                          float scale, T* __restrict__ out) {
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= n) return;
+  const int64_t id = ids[row];
+  const bool ok = id >= 0 && id < vocab;
+  for (int d = (blockIdx.y * blockDim.x + threadIdx.x) * VEC; d < dim; d += gridDim.y * blockDim.x * VEC) {
+    float x[VEC];
+    if (ok) load_vec<T, VEC>(w + id * ldw + d, x);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = ok ? x[i] * scale : __builtin_nanf("");
+    store_vec<T, VEC>(out + row * dim + d, x);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// stable sort of the positions by id, kDigitBits at a time from the low end.  The key of a
+// token that takes no part (outside the vocabulary, or the padding id) is `vocab`.
+// ---------------------------------------------------------------------------
+struct SortArgs {
+  const int64_t* ids;     // first pass: key from the ids, position the index
+  const uint32_t* key_in; // later passes
+  const uint32_t* pos_in;
+  uint32_t* key_out;
+  uint32_t* pos_out;
+  uint32_t* hist;         // [kBins][tiles]
+  int64_t n;
+  int64_t vocab, padding;
+  int tiles, shift;
+};
+
+__device__ __forceinline__ uint32_t key_at(const SortArgs& a, int64_t i) {
+  if (!a.ids) return a.key_in[i];
+  const int64_t id = a.ids[i];
+  return id < 0 || id >= a.vocab || id == a.padding ? (uint32_t)a.vocab : (uint32_t)id;
+}
+
+__global__ __launch_bounds__(kThreads) void sort_count_kernel(SortArgs a) {
+  __shared__ uint32_t bins[kBins];
+  for (int b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * kSortTile;
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = i0 + r * kThreads + threadIdx.x;
+    if (i < a.n) atomicAdd(&bins[(key_at(a, i) >> a.shift) & (kBins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += kThreads) a.hist[(int64_t)b * a.tiles + blockIdx.x] = bins[b];
+}
+
+// exclusive prefix sums of `count` values by one work-group
+constexpr int kScanThreads = 1024;
+__global__ __launch_bounds__(kScanThreads) void sort_scan_kernel(uint32_t* x, int64_t count) {
+  __shared__ uint32_t wave_sum[kScanThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t per = (count + kScanThreads - 1) / kScanThreads;
+  const int64_t b = min(count, threadIdx.x * per), e = min(count, b + per);
+  uint32_t sum = 0;
+  for (int64_t i = b; i < e; ++i) sum += x[i];
+  uint32_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) wave_sum[wave] = incl;
+  __syncthreads();
+  uint32_t before = incl - sum;
+  for (int w = 0; w < wave; ++w) before += wave_sum[w];
+  for (int64_t i = b; i < e; ++i) {
+    const uint32_t y = x[i];
+    x[i] = before;
+    before += y;
+  }
+}
+
+// Lanes of the wave whose digit equals this lane's, among the `on` ones.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool on) {
+  uint64_t m = __builtin_amdgcn_ballot_w64(on);
+#pragma unroll
+  for (int b = 0; b < kDigitBits; ++b) {
+    const uint64_t set = __builtin_amdgcn_ballot_w64((digit >> b) & 1);
+    m &= (digit >> b) & 1 ? set : ~set;
+  }
+  return m;
+}
+
+// A wave owns kRounds x 64 consecutive elements and takes them 64 at a time; an element's
+// place is its digit's base for the wave plus the number of earlier elements with the digit.
+__global__ __launch_bounds__(kThreads) void sort_scatter_kernel(SortArgs a) {
+  __shared__ uint32_t base[kWaves][kBins];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int b = threadIdx.x; b < kWaves * kBins; b += kThreads) (&base[0][0])[b] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * kSortTile + wave * (kRounds * 64) + lane;
+  uint32_t key[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = i0 + 64 * r;
+    key[r] = i < a.n ? key_at(a, i) : 0;
+    if (i < a.n) atomicAdd(&base[wave][(key[r] >> a.shift) & (kBins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    uint32_t at = a.hist[(int64_t)b * a.tiles + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t c = base[w][b];
+      base[w][b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = i0 + 64 * r;
+    const bool on = i < a.n;
+    const uint32_t digit = (key[r] >> a.shift) & (kBins - 1);
+    const uint64_t same = same_digit(digit, on);
+    const uint64_t before = same & ((1ull << lane) - 1);
+    uint32_t at = 0;
+    if (on) {
+      at = base[wave][digit] + (uint32_t)__popcll(before);
+      a.key_out[at] = key[r];
+      a.pos_out[at] = a.ids ? (uint32_t)i : a.pos_in[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (on && before == 0) base[wave][digit] += (uint32_t)__popcll(same);  // the digit's first lane
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void zero_kernel(u32x4* p, int64_t vectors, unsigned char* tail, int tail_bytes) {
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < vectors; i += step) p[i] = u32x4{0, 0, 0, 0};
+  if (blockIdx.x == 0 && (int)threadIdx.x < tail_bytes) tail[threadIdx.x] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// sums of the rows of dout over runs of equal ids
+// ---------------------------------------------------------------------------
+struct ReduceArgs {
+  const uint32_t* key;  // sorted ids
+  const uint32_t* pos;
+  int64_t n;
+  uint32_t vocab;       // the key of tokens that take no part
+  int64_t ldd;          // row stride of dout
+  int dim;
+  float scale;
+  float* part;          // [chunks][2][dim]: the run that began earlier, the run that goes on
+};
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(kThreads) void reduce_kernel(ReduceArgs a, const T* __restrict__ dout,
+                                                          T* __restrict__ dw) {
+  __shared__ uint32_t key[kChunk + 2], pos[kChunk];  // key[0], key[count + 1]: the neighbours'
+  const int64_t i0 = (int64_t)blockIdx.x * kChunk;
+  const int count = (int)min((int64_t)kChunk, a.n - i0);
+  const int t = threadIdx.x;
+  if (t < count) pos[t] = a.pos[i0 + t];
+  // `vocab` stands for no neighbour: runs of it are skipped anyway
+  if (t < count + 2) key[t] = i0 + t >= 1 && i0 + t <= a.n ? a.key[i0 + t - 1] : a.vocab;
+  __syncthreads();
+  const int d = (blockIdx.y * kThreads + t) * VEC;
+  if (d >= a.dim) return;
+  float acc[VEC] = {};
+  bool earlier = key[0] == key[1];
+  constexpr int U = 8;
+  for (int j0 = 0; j0 < count; j0 += U) {
+    float x[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = min(j0 + u, count - 1);
+      if (key[j + 1] != a.vocab) load_vec<T, VEC>(dout + pos[j] * a.ldd + d, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u;
+      if (j >= count) break;
+      const uint32_t id = key[j + 1];
+      if (id == a.vocab) break;  // sorted last: nothing follows
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += x[u][i];
+      const bool last = j + 1 == count;
+      if (!last && key[j + 2] == id) continue;
+      const bool goes_on = last && key[j + 2] == id;
+      if (earlier || goes_on) {
+        float* q = a.part + ((int64_t)blockIdx.x * 2 + (earlier ? 0 : 1)) * a.dim + d;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q[i] = acc[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] *= a.scale;
+        store_vec<T, VEC>(dw + (int64_t)id * a.dim + d, acc);
+      }
+      earlier = false;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+    }
+  }
+}
+
+// the runs that chunk borders cut: the chunk a run begins in adds its parts in chunk order
+template <typename T, int VEC>
+__global__ __launch_bounds__(kThreads) void join_kernel(ReduceArgs a, T* __restrict__ dw) {
+  const int64_t c = blockIdx.x, first = c * kChunk, next = first + kChunk;
+  if (next >= a.n) return;  // the last chunk: its last run goes nowhere
+  const uint32_t id = a.key[next - 1];
+  if (id == a.vocab || a.key[next] != id) return;
+  if (a.key[first] == id && first > 0 && a.key[first - 1] == id) return;  // began earlier
+  const int d = (blockIdx.y * kThreads + threadIdx.x) * VEC;
+  if (d >= a.dim) return;
+  // the chunks that the run reaches into
+  int64_t end = c + 2;
+  while (end * kChunk < a.n && a.key[end * kChunk - 1] == id && a.key[end * kChunk] == id) ++end;
+  float acc[VEC];
+  const float* q = a.part + (c * 2 + 1) * a.dim + d;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] = q[i];
+#pragma unroll 4
+  for (int64_t e = c + 1; e < end; ++e) {
+    const float* r = a.part + e * 2 * a.dim + d;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] += r[i];
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] *= a.scale;
+  store_vec<T, VEC>(dw + (int64_t)id * a.dim + d, acc);
+}
+
+bool ok16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int64_t tiles_of(int64_t n) { return (n + kSortTile - 1) / kSortTile; }
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
+
+// the workspace: two (key, position) buffers, the digit counts, the partial rows
+struct Workspace {
+  int64_t key[2], pos[2], hist, part, bytes;
+  Workspace(int64_t n, int64_t dim) {
+    int64_t at = 0;
+    auto take = [&](int64_t bytes_) {
+      const int64_t r = at;
+      at += up16(bytes_);
+      return r;
+    };
+    for (int i = 0; i < 2; ++i) {
+      key[i] = take(4 * n);
+      pos[i] = take(4 * n);
+    }
+    hist = take(4 * (int64_t)kBins * tiles_of(n));
+    part = take(8 * chunks_of(n) * dim);
+    bytes = at;
+  }
+};
+
+template <typename T>
+void launch_lookup(const int64_t* ids, int64_t n, const void* w, int64_t ldw, int64_t vocab, int64_t dim, float scale,
+                   void* out, hipStream_t s) {
+  const bool vec = ok16(w) && ok16(out) && dim % kVec<T> == 0 && ldw % kVec<T> == 0;
+  const int64_t lanes = vec ? dim / kVec<T> : dim;
+  int tx = 1;
+  while (tx < kThreads && tx < lanes) tx *= 2;
+  const dim3 block((unsigned)tx, (unsigned)(kThreads / tx));
+  const dim3 grid((unsigned)((n + block.y - 1) / block.y), (unsigned)((lanes + tx - 1) / tx));
+  if (vec)
+    hipLaunchKernelGGL((lookup_kernel<T, kVec<T>>), grid, block, 0, s, ids, n, (const T*)w, ldw, vocab, (int)dim, scale,
+                       (T*)out);
+  else
+    hipLaunchKernelGGL((lookup_kernel<T, 1>), grid, block, 0, s, ids, n, (const T*)w, ldw, vocab, (int)dim, scale,
+                       (T*)out);
+}
+
+template <typename T>
+void launch_sums(const ReduceArgs& a, const void* dout, void* dw, hipStream_t s) {
+  const bool vec = ok16(dout) && ok16(dw) && a.dim % kVec<T> == 0 && a.ldd % kVec<T> == 0;
+  const int64_t lanes = vec ? a.dim / kVec<T> : a.dim;
+  const dim3 grid((unsigned)chunks_of(a.n), (unsigned)((lanes + kThreads - 1) / kThreads));
+  {
+    TimedLaunch timed_("embedding.reduce_kernel", s);
+    if (vec) hipLaunchKernelGGL((reduce_kernel<T, kVec<T>>), grid, dim3(kThreads), 0, s, a, (const T*)dout, (T*)dw);
+    else hipLaunchKernelGGL((reduce_kernel<T, 1>), grid, dim3(kThreads), 0, s, a, (const T*)dout, (T*)dw);
+  }
+  if (grid.x == 1) return;
+  TimedLaunch timed_("embedding.join_kernel", s);
+  if (vec) hipLaunchKernelGGL((join_kernel<T, kVec<T>>), grid, dim3(kThreads), 0, s, a, (T*)dw);
+  else hipLaunchKernelGGL((join_kernel<T, 1>), grid, dim3(kThreads), 0, s, a, (T*)dw);
+}
+
+}  // namespace embed
+}  // namespace ts
+
+using namespace ts::embed;
+
+extern "C" {
+
+int ts_embedding_fwd(const int64_t* ids, int64_t n, const void* weight, int64_t ld_weight, int64_t vocab, int64_t dim,
+                     float scale, void* out, int dtype, void* stream) {
+  TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F16 || dtype == TS_BF16, "ts_embedding_fwd: dtype %d", dtype);
+  TS_CHECK_ARG(n >= 0 && n < (1ll << 31) && vocab >= 0 && vocab < (1ll << 31) && dim >= 1 && dim < (1 << 20) &&
+                   ld_weight >= dim,
+               "ts_embedding_fwd: bad shape n=%lld vocab=%lld dim=%lld", (long long)n, (long long)vocab,
+               (long long)dim);
+  if (n == 0) return TS_OK;
+  TS_CHECK_ARG(ids && out && (weight || vocab == 0), "ts_embedding_fwd: null pointer");
+  hipStream_t s = (hipStream_t)stream;
+  {
+    ts::TimedLaunch timed_("embedding.lookup_kernel", s);
+    if (dtype == TS_F32) launch_lookup<float>(ids, n, weight, ld_weight, vocab, dim, scale, out, s);
+    else if (dtype == TS_F16) launch_lookup<ts::f16>(ids, n, weight, ld_weight, vocab, dim, scale, out, s);
+    else launch_lookup<ts::bf16>(ids, n, weight, ld_weight, vocab, dim, scale, out, s);
+  }
+  return ts::check_launch("ts_embedding_fwd");
+}
+
+int64_t ts_embedding_bwd_workspace(int64_t n, int64_t dim) {
+  return n > 0 && dim > 0 ? Workspace(n, dim).bytes : 0;
+}
+
+int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_t ld_grad, int64_t vocab, int64_t dim,
+                     int64_t padding, float scale, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                     int dtype, void* stream) {
+  TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F16 || dtype == TS_BF16, "ts_embedding_bwd: dtype %d", dtype);
+  TS_CHECK_ARG(n >= 0 && n < (1ll << 31) && vocab >= 0 && vocab < (1ll << 31) - 1 && dim >= 1 && dim < (1 << 20),
+               "ts_embedding_bwd: bad shape n=%lld vocab=%lld dim=%lld", (long long)n, (long long)vocab,
+               (long long)dim);
+  if (vocab == 0) return TS_OK;
+  TS_CHECK_ARG(grad_weight && ok16(grad_weight), "ts_embedding_bwd: grad_weight null or not 16-byte aligned");
+  hipStream_t s = (hipStream_t)stream;
+  {
+    const int64_t bytes = vocab * dim * (dtype == TS_F32 ? 4 : 2);
+    ts::TimedLaunch timed_("embedding.zero_kernel", s);
+    const int64_t blocks = std::min<int64_t>((bytes / 16 + kThreads - 1) / kThreads, 4096);
+    hipLaunchKernelGGL(zero_kernel, dim3((unsigned)std::max<int64_t>(blocks, 1)), dim3(kThreads), 0, s,
+                       (ts::u32x4*)grad_weight, bytes / 16, (unsigned char*)grad_weight + bytes / 16 * 16,
+                       (int)(bytes % 16));
+  }
+  int st = ts::check_launch("ts_embedding_bwd (zero)");
+  if (st != TS_OK || n == 0) return st;
+  TS_CHECK_ARG(ids && grad_out && ld_grad >= 0, "ts_embedding_bwd: null pointer");
+  TS_CHECK_ARG(workspace && ok16(workspace) && workspace_bytes >= ts_embedding_bwd_workspace(n, dim),
+               "ts_embedding_bwd: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
+               (long long)ts_embedding_bwd_workspace(n, dim));
+  const Workspace ws(n, dim);
+  char* base = (char*)workspace;
+  SortArgs a;
+  a.n = n;
+  a.vocab = vocab;
+  a.padding = padding;
+  a.tiles = (int)tiles_of(n);
+  a.hist = (uint32_t*)(base + ws.hist);
+  int out = 0;
+  a.ids = ids;
+  a.key_in = a.pos_in = nullptr;
+  for (a.shift = 0; a.shift == 0 || (vocab >> a.shift) > 0; a.shift += kDigitBits) {
+    a.key_out = (uint32_t*)(base + ws.key[out]);
+    a.pos_out = (uint32_t*)(base + ws.pos[out]);
+    {
+      ts::TimedLaunch timed_("embedding.sort_count_kernel", s);
+      hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)a.tiles), dim3(kThreads), 0, s, a);
+    }
+    {
+      ts::TimedLaunch timed_("embedding.sort_scan_kernel", s);
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, a.hist, (int64_t)kBins * a.tiles);
+    }
+    {
+      ts::TimedLaunch timed_("embedding.sort_scatter_kernel", s);
+      hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)a.tiles), dim3(kThreads), 0, s, a);
+    }
+    a.ids = nullptr;
+    a.key_in = a.key_out;
+    a.pos_in = a.pos_out;
+    out ^= 1;
+  }
+  ReduceArgs r;
+  r.key = a.key_in;
+  r.pos = a.pos_in;
+  r.n = n;
+  r.vocab = (uint32_t)vocab;
+  r.ldd = ld_grad;
+  r.dim = (int)dim;
+  r.scale = scale;
+  r.part = (float*)(base + ws.part);
+  if (dtype == TS_F32) launch_sums<float>(r, grad_out, grad_weight, s);
+  else if (dtype == TS_F16) launch_sums<ts::f16>(r, grad_out, grad_weight, s);
+  else launch_sums<ts::bf16>(r, grad_out, grad_weight, s);
+  return ts::check_launch("ts_embedding_bwd");
+}
+
+}  // extern "C"

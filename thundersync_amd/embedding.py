@@ -1,0 +1,152 @@
+"""Embedding lookup with a scale and its gradient by sorted tokens, on the gfx950 kernels.
+
+:func:`embedding` is ``scale * weight[ids]`` for bf16, fp16 or fp32 tables
+(one rounding of the fp32 product).  Its gradient with respect to the table is
+dense, like ``torch.nn.functional.embedding``'s, but summed in fp32 in token
+order without atomics (``ts_embedding_bwd`` sorts the positions by token), so
+it has the same bytes every time, and rounded once.
+
+A token id outside ``[0, vocab)`` gives a row of NaN and no gradient (a bad id
+surfaces as a NaN loss, as a target of the fused logprob does);
+``THUNDERSYNC_CHECK_TARGETS=1`` checks the ids first and raises.
+
+:func:`use_hip_embedding` swaps a model's ``torch.nn.Embedding`` modules for
+:class:`HipEmbedding`, with the Parameter's identity kept (a head tied to the
+table stays tied).  GPU only: other dtypes and CPU tensors raise in
+:func:`embedding`; the swapped module keeps torch's forward for them.
+"""
+
+from __future__ import annotations
+
+import math
+import os
+
+import torch
+
+from . import _lib
+from .fused_logprob import CHECK_TARGETS_ENV, _check_targets
+from .operator_profiling import device_role, operator_range
+
+DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+ID_DTYPES = (torch.int64, torch.int32)
+
+
+def _validate(ids, weight, scale, padding_idx):
+    if weight.dim() != 2 or weight.shape[1] < 1:
+        raise ValueError(f"weight must be [V, D], got {tuple(weight.shape)}")
+    if ids.dtype not in ID_DTYPES:
+        raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
+    if not (isinstance(scale, (int, float)) and math.isfinite(scale)):
+        raise ValueError(f"scale must be a finite number, got {scale!r}")
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx {padding_idx} is outside the vocabulary [0, {weight.shape[0]})")
+    if not ids.is_cuda or not weight.is_cuda:
+        raise RuntimeError("thundersync_amd embedding runs on the GPU only; got a CPU tensor")
+    if ids.device != weight.device:
+        raise ValueError(f"ids on {ids.device} and weight on {weight.device}")
+    if weight.dtype not in DTYPES:
+        raise TypeError(f"thundersync_amd embedding takes a bf16, fp16 or fp32 weight, got {weight.dtype}")
+    if os.environ.get(CHECK_TARGETS_ENV, "0") not in ("", "0"):
+        _check_targets(ids.reshape(-1), weight.shape[0])
+
+
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    """``[N, D]`` with unit stride in the rows (which may repeat: a stride of 0)."""
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def embedding_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    """``scale * weight[ids]`` (ids of any shape), without autograd."""
+    lib = _lib.require_library()
+    flat = ids.reshape(-1).to(torch.int64).contiguous()
+    w = weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
+    v, d = w.shape
+    out = torch.empty(*ids.shape, d, dtype=w.dtype, device=w.device)
+    _lib.check(
+        lib.ts_embedding_fwd(flat.data_ptr(), flat.numel(), w.data_ptr(), max(w.stride(0), d), v, d, float(scale),
+                             out.data_ptr(), _lib.dtype_code(w.dtype), _lib.stream_of(w)),
+        lambda: f"ts_embedding_fwd(tokens={flat.numel()}, vocab={v}, dim={d})",
+    )
+    return out
+
+
+def embedding_backward(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int, *, scale: float = 1.0,
+                       padding_idx: int | None = None) -> torch.Tensor:
+    """The table's gradient ``[vocab, D]`` for ``grad_out`` ``[*ids.shape, D]``."""
+    lib = _lib.require_library()
+    d = grad_out.shape[-1]
+    flat = ids.reshape(-1).to(torch.int64).contiguous()
+    n = flat.numel()
+    g = _unit_rows(grad_out.reshape(n, d))
+    grad = torch.empty(vocab, d, dtype=g.dtype, device=g.device)
+    ws_bytes = int(lib.ts_embedding_bwd_workspace(n, d))
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=g.device)
+    _lib.check(
+        lib.ts_embedding_bwd(flat.data_ptr(), n, g.data_ptr(), g.stride(0), vocab, d,
+                             -1 if padding_idx is None else int(padding_idx), float(scale), grad.data_ptr(),
+                             ws.data_ptr(), ws_bytes, _lib.dtype_code(g.dtype), _lib.stream_of(g)),
+        lambda: f"ts_embedding_bwd(tokens={n}, vocab={vocab}, dim={d})",
+    )
+    return grad
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.vocab, ctx.dtype, ctx.scale, ctx.padding_idx = weight.shape[0], weight.dtype, scale, padding_idx
+        with torch.cuda.device(weight.device), operator_range(
+                "embedding_forward", role=device_role(weight.device), tokens=ids.numel(), hidden=weight.shape[1],
+                vocab=weight.shape[0], dtype=weight.dtype):
+            return embedding_forward(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        with torch.cuda.device(grad.device), operator_range(
+                "embedding_backward", role=device_role(grad.device), tokens=ids.numel(), hidden=grad.shape[-1],
+                vocab=ctx.vocab):
+            gw = embedding_backward(ids, grad.to(ctx.dtype), ctx.vocab, scale=ctx.scale, padding_idx=ctx.padding_idx)
+        return None, gw, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+              padding_idx: int | None = None) -> torch.Tensor:
+    """``scale * weight[ids]``: ``[*ids.shape, D]`` for int64 or int32 ``ids`` of any shape.
+
+    The row ``padding_idx`` of the table gets no gradient.
+    """
+    _validate(ids, weight, scale, padding_idx)
+    return _Embedding.apply(ids, weight, float(scale), padding_idx)
+
+
+class HipEmbedding(torch.nn.Embedding):
+    """``torch.nn.Embedding`` on the HIP kernels; a call they do not serve (a CPU
+    tensor, another dtype, the library switched off) runs torch's forward."""
+
+    def forward(self, input):  # noqa: A002 - torch's name
+        takes = (input.is_cuda and self.weight.is_cuda and input.dtype in ID_DTYPES and self.weight.dtype in DTYPES
+                 and input.device == self.weight.device and _lib.library() is not None)
+        if not takes:
+            return super().forward(input)
+        return embedding(input, self.weight, padding_idx=self.padding_idx)
+
+
+def use_hip_embedding(model: torch.nn.Module) -> int:
+    """Swap every plain ``torch.nn.Embedding`` below ``model`` for :class:`HipEmbedding`
+    and return the count.  Modules with ``max_norm``, ``scale_grad_by_freq`` or
+    ``sparse`` and subclasses of their own are left alone."""
+    count = 0
+    for name, module in list(model.named_modules()):
+        if not name or type(module) is not torch.nn.Embedding:
+            continue
+        if module.max_norm is not None or module.scale_grad_by_freq or module.sparse:
+            continue
+        with torch.device("meta"):
+            swapped = HipEmbedding(module.num_embeddings, module.embedding_dim, module.padding_idx)
+        swapped.weight = module.weight
+        swapped.train(module.training)
+        model.set_submodule(name, swapped)
+        count += 1
+    return count

@@ -119,22 +119,22 @@ def _forward_exact(hidden, weight, target, with_entropy):
     return lp, ent, lse
 
 
-def _backward_exact(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_weight_grad):
-    """fp32 / fp64: the reference's chunk loop (FL:137-193) with a [chunk, V]
-    dlogits block in the input type; grad_weight accumulated in it."""
+def head_vjp_exact(h, w, chunk, needs_weight_grad, dlogits, h_weight=None):
+    """:func:`head_vjp` at fp32 / fp64: the reference's chunk loop (FL:137-193)
+    with a [chunk, V] dlogits block in the input type; grad_weight accumulated in
+    it.  Rows of ``h``, ``w`` and ``h_weight`` have unit stride."""
     lib = _lib.require_library()
-    h, w = _unit_stride(hidden), _unit_stride(weight)
-    t = target.to(torch.int64).contiguous()
     n, d = h.shape
     v = w.shape[0]
     dt, dev = h.dtype, h.device
     grad_hidden = torch.empty(n, d, dtype=dt, device=dev)
     if n == 0:
         return grad_hidden, torch.zeros(v, d, dtype=dt, device=dev) if needs_weight_grad else None
+    h_weight = h if h_weight is None else h_weight
     # the first block writes the weight gradient, the others add to it
     grad_weight = torch.empty(v, d, dtype=dt, device=dev) if needs_weight_grad else None
     code, stream = _lib.dtype_code(dt), _lib.stream_of(h)
-    ldh, ldw = max(h.stride(0), d), max(w.stride(0), d)
+    ldw, ldhw = max(w.stride(0), d), max(h_weight.stride(0), d)
     block = min(max(1, int(chunk)), n)
     vp = (v + 3) // 4 * 4  # rows of whole 16-byte vectors
     dl = torch.empty(block, vp, dtype=dt, device=dev)
@@ -143,21 +143,11 @@ def _backward_exact(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, 
                 for s in ((rows, d, v), *([(v, d, rows)] if needs_weight_grad else []))]
     ws_bytes = max(int(lib.ts_matmul_exact_workspace(*s, code)) for s in products)
     ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
-    g_lp = grad_lp.to(dt).contiguous()
-    g_ent = grad_ent.to(dt).contiguous() if grad_ent is not None else None
     esize = h.element_size()
     for i in range(0, n, block):
         rows = min(block, n - i)
-        h_i = h.data_ptr() + i * ldh * esize
         with operator_range("logprob_head_coefficient_backward", role=device_role(dev), rows=rows, vocab=v):
-            _lib.check(
-                lib.ts_logprob_dlogits_exact(
-                    h_i, ldh, w.data_ptr(), ldw, t[i:].data_ptr(), lse[i:].data_ptr(),
-                    ent[i:].data_ptr() if g_ent is not None else None, g_lp[i:].data_ptr(),
-                    g_ent[i:].data_ptr() if g_ent is not None else None, rows, d, v, dl.data_ptr(), vp, code, stream,
-                ),
-                f"ts_logprob_dlogits_exact(rows={rows}, dim={d}, vocab={v})",
-            )
+            dlogits(i, rows, dl, vp)
         with operator_range("logprob_head_hidden_vjp", role=device_role(dev), rows=rows, hidden=d, vocab=v):
             # grad_hidden[i:i+rows] = dl . W
             _lib.check(
@@ -169,11 +159,36 @@ def _backward_exact(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, 
             with operator_range("logprob_head_weight_vjp", role=device_role(dev), rows=rows, hidden=d, vocab=v):
                 # grad_weight += dl^T . h[i:i+rows]
                 _lib.check(
-                    lib.ts_matmul_exact_ws(dl.data_ptr(), 1, vp, h_i, ldh, 1, v, d, rows, grad_weight.data_ptr(), d,
-                                           int(i > 0), ws.data_ptr(), ws_bytes, code, stream),
+                    lib.ts_matmul_exact_ws(dl.data_ptr(), 1, vp, h_weight.data_ptr() + i * ldhw * esize, ldhw, 1, v, d,
+                                           rows, grad_weight.data_ptr(), d, int(i > 0), ws.data_ptr(), ws_bytes, code,
+                                           stream),
                     f"ts_matmul_exact_ws(dlogits^T . hidden, rows={rows}, dim={d}, vocab={v})",
                 )
     return grad_hidden, grad_weight
+
+
+def _backward_exact(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_weight_grad):
+    """fp32 / fp64: the logits' gradient in the input type (FL:143-165)."""
+    lib = _lib.require_library()
+    h, w = _unit_stride(hidden), _unit_stride(weight)
+    t = target.to(torch.int64).contiguous()
+    d, v = h.shape[1], w.shape[0]
+    ldh, ldw = max(h.stride(0), d), max(w.stride(0), d)
+    code, stream = _lib.dtype_code(h.dtype), _lib.stream_of(h)
+    g_lp = grad_lp.to(h.dtype).contiguous()
+    g_ent = grad_ent.to(h.dtype).contiguous() if grad_ent is not None else None
+
+    def dlogits(i, rows, dl, ld):
+        _lib.check(
+            lib.ts_logprob_dlogits_exact(
+                h.data_ptr() + i * ldh * h.element_size(), ldh, w.data_ptr(), ldw, t[i:].data_ptr(),
+                lse[i:].data_ptr(), ent[i:].data_ptr() if g_ent is not None else None, g_lp[i:].data_ptr(),
+                g_ent[i:].data_ptr() if g_ent is not None else None, rows, d, v, dl.data_ptr(), ld, code, stream,
+            ),
+            f"ts_logprob_dlogits_exact(rows={rows}, dim={d}, vocab={v})",
+        )
+
+    return head_vjp_exact(h, w, chunk, needs_weight_grad, dlogits)
 
 
 def _forward(hidden, weight, target, with_entropy):
@@ -217,19 +232,20 @@ def backward_block_rows(n: int, chunk: int) -> int:
     return min(block, max(n, 1))
 
 
-def _backward(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_weight_grad):
-    if hidden.dtype in EXACT_DTYPES:
-        return _backward_exact(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_weight_grad)
+def head_vjp(h, w, d_in, chunk, needs_weight_grad, dlogits, h_weight=None):
+    """Both vector-Jacobian products of bf16/fp16 head logits, block of rows by
+    block: ``dlogits(i, rows, dl, ld)`` writes rows ``[i, i + rows)`` of the
+    logits' gradient into ``dl``.  ``h`` and ``w`` are padded and aligned,
+    ``d_in`` is the hidden dim before padding; ``h_weight`` (default ``h``) is
+    the left factor of the weight gradient."""
     lib = _lib.require_library()
-    d_in = hidden.shape[1]
-    h, w = _rows_ok(_pad_dim(hidden)), _rows_ok(_pad_dim(weight))
-    t = target.to(torch.int64).contiguous()
     n, d = h.shape
     v = w.shape[0]
     vp = (v + 7) // 8 * 8
     grad_hidden = torch.empty_like(h)
     if n == 0:
-        return grad_hidden[:, :d_in], torch.zeros_like(weight) if needs_weight_grad else None
+        return grad_hidden[:, :d_in], torch.zeros_like(w[:, :d_in]) if needs_weight_grad else None
+    h_weight = h if h_weight is None else h_weight
     stream = _lib.stream_of(h)
     code = _lib.dtype_code(h.dtype)
     block = backward_block_rows(n, chunk)
@@ -242,21 +258,10 @@ def _backward(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_
     # the weight gradient's fp32 sum over the blocks, which one block alone does not need
     grad_weight = torch.empty(v, d, dtype=w.dtype, device=h.device) if needs_weight_grad else None
     acc = torch.empty(v, d, dtype=torch.float32, device=h.device) if needs_weight_grad and n > block else None
-    g_lp = grad_lp.to(torch.float32).contiguous()
-    g_ent = grad_ent.to(torch.float32).contiguous() if grad_ent is not None else None
     for i in range(0, n, block):
         rows = min(block, n - i)
-        hi = h[i : i + rows]
         with operator_range("logprob_head_coefficient_backward", role=device_role(h.device), rows=rows, vocab=v):
-            _lib.check(
-                lib.ts_logprob_dlogits(
-                    hi.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), t[i:].data_ptr(),
-                    lse[i:].data_ptr(), ent[i:].data_ptr() if ent is not None else None,
-                    g_lp[i:].data_ptr(), g_ent[i:].data_ptr() if g_ent is not None else None,
-                    rows, d, v, dl.data_ptr(), vp, code, stream,
-                ),
-                f"ts_logprob_dlogits(rows={rows}, dim={d}, vocab={v})",
-            )
+            dlogits(i, rows, dl, vp)
         with operator_range("logprob_head_hidden_vjp", role=device_role(h.device), rows=rows, hidden=d, vocab=v):
             _lib.check(
                 lib.ts_logprob_grad_hidden(
@@ -271,8 +276,8 @@ def _backward(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_
             with operator_range("logprob_head_weight_vjp", role=device_role(h.device), rows=rows, hidden=d, vocab=v):
                 _lib.check(
                     lib.ts_logprob_grad_weight_block(
-                        dl.data_ptr(), vp, hi.data_ptr(), h.stride(0), rows, d, v, _lib.ptr(acc), d, int(i == 0),
-                        grad_weight.data_ptr() if last else None, d, code, stream,
+                        dl.data_ptr(), vp, h_weight[i:].data_ptr(), h_weight.stride(0), rows, d, v, _lib.ptr(acc), d,
+                        int(i == 0), grad_weight.data_ptr() if last else None, d, code, stream,
                     ),
                     f"ts_logprob_grad_weight_block(rows={rows}, dim={d}, vocab={v})",
                 )
@@ -280,6 +285,31 @@ def _backward(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_
         grad_hidden = grad_hidden[:, :d_in].contiguous()
         grad_weight = grad_weight[:, :d_in].contiguous() if grad_weight is not None else None
     return grad_hidden, grad_weight
+
+
+def _backward(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_weight_grad):
+    if hidden.dtype in EXACT_DTYPES:
+        return _backward_exact(hidden, weight, target, lse, ent, grad_lp, grad_ent, chunk, needs_weight_grad)
+    lib = _lib.require_library()
+    h, w = _rows_ok(_pad_dim(hidden)), _rows_ok(_pad_dim(weight))
+    t = target.to(torch.int64).contiguous()
+    d, v = h.shape[1], w.shape[0]
+    g_lp = grad_lp.to(torch.float32).contiguous()
+    g_ent = grad_ent.to(torch.float32).contiguous() if grad_ent is not None else None
+    code, stream = _lib.dtype_code(h.dtype), _lib.stream_of(h)
+
+    def dlogits(i, rows, dl, ld):
+        _lib.check(
+            lib.ts_logprob_dlogits(
+                h[i:].data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), t[i:].data_ptr(),
+                lse[i:].data_ptr(), ent[i:].data_ptr() if ent is not None else None,
+                g_lp[i:].data_ptr(), g_ent[i:].data_ptr() if g_ent is not None else None,
+                rows, d, v, dl.data_ptr(), ld, code, stream,
+            ),
+            f"ts_logprob_dlogits(rows={rows}, dim={d}, vocab={v})",
+        )
+
+    return head_vjp(h, w, hidden.shape[1], chunk, needs_weight_grad, dlogits)
 
 
 class _FusedLinearLogprob(torch.autograd.Function):
