@@ -421,6 +421,11 @@ int ts_logprob_grad_hidden(const void* dlogits, int64_t ld_dlogits, const void* 
                            void* grad_hidden, int64_t ld_grad, void* workspace,
                            int64_t workspace_bytes, int dtype, void* stream);
 
+/* ts_logprob_grad_hidden with the fp32 sums themselves, [rows, dim] dense. */
+int ts_logprob_grad_hidden_f32(const void* dlogits, int64_t ld_dlogits, const void* weight, int64_t ld_weight,
+                               int64_t rows, int64_t dim, int64_t vocab, float* grad_hidden, void* workspace,
+                               int64_t workspace_bytes, int dtype, void* stream);
+
 /* grad_weight [vocab, ld_grad] (fp32) += dlogits[:rows]^T . hidden[:rows]
  * on MFMA with fp32 accumulation; called once per dlogits block, it
  * accumulates the weight gradient across blocks in block order, to be cast to
@@ -527,35 +532,47 @@ int64_t ts_distill_fwd_workspace(int64_t rows, int64_t vocab);
 
 /* bf16 or fp16: loss, lse (of the logits over T, natural log) and slot_z (the
  * logits at the slots, not over T), all fp32.  hidden and weight as for
- * ts_logprob_fwd. */
+ * ts_logprob_fwd.  With exps not null the exponentials of (z - m) / T, m the
+ * maximum of the row's tile of 256 vocabulary rows, are stored there in the
+ * element type ([rows, ld_exps >= vocab rounded up to 8], pad columns zero); the
+ * workspace then begins with the maxima, [ceil(vocab / 256), rows] floats. */
 int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
                    int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
                    float* slot_z, int64_t pitch, int64_t top, const int32_t* state, float* loss, float* lse,
-                   void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+                   void* exps, int64_t ld_exps, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
-/* bf16 or fp16: dlogits [rows, ld_dlogits >= vocab rounded up to 8] in the
- * element type, each rounded once from fp32; columns past the vocabulary are
- * written as zero.  Inputs as ts_distill_fwd took and gave them. */
+/* fp32 or fp64: loss, lse and slot_z of a block of logits [rows, ld_logits]. */
+int ts_distill_fwd_exact(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, double temperature,
+                         const int32_t* slot_id, const void* slot_p, void* slot_z, int64_t pitch, int64_t top,
+                         const int32_t* state, void* loss, void* lse, int dtype, void* stream);
+
+/* dlogits from what a forward stored: ts_distill_fwd's exps and tile maxima
+ * (bf16, fp16), or the logits (fp32, fp64; tile_max null).  A null grad: q - p,
+ * without the 1 / T.  dlogits may be the stored block itself; columns past the
+ * vocabulary are zero in bf16 and fp16, untouched otherwise.  Entries are
+ * rounded once from the stored values, the slots' from slot_z. */
+int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_max, int64_t rows, int64_t vocab,
+                      double temperature, const int32_t* slot_id, const void* slot_p, const void* slot_z,
+                      int64_t pitch, int64_t top, const int32_t* state, const void* lse, const void* grad,
+                      void* dlogits, int64_t ld_dlogits, int dtype, void* stream);
+
+/* bf16 or fp16: dlogits [rows, ld_dlogits >= vocab rounded up to 8] with the
+ * logits formed again, each entry rounded once from fp32; columns past the
+ * vocabulary are zero.  Inputs as ts_distill_fwd took and gave them. */
 int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
                        int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
                        const float* slot_z, int64_t pitch, int64_t top, const int32_t* state, const float* lse,
                        const float* grad, void* dlogits, int64_t ld_dlogits, int dtype, void* stream);
 
-/* The parts of the fp32 and fp64 path, around ts_logprob_fwd_exact and
- * ts_logprob_dlogits_exact on rows divided by T: slot_z = hidden . weight[slot_id]
- * (any dtype), loss from slot_z and lse (both over T), the slots' entries of
- * dlogits = grad_scale grad (exp(logit_scale slot_z - lse) - slot_p), and
- * out = scale hidden with zeros in the rows whose state is 0. */
-int ts_distill_scores(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight,
-                      const int32_t* slot_id, int64_t pitch, int64_t rows, int64_t top, int64_t dim, void* slot_z,
-                      int dtype, void* stream);
-int ts_distill_loss(const int32_t* slot_id, const void* slot_p, const void* slot_z, int64_t pitch, int64_t top,
-                    const int32_t* state, const void* lse, int64_t rows, void* loss, int dtype, void* stream);
-int ts_distill_slots(const int32_t* slot_id, const void* slot_p, const void* slot_z, int64_t pitch, int64_t top,
-                     const void* lse, const void* grad, int64_t rows, double logit_scale, double grad_scale,
-                     void* dlogits, int64_t ld_dlogits, int dtype, void* stream);
-int ts_distill_rows(const void* hidden, int64_t ld_hidden, const int32_t* state, int64_t rows, int64_t dim,
-                    double scale, void* out, int64_t ld_out, int dtype, void* stream);
+/* out [rows, dim] = hidden, with zeros in the rows whose state is 0. */
+int ts_distill_rows(const void* hidden, int64_t ld_hidden, const int32_t* state, int64_t rows, int64_t dim, void* out,
+                    int dtype, void* stream);
+
+/* out [rows, dim] (dtype) = grad / T unit (fp64 for dtype TS_F64, otherwise
+ * fp32), with zeros in the rows whose state is 0: the hidden states' gradient
+ * from that of q - p. */
+int ts_distill_scale(const void* unit, const void* grad, const int32_t* state, int64_t rows, int64_t dim,
+                     double temperature, void* out, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Embedding (fp32, fp16 or bf16)

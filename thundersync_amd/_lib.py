@@ -57,6 +57,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "ts_logprob_grad_hidden_workspace": (_I64, [_I64, _I64, _I64]),
     "ts_logprob_grad_hidden": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _INT, _P]),
+    "ts_logprob_grad_hidden_f32": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _INT, _P]),
     "ts_logprob_grad_weight_block": (
         _INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _INT, _P, _I64, _INT, _P]),
     "ts_logprob_grad_weight": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _INT, _P]),
@@ -82,16 +83,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ts_distill_fwd_workspace": (_I64, [_I64, _I64]),
     "ts_distill_fwd": (
         _INT,
-        [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _INT, _P],
+        [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I64, _INT, _P],
     ),
-    "ts_distill_scores": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _INT, _P]),
-    "ts_distill_loss": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _I64, _P, _INT, _P]),
+    "ts_distill_fwd_exact": (_INT, [_P, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _INT, _P]),
+    "ts_distill_finish": (
+        _INT, [_P, _I64, _P, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _INT, _P]),
     "ts_distill_dlogits": (
         _INT,
         [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _INT, _P],
     ),
-    "ts_distill_slots": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _I64, _D, _D, _P, _I64, _INT, _P]),
-    "ts_distill_rows": (_INT, [_P, _I64, _P, _I64, _I64, _D, _P, _I64, _INT, _P]),
+    "ts_distill_rows": (_INT, [_P, _I64, _P, _I64, _I64, _P, _INT, _P]),
+    "ts_distill_scale": (_INT, [_P, _P, _P, _I64, _I64, _D, _P, _INT, _P]),
     "ts_embedding_fwd": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _F, _P, _INT, _P]),
     "ts_embedding_bwd_workspace": (_I64, [_I64, _I64]),
     "ts_embedding_bwd": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _I64, _INT, _P]),

@@ -6,13 +6,16 @@
 //   present slots of teacher[n] / T, the slots of one token added together
 //   loss[n] = sum_k p_k (log p_k - log q_k),  dz[n, v] = g[n] / T (q_v - p_v)
 //
-// Forward: teacher_kernel turns each row's slots into (token, p); stats_kernel reduces the
-// logits of a 256-row vocabulary tile to (max, sum exp) per token in its MFMA epilogue;
-// scores_kernel takes the logits at the slots' tokens as dot products; loss_kernel merges
-// the tiles and sums the slots.  Backward, per block of rows: dlogits_kernel recomputes the
-// logits and writes the block's q part in the element type, slots_kernel overwrites the
-// slots' entries with g / T (q - p) rounded once; the vector-Jacobian products with W and h
-// are the fused logprob's.  Bound by the products, as the fused logprob is (its GEMM core).
+// teacher_kernel turns each row's slots into (token, p).  16-bit types: stats_kernel reduces
+// the logits of a 256-row vocabulary tile to (max, sum exp) per token in its MFMA epilogue and,
+// where a gradient follows, stores the tile's exponentials in the element type;
+// scores_kernel takes the logits at the slots' tokens as dot products; loss_kernel merges the
+// tiles and sums the slots; finish_kernel scales the exponentials to q, in one pass over
+// 2 bytes an entry in place of a second product of 2 D flops an entry, and writes the slots'
+// entries from their fp32 logits.  Where the stored block would outgrow its bound,
+// dlogits_kernel forms it from the logits again.  fp32 and fp64: the logits of a block of
+// rows by the exact product, then one work-group a row.  The vector-Jacobian products with W
+// and h are the fused logprob's.  Bound by the products (the fused logprob's GEMM core).
 #include <algorithm>
 #include <type_traits>
 
@@ -130,12 +133,37 @@ struct StatsArgs {
   float unit;      // log2(e) / T
   float* part_m;   // [n_vtiles][rows]
   float* part_s;
+  bf16* exps;      // STORE: [rows][lde], exp((z - tile's max) / T) in E (pad columns 0)
+  int64_t lde;
+  int vocab_pad;
 };
 
-template <typename E, class S>
-__global__ __launch_bounds__(kGemmThreads, 1) void stats_kernel(StatsArgs p) {
-  GEMM_RING_OF(S)
-  constexpr int MI = S::MI, NI = S::NI;
+template <class S> constexpr int kPasses = S::BN > TN ? S::WN : 1;  // halves of a Wide tile take turns in the staging
+
+// coalesced store of the staged [PT tokens][TM vocabulary rows] of one pass
+template <class S, class Quarter>
+__device__ __forceinline__ void store_staged(Quarter&& quarter, bf16* out, int64_t ld, int n0, int rows, int v0,
+                                             int vocab_pad, int pass) {
+  constexpr int PT = S::BN / kPasses<S>;
+  const int vmax = min(TM, vocab_pad - v0);
+#pragma unroll 4
+  for (int it = 0; it < (PT * TM / 8) / kGemmThreads; ++it) {
+    const int c = it * kGemmThreads + threadIdx.x;
+    const int row = c / (TM / 8), chunk = (c % (TM / 8)) * 8;
+    const int n = n0 + pass * PT + row;
+    if (n < rows && chunk < vmax)
+      *reinterpret_cast<u32x4*>(out + (int64_t)n * ld + v0 + chunk) =
+          *reinterpret_cast<const u32x4*>(quarter(row >> 6) + (row & 63) * OPITCH + chunk);
+  }
+}
+
+// The tile's maximum is exchanged between the waves before the exponentials are formed, so
+// that all of a token's exponentials of the tile are relative to one number.  With STORE they
+// are staged through the ring as 16-bit values: tokens 64 q .. 64 q + 63 in stage q.
+template <typename E, class S, bool STORE>
+__device__ __forceinline__ void stats_tile(const StatsArgs& p, bf16* s0, bf16* s1, bf16* s2, bf16* s3, float* xm,
+                                           float* xs) {
+  constexpr int MI = S::MI, NI = S::NI, PASSES = kPasses<S>;
   int vt, tt;
   grouped_tile(xcd_logical(blockIdx.x, p.n_ttiles * p.n_vtiles), p.n_vtiles, p.n_ttiles, vt, tt);
   const int v0 = vt * TM, n0 = tt * S::BN;
@@ -144,8 +172,6 @@ __global__ __launch_bounds__(kGemmThreads, 1) void stats_kernel(StatsArgs p) {
                                 p.h + (int64_t)n0 * p.ldh, p.ldh, min(S::BN, p.rows - n0), p.dim, s0, s1, s2, s3);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave % S::WM, wn = wave / S::WM;
-  float* xm = reinterpret_cast<float*>(s0);  // [WM - 1][BN] per token, from the waves wm > 0
-  float* xs = xm + (S::WM - 1) * S::BN;
   // rows past the vocabulary (last vocabulary tile only) take no part
   if (v0 + TM > p.vocab) {
 #pragma unroll
@@ -159,34 +185,70 @@ __global__ __launch_bounds__(kGemmThreads, 1) void stats_kernel(StatsArgs p) {
   float mk[NI], sk[NI];
 #pragma unroll
   for (int ni = 0; ni < NI; ++ni) {
-    const int col = b_row<S>(ni, lane, wn);
     float m = neg_inf();
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) m = fmaxf(m, fmaxf(acc[mi][ni][i], acc[mi][ni][i + 1]));
-    float sum = 0.f;
-    if (m == neg_inf()) {  // nothing, or nothing but -inf and NaN, which a maximum does not show
+    mk[ni] = fmaxf(m, shfl_xor(m, 32));  // lane ^ 32 holds the column's other rows
+    if (lane < 32) xm[wm * S::BN + b_row<S>(ni, lane, wn)] = mk[ni];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+    for (int w = 0; w < S::WM; ++w) mk[ni] = fmaxf(mk[ni], xm[w * S::BN + b_row<S>(ni, lane, wn)]);
+  auto quarter = [&](int q) -> bf16* { return q == 0 ? s0 : q == 1 ? s1 : q == 2 ? s2 : s3; };
+  auto values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+      float sum = 0.f;
+      const float m2 = mk[ni] * p.unit;
+      // nothing, or nothing but -inf and NaN, which a maximum does not show
+      const bool none = mk[ni] == neg_inf();
+      const int col = b_row<S>(ni, lane, PASSES > 1 ? 0 : wn);  // token within the pass
+      bf16* out = quarter(col >> 6) + (col & 63) * OPITCH;
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (acc[mi][ni][i] != neg_inf()) sum = __builtin_nanf("");
-    } else {
-      const float m2 = m * p.unit;
+        for (int i4 = 0; i4 < 4; ++i4) {
+          float e[4];
 #pragma unroll
-      for (int mi = 0; mi < MI; ++mi)
+          for (int j = 0; j < 4; ++j) {
+            const float x = acc[mi][ni][4 * i4 + j];
+            e[j] = none ? (x == neg_inf() ? 0.f : __builtin_nanf("")) : fast_exp2(fmaf(x, p.unit, -m2));
+            sum += e[j];
+          }
+          if (STORE)
+            *reinterpret_cast<u32x2*>(out + a_row<S>(mi, 4 * i4, lane, wm)) =
+                u32x2{pack2<E>(e[0], e[1]), pack2<E>(e[2], e[3])};
+        }
+      sk[ni] = sum;
+      if (STORE && PASSES > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if constexpr (!STORE) {
+    values();
+  } else if constexpr (PASSES == 1) {
+    values();
+    __syncthreads();
+    store_staged<S>(quarter, p.exps, p.lde, n0, p.rows, v0, p.vocab_pad, 0);
+  } else {
+    static_assert(PASSES == 2, "two halves");
+    if (wn == 0) values();
+    __syncthreads();
+    store_staged<S>(quarter, p.exps, p.lde, n0, p.rows, v0, p.vocab_pad, 0);
+    __syncthreads();
+    if (wn == 1) values();
+    __syncthreads();
+    store_staged<S>(quarter, p.exps, p.lde, n0, p.rows, v0, p.vocab_pad, 1);
+  }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += fast_exp2(fmaf(acc[mi][ni][i], p.unit, -m2));
-    }
-    const float mo = shfl_xor(m, 32), so = shfl_xor(sum, 32);  // lane ^ 32 holds the other rows
-    merge(m, sum, mo, so, p.unit);
-    if (wm > 0 && lane < 32) {
-      xm[(wm - 1) * S::BN + col] = m;
-      xs[(wm - 1) * S::BN + col] = sum;
-    }
-    mk[ni] = m;
-    sk[ni] = sum;
+  for (int ni = 0; ni < NI; ++ni) {
+    const int col = b_row<S>(ni, lane, wn);
+    const float so = shfl_xor(sk[ni], 32);
+    sk[ni] += so;
+    if (wm > 0 && lane < 32) xs[(wm - 1) * S::BN + col] = sk[ni];
   }
   __syncthreads();
 #pragma unroll
@@ -194,63 +256,89 @@ __global__ __launch_bounds__(kGemmThreads, 1) void stats_kernel(StatsArgs p) {
     const int col = b_row<S>(ni, lane, wn), n = n0 + col;
     if (wm == 0 && lane < 32 && n < p.rows) {
 #pragma unroll
-      for (int w = 0; w < S::WM - 1; ++w) merge(mk[ni], sk[ni], xm[w * S::BN + col], xs[w * S::BN + col], p.unit);
+      for (int w = 0; w < S::WM - 1; ++w) sk[ni] += xs[w * S::BN + col];
       p.part_m[(int64_t)vt * p.rows + n] = mk[ni];
       p.part_s[(int64_t)vt * p.rows + n] = sk[ni];
     }
   }
 }
 
+template <typename E, class S>
+__global__ __launch_bounds__(kGemmThreads, 1) void stats_kernel(StatsArgs p) {
+  GEMM_RING_OF(S)
+  float* xm = reinterpret_cast<float*>(s0);
+  stats_tile<E, S, false>(p, s0, s1, s2, s3, xm, xm + S::WM * S::BN);
+}
+
+template <typename E, class S>
+__global__ __launch_bounds__(kGemmThreads, 1) void stats_store_kernel(StatsArgs p) {
+  GEMM_RING_OF(S)
+  __shared__ float xm[S::WM * S::BN], xs[S::WM * S::BN];  // the ring holds the staged values meanwhile
+  stats_tile<E, S, true>(p, s0, s1, s2, s3, xm, xs);
+}
+
 // ---------------------------------------------------------------------------
 // the logits at the slots: z[n, k] = h[n] . W[slot_id[n, k]], a wave per slot
 // ---------------------------------------------------------------------------
-template <typename T, typename C>
-__global__ __launch_bounds__(256) void scores_kernel(const T* __restrict__ h, int64_t ldh, const T* __restrict__ w,
-                                                     int64_t ldw, const int32_t* __restrict__ slot_id, int pitch,
-                                                     int top, int dim, C* __restrict__ z) {
+template <typename E>
+__global__ __launch_bounds__(256) void scores_kernel(const bf16* __restrict__ h, int64_t ldh,
+                                                     const bf16* __restrict__ w, int64_t ldw,
+                                                     const int32_t* __restrict__ slot_id, int pitch, int top, int dim,
+                                                     float* __restrict__ z) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n = blockIdx.x;
-  const T* hr = h + n * ldh;
+  const E* hr = reinterpret_cast<const E*>(h + n * ldh);
   for (int k = 4 * blockIdx.y + wave; k < top; k += 4 * gridDim.y) {
     const int id = slot_id[n * pitch + k];
     if (id < 0) continue;
-    const T* wr = w + (int64_t)id * ldw;
-    C acc = (C)0;
-    if constexpr (sizeof(T) == 2) {
-      for (int d = 8 * lane; d < dim; d += 512) {
-        float a[8], b[8];
-        load8(hr + d, a);
-        load8(wr + d, b);
+    const E* wr = reinterpret_cast<const E*>(w + (int64_t)id * ldw);
+    float acc = 0.f;
+    for (int d = 8 * lane; d < dim; d += 512) {
+      float a[8], b[8];
+      load8(hr + d, a);
+      load8(wr + d, b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc = fmaf(a[i], b[i], acc);
-      }
-    } else {
-      for (int d = lane; d < dim; d += 64) acc = fma(hr[d], wr[d], acc);
+      for (int i = 0; i < 8; ++i) acc = fmaf(a[i], b[i], acc);
     }
-    acc = wave_sum_of(acc);
+    acc = wave_sum(acc);
     if (lane == 0) z[n * pitch + k] = acc;
   }
 }
 
+// sum_k p_k (log p_k - (z_k / T - lse)) over a wave's slots of one row
+template <typename C>
+__device__ __forceinline__ C slots_loss(const int32_t* slot_id, const C* slot_p, const C* slot_z, int top, C inv_t,
+                                        C lse, int lane, int lanes) {
+  C sum = (C)0;
+  for (int k = lane; k < top; k += lanes) {
+    if (slot_id[k] < 0) continue;
+    const C p = slot_p[k];
+    if (p == (C)0) continue;
+    sum += p * (log(p) - (slot_z[k] * inv_t - lse));
+  }
+  return sum;
+}
+template <typename C> __device__ __forceinline__ C row_loss(int state, C sum) {
+  return state == kDead ? (C)0 : state == kBadId ? (C)__builtin_nan("") : sum;
+}
+
 // ---------------------------------------------------------------------------
-// loss[n] = sum_k p_k (log p_k - (z_k / T - lse)); lse of z / T.  With TILES the row's lse
-// is first merged from the tiles' statistics.  A work-group of 16 waves owns 16 tokens:
-// its 64 slots of 16 lanes merge the tiles t = slot, slot + 64, ..., then wave w sums
-// token w's slots.
+// lse of z / T from the tiles' statistics, and the loss.  A work-group of 16 waves owns 16
+// tokens: its 64 slots of 16 lanes merge the tiles t = slot, slot + 64, ..., then wave w
+// sums token w's teacher slots.
 // ---------------------------------------------------------------------------
 constexpr int kLossTokens = 16;
-template <typename C, bool TILES>
 __global__ __launch_bounds__(64 * kLossTokens) void loss_kernel(const float* __restrict__ pm,
                                                                 const float* __restrict__ ps, int n_vtiles, int rows,
                                                                 float unit, const int32_t* __restrict__ slot_id,
-                                                                const C* __restrict__ slot_p,
-                                                                const C* __restrict__ slot_z, int pitch, int top,
-                                                                const int32_t* __restrict__ state, C inv_t,
-                                                                C* __restrict__ lse, C* __restrict__ loss) {
+                                                                const float* __restrict__ slot_p,
+                                                                const float* __restrict__ slot_z, int pitch, int top,
+                                                                const int32_t* __restrict__ state, float inv_t,
+                                                                float* __restrict__ lse, float* __restrict__ loss) {
   __shared__ float sm[kLossTokens][kLossTokens], ss[kLossTokens][kLossTokens];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n0 = blockIdx.x * kLossTokens;
-  if constexpr (TILES) {
+  {
     const int tok = lane & 15, slot = 4 * wave + (lane >> 4), n = n0 + tok;
     float M = neg_inf(), S = 0.f;
     if (n < rows) {
@@ -273,26 +361,105 @@ __global__ __launch_bounds__(64 * kLossTokens) void loss_kernel(const float* __r
   }
   const int n = n0 + wave;
   if (n >= rows) return;
-  C l;
-  if constexpr (TILES) {
-    float M = sm[0][wave], S = ss[0][wave];
+  float M = sm[0][wave], S = ss[0][wave];
 #pragma unroll
-    for (int v = 1; v < kLossTokens; ++v) merge(M, S, sm[v][wave], ss[v][wave], unit);
-    l = (C)(M * inv_t + logf(S));
-    if (lane == 0) lse[n] = l;
+  for (int v = 1; v < kLossTokens; ++v) merge(M, S, sm[v][wave], ss[v][wave], unit);
+  const float l = M * inv_t + logf(S);
+  const int64_t o = (int64_t)n * pitch;
+  const float sum = wave_sum(slots_loss(slot_id + o, slot_p + o, slot_z + o, top, inv_t, l, lane, 64));
+  if (lane == 0) {
+    lse[n] = l;
+    loss[n] = row_loss(state[n], sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dlogits = grad / T (q - p) (grad null: q - p, without the 1 / T) from what the forward
+// stored: a work-group takes kFinish columns of one row.  E: exponentials relative to their
+// 256-column tile's maximum (FROM_EXPS), scaled once per tile; C: logits.  Bound by the
+// block's bytes, read and written once.
+// ---------------------------------------------------------------------------
+constexpr int kFinish = 2048;  // 256 threads of 8 columns
+template <typename T, typename C, bool FROM_EXPS>
+__global__ __launch_bounds__(256) void finish_kernel(const T* src, int64_t lds, const float* __restrict__ tile_max,
+                                                     int tile_rows, const C* __restrict__ lse,
+                                                     const C* __restrict__ grad, const int32_t* __restrict__ state,
+                                                     const int32_t* __restrict__ slot_id, const C* __restrict__ slot_p,
+                                                     const C* __restrict__ slot_z, int pitch, int top, int columns,
+                                                     C inv_t, T* dst, int64_t ldd) {
+  const int64_t n = blockIdx.x;
+  const int c0 = blockIdx.y * kFinish, c = c0 + 8 * threadIdx.x;
+  const bool dead = state[n] == kDead;
+  const C l = lse[n], coef = grad ? grad[n] * inv_t : (C)1;
+  if constexpr (FROM_EXPS) {
+    if (c < columns) {  // a multiple of 8
+      float x[8];
+      load8(src + n * lds + c, x);
+      const float f = fast_exp2((tile_max[(int64_t)(c / TM) * tile_rows + n] * inv_t - l) * kLog2e) * coef;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = dead ? 0.f : x[i] * f;
+      store8(dst + n * ldd + c, x);
+    }
   } else {
-    l = lse[n];
+    for (int i = threadIdx.x; i < kFinish; i += 256) {
+      if (c0 + i >= columns) break;
+      const C q = exp(src[n * lds + c0 + i] * inv_t - l);
+      dst[n * ldd + c0 + i] = dead ? (C)0 : q * coef;
+    }
   }
-  C sum = (C)0;
-  for (int k = lane; k < top; k += 64) {
-    const int64_t o = (int64_t)n * pitch + k;
-    if (slot_id[o] < 0) continue;
-    const C p = slot_p[o];
-    if (p == (C)0) continue;
-    sum += p * (log(p) - (slot_z[o] * inv_t - l));
+  if (dead) return;
+  __syncthreads();  // the slots' entries after the others', rounded once from their own logits
+  for (int k = threadIdx.x; k < top; k += 256) {
+    const int64_t o = n * pitch + k;
+    const int id = slot_id[o];
+    if (id < c0 || id >= c0 + kFinish) continue;
+    const C d = (exp(slot_z[o] * inv_t - l) - slot_p[o]) * coef;
+    if constexpr (std::is_same_v<T, C>) dst[n * ldd + id] = d;
+    else dst[n * ldd + id] = from_f<T>((float)d);
   }
-  sum = wave_sum_of(sum);
-  if (lane == 0) loss[n] = state[n] == kDead ? (C)0 : state[n] == kBadId ? (C)__builtin_nan("") : sum;
+}
+
+// ---------------------------------------------------------------------------
+// fp32 / fp64: lse, the slots' logits and the loss from a row of logits
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 512;
+template <typename C>
+__global__ __launch_bounds__(kRowThreads) void row_stats_kernel(const C* __restrict__ z, int64_t ldz, int vocab,
+                                                                C inv_t, const int32_t* __restrict__ slot_id,
+                                                                const C* __restrict__ slot_p, C* __restrict__ slot_z,
+                                                                int pitch, int top, const int32_t* __restrict__ state,
+                                                                C* __restrict__ lse, C* __restrict__ loss) {
+  __shared__ C sm[kRowThreads / 64], ss[kRowThreads / 64];
+  const int64_t n = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const C* row = z + n * ldz;
+  // the maximum (a NaN of the row shows in the sum)
+  C m = -(C)__builtin_huge_val();
+  for (int v = threadIdx.x; v < vocab; v += kRowThreads) m = fmax(m, row[v]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) m = fmax(m, __shfl_xor(m, o, kWave));
+  if (lane == 0) sm[wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 64; ++w) m = fmax(m, sm[w]);
+  C s = (C)0;
+  for (int v = threadIdx.x; v < vocab; v += kRowThreads) s += exp((row[v] - m) * inv_t);
+  s = wave_sum_of(s);
+  if (lane == 0) ss[wave] = s;
+  __syncthreads();
+  s = ss[0];
+#pragma unroll
+  for (int w = 1; w < kRowThreads / 64; ++w) s += ss[w];
+  const C l = m * inv_t + log(s);
+  if (wave != 0) return;
+  const int64_t o = n * pitch;
+  for (int k = lane; k < top; k += 64)
+    if (slot_id[o + k] >= 0) slot_z[o + k] = row[slot_id[o + k]];
+  const C sum = wave_sum_of(slots_loss(slot_id + o, slot_p + o, slot_z + o, top, inv_t, l, lane, 64));
+  if (lane == 0) {
+    lse[n] = l;
+    loss[n] = row_loss(state[n], sum);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -325,10 +492,7 @@ __global__ __launch_bounds__(kGemmThreads, 1) void dlogits_kernel(DlArgs p) {
                                 p.h + (int64_t)n0 * p.ldh, p.ldh, min(S::BN, p.rows - n0), p.dim, s0, s1, s2, s3);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave % S::WM, wn = wave / S::WM;
-  // tokens 64 q .. 64 q + 63 of the tile are staged in ring stage q as [64][OPITCH];
-  // a Wide tile does not fit, its waves' two halves of the tokens take turns
-  constexpr int PASSES = S::BN > TN ? S::WN : 1, PT = S::BN / PASSES;  // tokens per pass
-  static_assert(PT <= 256, "four stages of 64 tokens");
+  constexpr int PASSES = kPasses<S>;
   auto quarter = [&](int q) -> bf16* { return q == 0 ? s0 : q == 1 ? s1 : q == 2 ? s2 : s3; };
   auto values = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -356,24 +520,15 @@ __global__ __launch_bounds__(kGemmThreads, 1) void dlogits_kernel(DlArgs p) {
       if constexpr (PASSES > 1) __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const int vmax = min(TM, p.vocab_pad - v0);
   auto store = [&](int pass) __attribute__((always_inline)) {
-#pragma unroll 4
-    for (int it = 0; it < (PT * TM / 8) / kGemmThreads; ++it) {
-      const int c = it * kGemmThreads + tid;
-      const int row = c / (TM / 8), chunk = (c % (TM / 8)) * 8;
-      const int n = n0 + pass * PT + row;
-      if (n < p.rows && chunk < vmax)
-        *reinterpret_cast<u32x4*>(p.dl + (int64_t)n * p.ldl + v0 + chunk) =
-            *reinterpret_cast<const u32x4*>(quarter(row >> 6) + (row & 63) * OPITCH + chunk);
-    }
+    store_staged<S>(quarter, p.dl, p.ldl, n0, p.rows, v0, p.vocab_pad, pass);
   };
   if constexpr (PASSES == 1) {
     values();
     __syncthreads();
     store(0);
   } else {
-    static_assert(PASSES <= 2, "two halves");
+    static_assert(PASSES == 2, "two halves");
     if (wn == 0) values();
     __syncthreads();
     store(0);
@@ -384,35 +539,42 @@ __global__ __launch_bounds__(kGemmThreads, 1) void dlogits_kernel(DlArgs p) {
   }
 }
 
-// dl[n, slot_id] = grad_scale g (q - p) with q = exp(logit_scale z - lse), rounded once: the
-// slots' entries in full
-template <typename T, typename C>
-__global__ __launch_bounds__(256) void slots_kernel(const int32_t* __restrict__ slot_id, const C* __restrict__ slot_p,
-                                                    const C* __restrict__ slot_z, int pitch, int top, int64_t rows,
-                                                    const C* __restrict__ lse, const C* __restrict__ g, C logit_scale,
-                                                    C grad_scale, T* __restrict__ dl, int64_t ldl) {
+// dl[n, slot_id] = grad / T (q - p) with q = exp(z / T - lse), rounded once
+template <typename E>
+__global__ __launch_bounds__(256) void slots_kernel(const int32_t* __restrict__ slot_id,
+                                                    const float* __restrict__ slot_p,
+                                                    const float* __restrict__ slot_z, int pitch, int top, int64_t rows,
+                                                    const float* __restrict__ lse, const float* __restrict__ g,
+                                                    float inv_t, E* __restrict__ dl, int64_t ldl) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t n = i / pitch;
   const int k = (int)(i - n * pitch);
   if (n >= rows || k >= top) return;
   const int id = slot_id[i];
-  if (id < 0) return;
-  const C d = (exp(slot_z[i] * logit_scale - lse[n]) - slot_p[i]) * (g[n] * grad_scale);
-  if constexpr (std::is_same_v<T, C>) dl[n * ldl + id] = d;
-  else dl[n * ldl + id] = from_f<T>((float)d);
+  if (id >= 0) dl[n * ldl + id] = from_f<E>((expf(slot_z[i] * inv_t - lse[n]) - slot_p[i]) * (g[n] * inv_t));
 }
 
-// out[n] = live row ? scale h[n] : 0
-template <typename T, typename C>
+// out[n] = h[n], zeros where the row has no teacher
+template <typename T>
 __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ h, int64_t ldh,
-                                                   const int32_t* __restrict__ state, int64_t rows, int dim, C scale,
-                                                   T* __restrict__ out, int64_t ldo) {
+                                                   const int32_t* __restrict__ state, int dim, T* __restrict__ out) {
   const int64_t n = blockIdx.x;
   const bool dead = state[n] == kDead;
+  for (int d = threadIdx.x; d < dim; d += 256) out[n * dim + d] = dead ? (T)0.f : h[n * ldh + d];
+}
+
+// out[n] = grad[n] / T unit[n], zeros where the row has no teacher, rounded once
+template <typename T, typename C>
+__global__ __launch_bounds__(256) void scale_kernel(const C* __restrict__ unit, const C* __restrict__ grad,
+                                                    const int32_t* __restrict__ state, int dim, C inv_t,
+                                                    T* __restrict__ out) {
+  const int64_t n = blockIdx.x;
+  const bool dead = state[n] == kDead;
+  const C f = grad[n] * inv_t;
   for (int d = threadIdx.x; d < dim; d += 256) {
-    const T x = h[n * ldh + d];
-    if constexpr (std::is_same_v<T, C>) out[n * ldo + d] = dead ? (T)0 : x * scale;
-    else out[n * ldo + d] = dead ? from_f<T>(0.f) : scale == (C)1 ? x : from_f<T>(to_f(x) * scale);
+    const C x = dead ? (C)0 : unit[n * dim + d] * f;
+    if constexpr (std::is_same_v<T, C>) out[n * dim + d] = x;
+    else out[n * dim + d] = from_f<T>((float)x);
   }
 }
 
@@ -472,38 +634,10 @@ int64_t ts_distill_fwd_workspace(int64_t rows, int64_t vocab) {
   return 2 * ((vocab + TM - 1) / TM) * rows * (int64_t)sizeof(float);
 }
 
-int ts_distill_scores(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight,
-                      const int32_t* slot_id, int64_t pitch, int64_t rows, int64_t top, int64_t dim, void* slot_z,
-                      int dtype, void* stream) {
-  TS_CHECK_ARG(known(dtype), "ts_distill_scores: dtype %d", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && top > 0 && top <= pitch && pitch <= kMaxTop && dim > 0 &&
-                   dim < (1 << 20) && ld_hidden >= dim && ld_weight >= dim,
-               "ts_distill_scores: bad shape");
-  if (rows == 0) return TS_OK;
-  TS_CHECK_ARG(hidden && weight && slot_id && slot_z, "ts_distill_scores: null pointer");
-  TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F64 ||
-                   (ok16(hidden) && ok16(weight) && dim % 8 == 0 && ld_hidden % 8 == 0 && ld_weight % 8 == 0),
-               "ts_distill_scores: hidden/weight rows must be 16-byte aligned with dim %% 8 == 0");
-  hipStream_t s = (hipStream_t)stream;
-  {
-    ts::TimedLaunch timed_("distill.scores_kernel", s);
-    const dim3 grid((unsigned)rows, (unsigned)std::min<int64_t>((top + 3) / 4, 8));
-#define TS_SCORES(T, C)                                                                                          \
-  hipLaunchKernelGGL((scores_kernel<T, C>), grid, dim3(256), 0, s, (const T*)hidden, ld_hidden, (const T*)weight, \
-                     ld_weight, slot_id, (int)pitch, (int)top, (int)dim, (C*)slot_z)
-    if (dtype == TS_BF16) TS_SCORES(ts::bf16, float);
-    else if (dtype == TS_F16) TS_SCORES(ts::f16, float);
-    else if (dtype == TS_F32) TS_SCORES(float, float);
-    else TS_SCORES(double, double);
-#undef TS_SCORES
-  }
-  return ts::check_launch("ts_distill_scores");
-}
-
 int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
                    int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
                    float* slot_z, int64_t pitch, int64_t top, const int32_t* state, float* loss, float* lse,
-                   void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+                   void* exps, int64_t ld_exps, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
   TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_fwd: dtype %d (bf16 or fp16)", dtype);
   TS_CHECK_ARG(rows >= 0 && dim > 0 && vocab > 0 && rows < (1 << 30) && vocab < (1 << 30) && dim < (1 << 20) &&
                    top > 0 && top <= pitch && pitch <= kMaxTop,
@@ -520,6 +654,8 @@ int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, in
   TS_CHECK_ARG(workspace && workspace_bytes >= ts_distill_fwd_workspace(rows, vocab),
                "ts_distill_fwd: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
                (long long)ts_distill_fwd_workspace(rows, vocab));
+  TS_CHECK_ARG(!exps || (ok16(exps) && ld_exps % 8 == 0 && ld_exps >= (vocab + 7) / 8 * 8),
+               "ts_distill_fwd: exps' alignment or leading dimension");
   StatsArgs a;
   a.h = (const ts::bf16*)hidden;
   a.ldh = ld_hidden;
@@ -534,51 +670,93 @@ int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, in
   a.unit = (float)(1.4426950408889634 / temperature);
   a.part_m = (float*)workspace;
   a.part_s = a.part_m + (int64_t)a.n_vtiles * rows;
+  a.exps = (ts::bf16*)exps;
+  a.lde = ld_exps;
+  a.vocab_pad = (int)((vocab + 7) / 8 * 8);
   TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < (1ll << 31), "ts_distill_fwd: grid too large");
   hipStream_t s = (hipStream_t)stream;
   {
     ts::TimedLaunch timed_("distill.stats_kernel", s);
-    TS_LAUNCH_TOKENS(dtype, width, stats_kernel, dim3((unsigned)(a.n_ttiles * a.n_vtiles)), dim3(kGemmThreads), 0, s, a);
+    const dim3 grid((unsigned)(a.n_ttiles * a.n_vtiles));
+    if (exps) TS_LAUNCH_TOKENS(dtype, width, stats_store_kernel, grid, dim3(kGemmThreads), 0, s, a);
+    else TS_LAUNCH_TOKENS(dtype, width, stats_kernel, grid, dim3(kGemmThreads), 0, s, a);
   }
   int st = ts::check_launch("ts_distill_fwd (tiles)");
   if (st != TS_OK) return st;
-  st = ts_distill_scores(hidden, ld_hidden, weight, ld_weight, slot_id, pitch, rows, top, dim, slot_z, dtype, stream);
-  if (st != TS_OK) return st;
+  {
+    ts::TimedLaunch timed_("distill.scores_kernel", s);
+    TS_LAUNCH_E(dtype, scores_kernel, dim3((unsigned)rows, (unsigned)std::min<int64_t>((top + 3) / 4, 8)), dim3(256), 0,
+                s, a.h, ld_hidden, a.w, ld_weight, slot_id, (int)pitch, (int)top, (int)dim, slot_z);
+  }
   {
     ts::TimedLaunch timed_("distill.loss_kernel", s);
-    hipLaunchKernelGGL((loss_kernel<float, true>), dim3((unsigned)((rows + kLossTokens - 1) / kLossTokens)),
-                       dim3(64 * kLossTokens), 0, s, a.part_m, a.part_s, a.n_vtiles, (int)rows, a.unit, slot_id, slot_p,
-                       slot_z, (int)pitch, (int)top, state, (float)(1. / temperature), lse, loss);
+    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)((rows + kLossTokens - 1) / kLossTokens)), dim3(64 * kLossTokens),
+                       0, s, a.part_m, a.part_s, a.n_vtiles, (int)rows, a.unit, slot_id, slot_p, slot_z, (int)pitch,
+                       (int)top, state, (float)(1. / temperature), lse, loss);
   }
   return ts::check_launch("ts_distill_fwd (loss)");
 }
 
-int ts_distill_loss(const int32_t* slot_id, const void* slot_p, const void* slot_z, int64_t pitch, int64_t top,
-                    const int32_t* state, const void* lse, int64_t rows, void* loss, int dtype, void* stream) {
-  TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F64, "ts_distill_loss: dtype %d (fp32 or fp64)", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && top > 0 && top <= pitch && pitch <= kMaxTop,
-               "ts_distill_loss: bad shape");
+int ts_distill_fwd_exact(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, double temperature,
+                         const int32_t* slot_id, const void* slot_p, void* slot_z, int64_t pitch, int64_t top,
+                         const int32_t* state, void* loss, void* lse, int dtype, void* stream) {
+  TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F64, "ts_distill_fwd_exact: dtype %d (fp32 or fp64)", dtype);
+  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && vocab > 0 && vocab < (1 << 30) && ld_logits >= vocab && top > 0 &&
+                   top <= pitch && pitch <= kMaxTop,
+               "ts_distill_fwd_exact: bad shape");
+  TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_fwd_exact: temperature %g",
+               temperature);
   if (rows == 0) return TS_OK;
-  TS_CHECK_ARG(slot_id && slot_p && slot_z && state && lse && loss, "ts_distill_loss: null pointer");
+  TS_CHECK_ARG(logits && slot_id && slot_p && slot_z && state && loss && lse, "ts_distill_fwd_exact: null pointer");
   hipStream_t s = (hipStream_t)stream;
   {
-    ts::TimedLaunch timed_("distill.loss_kernel", s);
-    const dim3 grid((unsigned)((rows + kLossTokens - 1) / kLossTokens)), block(64 * kLossTokens);
+    ts::TimedLaunch timed_("distill.row_stats_kernel", s);
+    const dim3 grid((unsigned)rows), block(kRowThreads);
     if (dtype == TS_F64)
-      hipLaunchKernelGGL((loss_kernel<double, false>), grid, block, 0, s, (const float*)nullptr, (const float*)nullptr,
-                         0, (int)rows, 0.f, slot_id, (const double*)slot_p, (const double*)slot_z, (int)pitch, (int)top,
-                         state, 1., (double*)lse, (double*)loss);
+      hipLaunchKernelGGL(row_stats_kernel<double>, grid, block, 0, s, (const double*)logits, ld_logits, (int)vocab,
+                         1. / temperature, slot_id, (const double*)slot_p, (double*)slot_z, (int)pitch, (int)top, state,
+                         (double*)lse, (double*)loss);
     else
-      hipLaunchKernelGGL((loss_kernel<float, false>), grid, block, 0, s, (const float*)nullptr, (const float*)nullptr,
-                         0, (int)rows, 0.f, slot_id, (const float*)slot_p, (const float*)slot_z, (int)pitch, (int)top,
-                         state, 1.f, (float*)lse, (float*)loss);
+      hipLaunchKernelGGL(row_stats_kernel<float>, grid, block, 0, s, (const float*)logits, ld_logits, (int)vocab,
+                         (float)(1. / temperature), slot_id, (const float*)slot_p, (float*)slot_z, (int)pitch, (int)top,
+                         state, (float*)lse, (float*)loss);
   }
-  return ts::check_launch("ts_distill_loss");
+  return ts::check_launch("ts_distill_fwd_exact");
 }
 
-int ts_distill_slots(const int32_t* slot_id, const void* slot_p, const void* slot_z, int64_t pitch, int64_t top,
-                     const void* lse, const void* grad, int64_t rows, double logit_scale, double grad_scale,
-                     void* dlogits, int64_t ld_dlogits, int dtype, void* stream);
+int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_max, int64_t rows, int64_t vocab,
+                      double temperature, const int32_t* slot_id, const void* slot_p, const void* slot_z,
+                      int64_t pitch, int64_t top, const int32_t* state, const void* lse, const void* grad,
+                      void* dlogits, int64_t ld_dlogits, int dtype, void* stream) {
+  TS_CHECK_ARG(known(dtype), "ts_distill_finish: dtype %d", dtype);
+  const bool exact = dtype == TS_F32 || dtype == TS_F64;
+  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && vocab > 0 && vocab < 65535ll * kFinish && top > 0 && top <= pitch &&
+                   pitch <= kMaxTop && ld_stored >= vocab && ld_dlogits >= vocab,
+               "ts_distill_finish: bad shape");
+  TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_finish: temperature %g", temperature);
+  if (rows == 0) return TS_OK;
+  TS_CHECK_ARG(stored && dlogits && slot_id && slot_p && slot_z && state && lse && (exact || tile_max),
+               "ts_distill_finish: null pointer");
+  const int64_t columns = exact ? vocab : (vocab + 7) / 8 * 8;
+  TS_CHECK_ARG(exact || (ok16(stored) && ok16(dlogits) && ld_stored % 8 == 0 && ld_dlogits % 8 == 0 &&
+                         ld_stored >= columns && ld_dlogits >= columns),
+               "ts_distill_finish: alignment or leading dimensions");
+  hipStream_t s = (hipStream_t)stream;
+  {
+    ts::TimedLaunch timed_("distill.finish_kernel", s);
+    const dim3 grid((unsigned)rows, (unsigned)((columns + kFinish - 1) / kFinish));
+#define TS_FINISH(T, C, EXPS)                                                                                        \
+  hipLaunchKernelGGL((finish_kernel<T, C, EXPS>), grid, dim3(256), 0, s, (const T*)stored, ld_stored, tile_max,       \
+                     (int)rows, (const C*)lse, (const C*)grad, state, slot_id, (const C*)slot_p, (const C*)slot_z,    \
+                     (int)pitch, (int)top, (int)columns, (C)(1. / temperature), (T*)dlogits, ld_dlogits)
+    if (dtype == TS_BF16) TS_FINISH(ts::bf16, float, true);
+    else if (dtype == TS_F16) TS_FINISH(ts::f16, float, true);
+    else if (dtype == TS_F32) TS_FINISH(float, float, false);
+    else TS_FINISH(double, double, false);
+#undef TS_FINISH
+  }
+  return ts::check_launch("ts_distill_finish");
+}
 
 int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
                        int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
@@ -626,55 +804,62 @@ int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight
   }
   const int st = ts::check_launch("ts_distill_dlogits");
   if (st != TS_OK) return st;
-  return ts_distill_slots(slot_id, slot_p, slot_z, pitch, top, lse, grad, rows, 1. / temperature, 1. / temperature,
-                          dlogits, ld_dlogits, dtype, stream);
-}
-
-int ts_distill_slots(const int32_t* slot_id, const void* slot_p, const void* slot_z, int64_t pitch, int64_t top,
-                     const void* lse, const void* grad, int64_t rows, double logit_scale, double grad_scale,
-                     void* dlogits, int64_t ld_dlogits, int dtype, void* stream) {
-  TS_CHECK_ARG(known(dtype), "ts_distill_slots: dtype %d", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && top > 0 && top <= pitch && pitch <= kMaxTop && ld_dlogits > 0,
-               "ts_distill_slots: bad shape");
-  if (rows == 0) return TS_OK;
-  TS_CHECK_ARG(slot_id && slot_p && slot_z && lse && grad && dlogits, "ts_distill_slots: null pointer");
-  hipStream_t s = (hipStream_t)stream;
   {
     ts::TimedLaunch timed_("distill.slots_kernel", s);
     const dim3 grid((unsigned)((rows * pitch + 255) / 256));
-#define TS_SLOTS(T, C)                                                                                              \
-  hipLaunchKernelGGL((slots_kernel<T, C>), grid, dim3(256), 0, s, slot_id, (const C*)slot_p, (const C*)slot_z,       \
-                     (int)pitch, (int)top, rows, (const C*)lse, (const C*)grad, (C)logit_scale, (C)grad_scale,       \
-                     (T*)dlogits, ld_dlogits)
-    if (dtype == TS_BF16) TS_SLOTS(ts::bf16, float);
-    else if (dtype == TS_F16) TS_SLOTS(ts::f16, float);
-    else if (dtype == TS_F32) TS_SLOTS(float, float);
-    else TS_SLOTS(double, double);
-#undef TS_SLOTS
+    const float inv_t = (float)(1. / temperature);
+    if (dtype == TS_F16)
+      hipLaunchKernelGGL(slots_kernel<ts::f16>, grid, dim3(256), 0, s, slot_id, slot_p, slot_z, (int)pitch, (int)top,
+                         rows, lse, grad, inv_t, (ts::f16*)dlogits, ld_dlogits);
+    else
+      hipLaunchKernelGGL(slots_kernel<ts::bf16>, grid, dim3(256), 0, s, slot_id, slot_p, slot_z, (int)pitch, (int)top,
+                         rows, lse, grad, inv_t, (ts::bf16*)dlogits, ld_dlogits);
   }
-  return ts::check_launch("ts_distill_slots");
+  return ts::check_launch("ts_distill_dlogits (slots)");
 }
 
-int ts_distill_rows(const void* hidden, int64_t ld_hidden, const int32_t* state, int64_t rows, int64_t dim,
-                    double scale, void* out, int64_t ld_out, int dtype, void* stream) {
+int ts_distill_rows(const void* hidden, int64_t ld_hidden, const int32_t* state, int64_t rows, int64_t dim, void* out,
+                    int dtype, void* stream) {
   TS_CHECK_ARG(known(dtype), "ts_distill_rows: dtype %d", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && dim > 0 && dim < (1 << 20) && ld_hidden >= dim && ld_out >= dim,
+  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && dim > 0 && dim < (1 << 20) && ld_hidden >= dim,
                "ts_distill_rows: bad shape");
   if (rows == 0) return TS_OK;
   TS_CHECK_ARG(hidden && state && out && hidden != out, "ts_distill_rows: null or aliased pointer");
   hipStream_t s = (hipStream_t)stream;
   {
     ts::TimedLaunch timed_("distill.rows_kernel", s);
-#define TS_ROWS(T, C)                                                                                             \
-  hipLaunchKernelGGL((rows_kernel<T, C>), dim3((unsigned)rows), dim3(256), 0, s, (const T*)hidden, ld_hidden, state, \
-                     rows, (int)dim, (C)scale, (T*)out, ld_out)
-    if (dtype == TS_BF16) TS_ROWS(ts::bf16, float);
-    else if (dtype == TS_F16) TS_ROWS(ts::f16, float);
-    else if (dtype == TS_F32) TS_ROWS(float, float);
-    else TS_ROWS(double, double);
+#define TS_ROWS(T)                                                                                                   \
+  hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, (const T*)hidden, ld_hidden, state,       \
+                     (int)dim, (T*)out)
+    if (dtype == TS_BF16) TS_ROWS(ts::bf16);
+    else if (dtype == TS_F16) TS_ROWS(ts::f16);
+    else if (dtype == TS_F32) TS_ROWS(float);
+    else TS_ROWS(double);
 #undef TS_ROWS
   }
   return ts::check_launch("ts_distill_rows");
+}
+
+int ts_distill_scale(const void* unit, const void* grad, const int32_t* state, int64_t rows, int64_t dim,
+                     double temperature, void* out, int dtype, void* stream) {
+  TS_CHECK_ARG(known(dtype), "ts_distill_scale: dtype %d", dtype);
+  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && dim > 0 && dim < (1 << 20), "ts_distill_scale: bad shape");
+  TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_scale: temperature %g", temperature);
+  if (rows == 0) return TS_OK;
+  TS_CHECK_ARG(unit && grad && state && out, "ts_distill_scale: null pointer");
+  hipStream_t s = (hipStream_t)stream;
+  {
+    ts::TimedLaunch timed_("distill.scale_kernel", s);
+#define TS_SCALE(T, C)                                                                                               \
+  hipLaunchKernelGGL((scale_kernel<T, C>), dim3((unsigned)rows), dim3(256), 0, s, (const C*)unit, (const C*)grad,     \
+                     state, (int)dim, (C)(1. / temperature), (T*)out)
+    if (dtype == TS_BF16) TS_SCALE(ts::bf16, float);
+    else if (dtype == TS_F16) TS_SCALE(ts::f16, float);
+    else if (dtype == TS_F32) TS_SCALE(float, float);
+    else TS_SCALE(double, double);
+#undef TS_SCALE
+  }
+  return ts::check_launch("ts_distill_scale");
 }
 
 }  // extern "C"

@@ -386,7 +386,7 @@ struct DhArgs {
   int n_ttiles, n_dtiles, ksplit, kper;  // kper: vocabulary per range (multiple of TK)
   bf16* dh;
   int64_t ldd;
-  float* part;      // [ksplit][rows][dim] when ksplit > 1
+  float* part;      // [ksplit][rows][dim] when ksplit > 1, or fp32 results; else null
 };
 
 template <typename E, class S>
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kGemmThreads, 1) void grad_hidden_kernel(DhArgs p) 
         const int d = d0 + a_row<S>(mi, 4 * i4, lane, wm);
         const float a[4] = {acc[mi][ni][4 * i4], acc[mi][ni][4 * i4 + 1], acc[mi][ni][4 * i4 + 2],
                             acc[mi][ni][4 * i4 + 3]};
-        if (p.ksplit > 1) {
+        if (p.part) {
           float* q = p.part + ((int64_t)ks * p.rows + n) * p.dim + d;
           if (d + 3 < p.dim) {
             *reinterpret_cast<f32x4*>(q) = f32x4{a[0], a[1], a[2], a[3]};
@@ -435,11 +435,11 @@ __global__ __launch_bounds__(kGemmThreads, 1) void grad_hidden_kernel(DhArgs p) 
   }
 }
 
-// dh = bf16(sum_s part[s]) in range order; four elements per thread
+// dh = bf16(sum_s part[s]) in range order, or dh32 = the sum; four elements per thread
 template <typename E>
 __global__ __launch_bounds__(kThreads) void grad_hidden_reduce_kernel(const float* __restrict__ part, int ksplit,
                                                                       int rows, int dim, bf16* __restrict__ dh,
-                                                                      int64_t ldd) {
+                                                                      int64_t ldd, float* __restrict__ dh32) {
   const int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
   const int64_t total = (int64_t)rows * dim;
   if (e >= total) return;
@@ -447,7 +447,8 @@ __global__ __launch_bounds__(kThreads) void grad_hidden_reduce_kernel(const floa
   const int d = (int)(e - n * dim);
   f32x4 s = *reinterpret_cast<const f32x4*>(part + e);
   for (int k = 1; k < ksplit; ++k) s += *reinterpret_cast<const f32x4*>(part + (int64_t)k * total + e);
-  *reinterpret_cast<u32x2*>(dh + n * ldd + d) = u32x2{pack2<E>(s[0], s[1]), pack2<E>(s[2], s[3])};
+  if (dh32) *reinterpret_cast<f32x4*>(dh32 + n * ldd + d) = s;
+  else *reinterpret_cast<u32x2*>(dh + n * ldd + d) = u32x2{pack2<E>(s[0], s[1]), pack2<E>(s[2], s[3])};
 }
 
 // ---------------------------------------------------------------------------
@@ -663,7 +664,7 @@ namespace ts {
 int grad_hidden_launch(const void* dlogits, int64_t ld_dlogits, const void* weight, int64_t ld_weight, int64_t rows,
                        int64_t dim, int64_t vocab, void* grad_hidden, int64_t ld_grad, void* workspace,
                        int64_t workspace_bytes, int dtype, void* stream, const char* label,
-                       const char* reduce_label) {
+                       const char* reduce_label, bool wide) {
   using namespace ts::lp;
   TS_CHECK_ARG(dtype == ts::kBF16 || dtype == ts::kF16, "ts_logprob_grad_hidden: dtype %d (bf16 or fp16)", dtype);
   TS_CHECK_ARG(rows >= 0 && dim > 0 && vocab > 0 && rows < (1 << 30) && dim < (1 << 20) && vocab < (1 << 30),
@@ -673,6 +674,7 @@ int grad_hidden_launch(const void* dlogits, int64_t ld_dlogits, const void* weig
                    ld_dlogits % 8 == 0 && ld_weight % 8 == 0 && ld_grad % 8 == 0 && dim % 8 == 0 &&
                    ld_dlogits >= (vocab + 7) / 8 * 8 && ld_weight >= dim && ld_grad >= dim,
                "ts_logprob_grad_hidden: alignment or leading dimensions");
+  TS_CHECK_ARG(!wide || ld_grad == dim, "ts_logprob_grad_hidden: fp32 results are dense");
   TS_CHECK_ARG(255 * ld_dlogits < (1ll << 30) && 31 * ld_weight < (1ll << 30),
                "ts_logprob_grad_hidden: leading dimensions too large for 32-bit tile offsets");
   DhArgs a;
@@ -688,7 +690,7 @@ int grad_hidden_launch(const void* dlogits, int64_t ld_dlogits, const void* weig
   a.n_ttiles = grad_hidden_split(rows, dim, vocab, ld_dlogits, width, a.ksplit, a.kper);
   a.dh = (ts::bf16*)grad_hidden;
   a.ldd = ld_grad;
-  a.part = (float*)workspace;
+  a.part = a.ksplit > 1 ? (float*)workspace : wide ? (float*)grad_hidden : nullptr;
   if (a.ksplit > 1)
     TS_CHECK_ARG(workspace && workspace_bytes >= ts_logprob_grad_hidden_workspace(rows, dim, vocab) &&
                      ok16(workspace),
@@ -707,7 +709,8 @@ int grad_hidden_launch(const void* dlogits, int64_t ld_dlogits, const void* weig
   {
     ts::TimedLaunch timed_(reduce_label, s);
     TS_LAUNCH_E(dtype, grad_hidden_reduce_kernel, dim3((unsigned)((quads + kThreads - 1) / kThreads)), dim3(kThreads),
-                       0, s, (const float*)workspace, a.ksplit, (int)rows, (int)dim, (ts::bf16*)grad_hidden, ld_grad);
+                       0, s, (const float*)workspace, a.ksplit, (int)rows, (int)dim, (ts::bf16*)grad_hidden, ld_grad,
+                       wide ? (float*)grad_hidden : nullptr);
   }
   return ts::check_launch("ts_logprob_grad_hidden (reduce)");
 }
@@ -722,6 +725,14 @@ int ts_logprob_grad_hidden(const void* dlogits, int64_t ld_dlogits, const void* 
   return ts::grad_hidden_launch(dlogits, ld_dlogits, weight, ld_weight, rows, dim, vocab, grad_hidden, ld_grad,
                                 workspace, workspace_bytes, dtype, stream, "logprob.grad_hidden_kernel",
                                 "logprob.grad_hidden_reduce_kernel");
+}
+
+int ts_logprob_grad_hidden_f32(const void* dlogits, int64_t ld_dlogits, const void* weight, int64_t ld_weight,
+                               int64_t rows, int64_t dim, int64_t vocab, float* grad_hidden, void* workspace,
+                               int64_t workspace_bytes, int dtype, void* stream) {
+  return ts::grad_hidden_launch(dlogits, ld_dlogits, weight, ld_weight, rows, dim, vocab, grad_hidden, dim, workspace,
+                                workspace_bytes, dtype, stream, "logprob.grad_hidden_kernel",
+                                "logprob.grad_hidden_reduce_kernel", true);
 }
 
 int ts_logprob_grad_weight_block(const void* dlogits, int64_t ld_dlogits, const void* hidden, int64_t ld_hidden,

@@ -19,14 +19,24 @@ A token id at or past the vocabulary makes the row's loss NaN (and takes no
 part in its gradient), as a target of the fused logprob does;
 ``THUNDERSYNC_CHECK_TARGETS=1`` checks the ids first and raises.
 
-Forward: ``ts_distill_teacher`` turns the slots into probabilities and
-``ts_distill_fwd`` takes the logits' log-sum-exp tile by tile on MFMA and the
-logits at the slots.  Backward, per block of rows as in the fused logprob:
-``ts_distill_dlogits`` recomputes the logits and writes
-``grad / temperature (q - p)`` in the element type; the products with the
-weight and the hidden states are the fused logprob's
-(:func:`~thundersync_amd.fused_logprob.head_vjp`).  In fp16 an entry of that
-block below 6e-8 is lost, so scale the loss as fp16 training does.
+A block of rows (:func:`~thundersync_amd.fused_logprob.backward_block_rows` of
+``chunk``) has its ``[rows, V]`` block in the element type once, and that
+bounds the memory.  The logits are formed once:
+
+* no gradient: the tiles' statistics alone, for all rows;
+* a frozen weight: the forward goes on, block by block, from the stored
+  exponentials to ``q - p`` and its product with the weight, ``[N, D]`` in
+  fp32, which the backward multiplies by the upstream gradient (no block
+  outlives the call, and 2 N V D flops of logits formed again are saved);
+* a trainable weight and one block of rows: the block is kept for the
+  backward, which needs the upstream gradient first;
+* a trainable weight and more rows: the backward forms the logits again, block
+  by block, as the fused logprob does.
+
+The products with the weight and the hidden states are the fused logprob's
+(:func:`~thundersync_amd.fused_logprob.head_vjp`).  In fp16 an entry of the
+block below 6e-8 is lost, so scale the loss of a trainable head as fp16
+training does.
 
 bf16 or fp16 (fp32 losses), fp32 or fp64 (losses of their own type, computed
 at that precision).  GPU only: other dtypes and CPU tensors raise.
@@ -48,6 +58,7 @@ from .fused_logprob import (
     _pad_dim,
     _rows_ok,
     _unit_stride,
+    backward_block_rows,
     head_vjp,
     head_vjp_exact,
 )
@@ -108,135 +119,226 @@ def _teacher(ids, logits, vocab, temperature, dtype):
     return slot_id, slot_p, state
 
 
-def _live_rows(h, state, scale):
-    """``scale h`` with zeros in the rows without a teacher."""
+def _live_rows(h, state):
+    """``h`` with zeros in the rows without a teacher: 0 x NaN is NaN in the weight gradient's product."""
     out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     _lib.check(
         _lib.require_library().ts_distill_rows(h.data_ptr(), max(h.stride(0), h.shape[1]), state.data_ptr(), h.shape[0],
-                                               h.shape[1], float(scale), out.data_ptr(), h.shape[1],
-                                               _lib.dtype_code(h.dtype), _lib.stream_of(h)),
+                                               h.shape[1], out.data_ptr(), _lib.dtype_code(h.dtype), _lib.stream_of(h)),
         f"ts_distill_rows(rows={h.shape[0]}, dim={h.shape[1]})",
     )
     return out
 
 
-def _forward(hidden, weight, ids, logits, temperature):
-    lib = _lib.require_library()
-    exact = hidden.dtype in EXACT_DTYPES
-    dt = hidden.dtype if exact else torch.float32
-    n, v, k = hidden.shape[0], weight.shape[0], ids.shape[1]
-    slot_id, slot_p, state = _teacher(ids, logits, v, temperature, dt)
-    slot_z = torch.empty_like(slot_p)
-    pitch = slot_p.shape[1]
-    loss = torch.empty(n, dtype=dt, device=hidden.device)
-    lse = torch.empty(n, dtype=dt, device=hidden.device)
-    code, stream = _lib.dtype_code(hidden.dtype), _lib.stream_of(hidden)
-    if exact:
-        # the logits over the temperature: of the rows divided by it
-        h, w = _live_rows(_unit_stride(hidden), state, 1.0 / temperature), _unit_stride(weight)
-        d = h.shape[1]
-        ldw = max(w.stride(0), d)
-        target = torch.zeros(n, dtype=torch.int64, device=h.device)
-        unused = torch.empty(n, dtype=dt, device=h.device)
-        ws_bytes = int(lib.ts_logprob_fwd_exact_workspace(n, v, code))
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=h.device)
-        _lib.check(
-            lib.ts_logprob_fwd_exact(h.data_ptr(), d, w.data_ptr(), ldw, target.data_ptr(), n, d, v, unused.data_ptr(),
-                                     None, lse.data_ptr(), ws.data_ptr(), ws_bytes, code, stream),
-            f"ts_logprob_fwd_exact(rows={n}, dim={d}, vocab={v})",
-        )
-        _lib.check(
-            lib.ts_distill_scores(h.data_ptr(), d, w.data_ptr(), ldw, slot_id.data_ptr(), pitch, n, k, d,
-                                  slot_z.data_ptr(), code, stream),
-            f"ts_distill_scores(rows={n}, top={k}, dim={d})",
-        )
-        _lib.check(
-            lib.ts_distill_loss(slot_id.data_ptr(), slot_p.data_ptr(), slot_z.data_ptr(), pitch, k, state.data_ptr(),
-                                lse.data_ptr(), n, loss.data_ptr(), code, stream),
-            f"ts_distill_loss(rows={n}, top={k})",
-        )
-    else:
-        h, w = _rows_ok(_pad_dim(hidden)), _rows_ok(_pad_dim(weight))
-        d = h.shape[1]
-        ws_bytes = int(lib.ts_distill_fwd_workspace(n, v))
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=h.device)
-        _lib.check(
-            lib.ts_distill_fwd(h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), n, d, v, float(temperature),
-                               slot_id.data_ptr(), slot_p.data_ptr(), slot_z.data_ptr(), pitch, k, state.data_ptr(),
-                               loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, code, stream),
-            f"ts_distill_fwd(rows={n}, dim={d}, vocab={v}, top={k})",
-        )
-    return loss, lse, slot_id, slot_p, slot_z, state
+class _Rows:
+    """A call's tensors as its kernels take them, and what the kernels find out about each row."""
 
+    def __init__(self, hidden, weight, ids, logits, temperature):
+        self.exact = hidden.dtype in EXACT_DTYPES
+        self.dtype = hidden.dtype if self.exact else torch.float32  # of losses and statistics
+        self.top, self.temperature = ids.shape[1], float(temperature)
+        self._operands(hidden, weight)
+        self.slot_id, self.slot_p, self.state = _teacher(ids, logits, weight.shape[0], temperature, self.dtype)
+        self.slot_z = torch.empty_like(self.slot_p)
+        self.lse, self.loss = (torch.empty(self.n, dtype=self.dtype, device=hidden.device) for _ in range(2))
 
-def _backward(hidden, weight, lse, slot_id, slot_p, slot_z, state, grad, top, temperature, chunk, needs_weight_grad):
-    lib = _lib.require_library()
-    v, pitch = weight.shape[0], slot_p.shape[1]
-    g = grad.to(lse.dtype).contiguous()
-    code, stream = _lib.dtype_code(hidden.dtype), _lib.stream_of(hidden)
-    slots = (slot_id, slot_p, slot_z)
-    if hidden.dtype in EXACT_DTYPES:
-        rows_in, w = _unit_stride(hidden), _unit_stride(weight)
-        h = _live_rows(rows_in, state, 1.0 / temperature)
-        h_weight = _live_rows(rows_in, state, 1.0) if needs_weight_grad else None
-        d = h.shape[1]
-        ldw = max(w.stride(0), d)
-        none = torch.full((h.shape[0],), -1, dtype=torch.int64, device=h.device)
-        # the logprob's coefficient kernel gives -q g; a row without a teacher has none
-        coef = torch.where(state == 0, 0.0, g * (-1.0 / temperature))
+    def _operands(self, hidden, weight):
+        self.d_in = hidden.shape[1]
+        if self.exact:
+            self.h, self.w = _unit_stride(hidden), _unit_stride(weight)
+            self.ld = (weight.shape[0] + 3) // 4 * 4  # rows of whole 16-byte vectors
+        else:
+            self.h, self.w = _rows_ok(_pad_dim(hidden)), _rows_ok(_pad_dim(weight))
+            self.ld = (weight.shape[0] + 7) // 8 * 8
+        self.n, self.d = self.h.shape
+        self.v = weight.shape[0]
+        self.ldh, self.ldw = max(self.h.stride(0), self.d), max(self.w.stride(0), self.d)
+        self.code = _lib.dtype_code(hidden.dtype)
 
-        def dlogits(i, rows, dl, ld):
+    def saved(self):
+        return self.slot_id, self.slot_p, self.slot_z, self.state, self.lse
+
+    @classmethod
+    def again(cls, hidden, weight, saved, top, temperature):
+        """The rows of a forward that saved ``saved``, in its backward."""
+        rows = cls.__new__(cls)
+        rows.exact, rows.top, rows.temperature = hidden.dtype in EXACT_DTYPES, top, temperature
+        rows._operands(hidden, weight)
+        rows.slot_id, rows.slot_p, rows.slot_z, rows.state, rows.lse = saved
+        rows.dtype = rows.lse.dtype
+        return rows
+
+    def slots(self, i):
+        pitch = self.slot_p.shape[1]
+        return (self.slot_id[i:].data_ptr(), self.slot_p[i:].data_ptr(), self.slot_z[i:].data_ptr(), pitch, self.top,
+                self.state[i:].data_ptr())
+
+    def row(self, i):
+        return self.h.data_ptr() + i * self.ldh * self.h.element_size()
+
+    def what(self, name, rows):
+        return lambda: f"{name}(rows={rows}, dim={self.d}, vocab={self.v}, top={self.top})"
+
+    def logits(self, i, rows, block):
+        """fp32 / fp64: rows ``[i, i + rows)`` of hidden . weight^T into ``block``."""
+        lib = _lib.require_library()
+        ws_bytes = int(lib.ts_matmul_exact_workspace(rows, self.v, self.d, self.code))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=block.device)
+        _lib.check(
+            lib.ts_matmul_exact_ws(self.row(i), self.ldh, 1, self.w.data_ptr(), 1, self.ldw, rows, self.v, self.d,
+                                   block.data_ptr(), self.ld, 0, ws.data_ptr(), ws_bytes, self.code,
+                                   _lib.stream_of(block)),
+            self.what("ts_matmul_exact_ws", rows),
+        )
+
+    def forward(self, i, rows, block):
+        """Losses of rows ``[i, i + rows)``; with a ``block`` also what :meth:`finish` reads.  Returns the
+        tiles' maxima (16-bit types)."""
+        lib, stream = _lib.require_library(), _lib.stream_of(self.h)
+        if self.exact:
+            self.logits(i, rows, block)
             _lib.check(
-                lib.ts_logprob_dlogits_exact(h[i:].data_ptr(), d, w.data_ptr(), ldw, none[i:].data_ptr(),
-                                             lse[i:].data_ptr(), None, coef[i:].data_ptr(), None, rows, d, v,
-                                             dl.data_ptr(), ld, code, stream),
-                f"ts_logprob_dlogits_exact(rows={rows}, dim={d}, vocab={v})",
+                lib.ts_distill_fwd_exact(block.data_ptr(), self.ld, rows, self.v, self.temperature, *self.slots(i),
+                                         self.loss[i:].data_ptr(), self.lse[i:].data_ptr(), self.code, stream),
+                self.what("ts_distill_fwd_exact", rows),
             )
-            _lib.check(
-                lib.ts_distill_slots(*(s[i:].data_ptr() for s in slots), pitch, top, lse[i:].data_ptr(),
-                                     g[i:].data_ptr(), rows, 1.0, 1.0 / temperature, dl.data_ptr(), ld, code, stream),
-                f"ts_distill_slots(rows={rows}, top={top})",
-            )
-
-        return head_vjp_exact(h, w, chunk, needs_weight_grad, dlogits, h_weight)
-    h, w = _rows_ok(_pad_dim(hidden)), _rows_ok(_pad_dim(weight))
-    # 0 x NaN is NaN in the weight gradient's product: rows without a teacher enter it as zeros
-    h_weight = _live_rows(h, state, 1.0) if needs_weight_grad else None
-    d = h.shape[1]
-
-    def dlogits(i, rows, dl, ld):
+            return None
+        ws_bytes = int(lib.ts_distill_fwd_workspace(rows, self.v))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=self.h.device)
         _lib.check(
-            lib.ts_distill_dlogits(h[i:].data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), rows, d, v,
-                                   float(temperature), *(s[i:].data_ptr() for s in slots), pitch, top,
-                                   state[i:].data_ptr(), lse[i:].data_ptr(), g[i:].data_ptr(), dl.data_ptr(), ld, code,
-                                   stream),
-            f"ts_distill_dlogits(rows={rows}, dim={d}, vocab={v}, top={top})",
+            lib.ts_distill_fwd(self.row(i), self.ldh, self.w.data_ptr(), self.ldw, rows, self.d, self.v,
+                               self.temperature, *self.slots(i), self.loss[i:].data_ptr(), self.lse[i:].data_ptr(),
+                               _lib.ptr(block), self.ld, ws.data_ptr(), ws_bytes, self.code, stream),
+            self.what("ts_distill_fwd", rows),
+        )
+        return ws[: ws_bytes // 2]
+
+    def finish(self, i, rows, block, maxima, grad, out):
+        """``block`` (as :meth:`forward` left it) to the logits' gradient ``out`` (which may be the block)."""
+        _lib.check(
+            _lib.require_library().ts_distill_finish(
+                block.data_ptr(), self.ld, _lib.ptr(maxima), rows, self.v, self.temperature, *self.slots(i),
+                self.lse[i:].data_ptr(), None if grad is None else grad[i:].data_ptr(), out.data_ptr(), self.ld,
+                self.code, _lib.stream_of(out)),
+            self.what("ts_distill_finish", rows),
         )
 
-    return head_vjp(h, w, hidden.shape[1], chunk, needs_weight_grad, dlogits, h_weight)
+    def unit_gradient(self, i, rows, dl, out, ws):
+        """``out`` rows ``[i, i + rows)`` = (q - p) . weight, not rounded to the element type."""
+        lib, stream = _lib.require_library(), _lib.stream_of(out)
+        if self.exact:
+            status = lib.ts_matmul_exact_ws(dl.data_ptr(), self.ld, 1, self.w.data_ptr(), self.ldw, 1, rows, self.d,
+                                            self.v, out[i:].data_ptr(), self.d, 0, ws.data_ptr(), ws.numel(),
+                                            self.code, stream)
+        else:
+            status = lib.ts_logprob_grad_hidden_f32(dl.data_ptr(), self.ld, self.w.data_ptr(), self.ldw, rows, self.d,
+                                                    self.v, out[i:].data_ptr(), ws.data_ptr(), ws.numel(), self.code,
+                                                    stream)
+        _lib.check(status, self.what("distill gradient of hidden", rows))
+
+    def unit_workspace(self, sizes):
+        lib = _lib.require_library()
+        need = (lambda r: lib.ts_matmul_exact_workspace(r, self.d, self.v, self.code)) if self.exact else (
+            lambda r: lib.ts_logprob_grad_hidden_workspace(r, self.d, self.v))
+        return torch.empty(max(16, *(int(need(r)) for r in sizes)), dtype=torch.uint8, device=self.h.device)
+
+
+def _forward(rows: _Rows, chunk, need_hidden, need_weight):
+    """The losses, and what the backward wants: nothing, the hidden states' unit gradient, or a kept block and its
+    tiles' maxima."""
+    n, dev = rows.n, rows.h.device
+    block_rows = min(max(1, int(chunk)), max(n, 1)) if rows.exact else backward_block_rows(n, chunk)
+    frozen = need_hidden and not need_weight
+    keep = need_weight and 0 < n <= block_rows
+    if n == 0:
+        return (torch.empty(0, rows.d, dtype=rows.dtype, device=dev),) if frozen else ()
+    if not (rows.exact or frozen or keep):
+        rows.forward(0, n, None)
+        return ()
+    block = torch.empty(min(block_rows, n), rows.ld, dtype=rows.h.dtype, device=dev)
+    unit = torch.empty(n, rows.d, dtype=rows.dtype, device=dev) if frozen else None
+    ws = rows.unit_workspace({block_rows, n % block_rows or block_rows}) if frozen else None
+    maxima = None
+    for i in range(0, n, block_rows):
+        size = min(block_rows, n - i)
+        maxima = rows.forward(i, size, block)
+        if frozen:
+            with operator_range("distill_head_coefficient", role=device_role(dev), rows=size, vocab=rows.v):
+                rows.finish(i, size, block, maxima, None, block)
+            with operator_range("distill_head_hidden_vjp", role=device_role(dev), rows=size, hidden=rows.d, vocab=rows.v):
+                rows.unit_gradient(i, size, block, unit, ws)
+    if frozen:
+        return (unit,)
+    return (block, maxima) if keep else ()
+
+
+def _backward_frozen(unit, state, grad, temperature, dtype, d_in):
+    n, d = unit.shape
+    out = torch.empty(n, d, dtype=dtype, device=unit.device)
+    _lib.check(
+        _lib.require_library().ts_distill_scale(unit.data_ptr(), grad.to(unit.dtype).contiguous().data_ptr(),
+                                                state.data_ptr(), n, d, temperature, out.data_ptr(),
+                                                _lib.dtype_code(dtype), _lib.stream_of(unit)),
+        f"ts_distill_scale(rows={n}, dim={d})",
+    )
+    return out if d == d_in else out[:, :d_in].contiguous()
+
+
+def _backward_trainable(rows: _Rows, grad, chunk, block, maxima):
+    g = grad.to(rows.dtype).contiguous()
+    h_weight = _live_rows(rows.h, rows.state)
+    lib = _lib.require_library()
+
+    def dlogits(i, size, dl, ld):
+        if block is not None:
+            rows.finish(i, size, block, maxima, g, dl)
+        elif rows.exact:
+            rows.logits(i, size, dl)
+            rows.finish(i, size, dl, None, g, dl)
+        else:
+            _lib.check(
+                lib.ts_distill_dlogits(rows.row(i), rows.ldh, rows.w.data_ptr(), rows.ldw, size, rows.d, rows.v,
+                                       rows.temperature, *rows.slots(i), rows.lse[i:].data_ptr(), g[i:].data_ptr(),
+                                       dl.data_ptr(), ld, rows.code, _lib.stream_of(dl)),
+                rows.what("ts_distill_dlogits", size),
+            )
+
+    if rows.exact:
+        return head_vjp_exact(rows.h, rows.w, chunk, True, dlogits, h_weight)
+    return head_vjp(rows.h, rows.w, rows.d_in, chunk, True, dlogits, h_weight)
 
 
 class _FusedDistill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, ids, logits, temperature, chunk, needs_weight_grad):
+    def forward(ctx, hidden, weight, ids, logits, temperature, chunk, need_hidden, need_weight):
         with torch.cuda.device(hidden.device), operator_range(
                 "fused_distill_forward", role=device_role(hidden.device), tokens=hidden.shape[0],
                 hidden=hidden.shape[1], vocab=weight.shape[0], top=ids.shape[1], dtype=hidden.dtype):
-            loss, *saved = _forward(hidden, weight, ids, logits, temperature)
-        ctx.save_for_backward(hidden, weight, *saved)
-        ctx.top, ctx.temperature, ctx.chunk, ctx.needs_weight_grad = ids.shape[1], temperature, chunk, needs_weight_grad
-        return loss
+            rows = _Rows(hidden, weight, ids, logits, temperature)
+            kept = _forward(rows, chunk, need_hidden, need_weight)
+        ctx.frozen, ctx.chunk, ctx.top, ctx.temperature = not need_weight, chunk, rows.top, rows.temperature
+        if need_weight:
+            ctx.save_for_backward(hidden, weight, *rows.saved(), *kept)
+        elif need_hidden:
+            ctx.save_for_backward(*kept, rows.state)
+            ctx.dtype, ctx.d_in, ctx.vocab = hidden.dtype, hidden.shape[1], weight.shape[0]
+        return rows.loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, *saved = ctx.saved_tensors
-        with torch.cuda.device(hidden.device), operator_range(
-                "fused_distill_backward", role=device_role(hidden.device), tokens=hidden.shape[0],
-                hidden=hidden.shape[1], vocab=weight.shape[0], weight_grad=ctx.needs_weight_grad):
-            gh, gw = _backward(hidden, weight, *saved, grad, ctx.top, ctx.temperature, ctx.chunk,
-                               ctx.needs_weight_grad)
-        return gh, gw, None, None, None, None, None
+        with torch.cuda.device(grad.device), operator_range(
+                "fused_distill_backward", role=device_role(grad.device), tokens=grad.shape[0],
+                weight_grad=not ctx.frozen):
+            if ctx.frozen:
+                unit, state = ctx.saved_tensors
+                gh, gw = _backward_frozen(unit, state, grad, ctx.temperature, ctx.dtype, ctx.d_in), None
+            else:
+                hidden, weight, *saved = ctx.saved_tensors
+                block, maxima = [*saved[5:], None, None][:2]
+                rows = _Rows.again(hidden, weight, saved[:5], ctx.top, ctx.temperature)
+                gh, gw = _backward_trainable(rows, grad, ctx.chunk, block, maxima)
+        return gh, gw, None, None, None, None, None, None
 
 
 def fused_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
@@ -248,5 +350,6 @@ def fused_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch
     taken at ``temperature``; the loss is not multiplied by its square.
     """
     _validate(hidden, weight, teacher_ids, teacher_logits, temperature)
+    grad = torch.is_grad_enabled()
     return _FusedDistill.apply(hidden, weight, teacher_ids, teacher_logits, float(temperature), chunk,
-                               weight.requires_grad)
+                               grad and hidden.requires_grad, grad and weight.requires_grad)
