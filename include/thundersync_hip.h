@@ -599,6 +599,9 @@ int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_
  * Sampling (fp32, fp16 or bf16 logits)
  * ------------------------------------------------------------------------ */
 
+/* Workspace bytes ts_sample needs (for up to 4096 rows at a time). */
+int64_t ts_sample_workspace(int64_t rows, int64_t vocab);
+
 /* One token per row of logits [rows, vocab] from uniform[rows] (TS_F32 or
  * TS_F64, in [0, 1)) and the logprob of the token in the distribution it was
  * drawn from.  Weights are w = exp((logit - max) / temperature), their order is
@@ -614,7 +617,7 @@ int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_
 int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, const void* uniform,
               int uniform_dtype, const float* temperature, double temperature_all, const int32_t* top_k,
               int64_t top_k_all, const float* top_p, double top_p_all, const float* min_p, double min_p_all,
-              int64_t* tokens, float* logprobs, int dtype, void* stream);
+              int64_t* tokens, float* logprobs, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Merged-weight LoRA linear (bf16 or fp16 operands, fp32 accumulation)

@@ -145,6 +145,11 @@ def test_random_numbers_outside_their_range_draw_the_last(cuda):
         tokens, logprobs = sample_tokens(z, torch.full((2,), u, device=cuda))
         assert tokens.tolist() == [1, 2] and logprobs.isfinite().all()
     assert sample_tokens(z, torch.full((2,), -1.0, device=cuda))[0].tolist() == [0, 0]
+    wide = torch.full((1, 30000), -math.inf, device=cuda)
+    wide[0, 20000:20002] = 0.0
+    for u, want in ((-1.0, 20000), (0.0, 20000), (2.0, 20001), (math.nan, 20001)):
+        for options in ({}, {"top_p": 0.9}, {"top_k": 7}, {"min_p": 0.5}):
+            assert int(sample_tokens(wide, torch.full((1,), u, device=cuda), **options)[0]) == want
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])

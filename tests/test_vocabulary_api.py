@@ -98,9 +98,10 @@ def test_c_entries_refuse_without_a_device():
             (p, 2, p, 4, 1 << 31, 4, -1, 1.0, p, p, 1 << 20, bf16, None),
         ],
         "ts_sample": [
-            (p, 8, 2, (1 << 21) + 1, p, f32, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, bf16, None),
-            (p, 8, 2, 8, p, f32, None, math.nan, None, 0, None, 1.0, None, 0.0, p, p, bf16, None),
-            (p, 8, 2, 8, None, f32, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, bf16, None),
+            (p, 8, 2, (1 << 21) + 1, p, f32, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, p, 1 << 20, bf16, None),
+            (p, 8, 2, 8, p, f32, None, math.nan, None, 0, None, 1.0, None, 0.0, p, p, p, 1 << 20, bf16, None),
+            (p, 8, 2, 8, p, f32, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, p, 16, bf16, None),
+            (p, 8, 2, 8, None, f32, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, p, 1 << 20, bf16, None),
         ],
     }
     for name, cases in calls.items():

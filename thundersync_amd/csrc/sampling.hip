@@ -6,16 +6,22 @@
 //   of kept weights exceeds u times their total; logprob = log(w / total).  T = 0 draws
 //   the first maximum.
 //
-// Every filter keeps a prefix of the order, so a row's kept set is "logits above a
-// threshold, and the first m that equal it".  The threshold is found by counting, not by
-// sorting: a histogram over bins of log weight (64 octaves below the maximum), then, inside
-// the bin that the border falls into, over ranges of the logit's bits until at most
-// kCandidates logits are left, which are sorted in LDS.  A token depends on a border of the
-// running sum, and the tail's weights are far below fp32's rounding of the sum: weights are
-// fp64, sums over bins exact integers of 2^-scale (order-free), the running sum fp64 in a
-// fixed order.
+// Every filter keeps a prefix of the order, so a row's kept set is "logits above a border
+// element, and those that equal it up to its index".  The border is found by counting, not
+// by sorting the row.  A row is cut into slices of kSlice logits, and up to four launches of
+// work-groups over (rows x slices) work on it:
+//   maxima   each slice's maximum, minimum, NaN; without filters also its sum of weights
+//   bins     a histogram (count and mass) of the row over kBins bins of logit below its maximum
+//   gather   the bins that the borders fall into, their logits as candidates; per slice the
+//            sum of the weights above them
+//   draw     one work-group a row: sorts the candidates in LDS, finds the border, picks the
+//            slice that u falls into and reads that slice again for the token
+// A row with more than kCandidates logits in its border bins (equal logits, or very many in a
+// narrow range) is resolved by its draw work-group alone, which narrows the range bin by bin.
 //
-// One work-group per row.
+// A token depends on a border of the running sum, and the tail's weights are far below fp32's
+// rounding of the sum: weights are fp64, sums over bins exact integers of 2^-scale (order-free),
+// the running sum fp64 in a fixed order.
 #include <algorithm>
 #include <type_traits>
 
@@ -26,14 +32,16 @@
 namespace ts {
 namespace sample {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // the draw
 constexpr int kGroup = 8;                      // consecutive logits per thread and step
 constexpr int kBins = 2048;
 constexpr float kBinsPerOctave = 32.f;         // kBins / 64 octaves
 constexpr int kCandidates = 4096;              // logits sorted in LDS
 constexpr int kMaxVocab = 1 << 21;
-constexpr int kTile = kThreads * kGroup;       // logits per step of the work-group
-constexpr int kMaxTiles = kMaxVocab / kTile + 1;
+constexpr int kSlice = kThreads * kGroup;      // logits per slice
+constexpr int kMaxSlices = kMaxVocab / kSlice + 1;
+constexpr int kPartThreads = 256;              // maxima, bins, gather
+constexpr int kPartGroups = kSlice / kGroup / kPartThreads;  // a thread's groups of a slice
 
 struct Options {       // a value for every row, or one per row
   const float* temperature;
@@ -93,24 +101,53 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// What a row's weights are made of.
+// 2^(j / kTable) for j in [0, kTable), in LDS
+constexpr int kTable = 256;
+__device__ __forceinline__ void fill_table(double* table) {
+  for (int j = threadIdx.x; j < kTable; j += blockDim.x) table[j] = exp2((double)j / kTable);
+  __syncthreads();
+}
+
+// What a row's weights are made of.  exp((x - top) / T) = 2^(k / 256) 2^(r / 256) with k whole
+// and |r| <= 1/2: the first from the table and an exponent, the second by its Taylor series to
+// the fourth power (the next term is below 2^-54).
 struct Weights {
-  float top;      // the row's maximum
-  double inv_t;   // 1 / T
-  float octaves;  // log2(e) / T
+  const double* table;
+  double top;     // the maximum that weights are relative to
+  double units;   // kTable log2(e) / T
   double fixed;
+  float top_f;
+  float bins;     // bins per unit of logit
   __device__ __forceinline__ double of(float x) const {
-    if (x == top) return 1.;
-    return x == -inf() || top == inf() ? 0. : exp(((double)x - (double)top) * inv_t);
+    if (x == top_f) return 1.;
+    if (x == -inf() || top_f == inf()) return 0.;
+    const double y = fmax(((double)x - top) * units, -1100. * kTable);
+    const double k = rint(y);
+    const double t = (y - k) * (0.693147180559945309417 / kTable);
+    const double e = fma(fma(fma(fma(t, 1. / 24, 1. / 6), t, 0.5), t, 1.), t, 1.);
+    const int n = (int)k;
+    return ldexp(table[n & (kTable - 1)] * e, n >> 8);
   }
   __device__ __forceinline__ uint64_t fixed_of(float x) const { return (uint64_t)(of(x) * fixed + 0.5); }
   // falls with the logit, equal for equal logits
   __device__ __forceinline__ int bin(float x) const {
-    if (x == top) return 0;
-    const float b = (top - x) * octaves * kBinsPerOctave;
+    if (x == top_f) return 0;
+    const float b = (top_f - x) * bins;
     return b < (float)(kBins - 1) ? (int)b : kBins - 1;
   }
 };
+// `low`: the row's lowest finite logit, so that the bins cover no more than there is
+__device__ __forceinline__ Weights weights_of(const double* table, float top, float low, double temp, double fixed) {
+  Weights w;
+  w.table = table;
+  w.top = (double)top;
+  w.top_f = top;
+  w.units = kTable * (1.4426950408889634074 / temp);
+  w.fixed = fixed;
+  const float octave = (float)(0.693147180559945309 * temp);  // in units of logit
+  w.bins = fmaxf(kBinsPerOctave / octave, (float)kBins / (top - low));
+  return w;
+}
 
 // A border in the order: logits above `key` are kept, and the first `ties` (in index order)
 // of those that equal it.
@@ -126,15 +163,16 @@ struct Shared {
   uint64_t wave_u[kWaves];
   double wave_d[kWaves];
   uint32_t wave_c[kWaves];
-  double tile_sum[kMaxTiles];
-  uint32_t tile_ties[kMaxTiles];
+  double slice_sum[kMaxSlices];
+  uint64_t slice_add[kMaxSlices];  // candidates' kept mass, or (slow rows) ties
+  double table[kTable];
   int bin, n_cand;
   uint32_t lo, hi;
   uint64_t before_mass;
   uint32_t before_count;
   Border border;
   int token;
-  double weight, target;
+  double total, target, scale;
 };
 
 template <typename F> __device__ __forceinline__ void each(int n, F&& f) {
@@ -186,6 +224,27 @@ template <typename V> __device__ __forceinline__ V block_prefix(V x, V* per_wave
   // the lanes before this one, as the previous lane's inclusive sum
   const V prev = __shfl_up(incl, 1, 64);
   return lane ? before + prev : before;
+}
+
+// falling order of s.cand[0 .. have), padded with zeros to a power of two of at least 64
+__device__ void sort_candidates(Shared& s, int have) {
+  int size = 64;
+  while (size < have) size *= 2;
+  each(size - have, [&](int i) { s.cand[have + i] = 0; });
+  __syncthreads();
+  for (int len = 2; len <= size; len *= 2)
+    for (int step = len / 2; step >= 1; step /= 2) {
+      each(size / 2, [&](int i) {
+        const int p = 2 * step * (i / step) + i % step, q = p + step;
+        const uint64_t a = s.cand[p], c = s.cand[q];
+        const bool falling = (p & len) == 0;
+        if (falling ? a < c : a > c) {
+          s.cand[p] = c;
+          s.cand[q] = a;
+        }
+      });
+      __syncthreads();
+    }
 }
 
 // Where the running count (BY_MASS false: the first `want` elements) or the running mass
@@ -298,23 +357,7 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
         __syncthreads();
       }
       const int have = s.n_cand;
-      int size = 64;
-      while (size < have) size *= 2;
-      each(size - have, [&](int i) { s.cand[have + i] = 0; });
-      __syncthreads();
-      for (int len = 2; len <= size; len *= 2)
-        for (int step = len / 2; step >= 1; step /= 2) {
-          each(size / 2, [&](int i) {
-            const int p = 2 * step * (i / step) + i % step, q = p + step;
-            const uint64_t a = s.cand[p], c = s.cand[q];
-            const bool falling = (p & len) == 0;
-            if (falling ? a < c : a > c) {
-              s.cand[p] = c;
-              s.cand[q] = a;
-            }
-          });
-          __syncthreads();
-        }
+      sort_candidates(s, have);
       // the position of the border's element: four candidates a thread, by prefix sums
       constexpr int PER = kCandidates / kThreads;
       uint64_t mine = 0, sum = 0;
@@ -390,86 +433,439 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
-  __shared__ Shared s;
-  const int64_t r = blockIdx.x;
-  const int t = threadIdx.x;
-  const Row<T> row(a.logits, a.ld, r, a.vocab);
-  const double temp = a.o.temperature ? (double)a.o.temperature[r] : a.o.temperature_all;
-  const int64_t top_k = a.o.top_k ? (int64_t)a.o.top_k[r] : a.o.top_k_all;
-  const double top_p = a.o.top_p ? (double)a.o.top_p[r] : a.o.top_p_all;
-  const double min_p = fmin(a.o.min_p ? (double)a.o.min_p[r] : a.o.min_p_all, 1.);
-  const double u = a.uniform_wide ? ((const double*)a.uniform)[r] : (double)((const float*)a.uniform)[r];
-  const bool greedy = !(temp > 0.);
+// ---------------------------------------------------------------------------
+// a row's options and what the launches hand on
+// ---------------------------------------------------------------------------
+struct RowOptions {
+  double temp, top_p, min_p, u;
+  int64_t top_k;
+  bool greedy, by_k, by_p, by_min;
+  __device__ __forceinline__ RowOptions(const Args& a, int64_t r) {
+    temp = a.o.temperature ? (double)a.o.temperature[r] : a.o.temperature_all;
+    top_k = a.o.top_k ? (int64_t)a.o.top_k[r] : a.o.top_k_all;
+    top_p = a.o.top_p ? (double)a.o.top_p[r] : a.o.top_p_all;
+    min_p = fmin(a.o.min_p ? (double)a.o.min_p[r] : a.o.min_p_all, 1.);
+    u = a.uniform_wide ? ((const double*)a.uniform)[r] : (double)((const float*)a.uniform)[r];
+    u = u < 0. ? 0. : u;
+    greedy = !(temp > 0.) || top_k == 1;
+    by_k = !greedy && top_k > 0 && top_k < a.vocab;
+    by_p = !greedy && top_p < 1.;
+    by_min = !greedy && min_p > 0.;
+  }
+  __device__ __forceinline__ bool plain() const { return !greedy && !by_k && !by_p && !by_min; }
+};
 
-  // the maximum and its first index; a NaN shows in its own flag
-  float top = -inf();
+struct SliceStats {
+  float top, low;  // -inf / +inf: no logit above -inf
+  int at;          // first index of the maximum
+  int nan;
+};
+
+// Per row, written by the first gather work-group: the bins that hold the borders.
+struct Bins {
+  int lo, hi, k;          // border of p in [lo, hi], of k in k (or lo = hi = k, or none: kBins)
+  uint32_t k_before;      // elements above bin k
+  uint64_t k_mass, lo_mass;  // mass above bins k and lo
+};
+
+// The launches' workspace, of `rows` rows and `slices` slices.  From `bins` on only where some
+// row of the call has a top_k or top_p: null otherwise.
+struct Space {
+  SliceStats* stats;  // [rows][slices]
+  double* sums;       // [rows][slices]
+  Bins* bins;         // [rows]
+  uint64_t* mass;     // [rows][kBins]
+  uint32_t* count;    // [rows][kBins]
+  uint64_t* cand;     // [rows][kCandidates]
+  uint32_t* n_cand;   // [rows]
+  int slices;
+};
+
+// the row's maximum, lowest logit and NaN from its slices (every thread reads them all: few)
+struct RowStats {
+  float top, low;
+  int at;
+  bool nan;
+  __device__ __forceinline__ RowStats(const SliceStats* s, int slices) {
+    top = -inf();
+    low = inf();
+    at = 0x7fffffff;
+    int any = 0;
+    const int lane = threadIdx.x & 63;
+    for (int i = lane; i < slices; i += 64) {
+      const SliceStats x = s[i];
+      any |= x.nan;
+      low = fminf(low, x.low);
+      if (x.top > top) {  // slices in index order: the first of equal ones
+        top = x.top;
+        at = x.at;
+      }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const float xo = __shfl_xor(top, o, 64);
+      const int ao = __shfl_xor(at, o, 64);
+      if (xo > top || (xo == top && ao < at)) {
+        top = xo;
+        at = ao;
+      }
+      low = fminf(low, __shfl_xor(low, o, 64));
+      any |= __shfl_xor(any, o, 64);
+    }
+    nan = any != 0;
+  }
+  __device__ __forceinline__ bool empty() const { return nan || top == -inf(); }
+};
+
+constexpr int kPartWaves = kPartThreads / 64;
+
+// sum over the work-group of kPartThreads in a fixed order
+__device__ __forceinline__ double part_sum(double x, double* per_wave) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) per_wave[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double t = per_wave[0];
+#pragma unroll
+  for (int w = 1; w < kPartWaves; ++w) t += per_wave[w];
+  return t;
+}
+
+// ---------------------------------------------------------------------------
+// maxima: one slice, held in registers; a row without filters gets its slice's sum of
+// weights, relative to the slice's own maximum, from the same read
+// ---------------------------------------------------------------------------
+template <typename T, bool CLEAR>
+__global__ __launch_bounds__(kPartThreads) void maxima_kernel(Args a, Space sp) {
+  __shared__ double table[kTable], per_wave[kPartWaves];
+  __shared__ float tops[kPartWaves], lows[kPartWaves];
+  __shared__ int ats[kPartWaves];
+  const int64_t r = blockIdx.y;
+  const int slice = blockIdx.x, t = threadIdx.x;
+  if (CLEAR) {  // the histogram that the next launch adds to
+    for (int i = slice * kPartThreads + t; i < kBins; i += sp.slices * kPartThreads) {
+      sp.mass[r * kBins + i] = 0;
+      sp.count[r * kBins + i] = 0;
+    }
+    if (slice == 0 && t == 0) sp.n_cand[r] = 0;
+  }
+  const RowOptions o(a, r);
+  const Row<T> row(a.logits, a.ld, r, a.vocab);
+  float x[kPartGroups][kGroup];
+  float top = -inf(), low = inf();
   int at = 0x7fffffff;
   bool nan = false;
-  for (int g = t; g < row.groups; g += kThreads) {
+#pragma unroll
+  for (int i = 0; i < kPartGroups; ++i) {
+    const int g = slice * (kSlice / kGroup) + i * kPartThreads + t;
+    if (g < row.groups) {
+      row.load(g, x[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) x[i][j] = -inf();
+    }
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) {
+      nan |= x[i][j] != x[i][j];
+      if (x[i][j] > top) {
+        top = x[i][j];
+        at = row.first(g) + j;
+      }
+      if (x[i][j] > -inf()) low = fminf(low, x[i][j]);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    const float xo = __shfl_xor(top, d, 64);
+    const int ao = __shfl_xor(at, d, 64);
+    if (xo > top || (xo == top && ao < at)) {
+      top = xo;
+      at = ao;
+    }
+    low = fminf(low, __shfl_xor(low, d, 64));
+  }
+  if ((t & 63) == 0) {
+    tops[t >> 6] = top;
+    lows[t >> 6] = low;
+    ats[t >> 6] = at;
+  }
+  const bool any = __syncthreads_or(nan);
+#pragma unroll
+  for (int w = 0; w < kPartWaves; ++w) {
+    if (tops[w] > top || (tops[w] == top && ats[w] < at)) {
+      top = tops[w];
+      at = ats[w];
+    }
+    low = fminf(low, lows[w]);
+  }
+  if (t == 0) sp.stats[r * sp.slices + slice] = SliceStats{top, low, at, any};
+  if (!o.plain()) return;
+  if (any || top == -inf()) {
+    if (t == 0) sp.sums[r * sp.slices + slice] = 0.;
+    return;
+  }
+  fill_table(table);
+  const Weights w = weights_of(table, top, low, o.temp, a.fixed);
+  double sum = 0.;
+#pragma unroll
+  for (int i = 0; i < kPartGroups; ++i)
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) sum += w.of(x[i][j]);
+  sum = part_sum(sum, per_wave);
+  if (t == 0) sp.sums[r * sp.slices + slice] = sum;
+}
+
+// ---------------------------------------------------------------------------
+// bins: a work-group's share of the slices into a histogram in LDS, then into the row's.
+// The mass only where top_p asks for it.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void bins_kernel(Args a, Space sp) {
+  __shared__ double table[kTable];
+  __shared__ uint32_t count[kBins];
+  __shared__ uint64_t mass[kBins];
+  const int64_t r = blockIdx.y;
+  const int t = threadIdx.x;
+  const RowOptions o(a, r);
+  if (!o.by_k && !o.by_p) return;
+  const RowStats s(sp.stats + r * sp.slices, sp.slices);
+  if (s.empty()) return;
+  for (int i = t; i < kBins; i += kPartThreads) {
+    count[i] = 0;
+    mass[i] = 0;
+  }
+  fill_table(table);
+  const Weights w = weights_of(table, s.top, s.low, o.temp, a.fixed);
+  const Row<T> row(a.logits, a.ld, r, a.vocab);
+  for (int g = blockIdx.x * kPartThreads + t; g < row.groups; g += gridDim.x * kPartThreads) {
     float x[kGroup];
     row.load(g, x);
 #pragma unroll
     for (int j = 0; j < kGroup; ++j) {
-      nan |= x[j] != x[j];
-      if (x[j] > top) {
-        top = x[j];
-        at = row.first(g) + j;
-      }
-    }
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float xo = __shfl_xor(top, o, 64);
-    const int ao = __shfl_xor(at, o, 64);
-    if (xo > top || (xo == top && ao < at)) {
-      top = xo;
-      at = ao;
-    }
-  }
-  if ((t & 63) == 0) {
-    s.wave_d[t >> 6] = (double)top;
-    s.wave_c[t >> 6] = (uint32_t)at;
-  }
-  const bool any_nan = __syncthreads_or(nan);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float xo = (float)s.wave_d[w];
-    const int ao = (int)s.wave_c[w];
-    if (xo > top || (xo == top && ao < at)) {
-      top = xo;
-      at = ao;
+      if (x[j] == -inf()) continue;
+      const int b = w.bin(x[j]);
+      atomicAdd(&count[b], 1u);
+      if (o.by_p) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w.fixed_of(x[j]));
     }
   }
   __syncthreads();
-  if (any_nan || top == -inf()) {  // nothing to draw
-    if (t == 0) {
-      a.tokens[r] = -1;
-      a.logprobs[r] = __builtin_nanf("");
-    }
-    return;
+  for (int i = t; i < kBins; i += kPartThreads) {
+    if (count[i]) atomicAdd(&sp.count[r * kBins + i], count[i]);
+    if (mass[i]) atomicAdd((unsigned long long*)&sp.mass[r * kBins + i], (unsigned long long)mass[i]);
   }
-  if (greedy || top_k == 1) {
-    if (t == 0) {
-      a.tokens[r] = at;
-      a.logprobs[r] = 0.f;
-    }
-    return;
-  }
-  Weights w;
-  w.top = top;
-  w.inv_t = 1. / temp;
-  w.octaves = (float)(1.4426950408889634 / temp);
-  w.fixed = a.fixed;
+}
 
+// ---------------------------------------------------------------------------
+// gather: every work-group of a row finds the border bins from its histogram (2048 bins,
+// eight a thread), then goes through its slices
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void gather_kernel(Args a, Space sp) {
+  __shared__ double table[kTable], per_wave[kPartWaves];
+  __shared__ uint64_t wave_m[kPartWaves];
+  __shared__ uint32_t wave_c[kPartWaves];
+  __shared__ Bins found;
+  const int64_t r = blockIdx.y;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const RowOptions o(a, r);
+  if (o.greedy || o.plain()) return;
+  const RowStats s(sp.stats + r * sp.slices, sp.slices);
+  if (s.empty()) return;
+  if (t == 0) found = Bins{kBins, kBins, kBins, 0, 0, 0};
+  fill_table(table);
+  const Weights w = weights_of(table, s.top, s.low, o.temp, a.fixed);
+  if (o.by_k || o.by_p) {
+    constexpr int PER = kBins / kPartThreads;
+    uint32_t c[PER], cs = 0;
+    uint64_t m[PER], ms = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] = sp.count[r * kBins + PER * t + i];
+      m[i] = sp.mass[r * kBins + PER * t + i];
+      cs += c[i];
+      ms += m[i];
+    }
+    // exclusive prefix sums over the threads
+    uint32_t ci = cs;
+    uint64_t mi = ms;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t cy = __shfl_up(ci, d, 64);
+      const uint64_t my = __shfl_up(mi, d, 64);
+      if (lane >= d) {
+        ci += cy;
+        mi += my;
+      }
+    }
+    if (lane == 63) {
+      wave_c[wave] = ci;
+      wave_m[wave] = mi;
+    }
+    __syncthreads();
+    uint32_t c0 = ci - cs, all_c = 0;
+    uint64_t m0 = mi - ms, all_m = 0;
+#pragma unroll
+    for (int v = 0; v < kPartWaves; ++v) {
+      if (v < wave) {
+        c0 += wave_c[v];
+        m0 += wave_m[v];
+      }
+      all_c += wave_c[v];
+      all_m += wave_m[v];
+    }
+    const bool cut = o.by_k && (uint64_t)o.top_k < all_c;  // else there are no more than k
+    if (cut) {
+      uint32_t cc = c0;
+      uint64_t mm = m0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (cc < (uint64_t)o.top_k && cc + c[i] >= (uint64_t)o.top_k) {
+          found.k = PER * t + i;
+          found.k_before = cc;
+          found.k_mass = mm;
+          if (!o.by_p) {
+            found.lo = found.hi = found.k;
+            found.lo_mass = mm;
+          }
+        }
+        cc += c[i];
+        mm += m[i];
+      }
+    }
+    __syncthreads();
+    if (o.by_p) {
+      // p times the mass of the first k: between what is above bin k and that with all of bin k
+      const int k = found.k;
+      uint64_t most = all_m, least = all_m;
+      if (cut) {
+        least = found.k_mass;
+        most = least + sp.mass[r * kBins + k];
+      }
+      auto goal = [&](uint64_t total) {
+        const double x = ceil(o.top_p * (double)total);
+        return x > 1. ? (uint64_t)x : (uint64_t)1;
+      };
+      const uint64_t lo = goal(least), hi = goal(most);
+      uint64_t mm = m0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (mm < lo && mm + m[i] >= lo) {
+          found.lo = PER * t + i;
+          found.lo_mass = mm;
+        }
+        if (mm < hi && mm + m[i] >= hi) found.hi = PER * t + i;
+        mm += m[i];
+      }
+      __syncthreads();
+    }
+  }
+  const Bins f = found;
+  if (blockIdx.x == 0 && t == 0 && (o.by_k || o.by_p)) sp.bins[r] = f;  // (without either there is no room for it)
+  const Row<T> row(a.logits, a.ld, r, a.vocab);
+  for (int slice = blockIdx.x; slice < sp.slices; slice += gridDim.x) {
+    double sum = 0.;
+#pragma unroll
+    for (int i = 0; i < kPartGroups; ++i) {
+      const int g = slice * (kSlice / kGroup) + i * kPartThreads + t;
+      if (g >= row.groups) continue;
+      float x[kGroup];
+      row.load(g, x);
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) {
+        if (x[j] == -inf()) continue;
+        const int b = w.bin(x[j]);
+        if (b < f.lo) {
+          const double y = w.of(x[j]);
+          sum += y >= o.min_p ? y : 0.;
+        } else if (b <= f.hi || b == f.k) {
+          const uint32_t at = atomicAdd(&sp.n_cand[r], 1u);
+          if (at < (uint32_t)kCandidates)
+            sp.cand[r * kCandidates + at] =
+                ((uint64_t)key_of(x[j]) << 32) | (0xffffffffu - (uint32_t)(row.first(g) + j));
+        }
+      }
+    }
+    sum = part_sum(sum, per_wave);
+    if (t == 0) sp.sums[r * sp.slices + slice] = sum;
+  }
+}
+
+// The token within a slice: the first in index order whose running sum of `weight(x, index)`
+// exceeds s.target (an infinite target: the last with any).
+template <typename T, typename F>
+__device__ void draw_token(const Args& a, int64_t r, const Row<T>& row, int slice, F&& weight, Shared& s) {
+  const int g = slice * kThreads + (int)threadIdx.x;
+  float x[kGroup];
+  double y[kGroup], sum = 0.;
+  if (g < row.groups) row.load(g, x);
+  const int i0 = row.first(g);
+#pragma unroll
+  for (int j = 0; j < kGroup; ++j) {
+    y[j] = g < row.groups && x[j] != -inf() ? weight(x[j], i0 + j) : 0.;
+    sum += y[j];
+  }
+  double total;
+  double run = block_prefix<double>(sum, s.wave_d, total);
+  const double target = s.target;
+  int hit = -1, last = -1;
+#pragma unroll
+  for (int j = 0; j < kGroup; ++j) {
+    run += y[j];
+    if (y[j] > 0.) {
+      last = j;
+      if (hit < 0 && run > target) hit = j;
+    }
+  }
+  // the first hit of the work-group, or (by rounding) the slice's last kept logit
+  if (threadIdx.x == 0) {
+    s.token = 0x7fffffff;
+    s.n_cand = -1;
+  }
+  __syncthreads();
+  if (hit >= 0) atomicMin(&s.token, i0 + hit);
+  if (last >= 0) atomicMax(&s.n_cand, i0 + last);
+  __syncthreads();
+  const int token = s.token != 0x7fffffff ? s.token : s.n_cand;
+  if (token >= i0 && token < i0 + kGroup) {
+    double mine = 0.;
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) mine = token == i0 + j ? y[j] : mine;
+    a.tokens[r] = token;
+    a.logprobs[r] = (float)log(mine * s.scale / s.total);
+  }
+}
+
+// thread 0: the slice that u times the total falls into (s.bin), what is left of the target
+// there (s.target) and the total, from s.slice_sum
+__device__ __forceinline__ void pick_slice(Shared& s, int slices, double u) {
+  double total = 0.;
+  for (int i = 0; i < slices; ++i) total += s.slice_sum[i];
+  const double target = u * total;
+  double before = 0.;
+  int pick = -1, last = 0;
+  for (int i = 0; i < slices && pick < 0; ++i) {
+    if (s.slice_sum[i] > 0.) last = i;
+    if (before + s.slice_sum[i] > target) pick = i;
+    else before += s.slice_sum[i];
+  }
+  s.bin = pick < 0 ? last : pick;  // u of 1 or more, or NaN: the last one
+  s.target = pick < 0 ? __builtin_huge_val() : target - before;
+  s.total = total;
+  s.scale = 1.;
+}
+
+// A row by one work-group alone: see find_border.
+template <typename T>
+__device__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowOptions& o, const Weights& w, int slices,
+                         Shared& s) {
+  const int t = threadIdx.x;
   Border border{key_of(-inf()), 0};
-  const bool by_k = top_k > 0 && top_k < a.vocab, by_p = top_p < 1.;
-  if (by_k) {
-    find_border<T, false>(row, w, (uint64_t)top_k, nullptr, s);
+  if (o.by_k) {
+    find_border<T, false>(row, w, (uint64_t)o.top_k, nullptr, s);
     border = s.border;
   }
-  if (by_p) {
+  if (o.by_p) {
     // the mass of what top_k keeps, then the border of p times it
     uint64_t mass = 0;
     for (int g = t; g < row.groups; g += kThreads) {
@@ -483,25 +879,18 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     block_prefix<uint64_t>(mass, s.wave_u, total);
     if (border.ties) total += border.ties * w.fixed_of(of_key(border.key));
     // the smallest whole mass that is p times the total or more; at least the first element
-    const double goal = ceil(top_p * (double)total);
+    const double goal = ceil(o.top_p * (double)total);
     const uint64_t want = goal > 1. ? (uint64_t)goal : 1;
     const Border limit = border;
-    find_border<T, true>(row, w, want, by_k ? &limit : nullptr, s);
+    find_border<T, true>(row, w, want, o.by_k ? &limit : nullptr, s);
     border = s.border;
   }
-  // a partial tie only matters where not all of the logits that equal the border's are kept;
-  // counting them in index order covers both
   const float border_x = of_key(border.key);
-  auto above = [&](float x) { return x != -inf() && key_of(x) > border.key; };
   const double tie_weight = border.ties ? w.of(border_x) : 0.;
-  const bool tie_kept = border.ties && (tie_weight >= min_p);
-  auto weight = [&](float x) {
-    const double y = w.of(x);  // 1 for the maximum, which min_p never drops
-    return y >= min_p ? y : 0.;
-  };
-  // kept mass and ties per tile of kTile logits
-  const int tiles = (row.groups + kThreads - 1) / kThreads;
-  for (int i = 0; i < tiles; ++i) {
+  const bool tie_kept = border.ties && tie_weight >= o.min_p;
+  auto above = [&](float x) { return x != -inf() && key_of(x) > border.key; };
+  // kept mass and ties per slice
+  for (int i = 0; i < slices; ++i) {
     const int g = i * kThreads + t;
     double m = 0.;
     uint32_t ties = 0;
@@ -510,95 +899,234 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
       row.load(g, x);
 #pragma unroll
       for (int j = 0; j < kGroup; ++j) {
-        if (above(x[j])) m += weight(x[j]);
-        else if (tie_kept && x[j] == border_x) ++ties;
+        if (above(x[j])) {
+          const double y = w.of(x[j]);
+          m += y >= o.min_p ? y : 0.;
+        } else if (tie_kept && x[j] == border_x) {
+          ++ties;
+        }
       }
     }
     m = block_sum(m, s);
     if (tie_kept) ties = block_count(ties, s);
     if (t == 0) {
-      s.tile_sum[i] = m;
-      s.tile_ties[i] = ties;
+      s.slice_sum[i] = m;
+      s.slice_add[i] = ties;
     }
   }
   __syncthreads();
-  // the tile that the draw falls into
   if (t == 0) {
-    double total = 0.;
     uint32_t left = tie_kept ? (uint32_t)border.ties : 0;
-    for (int i = 0; i < tiles; ++i) {
-      const uint32_t n = min(left, s.tile_ties[i]);
-      s.tile_ties[i] = n;
+    for (int i = 0; i < slices; ++i) {
+      const uint32_t n = min(left, (uint32_t)s.slice_add[i]);
+      s.slice_add[i] = n;
       left -= n;
-      s.tile_sum[i] += n * tie_weight;
-      total += s.tile_sum[i];
+      s.slice_sum[i] += n * tie_weight;
     }
-    const double target = u * total;
-    double before = 0.;
-    int pick = -1, last = 0;
-    for (int i = 0; i < tiles && pick < 0; ++i) {
-      if (s.tile_sum[i] > 0.) last = i;
-      if (before + s.tile_sum[i] > target) pick = i;
-      else before += s.tile_sum[i];
-    }
-    if (pick < 0) {  // u of 1 or more, or NaN: the last one
-      pick = last;
-      before = -__builtin_huge_val();
-    }
-    s.bin = pick;
-    s.target = target - before;  // infinite: the last kept logit of the tile
-    s.weight = total;
-    s.token = -1;
-    s.n_cand = -1;
+    pick_slice(s, slices, o.u);
   }
   __syncthreads();
-  {
-    const int g = s.bin * kThreads + t;
+  // the slice's first ties, by their rank in it
+  const int slice = s.bin, g = slice * kThreads + t;
+  uint32_t ties = 0;
+  if (tie_kept && g < row.groups) {
     float x[kGroup];
-    double y[kGroup];
-    double sum = 0.;
-    uint32_t ties = 0;
-    if (g < row.groups) row.load(g, x);
+    row.load(g, x);
 #pragma unroll
-    for (int j = 0; j < kGroup; ++j) {
-      if (g >= row.groups) x[j] = -inf();
-      y[j] = above(x[j]) ? weight(x[j]) : 0.;
-      ties += tie_kept && x[j] == border_x;
+    for (int j = 0; j < kGroup; ++j) ties += x[j] == border_x;
+  }
+  uint32_t all_ties, rank = block_prefix<uint32_t>(ties, s.wave_c, all_ties);
+  const uint32_t take = (uint32_t)s.slice_add[slice];
+  draw_token(a, r, row, slice, [&](float x, int) {
+    if (above(x)) {
+      const double y = w.of(x);
+      return y >= o.min_p ? y : 0.;
     }
-    uint32_t all_ties, tie = block_prefix<uint32_t>(ties, s.wave_c, all_ties);
-#pragma unroll
-    for (int j = 0; j < kGroup; ++j) {
-      if (tie_kept && x[j] == border_x) {
-        if (tie < s.tile_ties[s.bin]) y[j] = tie_weight;
-        ++tie;
-      }
-      sum += y[j];
+    return tie_kept && x == border_x && rank++ < take ? tie_weight : 0.;
+  }, s);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void draw_kernel(Args a, Space sp) {
+  __shared__ Shared s;
+  const int64_t r = blockIdx.x;
+  const int t = threadIdx.x;
+  const RowOptions o(a, r);
+  const SliceStats* stats = sp.stats + r * sp.slices;
+  const RowStats rs(stats, sp.slices);
+  if (rs.empty()) {  // nothing to draw
+    if (t == 0) {
+      a.tokens[r] = -1;
+      a.logprobs[r] = __builtin_nanf("");
     }
-    double total;
-    double run = block_prefix<double>(sum, s.wave_d, total);
-    const double target = s.target;
-    int hit = -1, last = -1;
-#pragma unroll
-    for (int j = 0; j < kGroup; ++j) {
-      run += y[j];
-      if (y[j] > 0.) {
-        last = j;
-        if (hit < 0 && run > target) hit = j;
-      }
+    return;
+  }
+  if (o.greedy) {
+    if (t == 0) {
+      a.tokens[r] = rs.at;
+      a.logprobs[r] = 0.f;
     }
-    // the first hit of the work-group, or (by rounding) the tile's last kept logit
-    const int i0 = row.first(g);
-    if (t == 0) s.token = 0x7fffffff;
-    __syncthreads();
-    if (hit >= 0) atomicMin(&s.token, i0 + hit);
-    if (last >= 0) atomicMax(&s.n_cand, i0 + last);
+    return;
+  }
+  fill_table(s.table);
+  const Row<T> row(a.logits, a.ld, r, a.vocab);
+  Weights w = weights_of(s.table, rs.top, rs.low, o.temp, a.fixed);
+  if (o.plain()) {
+    // slices' sums are relative to their own maxima
+    each(sp.slices, [&](int i) { s.slice_sum[i] = sp.sums[r * sp.slices + i] * w.of(stats[i].top); });
     __syncthreads();
     if (t == 0) {
-      const int token = s.token != 0x7fffffff ? s.token : s.n_cand;
-      a.tokens[r] = token;
-      a.logprobs[r] = (float)log(w.of(to_f(row.z[token]) + 0.f) / s.weight);
+      pick_slice(s, sp.slices, o.u);
+      s.scale = w.of(stats[s.bin].top);
+      s.target /= s.scale;
+    }
+    __syncthreads();
+    const float top = stats[s.bin].top;
+    w = weights_of(s.table, top, rs.low, o.temp, a.fixed);
+    draw_token(a, r, row, s.bin, [&](float x, int) { return w.of(x); }, s);
+    return;
+  }
+  uint64_t border = 0;  // the last kept (key, index); 0: no border
+  each(sp.slices, [&](int i) {
+    s.slice_sum[i] = sp.sums[r * sp.slices + i];
+    s.slice_add[i] = 0;
+  });
+  if (o.by_k || o.by_p) {
+    const Bins f = sp.bins[r];
+    const uint32_t have = sp.n_cand[r];
+    if (have > (uint32_t)kCandidates) {
+      slow_row<T>(a, r, row, o, w, sp.slices, s);
+      return;
+    }
+    if (have) {
+      each((int)have, [&](int i) { s.cand[i] = sp.cand[r * kCandidates + i]; });
+      sort_candidates(s, (int)have);
+      // four candidates a thread: their bins, masses and prefix sums
+      constexpr int PER = kCandidates / kThreads;
+      uint64_t m[PER], ms = 0;
+      int b[PER];
+      uint32_t before_k = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const bool on = PER * t + i < (int)have;
+        const float x = on ? of_key((uint32_t)(s.cand[PER * t + i] >> 32)) : 0.f;
+        b[i] = on ? w.bin(x) : kBins;
+        m[i] = on ? w.fixed_of(x) : 0;
+        ms += m[i];
+        before_k += on && b[i] < f.k;
+      }
+      // the last of the first k: in bin k's group, which ends the candidates
+      int last = (int)have - 1;
+      uint64_t mass_k = 0;
+      uint64_t all;
+      const uint64_t m0 = block_prefix<uint64_t>(ms, s.wave_u, all);
+      if (f.k < kBins) {
+        last = (int)block_count(before_k, s) + (int)(o.top_k - (int64_t)f.k_before) - 1;
+        uint64_t kept = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (b[i] == f.k && PER * t + i <= last) kept += m[i];
+        block_prefix<uint64_t>(kept, s.wave_u, mass_k);
+        mass_k += f.k_mass;
+      }
+      if (o.by_p) {
+        // p times the mass of the first k, reached in the bins [lo, hi], which begin the candidates
+        if (f.k >= kBins) {
+          // the whole row's mass: the histogram's
+          uint64_t mine = 0;
+          each(kBins, [&](int i) { mine += sp.mass[r * kBins + i]; });
+          block_prefix<uint64_t>(mine, s.wave_u, mass_k);
+        }
+        const double goal = ceil(o.top_p * (double)mass_k);
+        const uint64_t want = goal > 1. ? (uint64_t)goal : 1;
+        uint64_t run = m0 + f.lo_mass;
+        if (t == 0) s.bin = last;  // where p times the mass rounds past it
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          if (run < want && run + m[i] >= want) s.bin = PER * t + i;  // one element
+          run += m[i];
+        }
+        __syncthreads();
+        last = s.bin;
+      }
+      border = s.cand[last];
+      // the kept candidates' mass, by slice
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int at = PER * t + i;
+        if (at > last) continue;
+        const float x = of_key((uint32_t)(s.cand[at] >> 32));
+        if (!(w.of(x) >= o.min_p)) continue;
+        const int idx = (int)(0xffffffffu - (uint32_t)s.cand[at]);
+        atomicAdd((unsigned long long*)&s.slice_add[(idx + row.lead) / kSlice], (unsigned long long)m[i]);
+      }
     }
   }
+  __syncthreads();
+  if (t == 0) {
+    for (int i = 0; i < sp.slices; ++i) s.slice_sum[i] += (double)s.slice_add[i] / a.fixed;
+    pick_slice(s, sp.slices, o.u);
+  }
+  __syncthreads();
+  draw_token(a, r, row, s.bin, [&](float x, int i) {
+    const uint64_t me = ((uint64_t)key_of(x) << 32) | (0xffffffffu - (uint32_t)i);
+    if (me < border) return 0.;
+    const double y = w.of(x);
+    return y >= o.min_p ? y : 0.;
+  }, s);
+}
+
+constexpr int64_t kRowsAtOnce = 4096;  // rows per set of launches: bounds the workspace
+
+int slices_of(int64_t vocab) {
+  return (int)((((vocab + 2 * kGroup - 2) / kGroup) + kThreads - 1) / kThreads);  // of a row at any alignment
+}
+int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
+
+int64_t space_of(int64_t rows, int64_t vocab, bool bins, char* base, Space* sp) {
+  const int64_t slices = slices_of(vocab);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    char* p = base + at;
+    at += up16(bytes);
+    return p;
+  };
+  Space s{};
+  s.slices = (int)slices;
+  s.stats = (SliceStats*)take(rows * slices * (int64_t)sizeof(SliceStats));
+  s.sums = (double*)take(rows * slices * 8);
+  if (bins) {
+    s.bins = (Bins*)take(rows * (int64_t)sizeof(Bins));
+    s.mass = (uint64_t*)take(rows * kBins * 8);
+    s.count = (uint32_t*)take(rows * kBins * 4);
+    s.cand = (uint64_t*)take(rows * kCandidates * 8);
+    s.n_cand = (uint32_t*)take(rows * 4);
+  }
+  if (sp) *sp = s;
+  return at;
+}
+
+template <typename T>
+void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bins, hipStream_t s) {
+  const dim3 grid((unsigned)sp.slices, (unsigned)rows), block(kPartThreads);
+  {
+    TimedLaunch timed_("sampling.maxima_kernel", s);
+    if (bins) hipLaunchKernelGGL((maxima_kernel<T, true>), grid, block, 0, s, a, sp);
+    else hipLaunchKernelGGL((maxima_kernel<T, false>), grid, block, 0, s, a, sp);
+  }
+  // work-groups a row where the histogram's merge, or its search, is paid by each
+  const dim3 parts((unsigned)std::max<int64_t>(1, std::min<int64_t>(sp.slices, 1024 / rows)), (unsigned)rows);
+  if (bins) {
+    TimedLaunch timed_("sampling.bins_kernel", s);
+    hipLaunchKernelGGL(bins_kernel<T>, parts, block, 0, s, a, sp);
+  }
+  if (filters) {
+    TimedLaunch timed_("sampling.gather_kernel", s);
+    hipLaunchKernelGGL(gather_kernel<T>, parts, block, 0, s, a, sp);
+  }
+  TimedLaunch timed_("sampling.draw_kernel", s);
+  hipLaunchKernelGGL(draw_kernel<T>, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp);
 }
 
 }  // namespace sample
@@ -606,10 +1134,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
 
 extern "C" {
 
+int64_t ts_sample_workspace(int64_t rows, int64_t vocab) {
+  using namespace ts::sample;
+  return rows > 0 && vocab > 0 && vocab <= kMaxVocab ? space_of(std::min(rows, kRowsAtOnce), vocab, true, nullptr, nullptr)
+                                                     : 0;
+}
+
 int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, const void* uniform,
               int uniform_dtype, const float* temperature, double temperature_all, const int32_t* top_k,
               int64_t top_k_all, const float* top_p, double top_p_all, const float* min_p, double min_p_all,
-              int64_t* tokens, float* logprobs, int dtype, void* stream) {
+              int64_t* tokens, float* logprobs, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
   using namespace ts::sample;
   TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F16 || dtype == TS_BF16, "ts_sample: dtype %d", dtype);
   TS_CHECK_ARG(uniform_dtype == TS_F32 || uniform_dtype == TS_F64, "ts_sample: uniform dtype %d", uniform_dtype);
@@ -632,13 +1166,30 @@ int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab
   a.fixed = (double)(1ull << (62 - bits));  // vocab weights of at most 1 stay below 2^62
   a.tokens = tokens;
   a.logprobs = logprobs;
+  const bool by_min = min_p || min_p_all > 0;
+  const bool bins = top_k || top_p || (top_k_all > 1 && top_k_all < vocab) || top_p_all < 1;
+  const int64_t at_once = std::min(rows, kRowsAtOnce);
+  const int64_t need = space_of(at_once, vocab, true, nullptr, nullptr);
+  TS_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need,
+               "ts_sample: workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)need);
   hipStream_t s = (hipStream_t)stream;
-  {
-    ts::TimedLaunch timed_("sampling.sample_kernel", s);
-    const dim3 grid((unsigned)rows), block(kThreads);
-    if (dtype == TS_F32) hipLaunchKernelGGL(sample_kernel<float>, grid, block, 0, s, a);
-    else if (dtype == TS_F16) hipLaunchKernelGGL(sample_kernel<ts::f16>, grid, block, 0, s, a);
-    else hipLaunchKernelGGL(sample_kernel<ts::bf16>, grid, block, 0, s, a);
+  const int64_t size = dtype == TS_F32 ? 4 : 2;
+  for (int64_t r0 = 0; r0 < rows; r0 += at_once) {
+    const int64_t n = std::min(at_once, rows - r0);
+    Args b = a;
+    b.logits = (const char*)logits + r0 * ld_logits * size;
+    b.uniform = (const char*)uniform + r0 * (a.uniform_wide ? 8 : 4);
+    if (temperature) b.o.temperature += r0;
+    if (top_k) b.o.top_k += r0;
+    if (top_p) b.o.top_p += r0;
+    if (min_p) b.o.min_p += r0;
+    b.tokens += r0;
+    b.logprobs += r0;
+    Space sp;
+    space_of(n, vocab, bins, (char*)workspace, &sp);
+    if (dtype == TS_F32) launch<float>(b, sp, n, bins || by_min, bins, s);
+    else if (dtype == TS_F16) launch<ts::f16>(b, sp, n, bins || by_min, bins, s);
+    else launch<ts::bf16>(b, sp, n, bins || by_min, bins, s);
   }
   return ts::check_launch("ts_sample");
 }

@@ -87,6 +87,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     b, v = z.shape
     tokens = torch.empty(b, dtype=torch.int64, device=z.device)
     logprobs = torch.empty(b, dtype=torch.float32, device=z.device)
+    ws_bytes = int(lib.ts_sample_workspace(b, v))
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=z.device)
     (t_rows, t_all), (k_rows, k_all), (p_rows, p_all), (m_rows, m_all) = options
     with torch.cuda.device(z.device), operator_range("sample_tokens", role=device_role(z.device), rows=b, vocab=v,
                                                      dtype=z.dtype):
@@ -94,7 +96,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
             lib.ts_sample(z.data_ptr(), z.stride(0), b, v, u.data_ptr(), _lib.dtype_code(u.dtype), _lib.ptr(t_rows),
                           float(t_all), _lib.ptr(k_rows), min(int(k_all), MAX_VOCAB), _lib.ptr(p_rows), float(p_all),
                           _lib.ptr(m_rows), min(float(m_all), 1.0), tokens.data_ptr(), logprobs.data_ptr(),
-                          _lib.dtype_code(z.dtype), _lib.stream_of(z)),
+                          ws.data_ptr(), ws_bytes, _lib.dtype_code(z.dtype), _lib.stream_of(z)),
             lambda: f"ts_sample(rows={b}, vocab={v}, {z.dtype})",
         )
     return tokens, logprobs
