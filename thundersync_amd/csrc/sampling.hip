@@ -17,7 +17,7 @@
 //   draw     one work-group a row: sorts the candidates in LDS, finds the border, picks the
 //            slice that u falls into and reads that slice again for the token
 // A row with more than kCandidates logits in its border bins (equal logits, or very many in a
-// narrow range) is resolved by its draw work-group alone, which narrows the range bin by bin.
+// narrow range) is left to one work-group of a fifth launch, which narrows the range bin by bin.
 //
 // A token depends on a border of the running sum, and the tail's weights are far below fp32's
 // rounding of the sum: weights are fp64, sums over bins exact integers of 2^-scale (order-free),
@@ -32,7 +32,8 @@
 namespace ts {
 namespace sample {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;  // the draw
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // a slow row
+constexpr int kDrawThreads = 256;
 constexpr int kGroup = 8;                      // consecutive logits per thread and step
 constexpr int kBins = 2048;
 constexpr float kBinsPerOctave = 32.f;         // kBins / 64 octaves
@@ -110,7 +111,9 @@ __device__ __forceinline__ void fill_table(double* table) {
 
 // What a row's weights are made of.  exp((x - top) / T) = 2^(k / 256) 2^(r / 256) with k whole
 // and |r| <= 1/2: the first from the table and an exponent, the second by its Taylor series to
-// the fourth power (the next term is below 2^-54).
+// the fourth power (the next term is below 2^-54).  k is rounded by adding 1.5 2^52, whose low
+// word then holds it, and the exponent is added to the high word: conversions, rounding and
+// ldexp of fp64 run at a quarter of the rate of these.
 struct Weights {
   const double* table;
   double top;     // the maximum that weights are relative to
@@ -118,15 +121,23 @@ struct Weights {
   double fixed;
   float top_f;
   float bins;     // bins per unit of logit
+  bool simple;    // top and units are finite
+  // of a logit above -inf (-inf: 2^-1000)
+  __device__ __forceinline__ double of_finite(float x) const {
+    constexpr double kRound = 6755399441055744., kL = 0.693147180559945309417 / kTable;
+    const double y = fmax(((double)x - top) * units, -1000. * kTable);
+    const double k = y + kRound;
+    const double t = y - (k - kRound);
+    const double e = fma(fma(fma(fma(t, kL * kL * kL * kL / 24, kL * kL * kL / 6), t, kL * kL / 2), t, kL), t, 1.);
+    const int n = __double2loint(k);
+    const double p = table[n & (kTable - 1)] * e;
+    return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+  }
   __device__ __forceinline__ double of(float x) const {
     if (x == top_f) return 1.;
     if (x == -inf() || top_f == inf()) return 0.;
-    const double y = fmax(((double)x - top) * units, -1100. * kTable);
-    const double k = rint(y);
-    const double t = (y - k) * (0.693147180559945309417 / kTable);
-    const double e = fma(fma(fma(fma(t, 1. / 24, 1. / 6), t, 0.5), t, 1.), t, 1.);
-    const int n = (int)k;
-    return ldexp(table[n & (kTable - 1)] * e, n >> 8);
+    if (!simple) return units > 0. ? 0. : 1.;  // T so small, or so large, that nothing is between
+    return ((double)x - top) * units < -1000. * kTable ? 0. : of_finite(x);
   }
   __device__ __forceinline__ uint64_t fixed_of(float x) const { return (uint64_t)(of(x) * fixed + 0.5); }
   // falls with the logit, equal for equal logits
@@ -144,6 +155,7 @@ __device__ __forceinline__ Weights weights_of(const double* table, float top, fl
   w.top_f = top;
   w.units = kTable * (1.4426950408889634074 / temp);
   w.fixed = fixed;
+  w.simple = top < inf() && w.units > 0. && w.units < __builtin_huge_val();
   const float octave = (float)(0.693147180559945309 * temp);  // in units of logit
   w.bins = fmaxf(kBinsPerOctave / octave, (float)kBins / (top - low));
   return w;
@@ -156,54 +168,47 @@ struct Border {
   int ties;
 };
 
-struct Shared {
-  uint32_t count[kBins];
-  uint64_t mass[kBins];
+// What a work-group of N threads that draws a row's token holds.
+template <int N> struct Scratch {
+  static constexpr int kN = N;
   uint64_t cand[kCandidates];
-  uint64_t wave_u[kWaves];
-  double wave_d[kWaves];
-  uint32_t wave_c[kWaves];
   double slice_sum[kMaxSlices];
   uint64_t slice_add[kMaxSlices];  // candidates' kept mass, or (slow rows) ties
   double table[kTable];
-  int bin, n_cand;
+  uint64_t wave_u[N / 64];
+  double wave_d[N / 64];
+  uint32_t wave_c[N / 64];
+  int bin, n_cand, token;
+  double total, target, scale;
+};
+// and one that finds a border by itself
+struct Shared : Scratch<kThreads> {
+  uint32_t count[kBins];
+  uint64_t mass[kBins];
   uint32_t lo, hi;
   uint64_t before_mass;
   uint32_t before_count;
   Border border;
-  int token;
-  double total, target, scale;
 };
 
-template <typename F> __device__ __forceinline__ void each(int n, F&& f) {
-  for (int i = threadIdx.x; i < n; i += kThreads) f(i);
+template <int N, typename F> __device__ __forceinline__ void each(int n, F&& f) {
+  for (int i = threadIdx.x; i < n; i += N) f(i);
 }
 
 // sums in a fixed order: lanes by halving distances, waves in order; every thread gets it
-__device__ __forceinline__ double block_sum(double x, Shared& s) {
+template <int N, typename V> __device__ __forceinline__ V block_sum(V x, V* per_wave) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.wave_d[threadIdx.x >> 6] = x;
+  if ((threadIdx.x & 63) == 0) per_wave[threadIdx.x >> 6] = x;
   __syncthreads();
-  double t = s.wave_d[0];
+  V t = per_wave[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) t += s.wave_d[w];
-  return t;
-}
-__device__ __forceinline__ uint32_t block_count(uint32_t x, Shared& s) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.wave_c[threadIdx.x >> 6] = x;
-  __syncthreads();
-  uint32_t t = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) t += s.wave_c[w];
+  for (int w = 1; w < N / 64; ++w) t += per_wave[w];
   return t;
 }
 // exclusive prefix sum over the threads
-template <typename V> __device__ __forceinline__ V block_prefix(V x, V* per_wave, V& total) {
+template <int N, typename V> __device__ __forceinline__ V block_prefix(V x, V* per_wave, V& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   V incl = x;
 #pragma unroll
@@ -217,7 +222,7 @@ template <typename V> __device__ __forceinline__ V block_prefix(V x, V* per_wave
   V before = (V)0;
   total = (V)0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < N / 64; ++w) {
     if (w == wave) before = total;
     total += per_wave[w];
   }
@@ -227,14 +232,14 @@ template <typename V> __device__ __forceinline__ V block_prefix(V x, V* per_wave
 }
 
 // falling order of s.cand[0 .. have), padded with zeros to a power of two of at least 64
-__device__ void sort_candidates(Shared& s, int have) {
+template <int N> __device__ void sort_candidates(Scratch<N>& s, int have) {
   int size = 64;
   while (size < have) size *= 2;
-  each(size - have, [&](int i) { s.cand[have + i] = 0; });
+  each<N>(size - have, [&](int i) { s.cand[have + i] = 0; });
   __syncthreads();
   for (int len = 2; len <= size; len *= 2)
     for (int step = len / 2; step >= 1; step /= 2) {
-      each(size / 2, [&](int i) {
+      each<N>(size / 2, [&](int i) {
         const int p = 2 * step * (i / step) + i % step, q = p + step;
         const uint64_t a = s.cand[p], c = s.cand[q];
         const bool falling = (p & len) == 0;
@@ -268,7 +273,7 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
     return k >= lo && k <= hi && w.bin(x) == bin0 ? (int)((hi - k) >> shift) : -1;
   };
   while (true) {
-    each(kBins, [&](int b) {
+    each<kThreads>(kBins, [&](int b) {
       s.count[b] = 0;
       s.mass[b] = 0;
     });
@@ -302,8 +307,8 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
     const uint64_t m0 = s.mass[2 * t], m1 = s.mass[2 * t + 1];
     uint32_t total_c;
     uint64_t total_m;
-    const uint32_t pc = block_prefix<uint32_t>(c0 + c1, s.wave_c, total_c) + before_count;
-    const uint64_t pm = block_prefix<uint64_t>(m0 + m1, s.wave_u, total_m) + before_mass;
+    const uint32_t pc = block_prefix<kThreads, uint32_t>(c0 + c1, s.wave_c, total_c) + before_count;
+    const uint64_t pm = block_prefix<kThreads, uint64_t>(m0 + m1, s.wave_u, total_m) + before_mass;
     if (t == 0) {
       s.bin = -1;
       s.lo = 0xffffffffu;
@@ -351,13 +356,13 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
       if (limited && bin_of(of_key(limit_key), limit_key) == b) {
         // the limit's ties, the last of the bin: one index is as good as another
         const int at = s.n_cand;
-        each((int)limit_ties, [&](int i) { s.cand[at + i] = ((uint64_t)limit_key << 32) | (0xffffffffu - (uint32_t)i); });
+        each<kThreads>((int)limit_ties, [&](int i) { s.cand[at + i] = ((uint64_t)limit_key << 32) | (0xffffffffu - (uint32_t)i); });
         __syncthreads();
         if (t == 0) s.n_cand = at + (int)limit_ties;
         __syncthreads();
       }
       const int have = s.n_cand;
-      sort_candidates(s, have);
+      sort_candidates<kThreads>(s, have);
       // the position of the border's element: four candidates a thread, by prefix sums
       constexpr int PER = kCandidates / kThreads;
       uint64_t mine = 0, sum = 0;
@@ -369,7 +374,7 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
         sum += part[i];
       }
       uint64_t total;
-      mine = block_prefix<uint64_t>(sum, s.wave_u, total) + (BY_MASS ? before_mass : before_count);
+      mine = block_prefix<kThreads, uint64_t>(sum, s.wave_u, total) + (BY_MASS ? before_mass : before_count);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int at = PER * t + i;
@@ -386,7 +391,7 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
         const int at = PER * t + i;
         ties += at <= last && (uint32_t)(s.cand[at] >> 32) == key;
       }
-      ties = block_count(ties, s);
+      ties = block_sum<kThreads, uint32_t>(ties, s.wave_c);
       if (t == 0) s.border = Border{key, (int)ties};
       __syncthreads();
       return;
@@ -519,25 +524,12 @@ struct RowStats {
 
 constexpr int kPartWaves = kPartThreads / 64;
 
-// sum over the work-group of kPartThreads in a fixed order
-__device__ __forceinline__ double part_sum(double x, double* per_wave) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) per_wave[threadIdx.x >> 6] = x;
-  __syncthreads();
-  double t = per_wave[0];
-#pragma unroll
-  for (int w = 1; w < kPartWaves; ++w) t += per_wave[w];
-  return t;
-}
-
 // ---------------------------------------------------------------------------
 // maxima: one slice, held in registers; a row without filters gets its slice's sum of
 // weights, relative to the slice's own maximum, from the same read
 // ---------------------------------------------------------------------------
 template <typename T, bool CLEAR>
-__global__ __launch_bounds__(kPartThreads) void maxima_kernel(Args a, Space sp) {
+__global__ __launch_bounds__(kPartThreads, 5) void maxima_kernel(Args a, Space sp) {
   __shared__ double table[kTable], per_wave[kPartWaves];
   __shared__ float tops[kPartWaves], lows[kPartWaves];
   __shared__ int ats[kPartWaves];
@@ -608,17 +600,24 @@ __global__ __launch_bounds__(kPartThreads) void maxima_kernel(Args a, Space sp) 
   fill_table(table);
   const Weights w = weights_of(table, top, low, o.temp, a.fixed);
   double sum = 0.;
+  if (w.simple) {  // 2^-1000 for a logit of -inf adds nothing to a sum of 1 or more
 #pragma unroll
-  for (int i = 0; i < kPartGroups; ++i)
+    for (int i = 0; i < kPartGroups; ++i)
 #pragma unroll
-    for (int j = 0; j < kGroup; ++j) sum += w.of(x[i][j]);
-  sum = part_sum(sum, per_wave);
+      for (int j = 0; j < kGroup; ++j) sum += w.of_finite(x[i][j]);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kPartGroups; ++i)
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) sum += w.of(x[i][j]);
+  }
+  sum = block_sum<kPartThreads, double>(sum, per_wave);
   if (t == 0) sp.sums[r * sp.slices + slice] = sum;
 }
 
 // ---------------------------------------------------------------------------
-// bins: a work-group's share of the slices into a histogram in LDS, then into the row's.
-// The mass only where top_p asks for it.
+// bins: a work-group's share of the slices into a histogram in LDS, then into the row's:
+// counts where top_k asks for them, mass where top_p does.  Bound by the LDS atomics.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kPartThreads) void bins_kernel(Args a, Space sp) {
@@ -645,7 +644,7 @@ __global__ __launch_bounds__(kPartThreads) void bins_kernel(Args a, Space sp) {
     for (int j = 0; j < kGroup; ++j) {
       if (x[j] == -inf()) continue;
       const int b = w.bin(x[j]);
-      atomicAdd(&count[b], 1u);
+      if (o.by_k) atomicAdd(&count[b], 1u);
       if (o.by_p) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w.fixed_of(x[j]));
     }
   }
@@ -779,87 +778,128 @@ __global__ __launch_bounds__(kPartThreads) void gather_kernel(Args a, Space sp) 
           const double y = w.of(x[j]);
           sum += y >= o.min_p ? y : 0.;
         } else if (b <= f.hi || b == f.k) {
-          const uint32_t at = atomicAdd(&sp.n_cand[r], 1u);
+          // one place for each of the wave's lanes that are here, from one atomic
+          const uint64_t here = __builtin_amdgcn_ballot_w64(true);
+          const int rank = __popcll(here & ((1ull << lane) - 1));
+          uint32_t at = 0;
+          if (rank == 0) at = atomicAdd(&sp.n_cand[r], (uint32_t)__popcll(here));
+          at = __builtin_amdgcn_readfirstlane(at) + rank;
           if (at < (uint32_t)kCandidates)
             sp.cand[r * kCandidates + at] =
                 ((uint64_t)key_of(x[j]) << 32) | (0xffffffffu - (uint32_t)(row.first(g) + j));
         }
       }
     }
-    sum = part_sum(sum, per_wave);
+    sum = block_sum<kPartThreads, double>(sum, per_wave);
     if (t == 0) sp.sums[r * sp.slices + slice] = sum;
   }
 }
 
 // The token within a slice: the first in index order whose running sum of `weight(x, index)`
-// exceeds s.target (an infinite target: the last with any).
-template <typename T, typename F>
-__device__ void draw_token(const Args& a, int64_t r, const Row<T>& row, int slice, F&& weight, Shared& s) {
-  const int g = slice * kThreads + (int)threadIdx.x;
-  float x[kGroup];
-  double y[kGroup], sum = 0.;
-  if (g < row.groups) row.load(g, x);
-  const int i0 = row.first(g);
+// exceeds s.target (an infinite target: the last with any).  A thread takes consecutive groups.
+template <typename T, int N, typename F>
+__device__ void draw_token(const Args& a, int64_t r, const Row<T>& row, int slice, F&& weight, Scratch<N>& s) {
+  constexpr int PER = kSlice / kGroup / N;
+  const int g0 = slice * (kSlice / kGroup) + PER * (int)threadIdx.x;
+  double y[PER][kGroup], sum = 0.;
 #pragma unroll
-  for (int j = 0; j < kGroup; ++j) {
-    y[j] = g < row.groups && x[j] != -inf() ? weight(x[j], i0 + j) : 0.;
-    sum += y[j];
-  }
-  double total;
-  double run = block_prefix<double>(sum, s.wave_d, total);
-  const double target = s.target;
-  int hit = -1, last = -1;
+  for (int q = 0; q < PER; ++q) {
+    float x[kGroup];
+    const int g = g0 + q, i0 = row.first(g);
+    if (g < row.groups) row.load(g, x);
 #pragma unroll
-  for (int j = 0; j < kGroup; ++j) {
-    run += y[j];
-    if (y[j] > 0.) {
-      last = j;
-      if (hit < 0 && run > target) hit = j;
+    for (int j = 0; j < kGroup; ++j) {
+      y[q][j] = g < row.groups && x[j] != -inf() ? weight(x[j], i0 + j) : 0.;
+      sum += y[q][j];
     }
   }
+  double all;
+  double run = block_prefix<N, double>(sum, s.wave_d, all);
+  const double target = s.target;
+  int hit = -1, last = -1;
+  double hit_y = 0., last_y = 0.;
+#pragma unroll
+  for (int q = 0; q < PER; ++q)
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) {
+      run += y[q][j];
+      if (y[q][j] > 0.) {
+        last = row.first(g0 + q) + j;
+        last_y = y[q][j];
+        if (hit < 0 && run > target) {
+          hit = last;
+          hit_y = last_y;
+        }
+      }
+    }
   // the first hit of the work-group, or (by rounding) the slice's last kept logit
   if (threadIdx.x == 0) {
     s.token = 0x7fffffff;
     s.n_cand = -1;
   }
   __syncthreads();
-  if (hit >= 0) atomicMin(&s.token, i0 + hit);
-  if (last >= 0) atomicMax(&s.n_cand, i0 + last);
+  if (hit >= 0) atomicMin(&s.token, hit);
+  if (last >= 0) atomicMax(&s.n_cand, last);
   __syncthreads();
-  const int token = s.token != 0x7fffffff ? s.token : s.n_cand;
-  if (token >= i0 && token < i0 + kGroup) {
-    double mine = 0.;
-#pragma unroll
-    for (int j = 0; j < kGroup; ++j) mine = token == i0 + j ? y[j] : mine;
+  const bool none = s.token == 0x7fffffff;
+  const int token = none ? s.n_cand : s.token;
+  if (token >= 0 && token == (none ? last : hit)) {
     a.tokens[r] = token;
-    a.logprobs[r] = (float)log(mine * s.scale / s.total);
+    a.logprobs[r] = (float)log((none ? last_y : hit_y) * s.scale / s.total);
   }
 }
 
-// thread 0: the slice that u times the total falls into (s.bin), what is left of the target
-// there (s.target) and the total, from s.slice_sum
-__device__ __forceinline__ void pick_slice(Shared& s, int slices, double u) {
-  double total = 0.;
-  for (int i = 0; i < slices; ++i) total += s.slice_sum[i];
+// The first wave: the slice that u times the total falls into (s.bin), what is left of the
+// target there (s.target) and the total, from s.slice_sum.  A lane takes consecutive slices.
+template <int N> __device__ __forceinline__ void pick_slice(Scratch<N>& s, int slices, double u) {
+  const int lane = threadIdx.x, per = (slices + 63) / 64;
+  const int b = min(slices, lane * per), e = min(slices, b + per);
+  double sum = 0.;
+  for (int i = b; i < e; ++i) sum += s.slice_sum[i];
+  double incl = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += y;
+  }
+  const double total = __shfl(incl, 63, 64), prev = __shfl_up(incl, 1, 64);
   const double target = u * total;
-  double before = 0.;
+  double before = lane ? prev : 0., left = 0.;
   int pick = -1, last = 0;
-  for (int i = 0; i < slices && pick < 0; ++i) {
+  for (int i = b; i < e; ++i) {
     if (s.slice_sum[i] > 0.) last = i;
-    if (before + s.slice_sum[i] > target) pick = i;
-    else before += s.slice_sum[i];
+    if (pick < 0 && before + s.slice_sum[i] > target) {
+      pick = i;
+      left = target - before;
+    }
+    before += s.slice_sum[i];
   }
-  s.bin = pick < 0 ? last : pick;  // u of 1 or more, or NaN: the last one
-  s.target = pick < 0 ? __builtin_huge_val() : target - before;
-  s.total = total;
-  s.scale = 1.;
+  const uint64_t found = __builtin_amdgcn_ballot_w64(pick >= 0);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
+  const int from = found ? __ffsll((unsigned long long)found) - 1 : 0;
+  pick = __shfl(pick, from, 64);
+  left = __shfl(left, from, 64);
+  if (lane == 0) {
+    s.bin = found ? pick : last;  // u of 1 or more, or NaN: the last one
+    s.target = found ? left : __builtin_huge_val();
+    s.total = total;
+    s.scale = 1.;
+  }
 }
 
-// A row by one work-group alone: see find_border.
+// A row whose border bins hold too many logits, by one work-group alone: see find_border.
 template <typename T>
-__device__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowOptions& o, const Weights& w, int slices,
-                         Shared& s) {
-  const int t = threadIdx.x;
+__global__ __launch_bounds__(kThreads) void slow_kernel(Args a, Space sp) {
+  __shared__ Shared s;
+  const int64_t r = blockIdx.x;
+  if (sp.n_cand[r] <= (uint32_t)kCandidates) return;
+  const int t = threadIdx.x, slices = sp.slices;
+  const RowOptions o(a, r);
+  const RowStats rs(sp.stats + r * slices, slices);
+  fill_table(s.table);
+  const Row<T> row(a.logits, a.ld, r, a.vocab);
+  const Weights w = weights_of(s.table, rs.top, rs.low, o.temp, a.fixed);
   Border border{key_of(-inf()), 0};
   if (o.by_k) {
     find_border<T, false>(row, w, (uint64_t)o.top_k, nullptr, s);
@@ -876,7 +916,7 @@ __device__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowO
         if (x[j] != -inf() && key_of(x[j]) > border.key) mass += w.fixed_of(x[j]);
     }
     uint64_t total;
-    block_prefix<uint64_t>(mass, s.wave_u, total);
+    block_prefix<kThreads, uint64_t>(mass, s.wave_u, total);
     if (border.ties) total += border.ties * w.fixed_of(of_key(border.key));
     // the smallest whole mass that is p times the total or more; at least the first element
     const double goal = ceil(o.top_p * (double)total);
@@ -907,8 +947,8 @@ __device__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowO
         }
       }
     }
-    m = block_sum(m, s);
-    if (tie_kept) ties = block_count(ties, s);
+    m = block_sum<kThreads, double>(m, s.wave_d);
+    if (tie_kept) ties = block_sum<kThreads, uint32_t>(ties, s.wave_c);
     if (t == 0) {
       s.slice_sum[i] = m;
       s.slice_add[i] = ties;
@@ -923,8 +963,9 @@ __device__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowO
       left -= n;
       s.slice_sum[i] += n * tie_weight;
     }
-    pick_slice(s, slices, o.u);
   }
+  __syncthreads();
+  if (t < 64) pick_slice(s, slices, o.u);
   __syncthreads();
   // the slice's first ties, by their rank in it
   const int slice = s.bin, g = slice * kThreads + t;
@@ -935,9 +976,9 @@ __device__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowO
 #pragma unroll
     for (int j = 0; j < kGroup; ++j) ties += x[j] == border_x;
   }
-  uint32_t all_ties, rank = block_prefix<uint32_t>(ties, s.wave_c, all_ties);
+  uint32_t all_ties, rank = block_prefix<kThreads, uint32_t>(ties, s.wave_c, all_ties);
   const uint32_t take = (uint32_t)s.slice_add[slice];
-  draw_token(a, r, row, slice, [&](float x, int) {
+  draw_token<T, kThreads>(a, r, row, slice, [&](float x, int) {
     if (above(x)) {
       const double y = w.of(x);
       return y >= o.min_p ? y : 0.;
@@ -947,12 +988,17 @@ __device__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowO
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void draw_kernel(Args a, Space sp) {
-  __shared__ Shared s;
+__global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
+  constexpr int N = kDrawThreads;
+  __shared__ Scratch<N> s;
   const int64_t r = blockIdx.x;
   const int t = threadIdx.x;
   const RowOptions o(a, r);
   const SliceStats* stats = sp.stats + r * sp.slices;
+  each<N>(sp.slices, [&](int i) {
+    s.slice_sum[i] = sp.sums[r * sp.slices + i];
+    s.slice_add[i] = 0;
+  });
   const RowStats rs(stats, sp.slices);
   if (rs.empty()) {  // nothing to draw
     if (t == 0) {
@@ -970,106 +1016,88 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Args a, Space sp) {
   }
   fill_table(s.table);
   const Row<T> row(a.logits, a.ld, r, a.vocab);
-  Weights w = weights_of(s.table, rs.top, rs.low, o.temp, a.fixed);
+  const Weights w = weights_of(s.table, rs.top, rs.low, o.temp, a.fixed);
   if (o.plain()) {
     // slices' sums are relative to their own maxima
-    each(sp.slices, [&](int i) { s.slice_sum[i] = sp.sums[r * sp.slices + i] * w.of(stats[i].top); });
+    each<N>(sp.slices, [&](int i) { s.slice_sum[i] *= w.of(stats[i].top); });
     __syncthreads();
-    if (t == 0) {
-      pick_slice(s, sp.slices, o.u);
-      s.scale = w.of(stats[s.bin].top);
-      s.target /= s.scale;
-    }
+    if (t < 64) pick_slice(s, sp.slices, o.u);
     __syncthreads();
     const float top = stats[s.bin].top;
-    w = weights_of(s.table, top, rs.low, o.temp, a.fixed);
-    draw_token(a, r, row, s.bin, [&](float x, int) { return w.of(x); }, s);
+    const double scale = w.of(top);
+    __syncthreads();
+    if (t == 0) {
+      s.scale = scale;
+      s.target /= scale;
+    }
+    __syncthreads();
+    const Weights v = weights_of(s.table, top, rs.low, o.temp, a.fixed);
+    draw_token<T, N>(a, r, row, s.bin, [&](float x, int) { return v.of(x); }, s);
     return;
   }
   uint64_t border = 0;  // the last kept (key, index); 0: no border
-  each(sp.slices, [&](int i) {
-    s.slice_sum[i] = sp.sums[r * sp.slices + i];
-    s.slice_add[i] = 0;
-  });
   if (o.by_k || o.by_p) {
     const Bins f = sp.bins[r];
-    const uint32_t have = sp.n_cand[r];
-    if (have > (uint32_t)kCandidates) {
-      slow_row<T>(a, r, row, o, w, sp.slices, s);
-      return;
-    }
+    const int have = (int)min(sp.n_cand[r], (uint32_t)kCandidates + 1);
+    if (have > kCandidates) return;  // slow_kernel's
     if (have) {
-      each((int)have, [&](int i) { s.cand[i] = sp.cand[r * kCandidates + i]; });
-      sort_candidates(s, (int)have);
-      // four candidates a thread: their bins, masses and prefix sums
-      constexpr int PER = kCandidates / kThreads;
-      uint64_t m[PER], ms = 0;
-      int b[PER];
-      uint32_t before_k = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const bool on = PER * t + i < (int)have;
-        const float x = on ? of_key((uint32_t)(s.cand[PER * t + i] >> 32)) : 0.f;
-        b[i] = on ? w.bin(x) : kBins;
-        m[i] = on ? w.fixed_of(x) : 0;
-        ms += m[i];
-        before_k += on && b[i] < f.k;
-      }
+      each<N>(have, [&](int i) { s.cand[i] = sp.cand[r * kCandidates + i]; });
+      sort_candidates<N>(s, have);
+      // a thread takes consecutive candidates
+      const int per = (have + N - 1) / N, b = min(have, per * t), e = min(have, b + per);
+      auto logit = [&](int i) { return of_key((uint32_t)(s.cand[i] >> 32)); };
       // the last of the first k: in bin k's group, which ends the candidates
-      int last = (int)have - 1;
+      int last = have - 1;
       uint64_t mass_k = 0;
-      uint64_t all;
-      const uint64_t m0 = block_prefix<uint64_t>(ms, s.wave_u, all);
       if (f.k < kBins) {
-        last = (int)block_count(before_k, s) + (int)(o.top_k - (int64_t)f.k_before) - 1;
-        uint64_t kept = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (b[i] == f.k && PER * t + i <= last) kept += m[i];
-        block_prefix<uint64_t>(kept, s.wave_u, mass_k);
-        mass_k += f.k_mass;
+        uint32_t before_k = 0;
+        for (int i = b; i < e; ++i) before_k += w.bin(logit(i)) < f.k;
+        before_k = block_sum<N, uint32_t>(before_k, s.wave_c);
+        last = (int)before_k + (int)(o.top_k - (int64_t)f.k_before) - 1;
+        if (o.by_p) {
+          uint64_t kept = 0;
+          for (int i = max(b, (int)before_k); i < min(e, last + 1); ++i) kept += w.fixed_of(logit(i));
+          mass_k = f.k_mass + block_sum<N, uint64_t>(kept, s.wave_u);
+        }
+      } else if (o.by_p) {  // the whole row's mass: the histogram's
+        uint64_t mine = 0;
+        each<N>(kBins, [&](int i) { mine += sp.mass[r * kBins + i]; });
+        mass_k = block_sum<N, uint64_t>(mine, s.wave_u);
       }
       if (o.by_p) {
         // p times the mass of the first k, reached in the bins [lo, hi], which begin the candidates
-        if (f.k >= kBins) {
-          // the whole row's mass: the histogram's
-          uint64_t mine = 0;
-          each(kBins, [&](int i) { mine += sp.mass[r * kBins + i]; });
-          block_prefix<uint64_t>(mine, s.wave_u, mass_k);
-        }
         const double goal = ceil(o.top_p * (double)mass_k);
         const uint64_t want = goal > 1. ? (uint64_t)goal : 1;
-        uint64_t run = m0 + f.lo_mass;
+        uint64_t mine = 0, all;
+        for (int i = b; i < e; ++i) mine += w.fixed_of(logit(i));
+        uint64_t run = block_prefix<N, uint64_t>(mine, s.wave_u, all) + f.lo_mass;
         if (t == 0) s.bin = last;  // where p times the mass rounds past it
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          if (run < want && run + m[i] >= want) s.bin = PER * t + i;  // one element
-          run += m[i];
+        for (int i = b; i < e; ++i) {
+          const uint64_t next = run + w.fixed_of(logit(i));
+          if (run < want && next >= want) s.bin = i;  // one element
+          run = next;
         }
         __syncthreads();
         last = s.bin;
       }
       border = s.cand[last];
       // the kept candidates' mass, by slice
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = PER * t + i;
-        if (at > last) continue;
-        const float x = of_key((uint32_t)(s.cand[at] >> 32));
+      for (int i = b; i < min(e, last + 1); ++i) {
+        const float x = logit(i);
         if (!(w.of(x) >= o.min_p)) continue;
-        const int idx = (int)(0xffffffffu - (uint32_t)s.cand[at]);
-        atomicAdd((unsigned long long*)&s.slice_add[(idx + row.lead) / kSlice], (unsigned long long)m[i]);
+        const int idx = (int)(0xffffffffu - (uint32_t)s.cand[i]);
+        atomicAdd((unsigned long long*)&s.slice_add[(idx + row.lead) / kSlice], (unsigned long long)w.fixed_of(x));
       }
     }
   }
   __syncthreads();
-  if (t == 0) {
-    for (int i = 0; i < sp.slices; ++i) s.slice_sum[i] += (double)s.slice_add[i] / a.fixed;
-    pick_slice(s, sp.slices, o.u);
-  }
+  const double unit = 1. / a.fixed;  // a power of two
+  each<N>(sp.slices, [&](int i) { s.slice_sum[i] += (double)s.slice_add[i] * unit; });
   __syncthreads();
-  draw_token(a, r, row, s.bin, [&](float x, int i) {
+  if (t < 64) pick_slice(s, sp.slices, o.u);
+  __syncthreads();
+  draw_token<T, N>(a, r, row, s.bin, [&](float x, int i) {
     const uint64_t me = ((uint64_t)key_of(x) << 32) | (0xffffffffu - (uint32_t)i);
     if (me < border) return 0.;
     const double y = w.of(x);
@@ -1125,8 +1153,14 @@ void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bin
     TimedLaunch timed_("sampling.gather_kernel", s);
     hipLaunchKernelGGL(gather_kernel<T>, parts, block, 0, s, a, sp);
   }
-  TimedLaunch timed_("sampling.draw_kernel", s);
-  hipLaunchKernelGGL(draw_kernel<T>, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp);
+  {
+    TimedLaunch timed_("sampling.draw_kernel", s);
+    hipLaunchKernelGGL(draw_kernel<T>, dim3((unsigned)rows), dim3(kDrawThreads), 0, s, a, sp);
+  }
+  if (bins) {
+    TimedLaunch timed_("sampling.slow_kernel", s);
+    hipLaunchKernelGGL(slow_kernel<T>, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp);
+  }
 }
 
 }  // namespace sample
