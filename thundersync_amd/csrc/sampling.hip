@@ -8,16 +8,16 @@
 //
 // Every filter keeps a prefix of the order, so a row's kept set is "logits above a border
 // element, and those that equal it up to its index".  The border is found by counting, not
-// by sorting the row.  A row is cut into slices of kSlice logits, and up to four launches of
+// by sorting the row.  A row is cut into slices of kSlice logits, and up to five launches of
 // work-groups over (rows x slices) work on it:
 //   maxima   each slice's maximum, minimum, NaN; without filters also its sum of weights
 //   bins     a histogram (count and mass) of the row over kBins bins of logit below its maximum
-//   gather   the bins that the borders fall into, their logits as candidates; per slice the
-//            sum of the weights above them
+//   search   the bins that the borders fall into
+//   gather   their logits as candidates; per slice the sum of the weights above them
 //   draw     one work-group a row: sorts the candidates in LDS, finds the border, picks the
 //            slice that u falls into and reads that slice again for the token
 // A row with more than kCandidates logits in its border bins (equal logits, or very many in a
-// narrow range) is left to one work-group of a fifth launch, which narrows the range bin by bin.
+// narrow range) is resolved by its draw work-group alone, which narrows the range bin by bin.
 //
 // A token depends on a border of the running sum, and the tail's weights are far below fp32's
 // rounding of the sum: weights are fp64, sums over bins exact integers of 2^-scale (order-free),
@@ -32,17 +32,16 @@
 namespace ts {
 namespace sample {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;  // a slow row
-constexpr int kDrawThreads = 256;
+constexpr int kMaxThreads = 256;                // maxima
+constexpr int kThreads = 512;                  // bins and gather: few work-groups a row, each pays the histogram
+constexpr int kDrawThreads = 512;              // draw
 constexpr int kGroup = 8;                      // consecutive logits per thread and step
 constexpr int kBins = 2048;
 constexpr float kBinsPerOctave = 32.f;         // kBins / 64 octaves
 constexpr int kCandidates = 4096;              // logits sorted in LDS
 constexpr int kMaxVocab = 1 << 21;
-constexpr int kSlice = kThreads * kGroup;      // logits per slice
+constexpr int kSliceGroups = 1024, kSlice = kSliceGroups * kGroup;  // logits per slice
 constexpr int kMaxSlices = kMaxVocab / kSlice + 1;
-constexpr int kPartThreads = 256;              // maxima, bins, gather
-constexpr int kPartGroups = kSlice / kGroup / kPartThreads;  // a thread's groups of a slice
 
 struct Options {       // a value for every row, or one per row
   const float* temperature;
@@ -78,8 +77,14 @@ template <typename T> struct Row {
     groups = (vocab + lead + kGroup - 1) / kGroup;
   }
   __device__ __forceinline__ int first(int g) const { return g * kGroup - lead; }
-  // logits of group g, -inf outside the row
+  // logits of group g, -inf outside the row; -0 and 0 are one logit
   __device__ __forceinline__ void load(int g, float (&x)[kGroup]) const {
+    load_raw(g, x);
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) x[j] += 0.f;
+  }
+  // the same without the zeros' care: for sums and maxima
+  __device__ __forceinline__ void load_raw(int g, float (&x)[kGroup]) const {
     const int i0 = first(g);
     if (i0 >= 0 && i0 + kGroup <= vocab) {
       load8(z + i0, x);
@@ -87,9 +92,6 @@ template <typename T> struct Row {
 #pragma unroll
       for (int j = 0; j < kGroup; ++j) x[j] = i0 + j >= 0 && i0 + j < vocab ? to_f(z[i0 + j]) : -inf();
     }
-    // -0 and 0 are one logit
-#pragma unroll
-    for (int j = 0; j < kGroup; ++j) x[j] += 0.f;
   }
 };
 
@@ -102,10 +104,23 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 2^(j / kTable) for j in [0, kTable), in LDS
+// 2^(j / kTable) for j in [0, kTable), worked out by the compiler: the exponential's series
+// of j ln 2 / kTable, whose terms fall below 2^-60 by the 20th, summed from the smallest
 constexpr int kTable = 256;
+struct Table {
+  double at[kTable];
+  constexpr Table() : at{} {
+    for (int j = 0; j < kTable; ++j) {
+      const double x = 0.693147180559945309417 * j / kTable;
+      double s = 1.;
+      for (int k = 20; k >= 1; --k) s = 1. + s * x / k;
+      at[j] = s;
+    }
+  }
+};
+__constant__ const Table kPowers = Table();
 __device__ __forceinline__ void fill_table(double* table) {
-  for (int j = threadIdx.x; j < kTable; j += blockDim.x) table[j] = exp2((double)j / kTable);
+  for (int j = threadIdx.x; j < kTable; j += blockDim.x) table[j] = kPowers.at[j];
   __syncthreads();
 }
 
@@ -122,8 +137,8 @@ struct Weights {
   float top_f;
   float bins;     // bins per unit of logit
   bool simple;    // top and units are finite
-  // of a logit above -inf (-inf: 2^-1000)
-  __device__ __forceinline__ double of_finite(float x) const {
+  // where `simple`; -inf gives 2^-1000, which adds nothing to a sum that holds the maximum's 1
+  __device__ __forceinline__ double of_simple(float x) const {
     constexpr double kRound = 6755399441055744., kL = 0.693147180559945309417 / kTable;
     const double y = fmax(((double)x - top) * units, -1000. * kTable);
     const double k = y + kRound;
@@ -131,20 +146,24 @@ struct Weights {
     const double e = fma(fma(fma(fma(t, kL * kL * kL * kL / 24, kL * kL * kL / 6), t, kL * kL / 2), t, kL), t, 1.);
     const int n = __double2loint(k);
     const double p = table[n & (kTable - 1)] * e;
-    return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+    return __hiloint2double(__double2hiint(p) + ((n & -kTable) << 12), __double2loint(p));
   }
   __device__ __forceinline__ double of(float x) const {
     if (x == top_f) return 1.;
     if (x == -inf() || top_f == inf()) return 0.;
     if (!simple) return units > 0. ? 0. : 1.;  // T so small, or so large, that nothing is between
-    return ((double)x - top) * units < -1000. * kTable ? 0. : of_finite(x);
+    return ((double)x - top) * units < -1000. * kTable ? 0. : of_simple(x);
   }
-  __device__ __forceinline__ uint64_t fixed_of(float x) const { return (uint64_t)(of(x) * fixed + 0.5); }
+  // a weight as a whole number of 1 / fixed (at most 2^50), by an addition whose rounding leaves it in the low bits
+  __device__ __forceinline__ uint64_t whole(double weight) const {
+    const double y = fma(weight, fixed, 4503599627370496.);
+    return ((uint64_t)(__double2hiint(y) & 0xfffff) << 32) | (uint32_t)__double2loint(y);
+  }
+  __device__ __forceinline__ uint64_t fixed_of(float x) const { return whole(of(x)); }
   // falls with the logit, equal for equal logits
   __device__ __forceinline__ int bin(float x) const {
-    if (x == top_f) return 0;
-    const float b = (top_f - x) * bins;
-    return b < (float)(kBins - 1) ? (int)b : kBins - 1;
+    const int b = (int)fminf((top_f - x) * bins, (float)(kBins - 1));
+    return x == top_f ? 0 : b;
   }
 };
 // `low`: the row's lowest finite logit, so that the bins cover no more than there is
@@ -157,7 +176,7 @@ __device__ __forceinline__ Weights weights_of(const double* table, float top, fl
   w.fixed = fixed;
   w.simple = top < inf() && w.units > 0. && w.units < __builtin_huge_val();
   const float octave = (float)(0.693147180559945309 * temp);  // in units of logit
-  w.bins = fmaxf(kBinsPerOctave / octave, (float)kBins / (top - low));
+  w.bins = fminf(fmaxf(kBinsPerOctave / octave, (float)kBins / (top - low)), 1e30f);
   return w;
 }
 
@@ -170,8 +189,13 @@ struct Border {
 
 // What a work-group of N threads that draws a row's token holds.
 template <int N> struct Scratch {
-  static constexpr int kN = N;
-  uint64_t cand[kCandidates];
+  union {
+    uint64_t cand[kCandidates];
+    struct {  // find_border's, before it gathers candidates
+      uint64_t mass[kBins];
+      uint32_t count[kBins];
+    };
+  };
   double slice_sum[kMaxSlices];
   uint64_t slice_add[kMaxSlices];  // candidates' kept mass, or (slow rows) ties
   double table[kTable];
@@ -180,14 +204,8 @@ template <int N> struct Scratch {
   uint32_t wave_c[N / 64];
   int bin, n_cand, token;
   double total, target, scale;
-};
-// and one that finds a border by itself
-struct Shared : Scratch<kThreads> {
-  uint32_t count[kBins];
-  uint64_t mass[kBins];
-  uint32_t lo, hi;
+  uint32_t lo, hi, before_count;
   uint64_t before_mass;
-  uint32_t before_count;
   Border border;
 };
 
@@ -231,8 +249,37 @@ template <int N, typename V> __device__ __forceinline__ V block_prefix(V x, V* p
   return lane ? before + prev : before;
 }
 
-// falling order of s.cand[0 .. have), padded with zeros to a power of two of at least 64
-template <int N> __device__ void sort_candidates(Scratch<N>& s, int have) {
+// s.cand[0 .. have) (all different) into falling order.  Few: each one's place is the number of
+// larger ones, counted by a thread that reads them all (480 in 256 threads: one step of 2 x 480
+// comparisons against 45 steps of the sorting network, each with its barrier).  Many: the
+// network, over a power of two padded with zeros.
+constexpr int kCounted = 1024;
+template <int N> __device__ __forceinline__ void sort_candidates(Scratch<N>& s, int have) {
+  if (have <= kCounted) {
+    constexpr int PER = kCounted / N;
+    uint64_t mine[PER];
+    int place[PER] = {};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine[i] = (int)threadIdx.x + N * i < have ? s.cand[threadIdx.x + N * i] : 0;
+    if (threadIdx.x == 0 && (have & 1)) s.cand[have] = 0;  // read in pairs; counts for nothing
+    __syncthreads();
+    auto count = [&](auto used) {
+#pragma unroll 8
+      for (int j = 0; j < have; j += 2) {
+        const uint64_t a = s.cand[j], c = s.cand[j + 1];
+#pragma unroll
+        for (int i = 0; i < decltype(used)::value; ++i) place[i] += (a > mine[i]) + (c > mine[i]);
+      }
+    };
+    if (have <= N) count(std::integral_constant<int, 1>{});
+    else count(std::integral_constant<int, PER>{});
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if ((int)threadIdx.x + N * i < have) s.cand[place[i]] = mine[i];
+    __syncthreads();
+    return;
+  }
   int size = 64;
   while (size < have) size *= 2;
   each<N>(size - have, [&](int i) { s.cand[have + i] = 0; });
@@ -255,8 +302,8 @@ template <int N> __device__ void sort_candidates(Scratch<N>& s, int have) {
 // Where the running count (BY_MASS false: the first `want` elements) or the running mass
 // (the first elements whose predecessors weigh less than `want`) ends, among the logits
 // above `limit` and its first ties.
-template <typename T, bool BY_MASS>
-__device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, const Border* limit, Shared& s) {
+template <typename T, int N, bool BY_MASS>
+__device__ __forceinline__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, const Border* limit, Scratch<N>& s) {
   const uint32_t limit_key = limit ? limit->key : 0;
   const uint32_t limit_ties = limit ? (uint32_t)limit->ties : 0;
   const bool limited = limit != nullptr;
@@ -273,12 +320,12 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
     return k >= lo && k <= hi && w.bin(x) == bin0 ? (int)((hi - k) >> shift) : -1;
   };
   while (true) {
-    each<kThreads>(kBins, [&](int b) {
+    each<N>(kBins, [&](int b) {
       s.count[b] = 0;
       s.mass[b] = 0;
     });
     __syncthreads();
-    for (int g = threadIdx.x; g < row.groups; g += kThreads) {
+    for (int g = threadIdx.x; g < row.groups; g += N) {
       float x[kGroup];
       row.load(g, x);
 #pragma unroll
@@ -301,14 +348,17 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
       }
     }
     __syncthreads();
-    // the first bin in which the wanted amount is reached: two bins a thread
+    // the first bin in which the wanted amount is reached: consecutive bins a thread
+    constexpr int BINS = kBins / N;
     const int t = threadIdx.x;
-    const uint32_t c0 = s.count[2 * t], c1 = s.count[2 * t + 1];
-    const uint64_t m0 = s.mass[2 * t], m1 = s.mass[2 * t + 1];
-    uint32_t total_c;
-    uint64_t total_m;
-    const uint32_t pc = block_prefix<kThreads, uint32_t>(c0 + c1, s.wave_c, total_c) + before_count;
-    const uint64_t pm = block_prefix<kThreads, uint64_t>(m0 + m1, s.wave_u, total_m) + before_mass;
+    uint32_t c = 0, total_c;
+    uint64_t m = 0, total_m;
+    for (int i = 0; i < BINS; ++i) {
+      c += s.count[BINS * t + i];
+      m += s.mass[BINS * t + i];
+    }
+    c = block_prefix<N, uint32_t>(c, s.wave_c, total_c) + before_count;
+    m = block_prefix<N, uint64_t>(m, s.wave_u, total_m) + before_mass;
     if (t == 0) {
       s.bin = -1;
       s.lo = 0xffffffffu;
@@ -316,17 +366,18 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
       s.n_cand = 0;
     }
     __syncthreads();
-    // reached in a bin: its end is at or past the wanted amount, its start is not
-    auto reached = [&](uint64_t at, uint64_t end, uint32_t n) { return n > 0 && at < want && end >= want; };
-    const uint64_t at0 = BY_MASS ? pm : pc, at1 = BY_MASS ? pm + m0 : pc + c0, at2 = BY_MASS ? pm + m0 + m1 : pc + c0 + c1;
-    if (reached(at0, at1, c0)) {
-      s.bin = 2 * t;
-      s.before_mass = pm;
-      s.before_count = pc;
-    } else if (reached(at1, at2, c1)) {
-      s.bin = 2 * t + 1;
-      s.before_mass = pm + m0;
-      s.before_count = pc + c0;
+    for (int i = 0; i < BINS; ++i) {
+      const uint32_t cb = s.count[BINS * t + i];
+      const uint64_t mb = s.mass[BINS * t + i];
+      // reached in this bin: its end is at or past the wanted amount, its start is not
+      const uint64_t at = BY_MASS ? m : c, end = BY_MASS ? m + mb : c + cb;
+      if (cb > 0 && at < want && end >= want) {
+        s.bin = BINS * t + i;
+        s.before_mass = m;
+        s.before_count = c;
+      }
+      c += cb;
+      m += mb;
     }
     __syncthreads();
     if (s.bin < 0) {
@@ -339,9 +390,10 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
     const uint32_t n = s.count[b];
     before_mass = s.before_mass;
     before_count = s.before_count;
+    __syncthreads();  // the candidates take the histogram's place
     if (n <= (uint32_t)kCandidates) {
       // gather the bin's logits, sort them, walk them
-      for (int g = threadIdx.x; g < row.groups; g += kThreads) {
+      for (int g = threadIdx.x; g < row.groups; g += N) {
         float x[kGroup];
         row.load(g, x);
 #pragma unroll
@@ -356,49 +408,38 @@ __device__ void find_border(const Row<T>& row, const Weights& w, uint64_t want, 
       if (limited && bin_of(of_key(limit_key), limit_key) == b) {
         // the limit's ties, the last of the bin: one index is as good as another
         const int at = s.n_cand;
-        each<kThreads>((int)limit_ties, [&](int i) { s.cand[at + i] = ((uint64_t)limit_key << 32) | (0xffffffffu - (uint32_t)i); });
+        each<N>((int)limit_ties, [&](int i) { s.cand[at + i] = ((uint64_t)limit_key << 32) | (0xffffffffu - (uint32_t)i); });
         __syncthreads();
         if (t == 0) s.n_cand = at + (int)limit_ties;
         __syncthreads();
       }
       const int have = s.n_cand;
-      sort_candidates<kThreads>(s, have);
-      // the position of the border's element: four candidates a thread, by prefix sums
-      constexpr int PER = kCandidates / kThreads;
-      uint64_t mine = 0, sum = 0;
-      uint64_t part[PER];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = PER * t + i;
-        part[i] = at < have ? (BY_MASS ? w.fixed_of(of_key((uint32_t)(s.cand[at] >> 32))) : 1) : 0;
-        sum += part[i];
-      }
-      uint64_t total;
-      mine = block_prefix<kThreads, uint64_t>(sum, s.wave_u, total) + (BY_MASS ? before_mass : before_count);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = PER * t + i;
-        if (at < have && mine < want && mine + part[i] >= want) s.bin = at;  // one element
-        mine += part[i];
+      sort_candidates<N>(s, have);
+      // the position of the border's element: consecutive candidates a thread, by prefix sums
+      const int per = (have + N - 1) / N, first = min(have, per * t), end = min(have, first + per);
+      auto part = [&](int i) { return BY_MASS ? w.fixed_of(of_key((uint32_t)(s.cand[i] >> 32))) : (uint64_t)1; };
+      uint64_t mine = 0, total;
+      for (int i = first; i < end; ++i) mine += part(i);
+      mine = block_prefix<N, uint64_t>(mine, s.wave_u, total) + (BY_MASS ? before_mass : before_count);
+      for (int i = first; i < end; ++i) {
+        const uint64_t next = mine + part(i);
+        if (mine < want && next >= want) s.bin = i;  // one element
+        mine = next;
       }
       __syncthreads();
       // its key and how many of that key's elements come up to it
       const int last = s.bin;
       const uint32_t key = (uint32_t)(s.cand[last] >> 32);
       uint32_t ties = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = PER * t + i;
-        ties += at <= last && (uint32_t)(s.cand[at] >> 32) == key;
-      }
-      ties = block_sum<kThreads, uint32_t>(ties, s.wave_c);
+      for (int i = first; i < min(end, last + 1); ++i) ties += (uint32_t)(s.cand[i] >> 32) == key;
+      ties = block_sum<N, uint32_t>(ties, s.wave_c);
       if (t == 0) s.border = Border{key, (int)ties};
       __syncthreads();
       return;
     }
     // too many: the range of keys in the bin
     uint32_t kmin = 0xffffffffu, kmax = 0;
-    for (int g = threadIdx.x; g < row.groups; g += kThreads) {
+    for (int g = threadIdx.x; g < row.groups; g += N) {
       float x[kGroup];
       row.load(g, x);
 #pragma unroll
@@ -460,27 +501,31 @@ struct RowOptions {
   __device__ __forceinline__ bool plain() const { return !greedy && !by_k && !by_p && !by_min; }
 };
 
+constexpr int kSums = kThreads / 64;
+constexpr int kBinParts = 8;  // work-groups a row for its histogram, at most
+
 struct SliceStats {
   float top, low;  // -inf / +inf: no logit above -inf
   int at;          // first index of the maximum
   int nan;
 };
 
-// Per row, written by the first gather work-group: the bins that hold the borders.
+// Per row: the bins that hold the borders.
 struct Bins {
   int lo, hi, k;          // border of p in [lo, hi], of k in k (or lo = hi = k, or none: kBins)
   uint32_t k_before;      // elements above bin k
   uint64_t k_mass, lo_mass;  // mass above bins k and lo
+  uint64_t all_mass;
 };
 
 // The launches' workspace, of `rows` rows and `slices` slices.  From `bins` on only where some
 // row of the call has a top_k or top_p: null otherwise.
 struct Space {
   SliceStats* stats;  // [rows][slices]
-  double* sums;       // [rows][slices]
+  double* sums;       // [rows][slices][kSums]: of a slice's waves (without filters the first alone)
   Bins* bins;         // [rows]
-  uint64_t* mass;     // [rows][kBins]
-  uint32_t* count;    // [rows][kBins]
+  uint64_t* mass;     // [rows][kBinParts][kBins]
+  uint32_t* count;    // [rows][kBinParts][kBins]
   uint64_t* cand;     // [rows][kCandidates]
   uint32_t* n_cand;   // [rows]
   int slices;
@@ -522,50 +567,54 @@ struct RowStats {
   __device__ __forceinline__ bool empty() const { return nan || top == -inf(); }
 };
 
-constexpr int kPartWaves = kPartThreads / 64;
-
 // ---------------------------------------------------------------------------
 // maxima: one slice, held in registers; a row without filters gets its slice's sum of
 // weights, relative to the slice's own maximum, from the same read
 // ---------------------------------------------------------------------------
-template <typename T, bool CLEAR>
-__global__ __launch_bounds__(kPartThreads, 5) void maxima_kernel(Args a, Space sp) {
-  __shared__ double table[kTable], per_wave[kPartWaves];
-  __shared__ float tops[kPartWaves], lows[kPartWaves];
-  __shared__ int ats[kPartWaves];
+template <typename T, bool BINS>
+__global__ __launch_bounds__(kMaxThreads, 5) void maxima_kernel(Args a, Space sp) {
+  constexpr int N = kMaxThreads, WAVES = N / 64, GROUPS = kSliceGroups / N;
+  __shared__ double table[kTable], per_wave[WAVES];
+  __shared__ float tops[WAVES], lows[WAVES];
+  __shared__ int ats[WAVES];
   const int64_t r = blockIdx.y;
   const int slice = blockIdx.x, t = threadIdx.x;
-  if (CLEAR) {  // the histogram that the next launch adds to
-    for (int i = slice * kPartThreads + t; i < kBins; i += sp.slices * kPartThreads) {
-      sp.mass[r * kBins + i] = 0;
-      sp.count[r * kBins + i] = 0;
-    }
-    if (slice == 0 && t == 0) sp.n_cand[r] = 0;
-  }
+  if (BINS && slice == 0 && t == 0) sp.n_cand[r] = 0;
   const RowOptions o(a, r);
   const Row<T> row(a.logits, a.ld, r, a.vocab);
-  float x[kPartGroups][kGroup];
+  float x[GROUPS][kGroup];
   float top = -inf(), low = inf();
-  int at = 0x7fffffff;
   bool nan = false;
 #pragma unroll
-  for (int i = 0; i < kPartGroups; ++i) {
-    const int g = slice * (kSlice / kGroup) + i * kPartThreads + t;
+  for (int i = 0; i < GROUPS; ++i) {
+    const int g = slice * kSliceGroups + i * N + t;
     if (g < row.groups) {
-      row.load(g, x[i]);
+      row.load_raw(g, x[i]);
     } else {
 #pragma unroll
       for (int j = 0; j < kGroup; ++j) x[i][j] = -inf();
     }
+  }
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
     for (int j = 0; j < kGroup; ++j) {
       nan |= x[i][j] != x[i][j];
-      if (x[i][j] > top) {
-        top = x[i][j];
-        at = row.first(g) + j;
-      }
-      if (x[i][j] > -inf()) low = fminf(low, x[i][j]);
+      top = fmaxf(top, x[i][j]);
     }
+  if (BINS) {  // the bins' range
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) low = fminf(low, x[i][j] == -inf() ? inf() : x[i][j]);
+  }
+  int at = 0x7fffffff;
+  if (o.greedy) {  // the first index of the thread's maximum
+#pragma unroll
+    for (int i = GROUPS - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = kGroup - 1; j >= 0; --j)
+        if (x[i][j] == top) at = row.first(slice * kSliceGroups + i * N + t) + j;
   }
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) {
@@ -584,7 +633,7 @@ __global__ __launch_bounds__(kPartThreads, 5) void maxima_kernel(Args a, Space s
   }
   const bool any = __syncthreads_or(nan);
 #pragma unroll
-  for (int w = 0; w < kPartWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     if (tops[w] > top || (tops[w] == top && ats[w] < at)) {
       top = tops[w];
       at = ats[w];
@@ -594,33 +643,35 @@ __global__ __launch_bounds__(kPartThreads, 5) void maxima_kernel(Args a, Space s
   if (t == 0) sp.stats[r * sp.slices + slice] = SliceStats{top, low, at, any};
   if (!o.plain()) return;
   if (any || top == -inf()) {
-    if (t == 0) sp.sums[r * sp.slices + slice] = 0.;
+    if (t == 0) sp.sums[(r * sp.slices + slice) * kSums] = 0.;
     return;
   }
   fill_table(table);
   const Weights w = weights_of(table, top, low, o.temp, a.fixed);
   double sum = 0.;
-  if (w.simple) {  // 2^-1000 for a logit of -inf adds nothing to a sum of 1 or more
+  if (w.simple) {
 #pragma unroll
-    for (int i = 0; i < kPartGroups; ++i)
+    for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-      for (int j = 0; j < kGroup; ++j) sum += w.of_finite(x[i][j]);
+      for (int j = 0; j < kGroup; ++j) sum += w.of_simple(x[i][j]);
   } else {
-#pragma unroll 1
-    for (int i = 0; i < kPartGroups; ++i)
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
       for (int j = 0; j < kGroup; ++j) sum += w.of(x[i][j]);
   }
-  sum = block_sum<kPartThreads, double>(sum, per_wave);
-  if (t == 0) sp.sums[r * sp.slices + slice] = sum;
+  sum = block_sum<N, double>(sum, per_wave);
+  if (t == 0) sp.sums[(r * sp.slices + slice) * kSums] = sum;
 }
 
 // ---------------------------------------------------------------------------
-// bins: a work-group's share of the slices into a histogram in LDS, then into the row's:
-// counts where top_k asks for them, mass where top_p does.  Bound by the LDS atomics.
+// bins: a work-group's share of the row into a histogram of its own, counts where top_k
+// asks for them and mass where top_p does.  (Shares added to one histogram by atomics, or added
+// up by every gather work-group, cost as much as the logits; a last work-group that adds them
+// waits for the XCDs' caches to be written back.)  Bound by the weights' instructions.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kPartThreads) void bins_kernel(Args a, Space sp) {
+__global__ __launch_bounds__(kThreads) void bins_kernel(Args a, Space sp) {
   __shared__ double table[kTable];
   __shared__ uint32_t count[kBins];
   __shared__ uint64_t mass[kBins];
@@ -630,177 +681,220 @@ __global__ __launch_bounds__(kPartThreads) void bins_kernel(Args a, Space sp) {
   if (!o.by_k && !o.by_p) return;
   const RowStats s(sp.stats + r * sp.slices, sp.slices);
   if (s.empty()) return;
-  for (int i = t; i < kBins; i += kPartThreads) {
+  for (int i = t; i < kBins; i += kThreads) {
     count[i] = 0;
     mass[i] = 0;
   }
   fill_table(table);
   const Weights w = weights_of(table, s.top, s.low, o.temp, a.fixed);
   const Row<T> row(a.logits, a.ld, r, a.vocab);
-  for (int g = blockIdx.x * kPartThreads + t; g < row.groups; g += gridDim.x * kPartThreads) {
-    float x[kGroup];
-    row.load(g, x);
+  // no branch in a group's eight, so that their chains overlap: -inf falls into the last bin with nothing
+  auto fill = [&](auto weight) __attribute__((always_inline)) {
+    for (int g = blockIdx.x * kThreads + t; g < row.groups; g += gridDim.x * kThreads) {
+      float x[kGroup];
+      row.load_raw(g, x);
+      int b[kGroup];
 #pragma unroll
-    for (int j = 0; j < kGroup; ++j) {
-      if (x[j] == -inf()) continue;
-      const int b = w.bin(x[j]);
-      if (o.by_k) atomicAdd(&count[b], 1u);
-      if (o.by_p) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w.fixed_of(x[j]));
+      for (int j = 0; j < kGroup; ++j) b[j] = w.bin(x[j]);
+      if (o.by_k) {
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) atomicAdd(&count[b[j]], x[j] == -inf() ? 0u : 1u);
+      }
+      if (o.by_p) {
+        uint64_t m[kGroup];
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) m[j] = w.whole(weight(x[j]));
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) atomicAdd((unsigned long long*)&mass[b[j]], (unsigned long long)m[j]);
+      }
     }
-  }
+  };
+  if (w.simple) fill([&](float x) { return w.of_simple(x); });
+  else fill([&](float x) { return w.of(x); });
   __syncthreads();
-  for (int i = t; i < kBins; i += kPartThreads) {
-    if (count[i]) atomicAdd(&sp.count[r * kBins + i], count[i]);
-    if (mass[i]) atomicAdd((unsigned long long*)&sp.mass[r * kBins + i], (unsigned long long)mass[i]);
+  const int64_t base = (r * kBinParts + blockIdx.x) * kBins;
+  for (int i = t; i < kBins; i += kThreads) {
+    if (o.by_k) sp.count[base + i] = count[i];
+    if (o.by_p) sp.mass[base + i] = mass[i];
   }
 }
 
 // ---------------------------------------------------------------------------
-// gather: every work-group of a row finds the border bins from its histogram (2048 bins,
-// eight a thread), then goes through its slices
+// search: the border bins from a row's shares of the histogram, consecutive bins a thread
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int parts) {
+  __shared__ uint64_t wave_m[kThreads / 64];
+  __shared__ uint32_t wave_c[kThreads / 64];
+  __shared__ Bins found;
+  __shared__ uint64_t bin_mass;  // of bin k
+  constexpr int PER = kBins / kThreads;
+  const int64_t r = blockIdx.x;
+  const int t = threadIdx.x;
+  const RowOptions o(a, r);
+  if (!o.by_k && !o.by_p) return;
+  if (RowStats(sp.stats + r * sp.slices, sp.slices).empty()) return;  // it has no histogram
+  const uint32_t* count = sp.count + r * kBinParts * kBins;
+  const uint64_t* mass = sp.mass + r * kBinParts * kBins;
+  if (t == 0) found = Bins{kBins, kBins, kBins, 0, 0, 0, 0};
+  uint32_t c[PER] = {}, cs = 0;
+  uint64_t m[PER] = {}, ms = 0;
+  // all loads before the first use: other XCDs wrote them (past the shares, the last again)
+  uint32_t cp[kBinParts][PER] = {};
+  uint64_t mp[kBinParts][PER] = {};
+#pragma unroll
+  for (int part = 0; part < kBinParts; ++part) {
+    const int64_t base = min(part, parts - 1) * kBins + PER * t;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (o.by_k) cp[part][i] = count[base + i];
+      if (o.by_p) mp[part][i] = mass[base + i];
+    }
+  }
+#pragma unroll
+  for (int part = 0; part < kBinParts; ++part)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] += part < parts ? cp[part][i] : 0;
+      m[i] += part < parts ? mp[part][i] : 0;
+    }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    cs += c[i];
+    ms += m[i];
+  }
+  uint32_t all_c;
+  uint64_t all_m;
+  const uint32_t c0 = block_prefix<kThreads, uint32_t>(cs, wave_c, all_c);
+  const uint64_t m0 = block_prefix<kThreads, uint64_t>(ms, wave_m, all_m);
+  if (t == 0) found.all_mass = all_m;
+  const bool cut = o.by_k && (uint64_t)o.top_k < all_c;  // else there are no more than k
+  if (cut) {
+    uint32_t cc = c0;
+    uint64_t mm = m0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (cc < (uint64_t)o.top_k && cc + c[i] >= (uint64_t)o.top_k) {
+        found.k = PER * t + i;
+        found.k_before = cc;
+        found.k_mass = mm;
+        bin_mass = m[i];
+        if (!o.by_p) {
+          found.lo = found.hi = found.k;
+          found.lo_mass = mm;
+        }
+      }
+      cc += c[i];
+      mm += m[i];
+    }
+  }
+  __syncthreads();
+  if (o.by_p) {
+    // p times the mass of the first k: between what is above bin k and that with all of bin k
+    uint64_t most = all_m, least = all_m;
+    if (cut) {
+      least = found.k_mass;
+      most = least + bin_mass;
+    }
+    auto goal = [&](uint64_t total) {
+      const double x = ceil(o.top_p * (double)total);
+      return x > 1. ? (uint64_t)x : (uint64_t)1;
+    };
+    const uint64_t lo = goal(least), hi = goal(most);
+    uint64_t mm = m0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (mm < lo && mm + m[i] >= lo) {
+        found.lo = PER * t + i;
+        found.lo_mass = mm;
+      }
+      if (mm < hi && mm + m[i] >= hi) found.hi = PER * t + i;
+      mm += m[i];
+    }
+    __syncthreads();
+  }
+  if (t == 0) sp.bins[r] = found;
+}
+
+// ---------------------------------------------------------------------------
+// gather: per slice the sum of the weights above the border bins, and their logits
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kPartThreads) void gather_kernel(Args a, Space sp) {
-  __shared__ double table[kTable], per_wave[kPartWaves];
-  __shared__ uint64_t wave_m[kPartWaves];
-  __shared__ uint32_t wave_c[kPartWaves];
-  __shared__ Bins found;
+__global__ __launch_bounds__(kThreads) void gather_kernel(Args a, Space sp) {
+  __shared__ double table[kTable];
+  __shared__ uint64_t cand[kCandidates];
+  __shared__ uint32_t n_cand, cand_at;
   const int64_t r = blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const RowOptions o(a, r);
   if (o.greedy || o.plain()) return;
   const RowStats s(sp.stats + r * sp.slices, sp.slices);
   if (s.empty()) return;
-  if (t == 0) found = Bins{kBins, kBins, kBins, 0, 0, 0};
+  if (t == 0) n_cand = 0;
   fill_table(table);
   const Weights w = weights_of(table, s.top, s.low, o.temp, a.fixed);
-  if (o.by_k || o.by_p) {
-    constexpr int PER = kBins / kPartThreads;
-    uint32_t c[PER], cs = 0;
-    uint64_t m[PER], ms = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      c[i] = sp.count[r * kBins + PER * t + i];
-      m[i] = sp.mass[r * kBins + PER * t + i];
-      cs += c[i];
-      ms += m[i];
-    }
-    // exclusive prefix sums over the threads
-    uint32_t ci = cs;
-    uint64_t mi = ms;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t cy = __shfl_up(ci, d, 64);
-      const uint64_t my = __shfl_up(mi, d, 64);
-      if (lane >= d) {
-        ci += cy;
-        mi += my;
-      }
-    }
-    if (lane == 63) {
-      wave_c[wave] = ci;
-      wave_m[wave] = mi;
-    }
-    __syncthreads();
-    uint32_t c0 = ci - cs, all_c = 0;
-    uint64_t m0 = mi - ms, all_m = 0;
-#pragma unroll
-    for (int v = 0; v < kPartWaves; ++v) {
-      if (v < wave) {
-        c0 += wave_c[v];
-        m0 += wave_m[v];
-      }
-      all_c += wave_c[v];
-      all_m += wave_m[v];
-    }
-    const bool cut = o.by_k && (uint64_t)o.top_k < all_c;  // else there are no more than k
-    if (cut) {
-      uint32_t cc = c0;
-      uint64_t mm = m0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (cc < (uint64_t)o.top_k && cc + c[i] >= (uint64_t)o.top_k) {
-          found.k = PER * t + i;
-          found.k_before = cc;
-          found.k_mass = mm;
-          if (!o.by_p) {
-            found.lo = found.hi = found.k;
-            found.lo_mass = mm;
-          }
-        }
-        cc += c[i];
-        mm += m[i];
-      }
-    }
-    __syncthreads();
-    if (o.by_p) {
-      // p times the mass of the first k: between what is above bin k and that with all of bin k
-      const int k = found.k;
-      uint64_t most = all_m, least = all_m;
-      if (cut) {
-        least = found.k_mass;
-        most = least + sp.mass[r * kBins + k];
-      }
-      auto goal = [&](uint64_t total) {
-        const double x = ceil(o.top_p * (double)total);
-        return x > 1. ? (uint64_t)x : (uint64_t)1;
-      };
-      const uint64_t lo = goal(least), hi = goal(most);
-      uint64_t mm = m0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (mm < lo && mm + m[i] >= lo) {
-          found.lo = PER * t + i;
-          found.lo_mass = mm;
-        }
-        if (mm < hi && mm + m[i] >= hi) found.hi = PER * t + i;
-        mm += m[i];
-      }
-      __syncthreads();
-    }
-  }
-  const Bins f = found;
-  if (blockIdx.x == 0 && t == 0 && (o.by_k || o.by_p)) sp.bins[r] = f;  // (without either there is no room for it)
+  const Bins f = o.by_k || o.by_p ? sp.bins[r] : Bins{kBins, kBins, kBins, 0, 0, 0, 0};
   const Row<T> row(a.logits, a.ld, r, a.vocab);
   for (int slice = blockIdx.x; slice < sp.slices; slice += gridDim.x) {
     double sum = 0.;
 #pragma unroll
-    for (int i = 0; i < kPartGroups; ++i) {
-      const int g = slice * (kSlice / kGroup) + i * kPartThreads + t;
-      if (g >= row.groups) continue;
+    for (int q = 0; q < kSliceGroups / kThreads; ++q) {
+      const int g = slice * kSliceGroups + q * kThreads + t;
+      if (g >= row.groups) break;
       float x[kGroup];
       row.load(g, x);
+      int b[kGroup], least = kBins;
+      bool found_one = false;
 #pragma unroll
       for (int j = 0; j < kGroup; ++j) {
-        if (x[j] == -inf()) continue;
-        const int b = w.bin(x[j]);
-        if (b < f.lo) {
-          const double y = w.of(x[j]);
-          sum += y >= o.min_p ? y : 0.;
-        } else if (b <= f.hi || b == f.k) {
-          // one place for each of the wave's lanes that are here, from one atomic
-          const uint64_t here = __builtin_amdgcn_ballot_w64(true);
-          const int rank = __popcll(here & ((1ull << lane) - 1));
-          uint32_t at = 0;
-          if (rank == 0) at = atomicAdd(&sp.n_cand[r], (uint32_t)__popcll(here));
-          at = __builtin_amdgcn_readfirstlane(at) + rank;
+        b[j] = x[j] == -inf() ? kBins : w.bin(x[j]);
+        least = min(least, b[j]);
+        found_one |= b[j] < kBins && ((b[j] >= f.lo && b[j] <= f.hi) || b[j] == f.k);
+      }
+      if (least < f.lo) {
+        if (w.simple) {
+#pragma unroll
+          for (int j = 0; j < kGroup; ++j) {
+            const double y = w.of_simple(x[j]);
+            sum += b[j] < f.lo && y >= o.min_p ? y : 0.;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kGroup; ++j) {
+            const double y = w.of(x[j]);
+            sum += b[j] < f.lo && y >= o.min_p ? y : 0.;
+          }
+        }
+      }
+      if (found_one) {
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+          if (b[j] >= kBins || !((b[j] >= f.lo && b[j] <= f.hi) || b[j] == f.k)) continue;
+          const uint32_t at = atomicAdd(&n_cand, 1u);
           if (at < (uint32_t)kCandidates)
-            sp.cand[r * kCandidates + at] =
-                ((uint64_t)key_of(x[j]) << 32) | (0xffffffffu - (uint32_t)(row.first(g) + j));
+            cand[at] = ((uint64_t)key_of(x[j]) << 32) | (0xffffffffu - (uint32_t)(row.first(g) + j));
         }
       }
     }
-    sum = block_sum<kPartThreads, double>(sum, per_wave);
-    if (t == 0) sp.sums[r * sp.slices + slice] = sum;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if (lane == 0) sp.sums[(r * sp.slices + slice) * kSums + wave] = sum;  // the draw adds them: no barrier per slice
   }
+  // the work-group's candidates to the row's, from one atomic (their order does not matter)
+  __syncthreads();
+  const uint32_t mine = n_cand;
+  if (mine == 0) return;
+  if (t == 0) cand_at = atomicAdd(&sp.n_cand[r], mine);
+  __syncthreads();
+  for (uint32_t i = t; i < mine; i += kThreads)
+    if (cand_at + i < (uint32_t)kCandidates && i < (uint32_t)kCandidates) sp.cand[r * kCandidates + cand_at + i] = cand[i];
 }
 
 // The token within a slice: the first in index order whose running sum of `weight(x, index)`
 // exceeds s.target (an infinite target: the last with any).  A thread takes consecutive groups.
 template <typename T, int N, typename F>
-__device__ void draw_token(const Args& a, int64_t r, const Row<T>& row, int slice, F&& weight, Scratch<N>& s) {
-  constexpr int PER = kSlice / kGroup / N;
-  const int g0 = slice * (kSlice / kGroup) + PER * (int)threadIdx.x;
+__device__ __forceinline__ void draw_token(const Args& a, int64_t r, const Row<T>& row, int slice, F&& weight, Scratch<N>& s) {
+  constexpr int PER = kSliceGroups / N;
+  const int g0 = slice * kSliceGroups + PER * (int)threadIdx.x;
   double y[PER][kGroup], sum = 0.;
 #pragma unroll
   for (int q = 0; q < PER; ++q) {
@@ -823,7 +917,7 @@ __device__ void draw_token(const Args& a, int64_t r, const Row<T>& row, int slic
 #pragma unroll
     for (int j = 0; j < kGroup; ++j) {
       run += y[q][j];
-      if (y[q][j] > 0.) {
+      if (y[q][j] > 1e-300) {  // (of_simple's 2^-1000 stands for nothing)
         last = row.first(g0 + q) + j;
         last_y = y[q][j];
         if (hit < 0 && run > target) {
@@ -888,53 +982,48 @@ template <int N> __device__ __forceinline__ void pick_slice(Scratch<N>& s, int s
   }
 }
 
-// A row whose border bins hold too many logits, by one work-group alone: see find_border.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void slow_kernel(Args a, Space sp) {
-  __shared__ Shared s;
-  const int64_t r = blockIdx.x;
-  if (sp.n_cand[r] <= (uint32_t)kCandidates) return;
-  const int t = threadIdx.x, slices = sp.slices;
-  const RowOptions o(a, r);
-  const RowStats rs(sp.stats + r * slices, slices);
-  fill_table(s.table);
-  const Row<T> row(a.logits, a.ld, r, a.vocab);
-  const Weights w = weights_of(s.table, rs.top, rs.low, o.temp, a.fixed);
+// A row whose border bins hold too many logits, by its work-group alone: see find_border.
+template <typename T, int N>
+__device__ __forceinline__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowOptions& o, const Weights& w, int slices,
+                         Scratch<N>& s) {
+  const int t = threadIdx.x;
   Border border{key_of(-inf()), 0};
   if (o.by_k) {
-    find_border<T, false>(row, w, (uint64_t)o.top_k, nullptr, s);
+    find_border<T, N, false>(row, w, (uint64_t)o.top_k, nullptr, s);
     border = s.border;
   }
   if (o.by_p) {
     // the mass of what top_k keeps, then the border of p times it
     uint64_t mass = 0;
-    for (int g = t; g < row.groups; g += kThreads) {
+    for (int g = t; g < row.groups; g += N) {
       float x[kGroup];
       row.load(g, x);
 #pragma unroll
       for (int j = 0; j < kGroup; ++j)
         if (x[j] != -inf() && key_of(x[j]) > border.key) mass += w.fixed_of(x[j]);
     }
-    uint64_t total;
-    block_prefix<kThreads, uint64_t>(mass, s.wave_u, total);
+    uint64_t total = block_sum<N, uint64_t>(mass, s.wave_u);
     if (border.ties) total += border.ties * w.fixed_of(of_key(border.key));
     // the smallest whole mass that is p times the total or more; at least the first element
     const double goal = ceil(o.top_p * (double)total);
     const uint64_t want = goal > 1. ? (uint64_t)goal : 1;
     const Border limit = border;
-    find_border<T, true>(row, w, want, o.by_k ? &limit : nullptr, s);
+    __syncthreads();
+    find_border<T, N, true>(row, w, want, o.by_k ? &limit : nullptr, s);
     border = s.border;
   }
   const float border_x = of_key(border.key);
   const double tie_weight = border.ties ? w.of(border_x) : 0.;
   const bool tie_kept = border.ties && tie_weight >= o.min_p;
   auto above = [&](float x) { return x != -inf() && key_of(x) > border.key; };
+  constexpr int PER = kSliceGroups / N;
   // kept mass and ties per slice
   for (int i = 0; i < slices; ++i) {
-    const int g = i * kThreads + t;
     double m = 0.;
     uint32_t ties = 0;
-    if (g < row.groups) {
+    for (int q = 0; q < PER; ++q) {
+      const int g = i * kSliceGroups + q * N + t;
+      if (g >= row.groups) break;
       float x[kGroup];
       row.load(g, x);
 #pragma unroll
@@ -947,8 +1036,8 @@ __global__ __launch_bounds__(kThreads) void slow_kernel(Args a, Space sp) {
         }
       }
     }
-    m = block_sum<kThreads, double>(m, s.wave_d);
-    if (tie_kept) ties = block_sum<kThreads, uint32_t>(ties, s.wave_c);
+    m = block_sum<N, double>(m, s.wave_d);
+    if (tie_kept) ties = block_sum<N, uint32_t>(ties, s.wave_c);
     if (t == 0) {
       s.slice_sum[i] = m;
       s.slice_add[i] = ties;
@@ -967,18 +1056,20 @@ __global__ __launch_bounds__(kThreads) void slow_kernel(Args a, Space sp) {
   __syncthreads();
   if (t < 64) pick_slice(s, slices, o.u);
   __syncthreads();
-  // the slice's first ties, by their rank in it
-  const int slice = s.bin, g = slice * kThreads + t;
+  // the slice's first ties, by their rank in it (a thread takes consecutive groups, as the draw does)
+  const int slice = s.bin;
   uint32_t ties = 0;
-  if (tie_kept && g < row.groups) {
+  for (int q = 0; tie_kept && q < PER; ++q) {
+    const int g = slice * kSliceGroups + PER * t + q;
+    if (g >= row.groups) break;
     float x[kGroup];
     row.load(g, x);
 #pragma unroll
     for (int j = 0; j < kGroup; ++j) ties += x[j] == border_x;
   }
-  uint32_t all_ties, rank = block_prefix<kThreads, uint32_t>(ties, s.wave_c, all_ties);
+  uint32_t all_ties, rank = block_prefix<N, uint32_t>(ties, s.wave_c, all_ties);
   const uint32_t take = (uint32_t)s.slice_add[slice];
-  draw_token<T, kThreads>(a, r, row, slice, [&](float x, int) {
+  draw_token<T, N>(a, r, row, slice, [&](float x, int) {
     if (above(x)) {
       const double y = w.of(x);
       return y >= o.min_p ? y : 0.;
@@ -996,7 +1087,12 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
   const RowOptions o(a, r);
   const SliceStats* stats = sp.stats + r * sp.slices;
   each<N>(sp.slices, [&](int i) {
-    s.slice_sum[i] = sp.sums[r * sp.slices + i];
+    const double* sums = sp.sums + (r * sp.slices + i) * kSums;
+    double sum = sums[0];
+    if (!o.plain())
+#pragma unroll
+      for (int q = 1; q < kSums; ++q) sum += sums[q];
+    s.slice_sum[i] = sum;
     s.slice_add[i] = 0;
   });
   const RowStats rs(stats, sp.slices);
@@ -1032,14 +1128,17 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
     }
     __syncthreads();
     const Weights v = weights_of(s.table, top, rs.low, o.temp, a.fixed);
-    draw_token<T, N>(a, r, row, s.bin, [&](float x, int) { return v.of(x); }, s);
+    draw_token<T, N>(a, r, row, s.bin, [&](float x, int) { return v.simple ? v.of_simple(x) : v.of(x); }, s);
     return;
   }
   uint64_t border = 0;  // the last kept (key, index); 0: no border
   if (o.by_k || o.by_p) {
     const Bins f = sp.bins[r];
     const int have = (int)min(sp.n_cand[r], (uint32_t)kCandidates + 1);
-    if (have > kCandidates) return;  // slow_kernel's
+    if (have > kCandidates) {
+      slow_row<T, N>(a, r, row, o, w, sp.slices, s);
+      return;
+    }
     if (have) {
       each<N>(have, [&](int i) { s.cand[i] = sp.cand[r * kCandidates + i]; });
       sort_candidates<N>(s, have);
@@ -1059,10 +1158,8 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
           for (int i = max(b, (int)before_k); i < min(e, last + 1); ++i) kept += w.fixed_of(logit(i));
           mass_k = f.k_mass + block_sum<N, uint64_t>(kept, s.wave_u);
         }
-      } else if (o.by_p) {  // the whole row's mass: the histogram's
-        uint64_t mine = 0;
-        each<N>(kBins, [&](int i) { mine += sp.mass[r * kBins + i]; });
-        mass_k = block_sum<N, uint64_t>(mine, s.wave_u);
+      } else {
+        mass_k = f.all_mass;
       }
       if (o.by_p) {
         // p times the mass of the first k, reached in the bins [lo, hi], which begin the candidates
@@ -1100,7 +1197,7 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
   draw_token<T, N>(a, r, row, s.bin, [&](float x, int i) {
     const uint64_t me = ((uint64_t)key_of(x) << 32) | (0xffffffffu - (uint32_t)i);
     if (me < border) return 0.;
-    const double y = w.of(x);
+    const double y = w.simple ? w.of_simple(x) : w.of(x);
     return y >= o.min_p ? y : 0.;
   }, s);
 }
@@ -1108,7 +1205,7 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
 constexpr int64_t kRowsAtOnce = 4096;  // rows per set of launches: bounds the workspace
 
 int slices_of(int64_t vocab) {
-  return (int)((((vocab + 2 * kGroup - 2) / kGroup) + kThreads - 1) / kThreads);  // of a row at any alignment
+  return (int)((((vocab + 2 * kGroup - 2) / kGroup) + kSliceGroups - 1) / kSliceGroups);  // of a row at any alignment
 }
 int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
 
@@ -1123,11 +1220,11 @@ int64_t space_of(int64_t rows, int64_t vocab, bool bins, char* base, Space* sp) 
   Space s{};
   s.slices = (int)slices;
   s.stats = (SliceStats*)take(rows * slices * (int64_t)sizeof(SliceStats));
-  s.sums = (double*)take(rows * slices * 8);
+  s.sums = (double*)take(rows * slices * kSums * 8);
   if (bins) {
     s.bins = (Bins*)take(rows * (int64_t)sizeof(Bins));
-    s.mass = (uint64_t*)take(rows * kBins * 8);
-    s.count = (uint32_t*)take(rows * kBins * 4);
+    s.mass = (uint64_t*)take(rows * kBinParts * kBins * 8);
+    s.count = (uint32_t*)take(rows * kBinParts * kBins * 4);
     s.cand = (uint64_t*)take(rows * kCandidates * 8);
     s.n_cand = (uint32_t*)take(rows * 4);
   }
@@ -1137,29 +1234,31 @@ int64_t space_of(int64_t rows, int64_t vocab, bool bins, char* base, Space* sp) 
 
 template <typename T>
 void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bins, hipStream_t s) {
-  const dim3 grid((unsigned)sp.slices, (unsigned)rows), block(kPartThreads);
+  const dim3 grid((unsigned)sp.slices, (unsigned)rows), block(kMaxThreads);
   {
     TimedLaunch timed_("sampling.maxima_kernel", s);
     if (bins) hipLaunchKernelGGL((maxima_kernel<T, true>), grid, block, 0, s, a, sp);
     else hipLaunchKernelGGL((maxima_kernel<T, false>), grid, block, 0, s, a, sp);
   }
-  // work-groups a row where the histogram's merge, or its search, is paid by each
-  const dim3 parts((unsigned)std::max<int64_t>(1, std::min<int64_t>(sp.slices, 1024 / rows)), (unsigned)rows);
+  auto per_row = [&](int64_t all, int64_t most) {  // work-groups a row, for about `all` in the launch
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)sp.slices, (all + rows / 2) / rows}));
+  };
   if (bins) {
-    TimedLaunch timed_("sampling.bins_kernel", s);
-    hipLaunchKernelGGL(bins_kernel<T>, parts, block, 0, s, a, sp);
+    const unsigned parts = per_row(1024, kBinParts);
+    {
+      TimedLaunch timed_("sampling.bins_kernel", s);
+      hipLaunchKernelGGL(bins_kernel<T>, dim3(parts, (unsigned)rows), dim3(kThreads), 0, s, a, sp);
+    }
+    TimedLaunch timed_("sampling.search_kernel", s);
+    hipLaunchKernelGGL(search_kernel, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp, (int)parts);
   }
   if (filters) {
     TimedLaunch timed_("sampling.gather_kernel", s);
-    hipLaunchKernelGGL(gather_kernel<T>, parts, block, 0, s, a, sp);
+    hipLaunchKernelGGL(gather_kernel<T>, dim3(per_row(1024, sp.slices), (unsigned)rows), dim3(kThreads), 0, s, a, sp);
   }
   {
     TimedLaunch timed_("sampling.draw_kernel", s);
     hipLaunchKernelGGL(draw_kernel<T>, dim3((unsigned)rows), dim3(kDrawThreads), 0, s, a, sp);
-  }
-  if (bins) {
-    TimedLaunch timed_("sampling.slow_kernel", s);
-    hipLaunchKernelGGL(slow_kernel<T>, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp);
   }
 }
 
@@ -1197,7 +1296,7 @@ int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab
   a.o = Options{temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all};
   int bits = 0;
   while ((1ll << bits) < vocab) ++bits;
-  a.fixed = (double)(1ull << (62 - bits));  // vocab weights of at most 1 stay below 2^62
+  a.fixed = (double)(1ull << std::min(62 - bits, 50));  // vocab weights of at most 1 stay below 2^62
   a.tokens = tokens;
   a.logprobs = logprobs;
   const bool by_min = min_p || min_p_all > 0;
