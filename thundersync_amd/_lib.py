@@ -18,6 +18,7 @@ not available -- there is no host fallback inside this package.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -268,6 +269,18 @@ def stream_of(tensor) -> int:
     if raw is not None and tensor.device.index is not None:
         return raw(tensor.device.index)
     return torch.cuda.current_stream(tensor.device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(tensor):
+    """A context in which ``tensor``'s device is the current one, as a launch on
+    its stream wants it (nothing to enter where it already is)."""
+    import torch
+
+    index = tensor.device.index
+    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def ptr(tensor) -> int | None:

@@ -3,7 +3,7 @@
 //   out[n] = scale W[ids[n]]        dW[v] = scale sum over n with ids[n] = v of dout[n]
 //
 // Lookup: bandwidth-bound, 16 bytes a lane.  Gradient: the tokens' positions are sorted by
-// id (stable, so equal ids keep the token order), and chunks of kChunk sorted positions add
+// id (stable, so equal ids keep the token order), and chunks of sorted positions add
 // up their rows of dout in fp32; an id whose positions end inside the chunk is written once,
 // one that a chunk border cuts leaves fp32 partial rows that join_kernel adds in chunk
 // order.  No atomics on values: the same bits every time.  Rows of the table that no token
@@ -19,7 +19,7 @@ namespace ts {
 namespace embed {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 32;      // sorted positions per work-group of the reduction
+constexpr int kChunk = 32;      // sorted positions per work-group of the reduction, at most
 constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
 constexpr int kRounds = 8, kWaves = kThreads / 64, kSortTile = kThreads * kRounds;
 
@@ -64,8 +64,12 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(const int64_t* __restr
 }
 
 // ---------------------------------------------------------------------------
-// stable sort of the positions by id, kDigitBits at a time from the low end.  The key of a
-// token that takes no part (outside the vocabulary, or the padding id) is `vocab`.
+// stable sort of the positions by id, kDigitBits at a time from the low end, in tiles of
+// kSortTile.  The key of a token that takes no part (outside the vocabulary, or the padding
+// id) is `vocab`.  A pass is two launches, of the tiles' digit counts and of their placement,
+// or with one tile all passes are one launch in LDS.  The sort occupies a few CUs, so the
+// rest of each launch's grid writes its share of the gradient's zeros: a training batch's
+// sort (16384 tokens, 48 us by itself) then costs nothing beside the zeros' 256 us.
 // ---------------------------------------------------------------------------
 struct SortArgs {
   const int64_t* ids;     // first pass: key from the ids, position the index
@@ -73,55 +77,28 @@ struct SortArgs {
   const uint32_t* pos_in;
   uint32_t* key_out;
   uint32_t* pos_out;
-  uint32_t* hist;         // [kBins][tiles]
+  uint32_t* hist;         // [tiles][kBins]
   int64_t n;
   int64_t vocab, padding;
   int tiles, shift;
+  // this launch's zeros: 16-byte words [zero0, zero1) of `zero`, and the bytes behind the last
+  u32x4* zero;
+  int64_t zero0, zero1;
+  unsigned char* tail;
+  int tail_bytes;
 };
+
+__device__ __forceinline__ void write_zeros(const SortArgs& a, int block, int blocks) {
+  const int64_t step = (int64_t)blocks * kThreads;
+  for (int64_t i = a.zero0 + (int64_t)block * kThreads + threadIdx.x; i < a.zero1; i += step)
+    a.zero[i] = u32x4{0, 0, 0, 0};
+  if (block == 0 && (int)threadIdx.x < a.tail_bytes) a.tail[threadIdx.x] = 0;
+}
 
 __device__ __forceinline__ uint32_t key_at(const SortArgs& a, int64_t i) {
   if (!a.ids) return a.key_in[i];
   const int64_t id = a.ids[i];
   return id < 0 || id >= a.vocab || id == a.padding ? (uint32_t)a.vocab : (uint32_t)id;
-}
-
-__global__ __launch_bounds__(kThreads) void sort_count_kernel(SortArgs a) {
-  __shared__ uint32_t bins[kBins];
-  for (int b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
-  __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kSortTile;
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = i0 + r * kThreads + threadIdx.x;
-    if (i < a.n) atomicAdd(&bins[(key_at(a, i) >> a.shift) & (kBins - 1)], 1u);
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kThreads) a.hist[(int64_t)b * a.tiles + blockIdx.x] = bins[b];
-}
-
-// exclusive prefix sums of `count` values by one work-group
-constexpr int kScanThreads = 1024;
-__global__ __launch_bounds__(kScanThreads) void sort_scan_kernel(uint32_t* x, int64_t count) {
-  __shared__ uint32_t wave_sum[kScanThreads / 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t per = (count + kScanThreads - 1) / kScanThreads;
-  const int64_t b = min(count, threadIdx.x * per), e = min(count, b + per);
-  uint32_t sum = 0;
-  for (int64_t i = b; i < e; ++i) sum += x[i];
-  uint32_t incl = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t y = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 63) wave_sum[wave] = incl;
-  __syncthreads();
-  uint32_t before = incl - sum;
-  for (int w = 0; w < wave; ++w) before += wave_sum[w];
-  for (int64_t i = b; i < e; ++i) {
-    const uint32_t y = x[i];
-    x[i] = before;
-    before += y;
-  }
 }
 
 // Lanes of the wave whose digit equals this lane's, among the `on` ones.
@@ -135,57 +112,161 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool on) {
   return m;
 }
 
-// A wave owns kRounds x 64 consecutive elements and takes them 64 at a time; an element's
-// place is its digit's base for the wave plus the number of earlier elements with the digit.
-__global__ __launch_bounds__(kThreads) void sort_scatter_kernel(SortArgs a) {
-  __shared__ uint32_t base[kWaves][kBins];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int b = threadIdx.x; b < kWaves * kBins; b += kThreads) (&base[0][0])[b] = 0;
+// A tile's elements are kRounds x 64 consecutive ones a wave, 64 at a time.  base[wave][digit]
+// holds the wave's counts, then (with each digit's first place in `first`) the place of the
+// wave's first element of the digit.
+struct Places {
+  uint32_t base[kWaves][kBins];
+  uint32_t wave_sum[kWaves];
+};
+__device__ __forceinline__ void count_digits(Places& p, const uint32_t (&key)[kRounds], const bool (&on)[kRounds],
+                                             int shift) {
+  const int wave = threadIdx.x >> 6;
+  for (int b = threadIdx.x; b < kWaves * kBins; b += kThreads) (&p.base[0][0])[b] = 0;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kSortTile + wave * (kRounds * 64) + lane;
-  uint32_t key[kRounds];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = i0 + 64 * r;
-    key[r] = i < a.n ? key_at(a, i) : 0;
-    if (i < a.n) atomicAdd(&base[wave][(key[r] >> a.shift) & (kBins - 1)], 1u);
-  }
+  for (int r = 0; r < kRounds; ++r)
+    if (on[r]) atomicAdd(&p.base[wave][(key[r] >> shift) & (kBins - 1)], 1u);
   __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kThreads) {
-    uint32_t at = a.hist[(int64_t)b * a.tiles + blockIdx.x];
+}
+// two consecutive digits a thread: `all` of each in the whole sort, `before` in earlier tiles
+__device__ __forceinline__ void place_digits(Places& p, const uint32_t (&all)[2], const uint32_t (&before)[2]) {
+  static_assert(kBins == 2 * kThreads, "two digits a thread");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t incl = all[0] + all[1];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) p.wave_sum[wave] = incl;
+  __syncthreads();
+  uint32_t first = incl - all[0] - all[1];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) first += w < wave ? p.wave_sum[w] : 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = 2 * threadIdx.x + i;
+    uint32_t at = first + (i ? all[0] : 0) + before[i];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const uint32_t c = base[w][b];
-      base[w][b] = at;
+      const uint32_t c = p.base[w][b];
+      p.base[w][b] = at;
       at += c;
     }
   }
   __syncthreads();
+}
+// an element's place is its digit's base for the wave plus the earlier elements with the digit
+template <typename F>
+__device__ __forceinline__ void put_digits(Places& p, const uint32_t (&key)[kRounds], const bool (&on)[kRounds],
+                                           int shift, F&& put) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = i0 + 64 * r;
-    const bool on = i < a.n;
-    const uint32_t digit = (key[r] >> a.shift) & (kBins - 1);
-    const uint64_t same = same_digit(digit, on);
+    const uint32_t digit = (key[r] >> shift) & (kBins - 1);
+    const uint64_t same = same_digit(digit, on[r]);
     const uint64_t before = same & ((1ull << lane) - 1);
-    uint32_t at = 0;
-    if (on) {
-      at = base[wave][digit] + (uint32_t)__popcll(before);
-      a.key_out[at] = key[r];
-      a.pos_out[at] = a.ids ? (uint32_t)i : a.pos_in[i];
-    }
+    if (on[r]) put(r, p.base[wave][digit] + (uint32_t)__popcll(before));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (on && before == 0) base[wave][digit] += (uint32_t)__popcll(same);  // the digit's first lane
+    if (on[r] && before == 0) p.base[wave][digit] += (uint32_t)__popcll(same);  // the digit's first lane
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
 }
 
-__global__ __launch_bounds__(kThreads) void zero_kernel(u32x4* p, int64_t vectors, unsigned char* tail, int tail_bytes) {
-  const int64_t step = (int64_t)gridDim.x * kThreads;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < vectors; i += step) p[i] = u32x4{0, 0, 0, 0};
-  if (blockIdx.x == 0 && (int)threadIdx.x < tail_bytes) tail[threadIdx.x] = 0;
+__global__ __launch_bounds__(kThreads) void sort_count_kernel(SortArgs a) {
+  if ((int)blockIdx.x >= a.tiles) return write_zeros(a, (int)blockIdx.x - a.tiles, (int)gridDim.x - a.tiles);
+  __shared__ uint32_t bins[kBins];
+  for (int b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * kSortTile;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = i0 + r * kThreads + threadIdx.x;
+    if (i < a.n) atomicAdd(&bins[(key_at(a, i) >> a.shift) & (kBins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += kThreads) a.hist[(int64_t)blockIdx.x * kBins + b] = bins[b];
+}
+
+// Each tile adds up the tiles' counts itself (two digits a thread, rows of 2 KB): for the
+// tiles of a batch less than a launch that would scan them.
+__global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
+  if ((int)blockIdx.x >= a.tiles) return write_zeros(a, (int)blockIdx.x - a.tiles, (int)gridDim.x - a.tiles);
+  __shared__ Places p;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t i0 = (int64_t)blockIdx.x * kSortTile + wave * (kRounds * 64) + lane;
+  uint32_t key[kRounds], pos[kRounds];
+  bool on[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = i0 + 64 * r;
+    on[r] = i < a.n;
+    key[r] = on[r] ? key_at(a, i) : 0;
+    pos[r] = on[r] ? (a.ids ? (uint32_t)i : a.pos_in[i]) : 0;
+  }
+  uint32_t all[2] = {}, before[2] = {};
+#pragma unroll 8
+  for (int tile = 0; tile < a.tiles; ++tile) {
+    const u32x2 c = *reinterpret_cast<const u32x2*>(a.hist + (int64_t)tile * kBins + 2 * threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      all[i] += c[i];
+      before[i] += tile < (int)blockIdx.x ? c[i] : 0;
+    }
+  }
+  count_digits(p, key, on, a.shift);
+  place_digits(p, all, before);
+  put_digits(p, key, on, a.shift, [&](int r, uint32_t at) {
+    a.key_out[at] = key[r];
+    a.pos_out[at] = pos[r];
+  });
+}
+
+// at most kSortTile tokens: every pass in LDS
+__global__ __launch_bounds__(kThreads) void sort_tile_kernel(SortArgs a) {
+  if ((int)blockIdx.x >= a.tiles) return write_zeros(a, (int)blockIdx.x - a.tiles, (int)gridDim.x - a.tiles);
+  __shared__ Places p;
+  __shared__ uint32_t keys[kSortTile], places[kSortTile];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i0 = wave * (kRounds * 64) + lane, n = (int)a.n;
+  uint32_t key[kRounds], pos[kRounds];
+  bool on[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    pos[r] = i0 + 64 * r;
+    on[r] = (int)pos[r] < n;
+    key[r] = on[r] ? key_at(a, pos[r]) : 0;
+  }
+  for (int shift = 0; shift == 0 || (a.vocab >> shift) > 0; shift += kDigitBits) {
+    if (shift) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r)
+        if (on[r]) {
+          key[r] = keys[i0 + 64 * r];
+          pos[r] = places[i0 + 64 * r];
+        }
+    }
+    count_digits(p, key, on, shift);  // (its barriers also end the reads above)
+    uint32_t all[2] = {};
+    const uint32_t before[2] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) all[i] += p.base[w][2 * threadIdx.x + i];
+    place_digits(p, all, before);
+    put_digits(p, key, on, shift, [&](int r, uint32_t at) {
+      keys[at] = key[r];
+      places[at] = pos[r];
+    });
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    a.key_out[i] = keys[i];
+    a.pos_out[i] = places[i];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -199,6 +280,7 @@ struct ReduceArgs {
   int64_t ldd;          // row stride of dout
   int dim;
   float scale;
+  int chunk;            // sorted positions per work-group
   float* part;          // [chunks][2][dim]: the run that began earlier, the run that goes on
 };
 
@@ -206,8 +288,8 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void reduce_kernel(ReduceArgs a, const T* __restrict__ dout,
                                                           T* __restrict__ dw) {
   __shared__ uint32_t key[kChunk + 2], pos[kChunk];  // key[0], key[count + 1]: the neighbours'
-  const int64_t i0 = (int64_t)blockIdx.x * kChunk;
-  const int count = (int)min((int64_t)kChunk, a.n - i0);
+  const int64_t i0 = (int64_t)blockIdx.x * a.chunk;
+  const int count = (int)min((int64_t)a.chunk, a.n - i0);
   const int t = threadIdx.x;
   if (t < count) pos[t] = a.pos[i0 + t];
   // `vocab` stands for no neighbour: runs of it are skipped anyway
@@ -255,7 +337,7 @@ __global__ __launch_bounds__(kThreads) void reduce_kernel(ReduceArgs a, const T*
 // the runs that chunk borders cut: the chunk a run begins in adds its parts in chunk order
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void join_kernel(ReduceArgs a, T* __restrict__ dw) {
-  const int64_t c = blockIdx.x, first = c * kChunk, next = first + kChunk;
+  const int64_t c = blockIdx.x, first = c * a.chunk, next = first + a.chunk;
   if (next >= a.n) return;  // the last chunk: its last run goes nowhere
   const uint32_t id = a.key[next - 1];
   if (id == a.vocab || a.key[next] != id) return;
@@ -264,7 +346,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ReduceArgs a, T* __restr
   if (d >= a.dim) return;
   // the chunks that the run reaches into
   int64_t end = c + 2;
-  while (end * kChunk < a.n && a.key[end * kChunk - 1] == id && a.key[end * kChunk] == id) ++end;
+  while (end * a.chunk < a.n && a.key[end * a.chunk - 1] == id && a.key[end * a.chunk] == id) ++end;
   float acc[VEC];
   const float* q = a.part + (c * 2 + 1) * a.dim + d;
 #pragma unroll
@@ -283,7 +365,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ReduceArgs a, T* __restr
 bool ok16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int64_t tiles_of(int64_t n) { return (n + kSortTile - 1) / kSortTile; }
-int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+// Few tokens: chunks of 8, for work-groups enough
+int chunk_of(int64_t n) { return n <= 4096 ? 8 : kChunk; }
+int64_t chunks_of(int64_t n) { return (n + chunk_of(n) - 1) / chunk_of(n); }
 int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
 
 // the workspace: two (key, position) buffers, the digit counts, the partial rows
@@ -379,51 +463,63 @@ int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_
   if (vocab == 0) return TS_OK;
   TS_CHECK_ARG(grad_weight && ok16(grad_weight), "ts_embedding_bwd: grad_weight null or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
-  {
-    const int64_t bytes = vocab * dim * (dtype == TS_F32 ? 4 : 2);
-    ts::TimedLaunch timed_("embedding.zero_kernel", s);
-    const int64_t blocks = std::min<int64_t>((bytes / 16 + kThreads - 1) / kThreads, 4096);
-    hipLaunchKernelGGL(zero_kernel, dim3((unsigned)std::max<int64_t>(blocks, 1)), dim3(kThreads), 0, s,
-                       (ts::u32x4*)grad_weight, bytes / 16, (unsigned char*)grad_weight + bytes / 16 * 16,
-                       (int)(bytes % 16));
-  }
-  int st = ts::check_launch("ts_embedding_bwd (zero)");
-  if (st != TS_OK || n == 0) return st;
-  TS_CHECK_ARG(ids && grad_out && ld_grad >= 0, "ts_embedding_bwd: null pointer");
-  TS_CHECK_ARG(workspace && ok16(workspace) && workspace_bytes >= ts_embedding_bwd_workspace(n, dim),
+  const int64_t bytes = vocab * dim * (dtype == TS_F32 ? 4 : 2);
+  TS_CHECK_ARG(n == 0 || (ids && grad_out && ld_grad >= 0), "ts_embedding_bwd: null pointer");
+  TS_CHECK_ARG(n == 0 || (workspace && ok16(workspace) && workspace_bytes >= ts_embedding_bwd_workspace(n, dim)),
                "ts_embedding_bwd: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
                (long long)ts_embedding_bwd_workspace(n, dim));
   const Workspace ws(n, dim);
   char* base = (char*)workspace;
-  SortArgs a;
+  SortArgs a{};
+  a.ids = ids;
   a.n = n;
   a.vocab = vocab;
   a.padding = padding;
   a.tiles = (int)tiles_of(n);
   a.hist = (uint32_t*)(base + ws.hist);
-  int out = 0;
-  a.ids = ids;
-  a.key_in = a.pos_in = nullptr;
-  for (a.shift = 0; a.shift == 0 || (vocab >> a.shift) > 0; a.shift += kDigitBits) {
-    a.key_out = (uint32_t*)(base + ws.key[out]);
-    a.pos_out = (uint32_t*)(base + ws.pos[out]);
-    {
-      ts::TimedLaunch timed_("embedding.sort_count_kernel", s);
-      hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)a.tiles), dim3(kThreads), 0, s, a);
-    }
-    {
-      ts::TimedLaunch timed_("embedding.sort_scan_kernel", s);
-      hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, a.hist, (int64_t)kBins * a.tiles);
-    }
-    {
-      ts::TimedLaunch timed_("embedding.sort_scatter_kernel", s);
-      hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)a.tiles), dim3(kThreads), 0, s, a);
-    }
-    a.ids = nullptr;
+  a.zero = (ts::u32x4*)grad_weight;
+  int passes = 1;
+  while ((vocab >> (passes * kDigitBits)) > 0) ++passes;
+  // launch i of `launches` writes its share of the zeros, the last one the bytes behind the last whole word
+  const int launches = a.tiles <= 1 ? 1 : 2 * passes;
+  auto share = [&](int i) {
+    a.zero0 = bytes / 16 * i / launches;
+    a.zero1 = bytes / 16 * (i + 1) / launches;
+    a.tail = (unsigned char*)grad_weight + bytes / 16 * 16;
+    a.tail_bytes = i + 1 == launches ? (int)(bytes % 16) : 0;
+    const int64_t blocks = std::min<int64_t>((a.zero1 - a.zero0 + kThreads - 1) / kThreads, 4096);
+    return dim3((unsigned)(a.tiles + std::max<int64_t>(blocks, 1)));
+  };
+  if (a.tiles <= 1) {
+    a.key_out = (uint32_t*)(base + ws.key[0]);
+    a.pos_out = (uint32_t*)(base + ws.pos[0]);
+    ts::TimedLaunch timed_("embedding.sort_tile_kernel", s);
+    const dim3 grid = share(0);
+    hipLaunchKernelGGL(sort_tile_kernel, grid, dim3(kThreads), 0, s, a);
     a.key_in = a.key_out;
     a.pos_in = a.pos_out;
-    out ^= 1;
+  } else {
+    for (int pass = 0; pass < passes; ++pass) {
+      a.shift = pass * kDigitBits;
+      a.key_out = (uint32_t*)(base + ws.key[pass % 2]);
+      a.pos_out = (uint32_t*)(base + ws.pos[pass % 2]);
+      {
+        ts::TimedLaunch timed_("embedding.sort_count_kernel", s);
+        const dim3 grid = share(2 * pass);
+        hipLaunchKernelGGL(sort_count_kernel, grid, dim3(kThreads), 0, s, a);
+      }
+      {
+        ts::TimedLaunch timed_("embedding.sort_place_kernel", s);
+        const dim3 grid = share(2 * pass + 1);
+        hipLaunchKernelGGL(sort_place_kernel, grid, dim3(kThreads), 0, s, a);
+      }
+      a.ids = nullptr;
+      a.key_in = a.key_out;
+      a.pos_in = a.pos_out;
+    }
   }
+  const int st = ts::check_launch("ts_embedding_bwd (sort)");
+  if (st != TS_OK || n == 0) return st;
   ReduceArgs r;
   r.key = a.key_in;
   r.pos = a.pos_in;
@@ -432,6 +528,7 @@ int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_
   r.ldd = ld_grad;
   r.dim = (int)dim;
   r.scale = scale;
+  r.chunk = chunk_of(n);
   r.part = (float*)(base + ws.part);
   if (dtype == TS_F32) launch_sums<float>(r, grad_out, grad_weight, s);
   else if (dtype == TS_F16) launch_sums<ts::f16>(r, grad_out, grad_weight, s);

@@ -95,7 +95,7 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
         ctx.vocab, ctx.dtype, ctx.scale, ctx.padding_idx = weight.shape[0], weight.dtype, scale, padding_idx
-        with torch.cuda.device(weight.device), operator_range(
+        with _lib.device_of(weight), operator_range(
                 "embedding_forward", role=device_role(weight.device), tokens=ids.numel(), hidden=weight.shape[1],
                 vocab=weight.shape[0], dtype=weight.dtype):
             return embedding_forward(ids, weight, scale)
@@ -104,7 +104,7 @@ class _Embedding(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
-        with torch.cuda.device(grad.device), operator_range(
+        with _lib.device_of(grad), operator_range(
                 "embedding_backward", role=device_role(grad.device), tokens=ids.numel(), hidden=grad.shape[-1],
                 vocab=ctx.vocab):
             gw = embedding_backward(ids, grad.to(ctx.dtype), ctx.vocab, scale=ctx.scale, padding_idx=ctx.padding_idx)
@@ -118,6 +118,9 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     The row ``padding_idx`` of the table gets no gradient.
     """
     _validate(ids, weight, scale, padding_idx)
+    if not (weight.requires_grad and torch.is_grad_enabled()):
+        with _lib.device_of(weight):
+            return embedding_forward(ids, weight.detach(), float(scale))
     return _Embedding.apply(ids, weight, float(scale), padding_idx)
 
 

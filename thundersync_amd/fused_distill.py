@@ -311,7 +311,7 @@ def _backward_trainable(rows: _Rows, grad, chunk, block, maxima):
 class _FusedDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, ids, logits, temperature, chunk, need_hidden, need_weight):
-        with torch.cuda.device(hidden.device), operator_range(
+        with _lib.device_of(hidden), operator_range(
                 "fused_distill_forward", role=device_role(hidden.device), tokens=hidden.shape[0],
                 hidden=hidden.shape[1], vocab=weight.shape[0], top=ids.shape[1], dtype=hidden.dtype):
             rows = _Rows(hidden, weight, ids, logits, temperature)
@@ -327,7 +327,7 @@ class _FusedDistill(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        with torch.cuda.device(grad.device), operator_range(
+        with _lib.device_of(grad), operator_range(
                 "fused_distill_backward", role=device_role(grad.device), tokens=grad.shape[0],
                 weight_grad=not ctx.frozen):
             if ctx.frozen:

@@ -90,7 +90,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     ws_bytes = int(lib.ts_sample_workspace(b, v))
     ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=z.device)
     (t_rows, t_all), (k_rows, k_all), (p_rows, p_all), (m_rows, m_all) = options
-    with torch.cuda.device(z.device), operator_range("sample_tokens", role=device_role(z.device), rows=b, vocab=v,
+    with _lib.device_of(z), operator_range("sample_tokens", role=device_role(z.device), rows=b, vocab=v,
                                                      dtype=z.dtype):
         _lib.check(
             lib.ts_sample(z.data_ptr(), z.stride(0), b, v, u.data_ptr(), _lib.dtype_code(u.dtype), _lib.ptr(t_rows),
