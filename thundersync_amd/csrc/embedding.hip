@@ -299,22 +299,29 @@ __global__ __launch_bounds__(kThreads) void reduce_kernel(ReduceArgs a, const T*
   if (d >= a.dim) return;
   float acc[VEC] = {};
   bool earlier = key[0] == key[1];
+  // U rows at a time, the next U in flight while these are added; a row past the chunk or of a
+  // token that takes no part is the chunk's first again
   constexpr int U = 8;
-  for (int j0 = 0; j0 < count; j0 += U) {
-    float x[U][VEC];
+  struct alignas(sizeof(T) * VEC) Raw {
+    T v[VEC];
+  };
+  auto fetch = [&](int j0, Raw (&x)[U]) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = min(j0 + u, count - 1);
-      if (key[j + 1] != a.vocab) load_vec<T, VEC>(dout + pos[j] * a.ldd + d, x[u]);
+      const int j = j0 + u < count && key[j0 + u + 1] != a.vocab ? j0 + u : 0;
+      x[u] = *reinterpret_cast<const Raw*>(dout + pos[j] * a.ldd + d);
     }
+  };
+  // false: nothing follows
+  auto add = [&](int j0, const Raw (&x)[U]) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u;
-      if (j >= count) break;
+      if (j >= count) return false;
       const uint32_t id = key[j + 1];
-      if (id == a.vocab) break;  // sorted last: nothing follows
+      if (id == a.vocab) return false;  // sorted last
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += x[u][i];
+      for (int i = 0; i < VEC; ++i) acc[i] += to_f(x[u].v[i]);
       const bool last = j + 1 == count;
       if (!last && key[j + 2] == id) continue;
       const bool goes_on = last && key[j + 2] == id;
@@ -331,6 +338,15 @@ __global__ __launch_bounds__(kThreads) void reduce_kernel(ReduceArgs a, const T*
 #pragma unroll
       for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
     }
+    return true;
+  };
+  Raw x[U], y[U];
+  fetch(0, x);
+  for (int j0 = 0; j0 < count; j0 += 2 * U) {
+    fetch(j0 + U, y);
+    if (!add(j0, x)) return;
+    fetch(j0 + 2 * U, x);
+    if (!add(j0 + U, y)) return;
   }
 }
 
@@ -342,16 +358,27 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ReduceArgs a, T* __restr
   const uint32_t id = a.key[next - 1];
   if (id == a.vocab || a.key[next] != id) return;
   if (a.key[first] == id && first > 0 && a.key[first - 1] == id) return;  // began earlier
+  // the first chunk that the run does not reach past, kThreads of them looked at at a time (one
+  // after the other the look-ups of a frequent token's 150 chunks took longer than their sums)
+  __shared__ int ends;
+  int64_t end = c + 2;
+  while (true) {
+    if (threadIdx.x == 0) ends = kThreads;
+    __syncthreads();
+    const int64_t e = end + threadIdx.x;
+    if (e * a.chunk >= a.n || a.key[e * a.chunk - 1] != id || a.key[e * a.chunk] != id) atomicMin(&ends, (int)threadIdx.x);
+    __syncthreads();
+    end += ends;
+    if (ends < kThreads) break;
+    __syncthreads();
+  }
   const int d = (blockIdx.y * kThreads + threadIdx.x) * VEC;
   if (d >= a.dim) return;
-  // the chunks that the run reaches into
-  int64_t end = c + 2;
-  while (end * a.chunk < a.n && a.key[end * a.chunk - 1] == id && a.key[end * a.chunk] == id) ++end;
   float acc[VEC];
   const float* q = a.part + (c * 2 + 1) * a.dim + d;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = q[i];
-#pragma unroll 4
+#pragma unroll 16
   for (int64_t e = c + 1; e < end; ++e) {
     const float* r = a.part + e * 2 * a.dim + d;
 #pragma unroll
