@@ -3,8 +3,9 @@
 The integration point of the reference's attention dispatch
 (engine/streaming.py:355-373, :414-548) for this library:
 
-* :func:`hip_attention_available` / :func:`hip_logprob_available` answer for
-  one call's tensors.  Under ``THUNDERSYNC_HIP=off`` (or ``auto`` without a
+* :func:`hip_attention_available` / :func:`hip_logprob_available` /
+  :func:`hip_distill_available` / :func:`hip_embedding_available` /
+  :func:`hip_sampling_available` answer for one call's tensors.  Under ``THUNDERSYNC_HIP=off`` (or ``auto`` without a
   loadable library) the answer is no; under ``require`` a library that cannot
   load raises at every call (``_lib.library``), and a loaded one is used
   without a trial, so that a kernel that cannot run on the device fails at
@@ -85,6 +86,45 @@ def logprob_trial(device: torch.device, dtype: torch.dtype, dim: int) -> None:
         raise RuntimeError("HIP logprob trial produced nonfinite values")
 
 
+def distill_trial(device: torch.device, dtype: torch.dtype, dim: int) -> None:
+    """Five rows against four teacher logits each over a 300-token head: losses and the hidden gradient, finite."""
+    from .fused_distill import fused_distill
+
+    g = torch.Generator(device=device).manual_seed(0)
+    h = torch.randn(5, dim, device=device, dtype=dtype, generator=g).requires_grad_()
+    w = torch.randn(300, dim, device=device, dtype=dtype, generator=g) * 0.02
+    ids = torch.randint(0, 300, (5, 4), device=device, generator=g)
+    loss = fused_distill(h, w, ids, torch.randn(5, 4, device=device, generator=g), chunk=4)
+    (grad,) = torch.autograd.grad(loss.sum(), (h,))
+    if not all(bool(x.isfinite().all()) for x in (loss, grad)):
+        raise RuntimeError("HIP distillation trial produced nonfinite values")
+
+
+def embedding_trial(device: torch.device, dtype: torch.dtype, dim: int) -> None:
+    """Forty tokens of a 30-row table: the rows themselves and as many gradients."""
+    from .embedding import embedding
+
+    g = torch.Generator(device=device).manual_seed(0)
+    w = torch.randn(30, dim, device=device, dtype=dtype, generator=g).requires_grad_()
+    ids = torch.randint(0, 30, (40,), device=device, generator=g)
+    out = embedding(ids, w)
+    (grad,) = torch.autograd.grad(out, w, torch.ones_like(out))
+    if not bool((out == w[ids]).all()) or not bool((grad[:, 0] == torch.bincount(ids, minlength=30)).all()):
+        raise RuntimeError("HIP embedding trial produced other rows or gradients")
+
+
+def sampling_trial(device: torch.device, dtype: torch.dtype, vocab: int) -> None:
+    """Two rows of one likely token each, drawn plainly and through every filter."""
+    from .sampling import sample_tokens
+
+    z = torch.zeros(2, vocab, device=device, dtype=dtype)
+    z[0, 0] = z[1, vocab - 1] = 60.0
+    u = torch.full((2,), 0.5, device=device)
+    for options in ({}, {"temperature": 0.7, "top_k": 2, "top_p": 0.9, "min_p": 0.1}):
+        if sample_tokens(z, u, **options)[0].tolist() != [0, vocab - 1]:
+            raise RuntimeError("HIP sampling trial drew other tokens")
+
+
 def _available(like: torch.Tensor, kernel: str, key: int, trial,
                dtypes=(torch.bfloat16, torch.float16)) -> bool:
     if not like.is_cuda or like.dtype not in dtypes:
@@ -110,3 +150,21 @@ def hip_logprob_available(hidden: torch.Tensor) -> bool:
     fp16 on MFMA; fp32 and fp64 at their own precision)."""
     return _available(hidden, "hip_logprob", int(hidden.shape[-1]), logprob_trial,
                       (torch.bfloat16, torch.float16, torch.float32, torch.float64))
+
+
+def hip_distill_available(hidden: torch.Tensor) -> bool:
+    """Whether these hidden states may take the HIP distillation (the fused logprob's types)."""
+    return _available(hidden, "hip_distill", int(hidden.shape[-1]), distill_trial,
+                      (torch.bfloat16, torch.float16, torch.float32, torch.float64))
+
+
+def hip_embedding_available(weight: torch.Tensor) -> bool:
+    """Whether this table may take the HIP embedding (bf16, fp16 and fp32)."""
+    return _available(weight, "hip_embedding", int(weight.shape[-1]), embedding_trial,
+                      (torch.bfloat16, torch.float16, torch.float32))
+
+
+def hip_sampling_available(logits: torch.Tensor) -> bool:
+    """Whether these logits may take the HIP sampling (bf16, fp16 and fp32)."""
+    return _available(logits, "hip_sampling", int(logits.shape[-1]), sampling_trial,
+                      (torch.bfloat16, torch.float16, torch.float32))

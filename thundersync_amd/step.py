@@ -36,6 +36,7 @@ from dataclasses import dataclass
 import torch
 
 from .attention import forest_context
+from .fused_distill import fused_distill
 from .fused_logprob import fused_logprob
 
 # class-name fragments of modules that carry state along the sequence
@@ -122,6 +123,20 @@ def _project(hidden, weight, rows, targets, chunk):
     return fused_logprob(hidden if rows is None else hidden.index_select(0, rows), weight, targets, chunk=chunk)
 
 
+def _forest_hidden(model, plan, hidden_fn):
+    """``[P, D]`` hidden states of a plan's physical stream, one pass of the decoder stack."""
+    assert_supported(model)
+    if hidden_fn is None:
+        stack = base_model(model)
+
+        def hidden_fn(ids, pos):
+            out = stack(input_ids=ids[None], position_ids=pos[None], attention_mask=None, use_cache=False)
+            return out.last_hidden_state[0]
+
+    with forest_context(plan):
+        return hidden_fn(plan.token_ids, plan.position_ids)
+
+
 def forest_logprobs(model: torch.nn.Module, plan, *, weight: torch.Tensor | None = None, chunk: int = 1024,
                     hidden_fn=None, return_stats: bool = False, gate: bool = True):
     """``log pi(token | context)`` of every scored token in logical order: ``[L]``,
@@ -133,16 +148,7 @@ def forest_logprobs(model: torch.nn.Module, plan, *, weight: torch.Tensor | None
     ``return_stats`` the result is ``(logprobs, StepStats)``.
     """
     head = weight if weight is not None else unembedding(model)
-    assert_supported(model)
-    if hidden_fn is None:
-        stack = base_model(model)
-
-        def hidden_fn(ids, pos):
-            out = stack(input_ids=ids[None], position_ids=pos[None], attention_mask=None, use_cache=False)
-            return out.last_hidden_state[0]
-
-    with forest_context(plan):
-        hidden = hidden_fn(plan.token_ids, plan.position_ids)  # [P, D]
+    hidden = _forest_hidden(model, plan, hidden_fn)
     src, tgt = plan.score_src, plan.score_tgt
     if gate:
         lp = _project(hidden, head, src, tgt, chunk)
@@ -166,6 +172,29 @@ def forest_logprobs(model: torch.nn.Module, plan, *, weight: torch.Tensor | None
         logical_scored=int(plan.logical_to_slot.numel()),
     )
     return logical, stats
+
+
+def forest_distillation(model: torch.nn.Module, plan, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                        temperature: float = 1.0, weight: torch.Tensor | None = None, chunk: int = 1024,
+                        hidden_fn=None) -> torch.Tensor:
+    """Divergence from a teacher's top tokens at every scored token in logical
+    order, ``[L]``: :func:`forest_logprobs`' gated form with
+    :func:`~thundersync_amd.fused_distill.fused_distill` in the logprob's place.
+
+    ``teacher_ids`` and ``teacher_logits`` are ``[S, K]``, a row for each of the
+    plan's scored positions (``plan.score_src``): siblings that share a token
+    share the teacher's row for it too.  :func:`split_by_trajectory` splits the
+    result as it does logprobs.
+    """
+    src = plan.score_src
+    if teacher_ids.dim() != 2 or teacher_ids.shape[0] != src.numel():
+        raise ValueError(f"teacher_ids must have one row per scored position ({src.numel()}), got "
+                         f"{tuple(teacher_ids.shape)}")
+    head = weight if weight is not None else unembedding(model)
+    hidden = _forest_hidden(model, plan, hidden_fn)
+    loss = fused_distill(hidden.index_select(0, src), head, teacher_ids, teacher_logits, temperature=temperature,
+                         chunk=chunk)
+    return loss.index_select(0, plan.logical_to_slot)
 
 
 def split_by_trajectory(plan, logical: torch.Tensor) -> dict[int, torch.Tensor]:
