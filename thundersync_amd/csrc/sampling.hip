@@ -738,24 +738,26 @@ __global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int 
   if (t == 0) found = Bins{kBins, kBins, kBins, 0, 0, 0, 0};
   uint32_t c[PER] = {}, cs = 0;
   uint64_t m[PER] = {}, ms = 0;
-  // all loads before the first use: other XCDs wrote them (past the shares, the last again)
+  // all loads before the first use: other XCDs wrote them
   uint32_t cp[kBinParts][PER] = {};
   uint64_t mp[kBinParts][PER] = {};
 #pragma unroll
   for (int part = 0; part < kBinParts; ++part) {
-    const int64_t base = min(part, parts - 1) * kBins + PER * t;
+    if (part < parts) {
+      const int base = part * kBins + PER * t;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (o.by_k) cp[part][i] = count[base + i];
-      if (o.by_p) mp[part][i] = mass[base + i];
+      for (int i = 0; i < PER; ++i) {
+        if (o.by_k) cp[part][i] = count[base + i];
+        if (o.by_p) mp[part][i] = mass[base + i];
+      }
     }
   }
 #pragma unroll
   for (int part = 0; part < kBinParts; ++part)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      c[i] += part < parts ? cp[part][i] : 0;
-      m[i] += part < parts ? mp[part][i] : 0;
+      c[i] += cp[part][i];
+      m[i] += mp[part][i];
     }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
