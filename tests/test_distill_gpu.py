@@ -184,6 +184,42 @@ def test_gradcheck(cuda, n, chunk):
                                     atol=1e-8)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_repeated_rows(cuda, dtype):
+    """One hidden row for every teacher's row, one teacher's row for every hidden row: expanded tensors."""
+    h, w, ids, teacher, grad = inputs(12, 40, 300, 5, dtype, ragged=False)
+    want = ref.distill(h[:1].expand(12, 40), w, ids[:1].expand(12, 5), teacher[:1].expand(12, 5), grad)
+    bound = ref.bounds(want, dtype, 5)
+    for train in (False, True):
+        hc = h[:1].to(cuda).requires_grad_()
+        wc = w.to(cuda).requires_grad_(train)
+        loss = fused_distill(hc.expand(12, 40), wc, ids[:1].to(cuda).expand(12, 5), teacher[:1].to(cuda).expand(12, 5))
+        (dh,) = torch.autograd.grad(loss, hc, grad.to(cuda))
+        check(loss, want["loss"], bound["loss"], "loss")
+        # twelve rounded gradients added by torch, in the element type
+        u = torch.finfo(dtype).eps / 2
+        total = want["dh"].sum(0, keepdim=True)
+        check(dh, total, bound["dh"].sum(0, keepdim=True) + 12 * u * want["dh"].abs().sum(0, keepdim=True), "dh")
+    one = fused_distill(h[:1].to(cuda).expand(1, 40), w.to(cuda), ids[:1].to(cuda), teacher[:1].to(cuda))
+    check(one, want["loss"][:1], bound["loss"][:1], "one row")
+
+
+def test_two_calls_at_once(cuda):
+    """Calls on two streams, each with its own gradients, interleaved: neither sees the other."""
+    case = [t.to(cuda) for t in inputs(200, 64, 2000, 9, BF16)]
+    want = [run(cuda, *case, train) for train in (False, True)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(run(cuda, *case, bool(i)))
+    torch.cuda.synchronize()
+    for results, w in zip(got, want):
+        assert all(torch.equal(a, b) for r in results for a, b in zip(r, w))
+
+
 def test_no_rows(cuda):
     for dtype in (BF16, FP32):
         h, w, ids, teacher, grad = inputs(0, 16, 40, 3, dtype)

@@ -132,6 +132,39 @@ def test_padding_and_ids_outside_the_table(cuda, monkeypatch):
         embedding(ids.to(cuda), wc)
 
 
+def test_tables_of_one_row_and_none(cuda):
+    w = torch.randn(1, 24, device=cuda).to(BF16).requires_grad_()
+    ids = torch.zeros(5000, dtype=torch.int64, device=cuda)
+    out = embedding(ids, w)
+    assert same_bits(out, ref.lookup(ids.cpu(), w.detach().cpu()))
+    dout = torch.randn(5000, 24, device=cuda).to(BF16)
+    (grad,) = torch.autograd.grad(out, w, dout)
+    check_gradient(grad, ids.cpu(), dout.cpu(), 1)
+    (grad,) = torch.autograd.grad(embedding(ids, w, padding_idx=0), w, dout)  # no token takes part
+    assert grad.abs().sum() == 0
+    empty = torch.zeros(0, 8, device=cuda, requires_grad=True)
+    out = embedding(ids[:3], empty)
+    assert out.shape == (3, 8) and out.isnan().all()
+    assert torch.autograd.grad(out.sum(), empty)[0].shape == (0, 8)
+
+
+def test_backward_twice(cuda):
+    ids, w, dout = (t.to(cuda) for t in inputs(3000, 500, 40, FP16))
+    w.requires_grad_()
+    out = embedding(ids, w)
+    one = torch.autograd.grad(out, w, dout, retain_graph=True)[0]
+    assert torch.equal(one, torch.autograd.grad(out, w, dout)[0])
+
+
+@pytest.mark.parametrize("n, v, d", [(300000, 1200, 16), (2048, 511, 8), (2049, 512, 8), (20000, 262143, 8)])
+def test_sort_sizes(cuda, n, v, d):
+    """Many tiles, exactly one, one more, and a vocabulary at a digit's edge."""
+    print(f"embedding sort n={n} v={v}", flush=True)
+    ids, w, dout = inputs(n, v, d, FP32, "any", seed=3)
+    got = embedding_backward(ids.to(cuda), dout.to(cuda), v)
+    check_gradient(got, ids, dout, v)
+
+
 def test_gradient_against_differences(cuda):
     """The lookup is linear: <dW, X> = <dout, lookup(X)>."""
     ids, w, dout = (t.to(cuda) for t in inputs(300, 64, 32, FP32))

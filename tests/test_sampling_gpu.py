@@ -183,6 +183,54 @@ def test_per_row_values_that_are_no_options(cuda):
     assert got == want
 
 
+def test_more_rows_than_a_set_of_launches(cuda):
+    """5000 rows with options of their own: the second set starts where the first ends."""
+    print("sample 5000 rows", flush=True)
+    b, v = 5000, 130
+    z, u = logits(b, v, FP16, seed=9)
+    g = torch.Generator().manual_seed(2)
+    rand = lambda: torch.rand(b, generator=g)  # noqa: E731
+    check(cuda, z, u, temperature=torch.where(rand() < 0.2, 0.0, 0.3 + rand()),
+          top_k=torch.randint(0, v + 5, (b,), generator=g).int(), top_p=0.3 + 0.8 * rand(), min_p=0.1 * rand())
+    check(cuda, z, u)
+    check(cuda, z, u, min_p=0.2)
+
+
+def test_endless_temperature_per_row(cuda):
+    """A row's infinite temperature draws evenly from what is kept, a denormal one the maximum."""
+    z = torch.randn(3, 20000, generator=torch.Generator().manual_seed(0))
+    z[:, ::3] = -math.inf
+    u = torch.full((3,), 0.6)
+    for options in ({}, {"top_k": 100}, {"top_p": 0.5}, {"min_p": 0.2}, {"top_k": 9000, "top_p": 0.9}):
+        check(cuda, z, u, temperature=torch.tensor([math.inf, 1e-40, 3e38]), **options)
+
+
+@pytest.mark.parametrize("b", [4, 5])
+def test_few_and_many_rows(cuda, b):
+    """Either side of the rows for which the border is searched in a launch of its own: the same tokens."""
+    z, u = logits(5, 60000, BF16, seed=21)
+    options = {"top_k": 300, "top_p": 0.8, "temperature": 1.2}
+    want = sample_tokens(z.to(cuda), u.to(cuda), **options)
+    got = sample_tokens(z[:b].to(cuda), u[:b].to(cuda), **options)
+    assert torch.equal(got[0], want[0][:b]) and torch.equal(got[1], want[1][:b])
+    check(cuda, z[:b], u[:b], **options)
+
+
+def test_two_calls_at_once(cuda):
+    z, u = (t.to(cuda) for t in logits(40, 50257, BF16, seed=8))
+    options = [{"top_p": 0.9}, {"top_k": 70, "temperature": 0.7}]
+    want = [sample_tokens(z, u, **o) for o in options]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(5):
+        for stream, o in zip(streams, options):
+            with torch.cuda.stream(stream):
+                got.append(sample_tokens(z, u, **o))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
 def test_frequencies(cuda):
     """Equally spaced random numbers draw every token as often as its probability says."""
     z = torch.randn(1, 300, generator=torch.Generator().manual_seed(0))

@@ -720,19 +720,18 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(Args a, Space sp) {
 }
 
 // ---------------------------------------------------------------------------
-// search: the border bins from a row's shares of the histogram, consecutive bins a thread
+// search: the border bins from a row's shares of the histogram, consecutive bins a thread.
+// A launch of its own, or for few rows the beginning of every gather work-group: a launch less
+// (one row: gather and search 8.5 + 12.5 -> 15.9 us, the pass 47 -> 45), where over many rows the
+// shares read again by each cost more (64 rows: gather 27 -> 42 us against a search of 9.6).
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int parts) {
+constexpr int kFewRows = 4;
+__device__ __forceinline__ void search_bins(const Space& sp, int64_t r, const RowOptions& o, int parts, Bins& found) {
   __shared__ uint64_t wave_m[kThreads / 64];
   __shared__ uint32_t wave_c[kThreads / 64];
-  __shared__ Bins found;
   __shared__ uint64_t bin_mass;  // of bin k
   constexpr int PER = kBins / kThreads;
-  const int64_t r = blockIdx.x;
   const int t = threadIdx.x;
-  const RowOptions o(a, r);
-  if (!o.by_k && !o.by_p) return;
-  if (RowStats(sp.stats + r * sp.slices, sp.slices).empty()) return;  // it has no histogram
   const uint32_t* count = sp.count + r * kBinParts * kBins;
   const uint64_t* mass = sp.mass + r * kBinParts * kBins;
   if (t == 0) found = Bins{kBins, kBins, kBins, 0, 0, 0, 0};
@@ -814,14 +813,25 @@ __global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int 
     }
     __syncthreads();
   }
-  if (t == 0) sp.bins[r] = found;
+}
+
+__global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int parts) {
+  __shared__ Bins found;
+  const int64_t r = blockIdx.x;
+  const RowOptions o(a, r);
+  if (!o.by_k && !o.by_p) return;
+  if (RowStats(sp.stats + r * sp.slices, sp.slices).empty()) return;  // it has no histogram
+  search_bins(sp, r, o, parts, found);
+  __syncthreads();
+  if (threadIdx.x == 0) sp.bins[r] = found;
 }
 
 // ---------------------------------------------------------------------------
 // gather: per slice the sum of the weights above the border bins, and their logits
 // ---------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(kThreads) void gather_kernel(Args a, Space sp) {
+template <typename T, bool SEARCH>
+__global__ __launch_bounds__(kThreads) void gather_kernel(Args a, Space sp, int parts) {
+  __shared__ Bins found;
   __shared__ double table[kTable];
   __shared__ uint64_t cand[kCandidates];
   __shared__ uint32_t n_cand, cand_at;
@@ -834,7 +844,12 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Args a, Space sp) {
   if (t == 0) n_cand = 0;
   fill_table(table);
   const Weights w = weights_of(table, s.top, s.low, o.temp, a.fixed);
-  const Bins f = o.by_k || o.by_p ? sp.bins[r] : Bins{kBins, kBins, kBins, 0, 0, 0, 0};
+  if (SEARCH && (o.by_k || o.by_p)) {
+    search_bins(sp, r, o, parts, found);
+    __syncthreads();
+    if (blockIdx.x == 0 && t == 0) sp.bins[r] = found;  // the draw's
+  }
+  const Bins f = !o.by_k && !o.by_p ? Bins{kBins, kBins, kBins, 0, 0, 0, 0} : SEARCH ? found : sp.bins[r];
   const Row<T> row(a.logits, a.ld, r, a.vocab);
   for (int slice = blockIdx.x; slice < sp.slices; slice += gridDim.x) {
     double sum = 0.;
@@ -1245,18 +1260,22 @@ void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bin
   auto per_row = [&](int64_t all, int64_t most) {  // work-groups a row, for about `all` in the launch
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)sp.slices, (all + rows / 2) / rows}));
   };
+  const unsigned parts = per_row(1024, kBinParts);
   if (bins) {
-    const unsigned parts = per_row(1024, kBinParts);
-    {
-      TimedLaunch timed_("sampling.bins_kernel", s);
-      hipLaunchKernelGGL(bins_kernel<T>, dim3(parts, (unsigned)rows), dim3(kThreads), 0, s, a, sp);
-    }
+    TimedLaunch timed_("sampling.bins_kernel", s);
+    hipLaunchKernelGGL(bins_kernel<T>, dim3(parts, (unsigned)rows), dim3(kThreads), 0, s, a, sp);
+  }
+  if (bins && rows > kFewRows) {
     TimedLaunch timed_("sampling.search_kernel", s);
     hipLaunchKernelGGL(search_kernel, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp, (int)parts);
   }
   if (filters) {
     TimedLaunch timed_("sampling.gather_kernel", s);
-    hipLaunchKernelGGL(gather_kernel<T>, dim3(per_row(1024, sp.slices), (unsigned)rows), dim3(kThreads), 0, s, a, sp);
+    const dim3 gathers(per_row(1024, sp.slices), (unsigned)rows), threads(kThreads);
+    if (bins && rows <= kFewRows)
+      hipLaunchKernelGGL((gather_kernel<T, true>), gathers, threads, 0, s, a, sp, (int)parts);
+    else
+      hipLaunchKernelGGL((gather_kernel<T, false>), gathers, threads, 0, s, a, sp, (int)parts);
   }
   {
     TimedLaunch timed_("sampling.draw_kernel", s);

@@ -130,6 +130,11 @@ def _live_rows(h, state):
     return out
 
 
+def _apart(t):
+    """``t`` with rows that do not overlap (an expanded row is copied)."""
+    return t if t.stride(0) >= t.shape[1] or t.shape[0] <= 1 else t.contiguous()
+
+
 class _Rows:
     """A call's tensors as its kernels take them, and what the kernels find out about each row."""
 
@@ -148,7 +153,7 @@ class _Rows:
             self.h, self.w = _unit_stride(hidden), _unit_stride(weight)
             self.ld = (weight.shape[0] + 3) // 4 * 4  # rows of whole 16-byte vectors
         else:
-            self.h, self.w = _rows_ok(_pad_dim(hidden)), _rows_ok(_pad_dim(weight))
+            self.h, self.w = (_rows_ok(_pad_dim(_apart(t))) for t in (hidden, weight))
             self.ld = (weight.shape[0] + 7) // 8 * 8
         self.n, self.d = self.h.shape
         self.v = weight.shape[0]
