@@ -136,11 +136,10 @@ struct Weights {
   double fixed;
   float top_f;
   float bins;     // bins per unit of logit
-  bool simple;    // top and units are finite
-  // where `simple`; -inf gives 2^-1000, which adds nothing to a sum that holds the maximum's 1
-  __device__ __forceinline__ double of_simple(float x) const {
+  // 2^(max(y, -1000 kTable) / kTable), for y of 0 or less; NaN counts as the least
+  __device__ __forceinline__ double power(double y) const {
     constexpr double kRound = 6755399441055744., kL = 0.693147180559945309417 / kTable;
-    const double y = fmax(((double)x - top) * units, -1000. * kTable);
+    y = fmax(y, -1000. * kTable);
     const double k = y + kRound;
     const double t = y - (k - kRound);
     const double e = fma(fma(fma(fma(t, kL * kL * kL * kL / 24, kL * kL * kL / 6), t, kL * kL / 2), t, kL), t, 1.);
@@ -148,18 +147,21 @@ struct Weights {
     const double p = table[n & (kTable - 1)] * e;
     return __hiloint2double(__double2hiint(p) + ((n & -kTable) << 12), __double2loint(p));
   }
+  // a logit's weight, 0 where it is more than 1000 octaves below the maximum (or -inf, or below an infinite one)
   __device__ __forceinline__ double of(float x) const {
-    if (x == top_f) return 1.;
-    if (x == -inf() || top_f == inf()) return 0.;
-    if (!simple) return units > 0. ? 0. : 1.;  // T so small, or so large, that nothing is between
-    return ((double)x - top) * units < -1000. * kTable ? 0. : of_simple(x);
+    const double y = ((double)x - top) * units, p = power(fmin(y, 0.));
+    return y < -1000. * kTable ? 0. : p;
   }
+  // the same with 2^-1000 for 0, which adds nothing to a sum that holds the maximum's 1 and no whole number
+  __device__ __forceinline__ double of_any(float x) const { return power(fmin(((double)x - top) * units, 0.)); }
+  // and where the maximum is finite
+  __device__ __forceinline__ double of_finite(float x) const { return power(((double)x - top) * units); }
   // a weight as a whole number of 1 / fixed (at most 2^50), by an addition whose rounding leaves it in the low bits
   __device__ __forceinline__ uint64_t whole(double weight) const {
     const double y = fma(weight, fixed, 4503599627370496.);
     return ((uint64_t)(__double2hiint(y) & 0xfffff) << 32) | (uint32_t)__double2loint(y);
   }
-  __device__ __forceinline__ uint64_t fixed_of(float x) const { return whole(of(x)); }
+  __device__ __forceinline__ uint64_t fixed_of(float x) const { return whole(of_any(x)); }
   // falls with the logit, equal for equal logits
   __device__ __forceinline__ int bin(float x) const {
     const int b = (int)fminf((top_f - x) * bins, (float)(kBins - 1));
@@ -170,11 +172,12 @@ struct Weights {
 __device__ __forceinline__ Weights weights_of(const double* table, float top, float low, double temp, double fixed) {
   Weights w;
   w.table = table;
-  w.top = (double)top;
+  // an infinite maximum: above every finite logit, and at its equals (whose difference is clamped to 0)
+  w.top = top < inf() ? (double)top : 1e300;
   w.top_f = top;
-  w.units = kTable * (1.4426950408889634074 / temp);
+  // a T so small or so large that nothing, or everything, is the maximum's equal keeps finite products
+  w.units = fmin(fmax(kTable * (1.4426950408889634074 / temp), 1e-300), 1e300);
   w.fixed = fixed;
-  w.simple = top < inf() && w.units > 0. && w.units < __builtin_huge_val();
   const float octave = (float)(0.693147180559945309 * temp);  // in units of logit
   w.bins = fminf(fmaxf(kBinsPerOctave / octave, (float)kBins / (top - low)), 1e30f);
   return w;
@@ -649,16 +652,16 @@ __global__ __launch_bounds__(kMaxThreads, 5) void maxima_kernel(Args a, Space sp
   fill_table(table);
   const Weights w = weights_of(table, top, low, o.temp, a.fixed);
   double sum = 0.;
-  if (w.simple) {
+  if (top < inf()) {
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-      for (int j = 0; j < kGroup; ++j) sum += w.of_simple(x[i][j]);
+      for (int j = 0; j < kGroup; ++j) sum += w.of_finite(x[i][j]);
   } else {
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-      for (int j = 0; j < kGroup; ++j) sum += w.of(x[i][j]);
+      for (int j = 0; j < kGroup; ++j) sum += x[i][j] == inf() ? 1. : 0.;
   }
   sum = block_sum<N, double>(sum, per_wave);
   if (t == 0) sp.sums[(r * sp.slices + slice) * kSums] = sum;
@@ -689,28 +692,24 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(Args a, Space sp) {
   const Weights w = weights_of(table, s.top, s.low, o.temp, a.fixed);
   const Row<T> row(a.logits, a.ld, r, a.vocab);
   // no branch in a group's eight, so that their chains overlap: -inf falls into the last bin with nothing
-  auto fill = [&](auto weight) __attribute__((always_inline)) {
-    for (int g = blockIdx.x * kThreads + t; g < row.groups; g += gridDim.x * kThreads) {
-      float x[kGroup];
-      row.load_raw(g, x);
-      int b[kGroup];
+  for (int g = blockIdx.x * kThreads + t; g < row.groups; g += gridDim.x * kThreads) {
+    float x[kGroup];
+    row.load_raw(g, x);
+    int b[kGroup];
 #pragma unroll
-      for (int j = 0; j < kGroup; ++j) b[j] = w.bin(x[j]);
-      if (o.by_k) {
+    for (int j = 0; j < kGroup; ++j) b[j] = w.bin(x[j]);
+    if (o.by_k) {
 #pragma unroll
-        for (int j = 0; j < kGroup; ++j) atomicAdd(&count[b[j]], x[j] == -inf() ? 0u : 1u);
-      }
-      if (o.by_p) {
-        uint64_t m[kGroup];
-#pragma unroll
-        for (int j = 0; j < kGroup; ++j) m[j] = w.whole(weight(x[j]));
-#pragma unroll
-        for (int j = 0; j < kGroup; ++j) atomicAdd((unsigned long long*)&mass[b[j]], (unsigned long long)m[j]);
-      }
+      for (int j = 0; j < kGroup; ++j) atomicAdd(&count[b[j]], x[j] == -inf() ? 0u : 1u);
     }
-  };
-  if (w.simple) fill([&](float x) { return w.of_simple(x); });
-  else fill([&](float x) { return w.of(x); });
+    if (o.by_p) {
+      uint64_t m[kGroup];
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) m[j] = w.fixed_of(x[j]);
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) atomicAdd((unsigned long long*)&mass[b[j]], (unsigned long long)m[j]);
+    }
+  }
   __syncthreads();
   const int64_t base = (r * kBinParts + blockIdx.x) * kBins;
   for (int i = t; i < kBins; i += kThreads) {
@@ -830,7 +829,7 @@ __global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int 
 // gather: per slice the sum of the weights above the border bins, and their logits
 // ---------------------------------------------------------------------------
 template <typename T, bool SEARCH>
-__global__ __launch_bounds__(kThreads) void gather_kernel(Args a, Space sp, int parts) {
+__global__ __launch_bounds__(kThreads, SEARCH ? 4 : 8) void gather_kernel(Args a, Space sp, int parts) {
   __shared__ Bins found;
   __shared__ double table[kTable];
   __shared__ uint64_t cand[kCandidates];
@@ -868,18 +867,10 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Args a, Space sp, int 
         found_one |= b[j] < kBins && ((b[j] >= f.lo && b[j] <= f.hi) || b[j] == f.k);
       }
       if (least < f.lo) {
-        if (w.simple) {
 #pragma unroll
-          for (int j = 0; j < kGroup; ++j) {
-            const double y = w.of_simple(x[j]);
-            sum += b[j] < f.lo && y >= o.min_p ? y : 0.;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kGroup; ++j) {
-            const double y = w.of(x[j]);
-            sum += b[j] < f.lo && y >= o.min_p ? y : 0.;
-          }
+        for (int j = 0; j < kGroup; ++j) {
+          const double y = w.of(x[j]);
+          sum += b[j] < f.lo && y >= o.min_p ? y : 0.;
         }
       }
       if (found_one) {
@@ -934,7 +925,7 @@ __device__ __forceinline__ void draw_token(const Args& a, int64_t r, const Row<T
 #pragma unroll
     for (int j = 0; j < kGroup; ++j) {
       run += y[q][j];
-      if (y[q][j] > 1e-300) {  // (of_simple's 2^-1000 stands for nothing)
+      if (y[q][j] > 0.) {
         last = row.first(g0 + q) + j;
         last_y = y[q][j];
         if (hit < 0 && run > target) {
@@ -949,8 +940,11 @@ __device__ __forceinline__ void draw_token(const Args& a, int64_t r, const Row<T
     s.n_cand = -1;
   }
   __syncthreads();
-  if (hit >= 0) atomicMin(&s.token, hit);
-  if (last >= 0) atomicMax(&s.n_cand, last);
+  // (lanes are in index order: a wave's first lane with a hit, its last with any)
+  const uint64_t hits = __builtin_amdgcn_ballot_w64(hit >= 0), lasts = __builtin_amdgcn_ballot_w64(last >= 0);
+  const int lane = threadIdx.x & 63;
+  if (hit >= 0 && lane == __ffsll((unsigned long long)hits) - 1) atomicMin(&s.token, hit);
+  if (last >= 0 && lane == 63 - __clzll((long long)lasts)) atomicMax(&s.n_cand, last);
   __syncthreads();
   const bool none = s.token == 0x7fffffff;
   const int token = none ? s.n_cand : s.token;
@@ -1145,7 +1139,7 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
     }
     __syncthreads();
     const Weights v = weights_of(s.table, top, rs.low, o.temp, a.fixed);
-    draw_token<T, N>(a, r, row, s.bin, [&](float x, int) { return v.simple ? v.of_simple(x) : v.of(x); }, s);
+    draw_token<T, N>(a, r, row, s.bin, [&](float x, int) { return v.of(x); }, s);
     return;
   }
   uint64_t border = 0;  // the last kept (key, index); 0: no border
@@ -1214,7 +1208,7 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
   draw_token<T, N>(a, r, row, s.bin, [&](float x, int i) {
     const uint64_t me = ((uint64_t)key_of(x) << 32) | (0xffffffffu - (uint32_t)i);
     if (me < border) return 0.;
-    const double y = w.simple ? w.of_simple(x) : w.of(x);
+    const double y = w.of(x);
     return y >= o.min_p ? y : 0.;
   }, s);
 }
