@@ -1251,8 +1251,12 @@ void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bin
     if (bins) hipLaunchKernelGGL((maxima_kernel<T, true>), grid, block, 0, s, a, sp);
     else hipLaunchKernelGGL((maxima_kernel<T, false>), grid, block, 0, s, a, sp);
   }
-  auto per_row = [&](int64_t all, int64_t most) {  // work-groups a row, for about `all` in the launch
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)sp.slices, (all + rows / 2) / rows}));
+  // work-groups a row, for about `all` in the launch, and no more than the slices fill evenly (19 slices over 16
+  // work-groups end when the three that have two do: 10 of two)
+  auto per_row = [&](int64_t all, int64_t most) {
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)sp.slices, (all + rows / 2) / rows}));
+    const int64_t each = (sp.slices + parts - 1) / parts;
+    return (unsigned)((sp.slices + each - 1) / each);
   };
   const unsigned parts = per_row(1024, kBinParts);
   if (bins) {
