@@ -44,7 +44,8 @@ template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, c
 }
 
 // ---------------------------------------------------------------------------
-// lookup; a token id outside [0, vocab) gives a row of NaN
+// lookup; a token id outside [0, vocab) gives a row of NaN.  Bound by HBM: 65536 fp32 rows of
+// 1024 in 81 us (268 MB written, 166 MB fetched: 5.4 TB/s), 16384 bf16 rows of 4096 in 46 us.
 // ---------------------------------------------------------------------------
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(const int64_t* __restrict__ ids, int64_t n,
@@ -69,7 +70,9 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(const int64_t* __restr
 // id) is `vocab`.  A pass is two launches, of the tiles' digit counts and of their placement,
 // or with one tile all passes are one launch in LDS.  The sort occupies a few CUs, so the
 // rest of each launch's grid writes its share of the gradient's zeros: a training batch's
-// sort (16384 tokens, 48 us by itself) then costs nothing beside the zeros' 256 us.
+// sort (16384 tokens, 48 us by itself) then costs nothing beside them.  The four launches that
+// write a [151936, 4096] bf16 gradient's 1.24 GB of zeros take 225 us (5.5 TB/s); the one launch
+// of 500 tokens, with [50257, 2560]'s 257 MB, 37 us (6.9 TB/s).
 // ---------------------------------------------------------------------------
 struct SortArgs {
   const int64_t* ids;     // first pass: key from the ids, position the index
@@ -270,7 +273,10 @@ __global__ __launch_bounds__(kThreads) void sort_tile_kernel(SortArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// sums of the rows of dout over runs of equal ids
+// sums of the rows of dout over runs of equal ids.  A work-group takes a chunk of sorted
+// positions and, with few rows of output a chunk, is bound by the latency of its gathered rows:
+// eight rows are loaded ahead of the sums.  65536 fp32 rows of 1024: 96 us (333 MB, 3.5 TB/s);
+// 16384 bf16 rows of 4096: 70 us; 500: 6 us.  The join: 12, 9 and 4 us.
 // ---------------------------------------------------------------------------
 struct ReduceArgs {
   const uint32_t* key;  // sorted ids

@@ -572,7 +572,9 @@ struct RowStats {
 
 // ---------------------------------------------------------------------------
 // maxima: one slice, held in registers; a row without filters gets its slice's sum of
-// weights, relative to the slice's own maximum, from the same read
+// weights, relative to the slice's own maximum, from the same read.  With filters bound by the
+// launch and the read (64 rows of 151936 fp32 logits: 9 us, 4.4 TB/s), without by the fp64
+// weights' instructions (512 bf16 rows of 151936: 69 us, 2.3 TB/s; the read alone is 30 at a copy's rate).
 // ---------------------------------------------------------------------------
 template <typename T, bool BINS>
 __global__ __launch_bounds__(kMaxThreads, 5) void maxima_kernel(Args a, Space sp) {
@@ -671,7 +673,9 @@ __global__ __launch_bounds__(kMaxThreads, 5) void maxima_kernel(Args a, Space sp
 // bins: a work-group's share of the row into a histogram of its own, counts where top_k
 // asks for them and mass where top_p does.  (Shares added to one histogram by atomics, or added
 // up by every gather work-group, cost as much as the logits; a last work-group that adds them
-// waits for the XCDs' caches to be written back.)  Bound by the weights' instructions.
+// waits for the XCDs' caches to be written back.)  Bound by the weights' instructions and
+// the histogram's LDS atomics (bank conflicts 14 % of the LDS cycles): 17 us at 64 rows of 151936
+// with top_p, 38 at 333 of 50257 with every option.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kThreads) void bins_kernel(Args a, Space sp) {
@@ -826,7 +830,8 @@ __global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int 
 }
 
 // ---------------------------------------------------------------------------
-// gather: per slice the sum of the weights above the border bins, and their logits
+// gather: per slice the sum of the weights above the border bins, and their logits.  21 us
+// at 64 rows of 151936, 28 at 333 of 50257, 13 with the search at one row.
 // ---------------------------------------------------------------------------
 template <typename T, bool SEARCH>
 __global__ __launch_bounds__(kThreads, SEARCH ? 4 : 8) void gather_kernel(Args a, Space sp, int parts) {
@@ -1089,6 +1094,8 @@ __device__ __forceinline__ void slow_row(const Args& a, int64_t r, const Row<T>&
   }, s);
 }
 
+// draw: one work-group a row.  Latency: the sort of its candidates, the sum over the slices and
+// the one slice read again follow one another: 11 us at one row, 18 at 64, 13 at 512 without filters.
 template <typename T>
 __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
   constexpr int N = kDrawThreads;
