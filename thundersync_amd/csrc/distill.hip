@@ -8,12 +8,12 @@
 //
 // teacher_kernel turns each row's slots into (token, p).  16-bit types: stats_kernel reduces
 // the logits of a 256-row vocabulary tile to (max, sum exp) per token in its MFMA epilogue and,
-// where a gradient follows, stores the tile's exponentials in the element type;
+// with a frozen head, stores the tile's exponentials in the element type;
 // scores_kernel takes the logits at the slots' tokens as dot products; loss_kernel merges the
 // tiles and sums the slots; finish_kernel scales the exponentials to q, in one pass over
 // 2 bytes an entry in place of a second product of 2 D flops an entry, and writes the slots'
-// entries from their fp32 logits.  Where the stored block would outgrow its bound,
-// dlogits_kernel forms it from the logits again.  fp32 and fp64: the logits of a block of
+// entries from their fp32 logits.  With a trainable head, whose gradient waits for the
+// upstream one, dlogits_kernel forms the logits again in the backward.  fp32 and fp64: the logits of a block of
 // rows by the exact product, then one work-group a row.  The vector-Jacobian products with W
 // and h are the fused logprob's.  Bound by the products (the fused logprob's GEMM core).
 #include <algorithm>

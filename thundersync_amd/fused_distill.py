@@ -20,16 +20,20 @@ part in its gradient), as a target of the fused logprob does;
 ``THUNDERSYNC_CHECK_TARGETS=1`` checks the ids first and raises.
 
 A block of rows (:func:`~thundersync_amd.fused_logprob.backward_block_rows` of
-``chunk``) has its ``[rows, V]`` block in the element type once, and that
-bounds the memory.  The logits are formed once:
+``chunk``) has its ``[rows, V]`` block in the element type, one at a time:
 
 * no gradient: the tiles' statistics alone, for all rows;
 * a frozen weight: the forward goes on, block by block, from the stored
   exponentials to ``q - p`` and its product with the weight, ``[N, D]`` in
   fp32, which the backward multiplies by the upstream gradient (no block
   outlives the call, and 2 N V D flops of logits formed again are saved);
-* a trainable weight and one block of rows: the block is kept for the
-  backward, which needs the upstream gradient first;
+* a trainable weight and one block of rows: the backward, which has the
+  upstream gradient, wants the block that the forward stored.  It is kept where
+  the blocks of all losses that wait for their backward then hold no more
+  than the weight does; otherwise the backward stores it again, by the same
+  kernels and with the same bits (:class:`_KeptBlocks`).  Its 16-bit entries
+  are rounded twice, as exponentials and with the row's factor: 2 bytes of
+  memory an entry, where the logits that would be rounded once take 4;
 * a trainable weight and more rows: the backward forms the logits again, block
   by block, as the fused logprob does.
 
@@ -44,8 +48,11 @@ at that precision).  GPU only: other dtypes and CPU tensors raise.
 
 from __future__ import annotations
 
+import copy
 import math
 import os
+import threading
+import weakref
 
 import torch
 
@@ -135,6 +142,29 @@ def _apart(t):
     return t if t.stride(0) >= t.shape[1] or t.shape[0] <= 1 else t.contiguous()
 
 
+class _KeptBlocks:
+    """The blocks that losses keep until their backward, so that together they hold no more than a weight does (a
+    1999 x 151936 block is 0.6 GB, beside a weight of D 2048 as large: a batch scored in sixteen calls kept 9.7 GB).
+    Kept, a step of that size takes 3.85 ms; stored again in the backward 5.07."""
+
+    def __init__(self):
+        self._lock, self._alive = threading.Lock(), []
+
+    def take(self, rows, ld, like, limit):
+        """An empty ``[rows, ld]`` block like ``like``, or None where it would take the blocks past ``limit`` bytes."""
+        with self._lock:
+            self._alive = [r for r in self._alive if r() is not None]
+            held = sum(t.nbytes for t in (r() for r in self._alive) if t is not None and t.device == like.device)
+            if held + rows * ld * like.element_size() > limit:
+                return None
+            block = torch.empty(rows, ld, dtype=like.dtype, device=like.device)
+            self._alive.append(weakref.ref(block))  # lives as long as what autograd saves
+            return block
+
+
+_kept = _KeptBlocks()
+
+
 class _Rows:
     """A call's tensors as its kernels take them, and what the kernels find out about each row."""
 
@@ -218,6 +248,12 @@ class _Rows:
         )
         return ws[: ws_bytes // 2]
 
+    def stored_again(self, i, rows, block):
+        """``block`` and its tiles' maxima as a :meth:`forward` that kept them left them; what autograd saved stays."""
+        again = copy.copy(self)
+        again.slot_z, again.lse, again.loss = (torch.empty_like(t) for t in (self.slot_z, self.lse, self.lse))
+        return again.forward(i, rows, block)
+
     def finish(self, i, rows, block, maxima, grad, out):
         """``block`` (as :meth:`forward` left it) to the logits' gradient ``out`` (which may be the block)."""
         _lib.check(
@@ -254,13 +290,13 @@ def _forward(rows: _Rows, chunk, need_hidden, need_weight):
     n, dev = rows.n, rows.h.device
     block_rows = min(max(1, int(chunk)), max(n, 1)) if rows.exact else backward_block_rows(n, chunk)
     frozen = need_hidden and not need_weight
-    keep = need_weight and 0 < n <= block_rows
     if n == 0:
         return (torch.empty(0, rows.d, dtype=rows.dtype, device=dev),) if frozen else ()
-    if not (rows.exact or frozen or keep):
+    kept = _kept.take(n, rows.ld, rows.h, rows.w.nbytes) if need_weight and n <= block_rows else None
+    if kept is None and not (rows.exact or frozen):
         rows.forward(0, n, None)
         return ()
-    block = torch.empty(min(block_rows, n), rows.ld, dtype=rows.h.dtype, device=dev)
+    block = torch.empty(min(block_rows, n), rows.ld, dtype=rows.h.dtype, device=dev) if kept is None else kept
     unit = torch.empty(n, rows.d, dtype=rows.dtype, device=dev) if frozen else None
     ws = rows.unit_workspace({block_rows, n % block_rows or block_rows}) if frozen else None
     maxima = None
@@ -274,7 +310,7 @@ def _forward(rows: _Rows, chunk, need_hidden, need_weight):
                 rows.unit_gradient(i, size, block, unit, ws)
     if frozen:
         return (unit,)
-    return (block, maxima) if keep else ()
+    return () if kept is None else (kept, maxima)
 
 
 def _backward_frozen(unit, state, grad, temperature, dtype, d_in):
@@ -293,6 +329,7 @@ def _backward_trainable(rows: _Rows, grad, chunk, block, maxima):
     g = grad.to(rows.dtype).contiguous()
     h_weight = _live_rows(rows.h, rows.state)
     lib = _lib.require_library()
+    one = not rows.exact and rows.n <= backward_block_rows(rows.n, chunk)
 
     def dlogits(i, size, dl, ld):
         if block is not None:
@@ -300,6 +337,8 @@ def _backward_trainable(rows: _Rows, grad, chunk, block, maxima):
         elif rows.exact:
             rows.logits(i, size, dl)
             rows.finish(i, size, dl, None, g, dl)
+        elif one:
+            rows.finish(i, size, dl, rows.stored_again(i, size, dl), g, dl)
         else:
             _lib.check(
                 lib.ts_distill_dlogits(rows.row(i), rows.ldh, rows.w.data_ptr(), rows.ldw, size, rows.d, rows.v,
