@@ -532,26 +532,44 @@ int64_t ts_distill_fwd_workspace(int64_t rows, int64_t vocab);
 
 /* bf16 or fp16: loss, lse (of the logits over T, natural log) and slot_z (the
  * logits at the slots, not over T), all fp32.  hidden and weight as for
- * ts_logprob_fwd.  With exps not null the exponentials of (z - m) / T, m the
- * maximum of the row's tile of 256 vocabulary rows, are stored there in the
- * element type ([rows, ld_exps >= vocab rounded up to 8], pad columns zero); the
- * workspace then begins with the maxima, [ceil(vocab / 256), rows] floats. */
+ * ts_logprob_fwd.  With exps not null 2^(z log2(e) / T - r) are stored there in
+ * the element type ([rows, ld_exps >= vocab rounded up to 8], pad columns zero), r
+ * being the maximum over the row's tile of 256 vocabulary rows rounded up to a
+ * whole number; the workspace then begins with these, [ceil(vocab / 256), rows]
+ * floats.  With row_scale not null it takes, per row, what ts_distill_softmax
+ * and ts_distill_slots go by ([rows, 2]: the reference of the row's block, and
+ * the factor that makes the block the softmax). */
 int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
                    int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
                    float* slot_z, int64_t pitch, int64_t top, const int32_t* state, float* loss, float* lse,
-                   void* exps, int64_t ld_exps, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+                   void* exps, int64_t ld_exps, float* row_scale, void* workspace, int64_t workspace_bytes, int dtype,
+                   void* stream);
+
+/* bf16 or fp16, in place: ts_distill_fwd's exps to one reference a row, so that
+ * the softmax is row_scale[n, 1] times the block, with zeros at the slots'
+ * tokens and in rows whose state is 0.  Entries are scaled by powers of two. */
+int ts_distill_softmax(void* block, int64_t ld_block, const float* tile_ref, const float* row_scale, int64_t rows,
+                       int64_t vocab, const int32_t* slot_id, int64_t pitch, int64_t top, const int32_t* state,
+                       int dtype, void* stream);
+
+/* unit [rows, dim] (fp32, dense; the block's product with weight) to the
+ * gradient of the row's loss times T: row_scale[n, 1] unit[n] + the sum over the
+ * slots of (q - p) weight[slot_id]. */
+int ts_distill_slots(float* unit, const float* row_scale, const void* weight, int64_t ld_weight, int64_t rows,
+                     int64_t dim, double temperature, const int32_t* slot_id, const float* slot_p, const float* slot_z,
+                     int64_t pitch, int64_t top, const float* lse, int dtype, void* stream);
 
 /* fp32 or fp64: loss, lse and slot_z of a block of logits [rows, ld_logits]. */
 int ts_distill_fwd_exact(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, double temperature,
                          const int32_t* slot_id, const void* slot_p, void* slot_z, int64_t pitch, int64_t top,
                          const int32_t* state, void* loss, void* lse, int dtype, void* stream);
 
-/* dlogits from what a forward stored: ts_distill_fwd's exps and tile maxima
- * (bf16, fp16), or the logits (fp32, fp64; tile_max null).  A null grad: q - p,
+/* dlogits from what a forward stored: ts_distill_fwd's exps and references
+ * (bf16, fp16), or the logits (fp32, fp64; tile_ref null).  A null grad: q - p,
  * without the 1 / T.  dlogits may be the stored block itself; columns past the
  * vocabulary are zero in bf16 and fp16, untouched otherwise.  Entries are
  * rounded once from the stored values, the slots' from slot_z. */
-int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_max, int64_t rows, int64_t vocab,
+int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_ref, int64_t rows, int64_t vocab,
                       double temperature, const int32_t* slot_id, const void* slot_p, const void* slot_z,
                       int64_t pitch, int64_t top, const int32_t* state, const void* lse, const void* grad,
                       void* dlogits, int64_t ld_dlogits, int dtype, void* stream);

@@ -84,8 +84,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ts_distill_fwd_workspace": (_I64, [_I64, _I64]),
     "ts_distill_fwd": (
         _INT,
-        [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I64, _INT, _P],
+        [_P, _I64, _P, _I64, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _INT, _P],
     ),
+    "ts_distill_softmax": (_INT, [_P, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _INT, _P]),
+    "ts_distill_slots": (_INT, [_P, _P, _P, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _INT, _P]),
     "ts_distill_fwd_exact": (_INT, [_P, _I64, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _INT, _P]),
     "ts_distill_finish": (
         _INT, [_P, _I64, _P, _I64, _I64, _D, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _INT, _P]),

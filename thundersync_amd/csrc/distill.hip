@@ -7,15 +7,18 @@
 //   loss[n] = sum_k p_k (log p_k - log q_k),  dz[n, v] = g[n] / T (q_v - p_v)
 //
 // teacher_kernel turns each row's slots into (token, p).  16-bit types: stats_kernel reduces
-// the logits of a 256-row vocabulary tile to (max, sum exp) per token in its MFMA epilogue and,
-// with a frozen head, stores the tile's exponentials in the element type;
+// the logits of a 256-row vocabulary tile to (reference, sum exp) per token in its MFMA epilogue
+// and, where the block is wanted, stores the tile's exponentials in the element type;
 // scores_kernel takes the logits at the slots' tokens as dot products; loss_kernel merges the
-// tiles and sums the slots; finish_kernel scales the exponentials to q, in one pass over
-// 2 bytes an entry in place of a second product of 2 D flops an entry, and writes the slots'
-// entries from their fp32 logits.  With a trainable head, whose gradient waits for the
-// upstream one, dlogits_kernel forms the logits again in the backward.  fp32 and fp64: the logits of a block of
-// rows by the exact product, then one work-group a row.  The vector-Jacobian products with W
-// and h are the fused logprob's.  Bound by the products (the fused logprob's GEMM core).
+// tiles and sums the slots.  One pass over 2 bytes an entry then stands in place of a second
+// product of 2 D flops an entry.  Frozen head: softmax_kernel shifts the exponentials by whole
+// octaves to one reference a row (no second rounding) and clears the slots' tokens, and
+// slots_kernel adds these to the block's product with W in fp32.  Trainable head, whose block
+// holds the upstream gradient: finish_kernel scales them to q and writes the slots' entries
+// from their fp32 logits; where the block would outgrow its bound, dlogits_kernel forms it from
+// the logits again.  fp32 and fp64: the logits of a block of rows by the exact product, then
+// one work-group a row.  The vector-Jacobian products with W and h are the fused logprob's.
+// Bound by the products (the fused logprob's GEMM core).
 #include <algorithm>
 #include <type_traits>
 
@@ -34,6 +37,7 @@ using namespace ts::head;
 constexpr int kMaxTop = 1024;   // slots per row
 constexpr int kRowWaves = 4;    // rows per work-group of the per-row kernels
 constexpr int kDead = 0, kLive = 1, kBadId = 2;  // row states
+constexpr int kHeadroom = 14;   // octaves of a frozen head's stored softmax above 1: below fp16's largest number
 
 template <typename T> __device__ __forceinline__ T wave_sum_of(T v) {
 #pragma unroll
@@ -109,7 +113,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void teacher_kernel(const int64_t* 
 }
 
 // ---------------------------------------------------------------------------
-// forward: per (vocabulary tile, token) max and sum exp of z / T
+// forward: per (vocabulary tile, token) reference and sum exp of z / T.  The reference is the
+// tile's maximum in octaves (of z log2(e) / T), rounded up to a whole one: exponentials of two
+// tiles differ by a power of two, which a 16-bit value is scaled by without another rounding.
 //
 // Few rows are bound by the weight's one read (48 rows, D 4096, V 151936: 286 us, 4.4 TB/s),
 // many by MFMA at the power-limited clock: 2048 rows take 2.23 ms with the exponentials stored,
@@ -117,16 +123,16 @@ __global__ __launch_bounds__(64 * kRowWaves) void teacher_kernel(const int64_t* 
 // staged through the ring's LDS) overlaps nothing, which is the distance to the 1373 TFLOP/s
 // that grad_hidden reaches at the same sizes.
 // ---------------------------------------------------------------------------
-// (max of z, sum exp((z - max) / T)) of two disjoint sets of logits, either of which may be
-// empty (max = -inf, sum 0); unit = log2(e) / T.  A set that holds a NaN has a NaN sum.
-__device__ __forceinline__ void merge(float& m, float& s, float mo, float so, float unit) {
+// (reference r, sum 2^(z unit - r)) of two disjoint sets of logits, either of which may be
+// empty (r = -inf, sum 0); unit = log2(e) / T.  A set that holds a NaN has a NaN sum.
+__device__ __forceinline__ void merge(float& m, float& s, float mo, float so) {
   if (mo == neg_inf() || m == neg_inf()) {
     m = fmaxf(m, mo);
     s += so;
     return;
   }
   const float mn = fmaxf(m, mo);
-  s = fast_exp2((m - mn) * unit) * s + fast_exp2((mo - mn) * unit) * so;
+  s = fast_exp2(m - mn) * s + fast_exp2(mo - mn) * so;
   m = mn;
 }
 
@@ -138,9 +144,9 @@ struct StatsArgs {
   int rows, dim, vocab;
   int n_ttiles, n_vtiles;
   float unit;      // log2(e) / T
-  float* part_m;   // [n_vtiles][rows]
+  float* part_m;   // [n_vtiles][rows]: references
   float* part_s;
-  bf16* exps;      // STORE: [rows][lde], exp((z - tile's max) / T) in E (pad columns 0)
+  bf16* exps;      // STORE: [rows][lde], 2^(z unit - the tile's reference) in E (pad columns 0)
   int64_t lde;
   int vocab_pad;
 };
@@ -205,12 +211,13 @@ __device__ __forceinline__ void stats_tile(const StatsArgs& p, bf16* s0, bf16* s
   for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
     for (int w = 0; w < S::WM; ++w) mk[ni] = fmaxf(mk[ni], xm[w * S::BN + b_row<S>(ni, lane, wn)]);
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) mk[ni] = ceilf(mk[ni] * p.unit);
   auto quarter = [&](int q) -> bf16* { return q == 0 ? s0 : q == 1 ? s1 : q == 2 ? s2 : s3; };
   auto values = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
       float sum = 0.f;
-      const float m2 = mk[ni] * p.unit;
       // nothing, or nothing but -inf and NaN, which a maximum does not show
       const bool none = mk[ni] == neg_inf();
       const int col = b_row<S>(ni, lane, PASSES > 1 ? 0 : wn);  // token within the pass
@@ -223,7 +230,7 @@ __device__ __forceinline__ void stats_tile(const StatsArgs& p, bf16* s0, bf16* s
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float x = acc[mi][ni][4 * i4 + j];
-            e[j] = none ? (x == neg_inf() ? 0.f : __builtin_nanf("")) : fast_exp2(fmaf(x, p.unit, -m2));
+            e[j] = none ? (x == neg_inf() ? 0.f : __builtin_nanf("")) : fast_exp2(fmaf(x, p.unit, -mk[ni]));
             sum += e[j];
           }
           if (STORE)
@@ -339,11 +346,12 @@ template <typename C> __device__ __forceinline__ C row_loss(int state, C sum) {
 constexpr int kLossTokens = 16;
 __global__ __launch_bounds__(64 * kLossTokens) void loss_kernel(const float* __restrict__ pm,
                                                                 const float* __restrict__ ps, int n_vtiles, int rows,
-                                                                float unit, const int32_t* __restrict__ slot_id,
+                                                                const int32_t* __restrict__ slot_id,
                                                                 const float* __restrict__ slot_p,
                                                                 const float* __restrict__ slot_z, int pitch, int top,
                                                                 const int32_t* __restrict__ state, float inv_t,
-                                                                float* __restrict__ lse, float* __restrict__ loss) {
+                                                                float* __restrict__ lse, float* __restrict__ loss,
+                                                                float2* __restrict__ row_scale) {
   __shared__ float sm[kLossTokens][kLossTokens], ss[kLossTokens][kLossTokens];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n0 = blockIdx.x * kLossTokens;
@@ -354,13 +362,13 @@ __global__ __launch_bounds__(64 * kLossTokens) void loss_kernel(const float* __r
 #pragma unroll 4
       for (int t = slot; t < n_vtiles; t += 64) {
         const int64_t o = (int64_t)t * rows + n;
-        merge(M, S, pm[o], ps[o], unit);
+        merge(M, S, pm[o], ps[o]);
       }
     }
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) {
       const float mo = shfl_xor(M, o), so = shfl_xor(S, o);
-      merge(M, S, mo, so, unit);
+      merge(M, S, mo, so);
     }
     if (lane < 16) {
       sm[wave][tok] = M;
@@ -372,25 +380,105 @@ __global__ __launch_bounds__(64 * kLossTokens) void loss_kernel(const float* __r
   if (n >= rows) return;
   float M = sm[0][wave], S = ss[0][wave];
 #pragma unroll
-  for (int v = 1; v < kLossTokens; ++v) merge(M, S, sm[v][wave], ss[v][wave], unit);
-  const float l = M * inv_t + logf(S);
+  for (int v = 1; v < kLossTokens; ++v) merge(M, S, sm[v][wave], ss[v][wave]);
+  const float l = M * kLn2 + logf(S);
   const int64_t o = (int64_t)n * pitch;
   const float sum = wave_sum(slots_loss(slot_id + o, slot_p + o, slot_z + o, top, inv_t, l, lane, 64));
   if (lane == 0) {
     lse[n] = l;
     loss[n] = row_loss(state[n], sum);
+    if (row_scale) row_scale[n] = float2{M - kHeadroom, 1.f / (ldexpf(1.f, kHeadroom) * S)};
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Frozen head, after the forward: the stored exponentials of a row to one reference, the
+// softmax then being row_scale[1] times the block, and zero at the slots' tokens.  An entry
+// keeps its one rounding: it is multiplied by a power of two, and kHeadroom octaves above 1
+// leave fp16's smallest normal number 28 below the row's largest (unscaled, the softmax of
+// 151936 equal logits is 6.6e-6 with four bits of it lost).  Bound as finish_kernel: 2048 x
+// 151936 in bf16 in 211 us, 5.9 TB/s.
+// ---------------------------------------------------------------------------
+constexpr int kFinish = 2048;  // columns of one row a work-group: 256 threads of 8
+template <typename T>
+__global__ __launch_bounds__(256) void softmax_kernel(T* __restrict__ block, int64_t ld,
+                                                      const float* __restrict__ tile_ref,
+                                                      const float2* __restrict__ row_scale, int rows,
+                                                      const int32_t* __restrict__ state,
+                                                      const int32_t* __restrict__ slot_id, int pitch, int top,
+                                                      int columns) {
+  const int64_t n = blockIdx.x;
+  const int c0 = blockIdx.y * kFinish, c = c0 + 8 * threadIdx.x;
+  const bool dead = state[n] == kDead;
+  if (c < columns) {  // a multiple of 8
+    float x[8];
+    load8(block + n * ld + c, x);
+    // (a reference that is no number belongs to a row whose factor is none)
+    const float f = ldexpf(1.f, (int)fmaxf(tile_ref[(int64_t)(c / TM) * rows + n] - row_scale[n].x, -200.f));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = dead ? 0.f : x[i] * f;
+    store8(block + n * ld + c, x);
+  }
+  if (dead) return;
+  __syncthreads();  // the slots' entries after the others'
+  for (int k = threadIdx.x; k < top; k += 256) {
+    const int id = slot_id[n * pitch + k];
+    if (id >= c0 && id < c0 + kFinish) block[n * ld + id] = from_f<T>(0.f);
+  }
+}
+
+// unit[n] = factor[n] unit[n] + sum_k (q_k - p_k) W[slot_id[n, k]], all in fp32: the slots are
+// the gradient's largest terms, and rounded in the block they alone made the error 1.4 times that
+// of the result's rounding.  A work-group takes 512 columns of one row, its waves every fourth
+// slot each, added in wave order.  Bound by the gathered rows of W: 2048 x 64 slots of
+// 8 KB, 1.07 GB, in 190 us.
+template <typename E>
+__global__ __launch_bounds__(256) void slots_kernel(float* __restrict__ unit, const float2* __restrict__ row_scale,
+                                                    const E* __restrict__ w, int64_t ldw,
+                                                    const int32_t* __restrict__ slot_id,
+                                                    const float* __restrict__ slot_p,
+                                                    const float* __restrict__ slot_z, int pitch, int top, int dim,
+                                                    float inv_t, const float* __restrict__ lse) {
+  __shared__ float part[3][8][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = blockIdx.x, o = n * pitch;
+  const int d = 512 * blockIdx.y + 8 * lane;
+  const bool on = d < dim;  // a multiple of 8
+  const float l = lse[n];
+  float acc[8] = {};
+#pragma unroll 4
+  for (int k = wave; k < top; k += 4) {
+    const int id = slot_id[o + k];
+    if (id < 0) continue;
+    const float c = expf(slot_z[o + k] * inv_t - l) - slot_p[o + k];
+    float x[8];
+    if (on) load8(w + (int64_t)id * ldw + d, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = on ? fmaf(c, x[i], acc[i]) : 0.f;
+  }
+  if (wave > 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[wave - 1][i][lane] = acc[i];
+  __syncthreads();
+  if (wave > 0 || !on) return;
+  const float f = row_scale[n].y;
+  float* out = unit + n * dim + d;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int v = 0; v < 3; ++v) acc[i] += part[v][i][lane];
+    out[i] = fmaf(out[i], f, acc[i]);
   }
 }
 
 // ---------------------------------------------------------------------------
 // dlogits = grad / T (q - p) (grad null: q - p, without the 1 / T) from what the forward
 // stored: a work-group takes kFinish columns of one row.  E: exponentials relative to their
-// 256-column tile's maximum (FROM_EXPS), scaled once per tile; C: logits.  Bound by the
+// 256-column tile's reference (FROM_EXPS), scaled once per tile; C: logits.  Bound by the
 // block's bytes, read and written once: 2048 x 151936 in bf16 in 211 us, 5.9 TB/s.
 // ---------------------------------------------------------------------------
-constexpr int kFinish = 2048;  // 256 threads of 8 columns
 template <typename T, typename C, bool FROM_EXPS>
-__global__ __launch_bounds__(256) void finish_kernel(const T* src, int64_t lds, const float* __restrict__ tile_max,
+__global__ __launch_bounds__(256) void finish_kernel(const T* src, int64_t lds, const float* __restrict__ tile_ref,
                                                      int tile_rows, const C* __restrict__ lse,
                                                      const C* __restrict__ grad, const int32_t* __restrict__ state,
                                                      const int32_t* __restrict__ slot_id, const C* __restrict__ slot_p,
@@ -404,7 +492,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const T* src, int64_t lds, 
     if (c < columns) {  // a multiple of 8
       float x[8];
       load8(src + n * lds + c, x);
-      const float f = fast_exp2((tile_max[(int64_t)(c / TM) * tile_rows + n] * inv_t - l) * kLog2e) * coef;
+      const float f = fast_exp2(fmaf(-l, kLog2e, tile_ref[(int64_t)(c / TM) * tile_rows + n])) * coef;
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = dead ? 0.f : x[i] * f;
       store8(dst + n * ldd + c, x);
@@ -552,11 +640,12 @@ __global__ __launch_bounds__(kGemmThreads, 1) void dlogits_kernel(DlArgs p) {
 
 // dl[n, slot_id] = grad / T (q - p) with q = exp(z / T - lse), rounded once
 template <typename E>
-__global__ __launch_bounds__(256) void slots_kernel(const int32_t* __restrict__ slot_id,
-                                                    const float* __restrict__ slot_p,
-                                                    const float* __restrict__ slot_z, int pitch, int top, int64_t rows,
-                                                    const float* __restrict__ lse, const float* __restrict__ g,
-                                                    float inv_t, E* __restrict__ dl, int64_t ldl) {
+__global__ __launch_bounds__(256) void dlogits_slots_kernel(const int32_t* __restrict__ slot_id,
+                                                            const float* __restrict__ slot_p,
+                                                            const float* __restrict__ slot_z, int pitch, int top,
+                                                            int64_t rows, const float* __restrict__ lse,
+                                                            const float* __restrict__ g, float inv_t,
+                                                            E* __restrict__ dl, int64_t ldl) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t n = i / pitch;
   const int k = (int)(i - n * pitch);
@@ -648,7 +737,8 @@ int64_t ts_distill_fwd_workspace(int64_t rows, int64_t vocab) {
 int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int64_t rows,
                    int64_t dim, int64_t vocab, double temperature, const int32_t* slot_id, const float* slot_p,
                    float* slot_z, int64_t pitch, int64_t top, const int32_t* state, float* loss, float* lse,
-                   void* exps, int64_t ld_exps, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+                   void* exps, int64_t ld_exps, float* row_scale, void* workspace, int64_t workspace_bytes, int dtype,
+                   void* stream) {
   TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_fwd: dtype %d (bf16 or fp16)", dtype);
   TS_CHECK_ARG(rows >= 0 && dim > 0 && vocab > 0 && rows < (1 << 30) && vocab < (1 << 30) && dim < (1 << 20) &&
                    top > 0 && top <= pitch && pitch <= kMaxTop,
@@ -667,6 +757,7 @@ int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, in
                (long long)ts_distill_fwd_workspace(rows, vocab));
   TS_CHECK_ARG(!exps || (ok16(exps) && ld_exps % 8 == 0 && ld_exps >= (vocab + 7) / 8 * 8),
                "ts_distill_fwd: exps' alignment or leading dimension");
+  TS_CHECK_ARG(((uintptr_t)row_scale & 7) == 0, "ts_distill_fwd: row_scale must be 8-byte aligned");
   StatsArgs a;
   a.h = (const ts::bf16*)hidden;
   a.ldh = ld_hidden;
@@ -702,8 +793,8 @@ int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, in
   {
     ts::TimedLaunch timed_("distill.loss_kernel", s);
     hipLaunchKernelGGL(loss_kernel, dim3((unsigned)((rows + kLossTokens - 1) / kLossTokens)), dim3(64 * kLossTokens),
-                       0, s, a.part_m, a.part_s, a.n_vtiles, (int)rows, a.unit, slot_id, slot_p, slot_z, (int)pitch,
-                       (int)top, state, (float)(1. / temperature), lse, loss);
+                       0, s, a.part_m, a.part_s, a.n_vtiles, (int)rows, slot_id, slot_p, slot_z, (int)pitch, (int)top,
+                       state, (float)(1. / temperature), lse, loss, (float2*)row_scale);
   }
   return ts::check_launch("ts_distill_fwd (loss)");
 }
@@ -735,7 +826,59 @@ int ts_distill_fwd_exact(const void* logits, int64_t ld_logits, int64_t rows, in
   return ts::check_launch("ts_distill_fwd_exact");
 }
 
-int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_max, int64_t rows, int64_t vocab,
+int ts_distill_softmax(void* block, int64_t ld_block, const float* tile_ref, const float* row_scale, int64_t rows,
+                       int64_t vocab, const int32_t* slot_id, int64_t pitch, int64_t top, const int32_t* state,
+                       int dtype, void* stream) {
+  TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_softmax: dtype %d (bf16 or fp16)", dtype);
+  const int64_t columns = (vocab + 7) / 8 * 8;
+  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && vocab > 0 && vocab < 65535ll * kFinish && top > 0 && top <= pitch &&
+                   pitch <= kMaxTop && ld_block >= columns && ld_block % 8 == 0,
+               "ts_distill_softmax: bad shape");
+  if (rows == 0) return TS_OK;
+  TS_CHECK_ARG(block && tile_ref && row_scale && slot_id && state, "ts_distill_softmax: null pointer");
+  TS_CHECK_ARG(ok16(block) && ((uintptr_t)row_scale & 7) == 0, "ts_distill_softmax: alignment");
+  hipStream_t s = (hipStream_t)stream;
+  {
+    ts::TimedLaunch timed_("distill.softmax_kernel", s);
+    const dim3 grid((unsigned)rows, (unsigned)((columns + kFinish - 1) / kFinish));
+    if (dtype == TS_F16)
+      hipLaunchKernelGGL(softmax_kernel<ts::f16>, grid, dim3(256), 0, s, (ts::f16*)block, ld_block, tile_ref,
+                         (const float2*)row_scale, (int)rows, state, slot_id, (int)pitch, (int)top, (int)columns);
+    else
+      hipLaunchKernelGGL(softmax_kernel<ts::bf16>, grid, dim3(256), 0, s, (ts::bf16*)block, ld_block, tile_ref,
+                         (const float2*)row_scale, (int)rows, state, slot_id, (int)pitch, (int)top, (int)columns);
+  }
+  return ts::check_launch("ts_distill_softmax");
+}
+
+int ts_distill_slots(float* unit, const float* row_scale, const void* weight, int64_t ld_weight, int64_t rows,
+                     int64_t dim, double temperature, const int32_t* slot_id, const float* slot_p, const float* slot_z,
+                     int64_t pitch, int64_t top, const float* lse, int dtype, void* stream) {
+  TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_slots: dtype %d (bf16 or fp16)", dtype);
+  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && dim > 0 && dim < (1 << 20) && dim % 8 == 0 && ld_weight >= dim &&
+                   ld_weight % 8 == 0 && top > 0 && top <= pitch && pitch <= kMaxTop,
+               "ts_distill_slots: bad shape");
+  TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_slots: temperature %g", temperature);
+  if (rows == 0) return TS_OK;
+  TS_CHECK_ARG(unit && row_scale && weight && slot_id && slot_p && slot_z && lse, "ts_distill_slots: null pointer");
+  TS_CHECK_ARG(ok16(weight) && ((uintptr_t)row_scale & 7) == 0, "ts_distill_slots: alignment");
+  hipStream_t s = (hipStream_t)stream;
+  {
+    ts::TimedLaunch timed_("distill.slots_kernel", s);
+    const dim3 grid((unsigned)rows, (unsigned)((dim + 511) / 512));
+    if (dtype == TS_F16)
+      hipLaunchKernelGGL(slots_kernel<ts::f16>, grid, dim3(256), 0, s, unit, (const float2*)row_scale,
+                         (const ts::f16*)weight, ld_weight, slot_id, slot_p, slot_z, (int)pitch, (int)top, (int)dim,
+                         (float)(1. / temperature), lse);
+    else
+      hipLaunchKernelGGL(slots_kernel<ts::bf16>, grid, dim3(256), 0, s, unit, (const float2*)row_scale,
+                         (const ts::bf16*)weight, ld_weight, slot_id, slot_p, slot_z, (int)pitch, (int)top, (int)dim,
+                         (float)(1. / temperature), lse);
+  }
+  return ts::check_launch("ts_distill_slots");
+}
+
+int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_ref, int64_t rows, int64_t vocab,
                       double temperature, const int32_t* slot_id, const void* slot_p, const void* slot_z,
                       int64_t pitch, int64_t top, const int32_t* state, const void* lse, const void* grad,
                       void* dlogits, int64_t ld_dlogits, int dtype, void* stream) {
@@ -746,7 +889,7 @@ int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_m
                "ts_distill_finish: bad shape");
   TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_finish: temperature %g", temperature);
   if (rows == 0) return TS_OK;
-  TS_CHECK_ARG(stored && dlogits && slot_id && slot_p && slot_z && state && lse && (exact || tile_max),
+  TS_CHECK_ARG(stored && dlogits && slot_id && slot_p && slot_z && state && lse && (exact || tile_ref),
                "ts_distill_finish: null pointer");
   const int64_t columns = exact ? vocab : (vocab + 7) / 8 * 8;
   TS_CHECK_ARG(exact || (ok16(stored) && ok16(dlogits) && ld_stored % 8 == 0 && ld_dlogits % 8 == 0 &&
@@ -757,7 +900,7 @@ int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_m
     ts::TimedLaunch timed_("distill.finish_kernel", s);
     const dim3 grid((unsigned)rows, (unsigned)((columns + kFinish - 1) / kFinish));
 #define TS_FINISH(T, C, EXPS)                                                                                        \
-  hipLaunchKernelGGL((finish_kernel<T, C, EXPS>), grid, dim3(256), 0, s, (const T*)stored, ld_stored, tile_max,       \
+  hipLaunchKernelGGL((finish_kernel<T, C, EXPS>), grid, dim3(256), 0, s, (const T*)stored, ld_stored, tile_ref,       \
                      (int)rows, (const C*)lse, (const C*)grad, state, slot_id, (const C*)slot_p, (const C*)slot_z,    \
                      (int)pitch, (int)top, (int)columns, (C)(1. / temperature), (T*)dlogits, ld_dlogits)
     if (dtype == TS_BF16) TS_FINISH(ts::bf16, float, true);
@@ -816,14 +959,14 @@ int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight
   const int st = ts::check_launch("ts_distill_dlogits");
   if (st != TS_OK) return st;
   {
-    ts::TimedLaunch timed_("distill.slots_kernel", s);
+    ts::TimedLaunch timed_("distill.dlogits_slots_kernel", s);
     const dim3 grid((unsigned)((rows * pitch + 255) / 256));
     const float inv_t = (float)(1. / temperature);
     if (dtype == TS_F16)
-      hipLaunchKernelGGL(slots_kernel<ts::f16>, grid, dim3(256), 0, s, slot_id, slot_p, slot_z, (int)pitch, (int)top,
+      hipLaunchKernelGGL(dlogits_slots_kernel<ts::f16>, grid, dim3(256), 0, s, slot_id, slot_p, slot_z, (int)pitch, (int)top,
                          rows, lse, grad, inv_t, (ts::f16*)dlogits, ld_dlogits);
     else
-      hipLaunchKernelGGL(slots_kernel<ts::bf16>, grid, dim3(256), 0, s, slot_id, slot_p, slot_z, (int)pitch, (int)top,
+      hipLaunchKernelGGL(dlogits_slots_kernel<ts::bf16>, grid, dim3(256), 0, s, slot_id, slot_p, slot_z, (int)pitch, (int)top,
                          rows, lse, grad, inv_t, (ts::bf16*)dlogits, ld_dlogits);
   }
   return ts::check_launch("ts_distill_dlogits (slots)");

@@ -26,7 +26,9 @@ A block of rows (:func:`~thundersync_amd.fused_logprob.backward_block_rows` of
 * a frozen weight: the forward goes on, block by block, from the stored
   exponentials to ``q - p`` and its product with the weight, ``[N, D]`` in
   fp32, which the backward multiplies by the upstream gradient (no block
-  outlives the call, and 2 N V D flops of logits formed again are saved);
+  outlives the call, and 2 N V D flops of logits formed again are saved).
+  The block's 16-bit entries are rounded once, with the exponent range of a
+  row's own reference, and the teacher's tokens are added in fp32;
 * a trainable weight and one block of rows: the backward, which has the
   upstream gradient, wants the block that the forward stored.  It is kept where
   the blocks of all losses that wait for their backward then hold no more
@@ -176,6 +178,7 @@ class _Rows:
         self.slot_id, self.slot_p, self.state = _teacher(ids, logits, weight.shape[0], temperature, self.dtype)
         self.slot_z = torch.empty_like(self.slot_p)
         self.lse, self.loss = (torch.empty(self.n, dtype=self.dtype, device=hidden.device) for _ in range(2))
+        self.row_scale = None
 
     def _operands(self, hidden, weight):
         self.d_in = hidden.shape[1]
@@ -200,7 +203,7 @@ class _Rows:
         rows.exact, rows.top, rows.temperature = hidden.dtype in EXACT_DTYPES, top, temperature
         rows._operands(hidden, weight)
         rows.slot_id, rows.slot_p, rows.slot_z, rows.state, rows.lse = saved
-        rows.dtype = rows.lse.dtype
+        rows.dtype, rows.row_scale = rows.lse.dtype, None
         return rows
 
     def slots(self, i):
@@ -227,8 +230,8 @@ class _Rows:
         )
 
     def forward(self, i, rows, block):
-        """Losses of rows ``[i, i + rows)``; with a ``block`` also what :meth:`finish` reads.  Returns the
-        tiles' maxima (16-bit types)."""
+        """Losses of rows ``[i, i + rows)``; with a ``block`` also what :meth:`finish` and :meth:`softmax` read.
+        Returns the tiles' references (16-bit types)."""
         lib, stream = _lib.require_library(), _lib.stream_of(self.h)
         if self.exact:
             self.logits(i, rows, block)
@@ -243,29 +246,52 @@ class _Rows:
         _lib.check(
             lib.ts_distill_fwd(self.row(i), self.ldh, self.w.data_ptr(), self.ldw, rows, self.d, self.v,
                                self.temperature, *self.slots(i), self.loss[i:].data_ptr(), self.lse[i:].data_ptr(),
-                               _lib.ptr(block), self.ld, ws.data_ptr(), ws_bytes, self.code, stream),
+                               _lib.ptr(block), self.ld, self.scale(i), ws.data_ptr(), ws_bytes, self.code, stream),
             self.what("ts_distill_fwd", rows),
         )
         return ws[: ws_bytes // 2]
 
     def stored_again(self, i, rows, block):
-        """``block`` and its tiles' maxima as a :meth:`forward` that kept them left them; what autograd saved stays."""
+        """``block`` and its tiles' references as a :meth:`forward` that kept them left them; what autograd saved stays."""
         again = copy.copy(self)
         again.slot_z, again.lse, again.loss = (torch.empty_like(t) for t in (self.slot_z, self.lse, self.lse))
         return again.forward(i, rows, block)
 
-    def finish(self, i, rows, block, maxima, grad, out):
+    def scale(self, i):
+        return None if self.row_scale is None else self.row_scale[i:].data_ptr()
+
+    def softmax(self, i, rows, block, references):
+        """16-bit types: ``block`` to the softmax over ``row_scale``, without the slots' tokens."""
+        slot_id, _, _, pitch, top, state = self.slots(i)
+        _lib.check(
+            _lib.require_library().ts_distill_softmax(block.data_ptr(), self.ld, references.data_ptr(), self.scale(i),
+                                                      rows, self.v, slot_id, pitch, top, state, self.code,
+                                                      _lib.stream_of(block)),
+            self.what("ts_distill_softmax", rows),
+        )
+
+    def add_slots(self, unit):
+        """16-bit types: the products with the weight to those of ``q - p``."""
+        *slots, _ = self.slots(0)
+        _lib.check(
+            _lib.require_library().ts_distill_slots(unit.data_ptr(), self.scale(0), self.w.data_ptr(), self.ldw, self.n,
+                                                    self.d, self.temperature, *slots, self.lse.data_ptr(), self.code,
+                                                    _lib.stream_of(unit)),
+            self.what("ts_distill_slots", self.n),
+        )
+
+    def finish(self, i, rows, block, references, grad, out):
         """``block`` (as :meth:`forward` left it) to the logits' gradient ``out`` (which may be the block)."""
         _lib.check(
             _lib.require_library().ts_distill_finish(
-                block.data_ptr(), self.ld, _lib.ptr(maxima), rows, self.v, self.temperature, *self.slots(i),
+                block.data_ptr(), self.ld, _lib.ptr(references), rows, self.v, self.temperature, *self.slots(i),
                 self.lse[i:].data_ptr(), None if grad is None else grad[i:].data_ptr(), out.data_ptr(), self.ld,
                 self.code, _lib.stream_of(out)),
             self.what("ts_distill_finish", rows),
         )
 
     def unit_gradient(self, i, rows, dl, out, ws):
-        """``out`` rows ``[i, i + rows)`` = (q - p) . weight, not rounded to the element type."""
+        """``out`` rows ``[i, i + rows)`` = ``dl`` . weight, not rounded to the element type."""
         lib, stream = _lib.require_library(), _lib.stream_of(out)
         if self.exact:
             status = lib.ts_matmul_exact_ws(dl.data_ptr(), self.ld, 1, self.w.data_ptr(), self.ldw, 1, rows, self.d,
@@ -286,7 +312,7 @@ class _Rows:
 
 def _forward(rows: _Rows, chunk, need_hidden, need_weight):
     """The losses, and what the backward wants: nothing, the hidden states' unit gradient, or a kept block and its
-    tiles' maxima."""
+    tiles' references."""
     n, dev = rows.n, rows.h.device
     block_rows = min(max(1, int(chunk)), max(n, 1)) if rows.exact else backward_block_rows(n, chunk)
     frozen = need_hidden and not need_weight
@@ -299,18 +325,25 @@ def _forward(rows: _Rows, chunk, need_hidden, need_weight):
     block = torch.empty(min(block_rows, n), rows.ld, dtype=rows.h.dtype, device=dev) if kept is None else kept
     unit = torch.empty(n, rows.d, dtype=rows.dtype, device=dev) if frozen else None
     ws = rows.unit_workspace({block_rows, n % block_rows or block_rows}) if frozen else None
-    maxima = None
+    if frozen and not rows.exact:
+        rows.row_scale = torch.empty(n, 2, dtype=torch.float32, device=dev)
+    references = None
     for i in range(0, n, block_rows):
         size = min(block_rows, n - i)
-        maxima = rows.forward(i, size, block)
+        references = rows.forward(i, size, block)
         if frozen:
             with operator_range("distill_head_coefficient", role=device_role(dev), rows=size, vocab=rows.v):
-                rows.finish(i, size, block, maxima, None, block)
+                if rows.exact:
+                    rows.finish(i, size, block, None, None, block)
+                else:
+                    rows.softmax(i, size, block, references)
             with operator_range("distill_head_hidden_vjp", role=device_role(dev), rows=size, hidden=rows.d, vocab=rows.v):
                 rows.unit_gradient(i, size, block, unit, ws)
     if frozen:
+        if not rows.exact:
+            rows.add_slots(unit)
         return (unit,)
-    return () if kept is None else (kept, maxima)
+    return () if kept is None else (kept, references)
 
 
 def _backward_frozen(unit, state, grad, temperature, dtype, d_in):
@@ -325,7 +358,7 @@ def _backward_frozen(unit, state, grad, temperature, dtype, d_in):
     return out if d == d_in else out[:, :d_in].contiguous()
 
 
-def _backward_trainable(rows: _Rows, grad, chunk, block, maxima):
+def _backward_trainable(rows: _Rows, grad, chunk, block, references):
     g = grad.to(rows.dtype).contiguous()
     h_weight = _live_rows(rows.h, rows.state)
     lib = _lib.require_library()
@@ -333,7 +366,7 @@ def _backward_trainable(rows: _Rows, grad, chunk, block, maxima):
 
     def dlogits(i, size, dl, ld):
         if block is not None:
-            rows.finish(i, size, block, maxima, g, dl)
+            rows.finish(i, size, block, references, g, dl)
         elif rows.exact:
             rows.logits(i, size, dl)
             rows.finish(i, size, dl, None, g, dl)
@@ -379,9 +412,9 @@ class _FusedDistill(torch.autograd.Function):
                 gh, gw = _backward_frozen(unit, state, grad, ctx.temperature, ctx.dtype, ctx.d_in), None
             else:
                 hidden, weight, *saved = ctx.saved_tensors
-                block, maxima = [*saved[5:], None, None][:2]
+                block, references = [*saved[5:], None, None][:2]
                 rows = _Rows.again(hidden, weight, saved[:5], ctx.top, ctx.temperature)
-                gh, gw = _backward_trainable(rows, grad, ctx.chunk, block, maxima)
+                gh, gw = _backward_trainable(rows, grad, ctx.chunk, block, references)
         return gh, gw, None, None, None, None, None, None
 
 
