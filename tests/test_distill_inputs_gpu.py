@@ -1,0 +1,41 @@
+"""Inputs of distillation and of the fused logprob that are valid as torch hands them over."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from thundersync_amd.fused_distill import fused_distill
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def inputs(cuda, n, d, v, k, dtype, seed=0):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    h = torch.randn(n, d, generator=g, device=cuda).to(dtype)
+    w = (torch.randn(v, d, generator=g, device=cuda) * 0.1).to(dtype)
+    ids = torch.stack([torch.randperm(v, generator=g, device=cuda)[:k] for _ in range(n)])
+    return h, w, ids, torch.randn(n, k, generator=g, device=cuda) * 2
+
+
+def both(h, w, ids, teacher):
+    """Loss and gradients with a trainable head."""
+    h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = fused_distill(h, w, ids, teacher)
+    return [loss.detach(), *torch.autograd.grad(loss.sum(), (h, w))]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_one_row_of_a_teacher(cuda, dtype):
+    """A column seen as a row has a row stride of 1, and one row of an expanded teacher one of 0: torch calls both
+    contiguous."""
+    h, w, ids, teacher = inputs(cuda, 1, 32, 300, 6, dtype)
+    want = both(h, w, ids, teacher)
+    column = teacher.T.contiguous().T
+    assert column.stride() == (1, 1)
+    expanded = teacher.expand(4, 6)[:1].as_strided((1, 6), (0, 1))
+    for t in (column, expanded):
+        assert all(torch.equal(a, b) for a, b in zip(both(h, w, ids, t), want))
+    assert all(torch.equal(a, b) for a, b in zip(both(h, w, ids.T.contiguous().T, teacher), want))

@@ -120,9 +120,10 @@ def _teacher(ids, logits, vocab, temperature, dtype):
     slot_p = torch.empty(n, pitch, dtype=dtype, device=ids.device)
     state = torch.empty(n, dtype=torch.int32, device=ids.device)
     _lib.check(
-        lib.ts_distill_teacher(ids.data_ptr(), logits.data_ptr(), logits.stride(0), _lib.dtype_code(logits.dtype), n, k,
-                               vocab, float(temperature), slot_id.data_ptr(), slot_p.data_ptr(), pitch,
-                               state.data_ptr(), _lib.dtype_code(dtype), _lib.stream_of(ids)),
+        lib.ts_distill_teacher(ids.data_ptr(), logits.data_ptr(), max(logits.stride(0), k),  # one row: any stride
+                               _lib.dtype_code(logits.dtype), n, k, vocab, float(temperature), slot_id.data_ptr(),
+                               slot_p.data_ptr(), pitch, state.data_ptr(), _lib.dtype_code(dtype),
+                               _lib.stream_of(ids)),
         f"ts_distill_teacher(rows={n}, top={k}, vocab={vocab})",
     )
     return slot_id, slot_p, state
