@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -39,3 +41,17 @@ def test_one_row_of_a_teacher(cuda, dtype):
     for t in (column, expanded):
         assert all(torch.equal(a, b) for a, b in zip(both(h, w, ids, t), want))
     assert all(torch.equal(a, b) for a, b in zip(both(h, w, ids.reshape(6, 1).T, teacher), want))
+
+
+@pytest.mark.parametrize("absent_id", [300, 1 << 40])
+def test_checked_ids_pass_absent_slots(cuda, absent_id, monkeypatch):
+    """THUNDERSYNC_CHECK_TARGETS looks at present slots: an absent one may name any token."""
+    h, w, ids, teacher = inputs(cuda, 3, 32, 300, 6, BF16)
+    teacher[1, 4] = -math.inf
+    want = both(h, w, ids, teacher)
+    ids[1, 4] = absent_id
+    monkeypatch.setenv("THUNDERSYNC_CHECK_TARGETS", "1")
+    assert all(torch.equal(a, b) for a, b in zip(both(h, w, ids, teacher), want))
+    ids[2, 0] = absent_id
+    with pytest.raises(ValueError, match=rf"target\[2\] = {absent_id} is outside the vocabulary"):
+        fused_distill(h, w, ids, teacher)

@@ -17,7 +17,7 @@ bring fewer than K; slots that name one token twice add up.  A row without
 any present slot has loss 0 and no gradient, whatever its hidden state holds.
 A token id at or past the vocabulary makes the row's loss NaN (and takes no
 part in its gradient), as a target of the fused logprob does;
-``THUNDERSYNC_CHECK_TARGETS=1`` checks the ids first and raises.
+``THUNDERSYNC_CHECK_TARGETS=1`` checks the present slots' ids first and raises.
 
 A block of rows (:func:`~thundersync_amd.fused_logprob.backward_block_rows` of
 ``chunk``) has its ``[rows, V]`` block in the element type, one at a time:
@@ -106,7 +106,8 @@ def _validate(hidden, weight, ids, logits, temperature):
             f"{hidden.dtype}/{weight.dtype}"
         )
     if os.environ.get(CHECK_TARGETS_ENV, "0") not in ("", "0") and ids.numel():
-        _check_targets(ids.amax(dim=1).clamp(min=0), weight.shape[0])  # an absent slot's negative id is no bad target
+        present = (ids >= 0) & (logits != -math.inf)  # an absent slot's id is no target
+        _check_targets(torch.where(present, ids, 0).amax(dim=1), weight.shape[0])
 
 
 def _teacher(ids, logits, vocab, temperature, dtype):
