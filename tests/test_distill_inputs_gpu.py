@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from thundersync_amd.fused_distill import fused_distill
+from thundersync_amd.fused_logprob import fused_logprob
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,50 @@ def test_checked_ids_pass_absent_slots(cuda, absent_id, monkeypatch):
     ids[2, 0] = absent_id
     with pytest.raises(ValueError, match=rf"target\[2\] = {absent_id} is outside the vocabulary"):
         fused_distill(h, w, ids, teacher)
+
+
+def off_border(t):
+    """``t`` contiguous, two bytes past a 16-byte border."""
+    flat = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)[1 : t.numel() + 1]
+    out = flat.view(t.shape)
+    out.copy_(t)
+    assert out.is_contiguous() and out.data_ptr() % 16
+    return out
+
+
+def one_row_of(t, width):
+    """The one row of ``t`` in a buffer whose rows are ``width`` apart."""
+    buffer = torch.zeros(2, width, dtype=t.dtype, device=t.device)
+    buffer[0, : t.shape[1]] = t[0]
+    return buffer[:1, : t.shape[1]]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_rows_off_a_16_byte_border(cuda, dtype):
+    h, w, ids, teacher = inputs(cuda, 9, 64, 300, 6, dtype)
+    want = both(h, w, ids, teacher)
+    assert all(torch.equal(a, b) for a, b in zip(both(off_border(h), off_border(w), ids, teacher), want))
+    frozen = fused_distill(off_border(h), off_border(w), ids, teacher)
+    assert torch.equal(frozen, want[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_logprob_rows_off_a_16_byte_border(cuda, dtype):
+    def logprob(h, w, target):
+        h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+        lp = fused_logprob(h, w, target)
+        return [lp.detach(), *torch.autograd.grad(lp.sum(), (h, w))]
+
+    h, w, ids, _ = inputs(cuda, 9, 64, 300, 1, dtype)
+    target = ids[:, 0].contiguous()
+    want = logprob(h, w, target)
+    assert all(torch.equal(a, b) for a, b in zip(logprob(off_border(h), off_border(w), target), want))
+    want = logprob(h[:1], w, target[:1])
+    assert all(torch.equal(a, b) for a, b in zip(logprob(one_row_of(h, 131), w, target[:1]), want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_one_row_of_wider_rows(cuda, dtype):
+    h, w, ids, teacher = inputs(cuda, 1, 64, 300, 6, dtype)
+    want = both(h, w, ids, teacher)
+    assert all(torch.equal(a, b) for a, b in zip(both(one_row_of(h, 131), w, ids, teacher), want))

@@ -86,9 +86,11 @@ def _pad_dim(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows_ok(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with rows of unit stride that start on 16-byte borders.  (A copy where they do not: torch
+    calls a tensor contiguous wherever it starts, and one row whatever its stride.)"""
     if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _unit_stride(t: torch.Tensor) -> torch.Tensor:
