@@ -83,13 +83,14 @@ def test_rows_off_a_16_byte_border(cuda, dtype):
     assert torch.equal(frozen, want[0])
 
 
+def logprob(h, w, target):
+    h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+    lp = fused_logprob(h, w, target)
+    return [lp.detach(), *torch.autograd.grad(lp.sum(), (h, w))]
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_logprob_rows_off_a_16_byte_border(cuda, dtype):
-    def logprob(h, w, target):
-        h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
-        lp = fused_logprob(h, w, target)
-        return [lp.detach(), *torch.autograd.grad(lp.sum(), (h, w))]
-
     h, w, ids, _ = inputs(cuda, 9, 64, 300, 1, dtype)
     target = ids[:, 0].contiguous()
     want = logprob(h, w, target)
@@ -103,3 +104,16 @@ def test_one_row_of_wider_rows(cuda, dtype):
     h, w, ids, teacher = inputs(cuda, 1, 64, 300, 6, dtype)
     want = both(h, w, ids, teacher)
     assert all(torch.equal(a, b) for a, b in zip(both(one_row_of(h, 131), w, ids, teacher), want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("d", [64, 50])
+def test_logprob_of_repeated_rows(cuda, dtype, d):
+    """One hidden row for every target, and a head of one row repeated: expanded tensors."""
+    h, w, ids, _ = inputs(cuda, 9, d, 300, 1, dtype)
+    target = ids[:, 0].contiguous()
+    want = logprob(h[:1].expand(9, d).contiguous(), w, target)
+    assert all(torch.equal(a, b) for a, b in zip(logprob(h[:1].expand(9, d), w, target), want))
+    one = w[:1].expand(300, d)
+    want = logprob(h, one.contiguous(), target)
+    assert all(torch.equal(a, b) for a, b in zip(logprob(h, one, target), want))

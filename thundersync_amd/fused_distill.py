@@ -141,11 +141,6 @@ def _live_rows(h, state):
     return out
 
 
-def _apart(t):
-    """``t`` with rows that do not overlap (an expanded row is copied)."""
-    return t if t.stride(0) >= t.shape[1] or t.shape[0] <= 1 else t.contiguous()
-
-
 class _KeptBlocks:
     """The blocks that losses keep until their backward, so that together they hold no more than a weight does (a
     1999 x 151936 block is 0.6 GB, beside a weight of D 2048 as large: a batch scored in sixteen calls kept 9.7 GB).
@@ -188,7 +183,7 @@ class _Rows:
             self.h, self.w = _unit_stride(hidden), _unit_stride(weight)
             self.ld = (weight.shape[0] + 3) // 4 * 4  # rows of whole 16-byte vectors
         else:
-            self.h, self.w = (_rows_ok(_pad_dim(_apart(t))) for t in (hidden, weight))
+            self.h, self.w = (_rows_ok(_pad_dim(t)) for t in (hidden, weight))
             self.ld = (weight.shape[0] + 7) // 8 * 8
         self.n, self.d = self.h.shape
         self.v = weight.shape[0]

@@ -86,9 +86,9 @@ def _pad_dim(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows_ok(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with rows of unit stride that start on 16-byte borders.  (A copy where they do not: torch
-    calls a tensor contiguous wherever it starts, and one row whatever its stride.)"""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+    """``t`` with rows of unit stride that start on 16-byte borders and do not overlap.  (A copy where
+    not: torch calls a tensor contiguous wherever it starts, and one row whatever its stride.)"""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
