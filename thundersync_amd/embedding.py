@@ -10,10 +10,10 @@ A token id outside ``[0, vocab)`` gives a row of NaN and no gradient (a bad id
 surfaces as a NaN loss, as a target of the fused logprob does);
 ``THUNDERSYNC_CHECK_TARGETS=1`` checks the ids first and raises.
 
-:func:`use_hip_embedding` swaps a model's ``torch.nn.Embedding`` modules for
-:class:`HipEmbedding`, with the Parameter's identity kept (a head tied to the
-table stays tied).  GPU only: other dtypes and CPU tensors raise in
-:func:`embedding`; the swapped module keeps torch's forward for them.
+:func:`use_hip_embedding` turns a model's ``torch.nn.Embedding`` modules into
+:class:`HipEmbedding`, in place (a head tied to a table stays tied, hooks stay).
+GPU only: other dtypes and CPU tensors raise in :func:`embedding`; the module
+keeps torch's forward for them.
 """
 
 from __future__ import annotations
@@ -137,19 +137,16 @@ class HipEmbedding(torch.nn.Embedding):
 
 
 def use_hip_embedding(model: torch.nn.Module) -> int:
-    """Swap every plain ``torch.nn.Embedding`` below ``model`` for :class:`HipEmbedding`
-    and return the count.  Modules with ``max_norm``, ``scale_grad_by_freq`` or
-    ``sparse`` and subclasses of their own are left alone."""
+    """Make every plain ``torch.nn.Embedding`` below ``model`` a :class:`HipEmbedding`
+    and return the count.  The modules stay the same objects, with their Parameter,
+    hooks and attributes, under every name they go by.  Modules with ``max_norm``,
+    ``scale_grad_by_freq`` or ``sparse`` and subclasses of their own are left alone."""
     count = 0
-    for name, module in list(model.named_modules()):
+    for name, module in model.named_modules():
         if not name or type(module) is not torch.nn.Embedding:
             continue
         if module.max_norm is not None or module.scale_grad_by_freq or module.sparse:
             continue
-        with torch.device("meta"):
-            swapped = HipEmbedding(module.num_embeddings, module.embedding_dim, module.padding_idx)
-        swapped.weight = module.weight
-        swapped.train(module.training)
-        model.set_submodule(name, swapped)
+        module.__class__ = HipEmbedding  # no state of its own
         count += 1
     return count
