@@ -22,6 +22,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .fused_logprob import CHECK_TARGETS_ENV, _check_targets
@@ -94,6 +95,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         ctx.vocab, ctx.dtype, ctx.scale, ctx.padding_idx = weight.shape[0], weight.dtype, scale, padding_idx
         with _lib.device_of(weight), operator_range(
                 "embedding_forward", role=device_role(weight.device), tokens=ids.numel(), hidden=weight.shape[1],
@@ -110,15 +112,22 @@ class _Embedding(torch.autograd.Function):
             gw = embedding_backward(ids, grad.to(ctx.dtype), ctx.vocab, scale=ctx.scale, padding_idx=ctx.padding_idx)
         return None, gw, None, None
 
+    @staticmethod
+    def jvp(ctx, ids_tangent, weight_tangent, *_):
+        (ids,) = ctx.saved_tensors
+        with _lib.device_of(weight_tangent):
+            return embedding_forward(ids, weight_tangent, ctx.scale)
+
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
               padding_idx: int | None = None) -> torch.Tensor:
     """``scale * weight[ids]``: ``[*ids.shape, D]`` for int64 or int32 ``ids`` of any shape.
 
-    The row ``padding_idx`` of the table gets no gradient.
+    The row ``padding_idx`` of the table gets no gradient.  A table's forward-mode
+    tangent reaches the rows.
     """
     _validate(ids, weight, scale, padding_idx)
-    if not (weight.requires_grad and torch.is_grad_enabled()):
+    if not (weight.requires_grad and torch.is_grad_enabled()) and forward_ad.unpack_dual(weight).tangent is None:
         with _lib.device_of(weight):
             return embedding_forward(ids, weight.detach(), float(scale))
     return _Embedding.apply(ids, weight, float(scale), padding_idx)
