@@ -493,7 +493,8 @@ struct RowOptions {
     temp = a.o.temperature ? (double)a.o.temperature[r] : a.o.temperature_all;
     top_k = a.o.top_k ? (int64_t)a.o.top_k[r] : a.o.top_k_all;
     top_p = a.o.top_p ? (double)a.o.top_p[r] : a.o.top_p_all;
-    min_p = fmin(a.o.min_p ? (double)a.o.min_p[r] : a.o.min_p_all, 1.);
+    min_p = a.o.min_p ? (double)a.o.min_p[r] : a.o.min_p_all;
+    min_p = min_p > 0. ? fmin(min_p, 1.) : 0.;  // NaN: none
     u = a.uniform_wide ? ((const double*)a.uniform)[r] : (double)((const float*)a.uniform)[r];
     u = u < 0. ? 0. : u;
     greedy = !(temp > 0.) || top_k == 1;

@@ -59,7 +59,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     ``temperature``, ``top_p`` and ``min_p`` are numbers or fp32 tensors
     ``[B]``, ``top_k`` a whole number or an int32 tensor ``[B]``; per-row values
     are not looked at on the host (a negative or NaN temperature counts as 0,
-    a ``top_k`` below 1 and a NaN ``top_p`` as none, a ``min_p`` above 1 as 1).
+    a ``top_k`` below 1, a NaN ``top_p`` and a NaN ``min_p`` as none, a ``min_p``
+    above 1 as 1).
     """
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
