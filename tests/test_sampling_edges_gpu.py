@@ -26,3 +26,18 @@ def test_a_rows_nan_options_filter_nothing(cuda):
     want = sample_tokens(z, u, top_p=half)
     got = sample_tokens(z, u, top_p=half, min_p=nan)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("temperature", [1e30, 1e292, 1.7e308])
+@pytest.mark.parametrize("options", [{}, {"top_p": 0.9}, {"top_k": 7}, {"min_p": 0.5}])
+def test_infinite_logits_at_any_temperature(cuda, temperature, options):
+    """A logit below an infinite one has no weight, however hot the row; among finite ones everything is even (0.1 in
+    fp32 is above a tenth, 0.9 below nine)."""
+    z = torch.zeros(2, 3000, device=cuda)
+    z[0, 17] = z[0, 2900] = math.inf
+    z[1] = torch.arange(3000, device=cuda) % 7
+    for u, first, second in ((0.1, 17, 300), (0.9, 2900, 2699)):
+        tokens, logprobs = sample_tokens(z, torch.full((2,), u, device=cuda), temperature=temperature, **options)
+        assert tokens[0] == first and abs(logprobs[0].item() - math.log(0.5)) <= 2.0 ** -24
+        if not options:
+            assert tokens[1] == second and abs(logprobs[1].item() + math.log(3000)) <= 2.0 ** -20

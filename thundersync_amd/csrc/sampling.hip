@@ -175,8 +175,9 @@ __device__ __forceinline__ Weights weights_of(const double* table, float top, fl
   // an infinite maximum: above every finite logit, and at its equals (whose difference is clamped to 0)
   w.top = top < inf() ? (double)top : 1e300;
   w.top_f = top;
-  // a T so small or so large that nothing, or everything, is the maximum's equal keeps finite products
-  w.units = fmin(fmax(kTable * (1.4426950408889634074 / temp), 1e-300), 1e300);
+  // a T so small or so large that nothing, or everything, is the maximum's equal keeps finite products,
+  // and one so large still has every finite logit 1000 octaves below an infinite one's 1e300
+  w.units = fmin(fmax(kTable * (1.4426950408889634074 / temp), 1e-290), 1e300);
   w.fixed = fixed;
   const float octave = (float)(0.693147180559945309 * temp);  // in units of logit
   w.bins = fminf(fmaxf(kBinsPerOctave / octave, (float)kBins / (top - low)), 1e30f);
