@@ -617,8 +617,10 @@ int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_
  * Sampling (fp32, fp16 or bf16 logits)
  * ------------------------------------------------------------------------ */
 
-/* Workspace bytes ts_sample needs (for up to 4096 rows at a time). */
-int64_t ts_sample_workspace(int64_t rows, int64_t vocab);
+/* Workspace bytes ts_sample needs: for a call with a top_k (a pointer, or one
+ * above 1 and below vocab) or top_p (a pointer, or one below 1) with filters 1,
+ * for any other with 0.  Many rows are taken in sets of about 128 MB. */
+int64_t ts_sample_workspace(int64_t rows, int64_t vocab, int filters);
 
 /* One token per row of logits [rows, vocab] from uniform[rows] (TS_F32 or
  * TS_F64, in [0, 1)) and the logprob of the token in the distribution it was

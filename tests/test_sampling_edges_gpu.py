@@ -41,3 +41,20 @@ def test_infinite_logits_at_any_temperature(cuda, temperature, options):
         assert tokens[0] == first and abs(logprobs[0].item() - math.log(0.5)) <= 2.0 ** -24
         if not options:
             assert tokens[1] == second and abs(logprobs[1].item() + math.log(3000)) <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("options", [{}, {"top_p": 0.9, "top_k": 40}])
+def test_rows_of_several_sets(cuda, options):
+    """Rows past one set of launches, the last set shorter: each row's token is its own."""
+    g = torch.Generator(device=cuda).manual_seed(3)
+    z = torch.randn(5003, 3000, generator=g, device=cuda)
+    u = torch.rand(5003, generator=g, device=cuda)
+    got = sample_tokens(z, u, **options)
+    for part in (slice(0, 5), slice(1666, 1672), slice(2500, 2504), slice(4990, 5003)):
+        want = sample_tokens(z[part], u[part], **options)
+        assert torch.equal(got[0][part], want[0]) and torch.equal(got[1][part], want[1])
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    sample_tokens(z, u, **options)
+    assert torch.cuda.max_memory_allocated() - before <= (136 << 20 if options else 8 << 20)

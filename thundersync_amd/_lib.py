@@ -100,7 +100,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ts_embedding_fwd": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _F, _P, _INT, _P]),
     "ts_embedding_bwd_workspace": (_I64, [_I64, _I64]),
     "ts_embedding_bwd": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _F, _P, _P, _I64, _INT, _P]),
-    "ts_sample_workspace": (_I64, [_I64, _I64]),
+    "ts_sample_workspace": (_I64, [_I64, _I64, _INT]),
     "ts_sample": (
         _INT, [_P, _I64, _I64, _I64, _P, _INT, _P, _D, _P, _I64, _P, _D, _P, _D, _P, _P, _P, _I64, _INT, _P]),
     "ts_adjoint_reduce": (_INT, [ctypes.POINTER(_P), _INT, _P, _P, _I64, _INT, _P]),

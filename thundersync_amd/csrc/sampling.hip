@@ -523,17 +523,17 @@ struct Bins {
   uint64_t all_mass;
 };
 
-// The launches' workspace, of `rows` rows and `slices` slices.  From `bins` on only where some
-// row of the call has a top_k or top_p: null otherwise.
+// The launches' workspace, of `rows` rows, `slices` slices and `parts` shares of a row's
+// histogram.  From `bins` on only where some row of the call has a top_k or top_p: null otherwise.
 struct Space {
   SliceStats* stats;  // [rows][slices]
   double* sums;       // [rows][slices][kSums]: of a slice's waves (without filters the first alone)
   Bins* bins;         // [rows]
-  uint64_t* mass;     // [rows][kBinParts][kBins]
-  uint32_t* count;    // [rows][kBinParts][kBins]
+  uint64_t* mass;     // [rows][parts][kBins]
+  uint32_t* count;    // [rows][parts][kBins]
   uint64_t* cand;     // [rows][kCandidates]
   uint32_t* n_cand;   // [rows]
-  int slices;
+  int slices, parts;
 };
 
 // the row's maximum, lowest logit and NaN from its slices (every thread reads them all: few)
@@ -717,7 +717,7 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(Args a, Space sp) {
     }
   }
   __syncthreads();
-  const int64_t base = (r * kBinParts + blockIdx.x) * kBins;
+  const int64_t base = (r * sp.parts + blockIdx.x) * kBins;
   for (int i = t; i < kBins; i += kThreads) {
     if (o.by_k) sp.count[base + i] = count[i];
     if (o.by_p) sp.mass[base + i] = mass[i];
@@ -731,14 +731,15 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(Args a, Space sp) {
 // shares read again by each cost more (64 rows: gather 27 -> 42 us against a search of 9.6).
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 4;
-__device__ __forceinline__ void search_bins(const Space& sp, int64_t r, const RowOptions& o, int parts, Bins& found) {
+__device__ __forceinline__ void search_bins(const Space& sp, int64_t r, const RowOptions& o, Bins& found) {
   __shared__ uint64_t wave_m[kThreads / 64];
   __shared__ uint32_t wave_c[kThreads / 64];
   __shared__ uint64_t bin_mass;  // of bin k
   constexpr int PER = kBins / kThreads;
   const int t = threadIdx.x;
-  const uint32_t* count = sp.count + r * kBinParts * kBins;
-  const uint64_t* mass = sp.mass + r * kBinParts * kBins;
+  const int parts = sp.parts;
+  const uint32_t* count = sp.count + r * parts * kBins;
+  const uint64_t* mass = sp.mass + r * parts * kBins;
   if (t == 0) found = Bins{kBins, kBins, kBins, 0, 0, 0, 0};
   uint32_t c[PER] = {}, cs = 0;
   uint64_t m[PER] = {}, ms = 0;
@@ -820,13 +821,13 @@ __device__ __forceinline__ void search_bins(const Space& sp, int64_t r, const Ro
   }
 }
 
-__global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int parts) {
+__global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp) {
   __shared__ Bins found;
   const int64_t r = blockIdx.x;
   const RowOptions o(a, r);
   if (!o.by_k && !o.by_p) return;
   if (RowStats(sp.stats + r * sp.slices, sp.slices).empty()) return;  // it has no histogram
-  search_bins(sp, r, o, parts, found);
+  search_bins(sp, r, o, found);
   __syncthreads();
   if (threadIdx.x == 0) sp.bins[r] = found;
 }
@@ -836,7 +837,7 @@ __global__ __launch_bounds__(kThreads) void search_kernel(Args a, Space sp, int 
 // at 64 rows of 151936, 28 at 333 of 50257, 13 with the search at one row.
 // ---------------------------------------------------------------------------
 template <typename T, bool SEARCH>
-__global__ __launch_bounds__(kThreads, SEARCH ? 4 : 8) void gather_kernel(Args a, Space sp, int parts) {
+__global__ __launch_bounds__(kThreads, SEARCH ? 4 : 8) void gather_kernel(Args a, Space sp) {
   __shared__ Bins found;
   __shared__ double table[kTable];
   __shared__ uint64_t cand[kCandidates];
@@ -851,7 +852,7 @@ __global__ __launch_bounds__(kThreads, SEARCH ? 4 : 8) void gather_kernel(Args a
   fill_table(table);
   const Weights w = weights_of(table, s.top, s.low, o.temp, a.fixed);
   if (SEARCH && (o.by_k || o.by_p)) {
-    search_bins(sp, r, o, parts, found);
+    search_bins(sp, r, o, found);
     __syncthreads();
     if (blockIdx.x == 0 && t == 0) sp.bins[r] = found;  // the draw's
   }
@@ -1222,14 +1223,20 @@ __global__ __launch_bounds__(kDrawThreads) void draw_kernel(Args a, Space sp) {
   }, s);
 }
 
-constexpr int64_t kRowsAtOnce = 4096;  // rows per set of launches: bounds the workspace
-
 int slices_of(int64_t vocab) {
   return (int)((((vocab + 2 * kGroup - 2) / kGroup) + kSliceGroups - 1) / kSliceGroups);  // of a row at any alignment
 }
 int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
 
-int64_t space_of(int64_t rows, int64_t vocab, bool bins, char* base, Space* sp) {
+// Work-groups a row, for about 1024 in the launch, and no more than the slices fill evenly (19 slices over 16
+// work-groups end when the three that have two do: 10 of two).
+int64_t per_row(int64_t rows, int64_t slices, int64_t most) {
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({most, slices, (1024 + rows / 2) / rows}));
+  const int64_t each = (slices + parts - 1) / parts;
+  return (slices + each - 1) / each;
+}
+
+int64_t space_of(int64_t rows, int64_t vocab, bool bins, int64_t parts, char* base, Space* sp) {
   const int64_t slices = slices_of(vocab);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1239,18 +1246,34 @@ int64_t space_of(int64_t rows, int64_t vocab, bool bins, char* base, Space* sp) 
   };
   Space s{};
   s.slices = (int)slices;
+  s.parts = (int)parts;
   s.stats = (SliceStats*)take(rows * slices * (int64_t)sizeof(SliceStats));
   s.sums = (double*)take(rows * slices * kSums * 8);
   if (bins) {
     s.bins = (Bins*)take(rows * (int64_t)sizeof(Bins));
-    s.mass = (uint64_t*)take(rows * kBinParts * kBins * 8);
-    s.count = (uint32_t*)take(rows * kBinParts * kBins * 4);
+    s.mass = (uint64_t*)take(rows * parts * kBins * 8);
+    s.count = (uint32_t*)take(rows * parts * kBins * 4);
     s.cand = (uint64_t*)take(rows * kCandidates * 8);
     s.n_cand = (uint32_t*)take(rows * 4);
   }
   if (sp) *sp = s;
   return at;
 }
+
+// How a call's rows are cut into sets of launches of equal size (but the last), so that a set's workspace stays below
+// about kSpaceBytes (filters over 151936 tokens: 2277 rows; a histogram of several parts comes with few rows), and
+// the parts of a row's histogram in all of them.
+constexpr int64_t kSpaceBytes = 128 << 20;
+struct Sets {
+  int64_t rows, parts, bytes;
+  Sets(int64_t all, int64_t vocab, bool bins) {
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096, kSpaceBytes / space_of(1, vocab, bins, 1, nullptr, nullptr)));
+    const int64_t sets = (all + most - 1) / most;
+    rows = (all + sets - 1) / sets;
+    parts = per_row(rows, slices_of(vocab), kBinParts);
+    bytes = space_of(rows, vocab, bins, parts, nullptr, nullptr);
+  }
+};
 
 template <typename T>
 void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bins, hipStream_t s) {
@@ -1260,29 +1283,19 @@ void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bin
     if (bins) hipLaunchKernelGGL((maxima_kernel<T, true>), grid, block, 0, s, a, sp);
     else hipLaunchKernelGGL((maxima_kernel<T, false>), grid, block, 0, s, a, sp);
   }
-  // work-groups a row, for about `all` in the launch, and no more than the slices fill evenly (19 slices over 16
-  // work-groups end when the three that have two do: 10 of two)
-  auto per_row = [&](int64_t all, int64_t most) {
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)sp.slices, (all + rows / 2) / rows}));
-    const int64_t each = (sp.slices + parts - 1) / parts;
-    return (unsigned)((sp.slices + each - 1) / each);
-  };
-  const unsigned parts = per_row(1024, kBinParts);
   if (bins) {
     TimedLaunch timed_("sampling.bins_kernel", s);
-    hipLaunchKernelGGL(bins_kernel<T>, dim3(parts, (unsigned)rows), dim3(kThreads), 0, s, a, sp);
+    hipLaunchKernelGGL(bins_kernel<T>, dim3((unsigned)sp.parts, (unsigned)rows), dim3(kThreads), 0, s, a, sp);
   }
   if (bins && rows > kFewRows) {
     TimedLaunch timed_("sampling.search_kernel", s);
-    hipLaunchKernelGGL(search_kernel, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp, (int)parts);
+    hipLaunchKernelGGL(search_kernel, dim3((unsigned)rows), dim3(kThreads), 0, s, a, sp);
   }
   if (filters) {
     TimedLaunch timed_("sampling.gather_kernel", s);
-    const dim3 gathers(per_row(1024, sp.slices), (unsigned)rows), threads(kThreads);
-    if (bins && rows <= kFewRows)
-      hipLaunchKernelGGL((gather_kernel<T, true>), gathers, threads, 0, s, a, sp, (int)parts);
-    else
-      hipLaunchKernelGGL((gather_kernel<T, false>), gathers, threads, 0, s, a, sp, (int)parts);
+    const dim3 gathers((unsigned)per_row(rows, sp.slices, sp.slices), (unsigned)rows), threads(kThreads);
+    if (bins && rows <= kFewRows) hipLaunchKernelGGL((gather_kernel<T, true>), gathers, threads, 0, s, a, sp);
+    else hipLaunchKernelGGL((gather_kernel<T, false>), gathers, threads, 0, s, a, sp);
   }
   {
     TimedLaunch timed_("sampling.draw_kernel", s);
@@ -1295,10 +1308,9 @@ void launch(const Args& a, const Space& sp, int64_t rows, bool filters, bool bin
 
 extern "C" {
 
-int64_t ts_sample_workspace(int64_t rows, int64_t vocab) {
+int64_t ts_sample_workspace(int64_t rows, int64_t vocab, int filters) {
   using namespace ts::sample;
-  return rows > 0 && vocab > 0 && vocab <= kMaxVocab ? space_of(std::min(rows, kRowsAtOnce), vocab, true, nullptr, nullptr)
-                                                     : 0;
+  return rows > 0 && vocab > 0 && vocab <= kMaxVocab ? Sets(rows, vocab, filters != 0).bytes : 0;
 }
 
 int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, const void* uniform,
@@ -1329,14 +1341,13 @@ int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab
   a.logprobs = logprobs;
   const bool by_min = min_p || min_p_all > 0;
   const bool bins = top_k || top_p || (top_k_all > 1 && top_k_all < vocab) || top_p_all < 1;
-  const int64_t at_once = std::min(rows, kRowsAtOnce);
-  const int64_t need = space_of(at_once, vocab, true, nullptr, nullptr);
-  TS_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need,
-               "ts_sample: workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)need);
+  const Sets sets(rows, vocab, bins);
+  TS_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= sets.bytes,
+               "ts_sample: workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)sets.bytes);
   hipStream_t s = (hipStream_t)stream;
   const int64_t size = dtype == TS_F32 ? 4 : 2;
-  for (int64_t r0 = 0; r0 < rows; r0 += at_once) {
-    const int64_t n = std::min(at_once, rows - r0);
+  for (int64_t r0 = 0; r0 < rows; r0 += sets.rows) {
+    const int64_t n = std::min(sets.rows, rows - r0);
     Args b = a;
     b.logits = (const char*)logits + r0 * ld_logits * size;
     b.uniform = (const char*)uniform + r0 * (a.uniform_wide ? 8 : 4);
@@ -1347,7 +1358,7 @@ int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab
     b.tokens += r0;
     b.logprobs += r0;
     Space sp;
-    space_of(n, vocab, bins, (char*)workspace, &sp);
+    space_of(n, vocab, bins, sets.parts, (char*)workspace, &sp);
     if (dtype == TS_F32) launch<float>(b, sp, n, bins || by_min, bins, s);
     else if (dtype == TS_F16) launch<ts::f16>(b, sp, n, bins || by_min, bins, s);
     else launch<ts::bf16>(b, sp, n, bins || by_min, bins, s);

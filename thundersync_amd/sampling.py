@@ -88,9 +88,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     b, v = z.shape
     tokens = torch.empty(b, dtype=torch.int64, device=z.device)
     logprobs = torch.empty(b, dtype=torch.float32, device=z.device)
-    ws_bytes = int(lib.ts_sample_workspace(b, v))
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=z.device)
     (t_rows, t_all), (k_rows, k_all), (p_rows, p_all), (m_rows, m_all) = options
+    filters = k_rows is not None or p_rows is not None or 1 < k_all < v or p_all < 1
+    ws_bytes = int(lib.ts_sample_workspace(b, v, int(filters)))
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=z.device)
     with _lib.device_of(z), operator_range("sample_tokens", role=device_role(z.device), rows=b, vocab=v,
                                                      dtype=z.dtype):
         _lib.check(
