@@ -7,6 +7,7 @@ import math
 import pytest
 import torch
 
+from oracle import sampling as ref
 from thundersync_amd.sampling import sample_tokens
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +59,22 @@ def test_rows_of_several_sets(cuda, options):
     before = torch.cuda.memory_allocated()
     sample_tokens(z, u, **options)
     assert torch.cuda.max_memory_allocated() - before <= (136 << 20 if options else 8 << 20)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("options", [{"temperature": 5.0, "top_p": 0.9}, {"temperature": 5.0, "top_k": 9000},
+                                     {"temperature": 3.0, "top_k": 20000, "top_p": 0.8, "min_p": 0.01}])
+def test_masks_of_the_lowest_finite_value(cuda, dtype, options):
+    """Such a mask stretches the row's range to the type's, and close logits then share a few bins, more of them than
+    are sorted at once: the same tokens as with masks of -inf."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    z = (0.3 * torch.randn(3, 40001, generator=g, device=cuda)).to(dtype)
+    masked = torch.rand(3, 40001, generator=g, device=cuda) < 0.2
+    u = torch.rand(3, generator=g, device=cuda, dtype=torch.float64)
+    want = sample_tokens(z.masked_fill(masked, -math.inf), u, **options)
+    low = z.masked_fill(masked, torch.finfo(dtype).min)
+    got = sample_tokens(low, u, **options)
+    assert torch.equal(got[0], want[0])
+    for i in range(3):
+        token, logprob = ref.sample(low[i].double().cpu().numpy(), float(u[i]), **options)
+        assert got[0][i] == token and abs(got[1][i].item() - logprob) <= 2.0 ** -23 * max(1.0, abs(logprob))

@@ -1001,7 +1001,12 @@ template <int N> __device__ __forceinline__ void pick_slice(Scratch<N>& s, int s
   }
 }
 
-// A row whose border bins hold too many logits, by its work-group alone: see find_border.
+// A row whose border bins hold too many logits, by its work-group alone: see find_border.  Logits
+// that are all equal, or close together in a row whose range a mask of the lowest finite value
+// stretches (the bins are then 1/32 octave wide).  A launch of such rows takes, with 151936 fp32
+// tokens, T = 5 and top_p (top_k 50000 and top_p): 64 rows masked by -inf, none of them slow, 76
+// (100) us, masked by the lowest value 135 (662), all equal 501 (454); 512 rows 309 (361), 388
+// (1139), 1129 (1179).
 template <typename T, int N>
 __device__ __forceinline__ void slow_row(const Args& a, int64_t r, const Row<T>& row, const RowOptions& o, const Weights& w, int slices,
                          Scratch<N>& s) {
