@@ -49,9 +49,14 @@ def bounds(ref, dtype, top, temperature=1.0):
     """How far loss, dh and dw may be off ``ref`` (an oracle's result), per element.
 
     With a = 2^-24 (fp32 sums; 2^-53 for fp64) and u the element type's half step:
-    * a logit over T is off by at most e = (D + 4) a max_v sum_d |h w| / T (D products added in any order);
-    * its exponential by e + 4 ulp of the argument and the function, |z| <= Z: rel = e + (8 + 2 Z) a; sums of V of
-      them by V a more, lse likewise;
+    * a logit over T, in fp32 or fp64, is off by at most e = (D + 4) a max_v sum_d |h w| / T (D products added in any
+      order).  bf16 and fp16: MFMA adds 16 products at a time, so the sum is rounded D / 16 + 20 times (the last of a
+      block of its own), each time by a of what it then is: no more than sum_d |h w|, and of terms of either sign within
+      |z| + 4 (sum_d (h w)^2)^(1/2), four deviations of its random walk;
+    * its exponential by e + 4 ulp of the argument and the function, |z| <= Z: rel = e + (8 + 2 Z) a.  The sum of V of
+      them is added in blocks, by at most a a step: 128 of a tile's 256 in a lane and 6 across the lanes, then
+      V / 16384 tiles of a slot and 18 slots, three roundings each (fp32 and fp64: V / 512 of a thread and 16 across
+      them); lse likewise;
     * the loss, a sum of K terms p (log p - z + lse), by 2 rel + (K + 8) a (its terms' size).
     * dz's entries are rounded to the element type twice at most (the exponential, its product with the row's
       factors) on top of that: each by (2 u + 2 rel + V a) g (q + p), and below the smallest normal number by
@@ -65,7 +70,13 @@ def bounds(ref, dtype, top, temperature=1.0):
     d = h.shape[1]
     finite = torch.isfinite(z)
     size = torch.where(finite, z.abs(), 0.0).amax(dim=1, keepdim=True) if v else z
-    rel = (d + 4) * a * (h.abs() @ w.abs().T).amax(dim=1, keepdim=True) / temperature + (8 + 2 * size) * a + v * a
+    added = h.abs() @ w.abs().T
+    if dtype in (torch.bfloat16, torch.float16):
+        walk = torch.where(finite, z.abs() * temperature, math.inf) + 4 * ((h * h) @ (w * w).T).sqrt()
+        added, steps, depth = torch.minimum(added, walk), d / 16 + 20, 134 + 3 * (v / 16384 + 18)
+    else:
+        steps, depth = d + 4, v / 512 + 16
+    rel = steps * a * added.amax(dim=1, keepdim=True) / temperature + (8 + 2 * size) * a + depth * a
     terms = torch.where(p > 0, p * (torch.log(torch.where(p > 0, p, 1.0)).abs() + size + math.log(v) + 1), 0.0).sum(dim=1)
     loss = 2 * rel[:, 0] + (top + 8) * a * (1 + terms)
     tiny = 2.0 ** -24 if dtype == torch.float16 else 0.0
