@@ -608,7 +608,7 @@ int64_t ts_embedding_bwd_workspace(int64_t n, int64_t dim);
  * grad_out's rows (row stride ld_grad, 0 for one row for all) by id, in fp32 in
  * token order and rounded once: the same bytes on every call.  Ids outside the
  * vocabulary and the id `padding` (-1: none) take no part; rows no id names are
- * zero.  n and vocab below 2^31 - 1. */
+ * zero.  n below 2^28, vocab below 2^31 - 1. */
 int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_t ld_grad, int64_t vocab, int64_t dim,
                      int64_t padding, float scale, void* grad_weight, void* workspace, int64_t workspace_bytes,
                      int dtype, void* stream);

@@ -19,6 +19,8 @@ namespace ts {
 namespace embed {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMaxBlocks = 1 << 23;  // of kThreads along one axis: a launch takes fewer than 2^32 threads there
+constexpr int64_t kMaxTokens = 1 << 28;  // of a gradient: every tile of its sort reads all tiles' counts
 constexpr int kChunk = 32;      // sorted positions per work-group of the reduction, at most
 constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
 constexpr int kRounds = 8, kWaves = kThreads / 64, kSortTile = kThreads * kRounds;
@@ -51,16 +53,16 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(const int64_t* __restrict__ ids, int64_t n,
                                                           const T* __restrict__ w, int64_t ldw, int64_t vocab, int dim,
                                                           float scale, T* __restrict__ out) {
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= n) return;
-  const int64_t id = ids[row];
-  const bool ok = id >= 0 && id < vocab;
-  for (int d = (blockIdx.y * blockDim.x + threadIdx.x) * VEC; d < dim; d += gridDim.y * blockDim.x * VEC) {
-    float x[VEC];
-    if (ok) load_vec<T, VEC>(w + id * ldw + d, x);
+  for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < n; row += (int64_t)gridDim.x * blockDim.y) {
+    const int64_t id = ids[row];
+    const bool ok = id >= 0 && id < vocab;
+    for (int d = (blockIdx.y * blockDim.x + threadIdx.x) * VEC; d < dim; d += gridDim.y * blockDim.x * VEC) {
+      float x[VEC];
+      if (ok) load_vec<T, VEC>(w + id * ldw + d, x);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = ok ? x[i] * scale : __builtin_nanf("");
-    store_vec<T, VEC>(out + row * dim + d, x);
+      for (int i = 0; i < VEC; ++i) x[i] = ok ? x[i] * scale : __builtin_nanf("");
+      store_vec<T, VEC>(out + row * dim + d, x);
+    }
   }
 }
 
@@ -431,7 +433,7 @@ void launch_lookup(const int64_t* ids, int64_t n, const void* w, int64_t ldw, in
   int tx = 1;
   while (tx < kThreads && tx < lanes) tx *= 2;
   const dim3 block((unsigned)tx, (unsigned)(kThreads / tx));
-  const dim3 grid((unsigned)((n + block.y - 1) / block.y), (unsigned)((lanes + tx - 1) / tx));
+  const dim3 grid((unsigned)std::min<int64_t>((n + block.y - 1) / block.y, kMaxBlocks), (unsigned)((lanes + tx - 1) / tx));
   if (vec)
     hipLaunchKernelGGL((lookup_kernel<T, kVec<T>>), grid, block, 0, s, ids, n, (const T*)w, ldw, vocab, (int)dim, scale,
                        (T*)out);
@@ -490,7 +492,7 @@ int ts_embedding_bwd(const int64_t* ids, int64_t n, const void* grad_out, int64_
                      int64_t padding, float scale, void* grad_weight, void* workspace, int64_t workspace_bytes,
                      int dtype, void* stream) {
   TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F16 || dtype == TS_BF16, "ts_embedding_bwd: dtype %d", dtype);
-  TS_CHECK_ARG(n >= 0 && n < (1ll << 31) && vocab >= 0 && vocab < (1ll << 31) - 1 && dim >= 1 && dim < (1 << 20),
+  TS_CHECK_ARG(n >= 0 && n < kMaxTokens && vocab >= 0 && vocab < (1ll << 31) - 1 && dim >= 1 && dim < (1 << 20),
                "ts_embedding_bwd: bad shape n=%lld vocab=%lld dim=%lld", (long long)n, (long long)vocab,
                (long long)dim);
   if (vocab == 0) return TS_OK;
