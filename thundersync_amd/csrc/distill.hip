@@ -35,6 +35,8 @@ using namespace ts::gemm;
 using namespace ts::head;
 
 constexpr int kMaxTop = 1024;   // slots per row
+constexpr int kRowThreads = 512;  // of the kernels that give a row a work-group, at most
+constexpr int64_t kMaxRows = (1ll << 32) / kRowThreads;  // a launch of 2^32 threads along an axis wraps
 constexpr int kRowWaves = 4;    // rows per work-group of the per-row kernels
 constexpr int kDead = 0, kLive = 1, kBadId = 2;  // row states
 constexpr int kHeadroom = 14;   // octaves of a frozen head's stored softmax above 1: below fp16's largest number
@@ -521,7 +523,6 @@ __global__ __launch_bounds__(256) void finish_kernel(const T* src, int64_t lds, 
 // 50 us at 600 x 32003 in fp32, beside 1.2 ms of the three products (0.4 ms each, 99 TFLOP/s
 // of fp32 MFMA).
 // ---------------------------------------------------------------------------
-constexpr int kRowThreads = 512;
 template <typename C>
 __global__ __launch_bounds__(kRowThreads) void row_stats_kernel(const C* __restrict__ z, int64_t ldz, int vocab,
                                                                 C inv_t, const int32_t* __restrict__ slot_id,
@@ -704,7 +705,7 @@ int ts_distill_teacher(const int64_t* ids, const void* teacher, int64_t ld_teach
                        int64_t top, int64_t vocab, double temperature, int32_t* slot_id, void* slot_p,
                        int64_t pitch, int32_t* state, int dtype, void* stream) {
   TS_CHECK_ARG(known(teacher_dtype) && known(dtype), "ts_distill_teacher: dtypes %d, %d", teacher_dtype, dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && top > 0 && top <= kMaxTop && vocab > 0 && vocab < (1 << 30) &&
+  TS_CHECK_ARG(rows >= 0 && rows < kMaxRows && top > 0 && top <= kMaxTop && vocab > 0 && vocab < (1 << 30) &&
                    pitch >= top && pitch <= kMaxTop && ld_teacher >= top,
                "ts_distill_teacher: bad shape rows=%lld top=%lld (1 .. %d) vocab=%lld", (long long)rows,
                (long long)top, kMaxTop, (long long)vocab);
@@ -740,7 +741,7 @@ int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, in
                    void* exps, int64_t ld_exps, float* row_scale, void* workspace, int64_t workspace_bytes, int dtype,
                    void* stream) {
   TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_fwd: dtype %d (bf16 or fp16)", dtype);
-  TS_CHECK_ARG(rows >= 0 && dim > 0 && vocab > 0 && rows < (1 << 30) && vocab < (1 << 30) && dim < (1 << 20) &&
+  TS_CHECK_ARG(rows >= 0 && dim > 0 && vocab > 0 && rows < kMaxRows && vocab < (1 << 30) && dim < (1 << 20) &&
                    top > 0 && top <= pitch && pitch <= kMaxTop,
                "ts_distill_fwd: bad shape rows=%lld dim=%lld vocab=%lld top=%lld", (long long)rows, (long long)dim,
                (long long)vocab, (long long)top);
@@ -775,7 +776,7 @@ int ts_distill_fwd(const void* hidden, int64_t ld_hidden, const void* weight, in
   a.exps = (ts::bf16*)exps;
   a.lde = ld_exps;
   a.vocab_pad = (int)((vocab + 7) / 8 * 8);
-  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < (1ll << 31), "ts_distill_fwd: grid too large");
+  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < kMaxGrid, "ts_distill_fwd: grid too large");
   hipStream_t s = (hipStream_t)stream;
   {
     ts::TimedLaunch timed_("distill.stats_kernel", s);
@@ -803,7 +804,7 @@ int ts_distill_fwd_exact(const void* logits, int64_t ld_logits, int64_t rows, in
                          const int32_t* slot_id, const void* slot_p, void* slot_z, int64_t pitch, int64_t top,
                          const int32_t* state, void* loss, void* lse, int dtype, void* stream) {
   TS_CHECK_ARG(dtype == TS_F32 || dtype == TS_F64, "ts_distill_fwd_exact: dtype %d (fp32 or fp64)", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && vocab > 0 && vocab < (1 << 30) && ld_logits >= vocab && top > 0 &&
+  TS_CHECK_ARG(rows >= 0 && rows < kMaxRows && vocab > 0 && vocab < (1 << 30) && ld_logits >= vocab && top > 0 &&
                    top <= pitch && pitch <= kMaxTop,
                "ts_distill_fwd_exact: bad shape");
   TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_fwd_exact: temperature %g",
@@ -831,7 +832,7 @@ int ts_distill_softmax(void* block, int64_t ld_block, const float* tile_ref, con
                        int dtype, void* stream) {
   TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_softmax: dtype %d (bf16 or fp16)", dtype);
   const int64_t columns = (vocab + 7) / 8 * 8;
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && vocab > 0 && vocab < 65535ll * kFinish && top > 0 && top <= pitch &&
+  TS_CHECK_ARG(rows >= 0 && rows < kMaxRows && vocab > 0 && vocab < 65535ll * kFinish && top > 0 && top <= pitch &&
                    pitch <= kMaxTop && ld_block >= columns && ld_block % 8 == 0,
                "ts_distill_softmax: bad shape");
   if (rows == 0) return TS_OK;
@@ -855,7 +856,7 @@ int ts_distill_slots(float* unit, const float* row_scale, const void* weight, in
                      int64_t dim, double temperature, const int32_t* slot_id, const float* slot_p, const float* slot_z,
                      int64_t pitch, int64_t top, const float* lse, int dtype, void* stream) {
   TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_slots: dtype %d (bf16 or fp16)", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && dim > 0 && dim < (1 << 20) && dim % 8 == 0 && ld_weight >= dim &&
+  TS_CHECK_ARG(rows >= 0 && rows < kMaxRows && dim > 0 && dim < (1 << 20) && dim % 8 == 0 && ld_weight >= dim &&
                    ld_weight % 8 == 0 && top > 0 && top <= pitch && pitch <= kMaxTop,
                "ts_distill_slots: bad shape");
   TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_slots: temperature %g", temperature);
@@ -884,7 +885,7 @@ int ts_distill_finish(const void* stored, int64_t ld_stored, const float* tile_r
                       void* dlogits, int64_t ld_dlogits, int dtype, void* stream) {
   TS_CHECK_ARG(known(dtype), "ts_distill_finish: dtype %d", dtype);
   const bool exact = dtype == TS_F32 || dtype == TS_F64;
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && vocab > 0 && vocab < 65535ll * kFinish && top > 0 && top <= pitch &&
+  TS_CHECK_ARG(rows >= 0 && rows < kMaxRows && vocab > 0 && vocab < 65535ll * kFinish && top > 0 && top <= pitch &&
                    pitch <= kMaxTop && ld_stored >= vocab && ld_dlogits >= vocab,
                "ts_distill_finish: bad shape");
   TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_finish: temperature %g", temperature);
@@ -917,7 +918,7 @@ int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight
                        const float* slot_z, int64_t pitch, int64_t top, const int32_t* state, const float* lse,
                        const float* grad, void* dlogits, int64_t ld_dlogits, int dtype, void* stream) {
   TS_CHECK_ARG(dtype == TS_BF16 || dtype == TS_F16, "ts_distill_dlogits: dtype %d (bf16 or fp16)", dtype);
-  TS_CHECK_ARG(rows >= 0 && dim > 0 && vocab > 0 && rows < (1 << 30) && vocab < (1 << 30) && dim < (1 << 20) &&
+  TS_CHECK_ARG(rows >= 0 && dim > 0 && vocab > 0 && rows < kMaxRows && vocab < (1 << 30) && dim < (1 << 20) &&
                    top > 0 && top <= pitch && pitch <= kMaxTop,
                "ts_distill_dlogits: bad shape");
   TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_dlogits: temperature %g",
@@ -950,7 +951,7 @@ int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight
   a.inv_t = (float)(1. / temperature);
   a.dl = (ts::bf16*)dlogits;
   a.ldl = ld_dlogits;
-  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < (1ll << 31), "ts_distill_dlogits: grid too large");
+  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < kMaxGrid, "ts_distill_dlogits: grid too large");
   hipStream_t s = (hipStream_t)stream;
   {
     ts::TimedLaunch timed_("distill.dlogits_kernel", s);
@@ -975,7 +976,7 @@ int ts_distill_dlogits(const void* hidden, int64_t ld_hidden, const void* weight
 int ts_distill_rows(const void* hidden, int64_t ld_hidden, const int32_t* state, int64_t rows, int64_t dim, void* out,
                     int dtype, void* stream) {
   TS_CHECK_ARG(known(dtype), "ts_distill_rows: dtype %d", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && dim > 0 && dim < (1 << 20) && ld_hidden >= dim,
+  TS_CHECK_ARG(rows >= 0 && rows < kMaxRows && dim > 0 && dim < (1 << 20) && ld_hidden >= dim,
                "ts_distill_rows: bad shape");
   if (rows == 0) return TS_OK;
   TS_CHECK_ARG(hidden && state && out && hidden != out, "ts_distill_rows: null or aliased pointer");
@@ -997,7 +998,7 @@ int ts_distill_rows(const void* hidden, int64_t ld_hidden, const int32_t* state,
 int ts_distill_scale(const void* unit, const void* grad, const int32_t* state, int64_t rows, int64_t dim,
                      double temperature, void* out, int dtype, void* stream) {
   TS_CHECK_ARG(known(dtype), "ts_distill_scale: dtype %d", dtype);
-  TS_CHECK_ARG(rows >= 0 && rows < (1 << 30) && dim > 0 && dim < (1 << 20), "ts_distill_scale: bad shape");
+  TS_CHECK_ARG(rows >= 0 && rows < kMaxRows && dim > 0 && dim < (1 << 20), "ts_distill_scale: bad shape");
   TS_CHECK_ARG(temperature > 0 && temperature < __builtin_huge_val(), "ts_distill_scale: temperature %g", temperature);
   if (rows == 0) return TS_OK;
   TS_CHECK_ARG(unit && grad && state && out, "ts_distill_scale: null pointer");

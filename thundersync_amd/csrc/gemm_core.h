@@ -23,6 +23,8 @@ namespace gemm {
 
 constexpr int kWaves = 8;  // waves per work-group, two per SIMD
 constexpr int kGemmThreads = 64 * kWaves;
+// work-groups of a launch: one of 2^32 threads or more along an axis wraps, without an error
+constexpr int64_t kMaxGrid = (1ll << 32) / kGemmThreads;
 constexpr int TM = 256;  // A rows (vocab rows, or hidden dims) per work-group
 constexpr int TN = 256;  // B rows (tokens) per work-group
 constexpr int TK = 32;   // K per LDS stage

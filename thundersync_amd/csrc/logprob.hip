@@ -592,7 +592,8 @@ int ts_logprob_fwd(const void* hidden, int64_t ld_hidden, const void* weight, in
   a.part_m = ws;
   a.part_s = ws + (int64_t)a.n_vtiles * rows;
   a.part_e = ws + 2 * (int64_t)a.n_vtiles * rows;
-  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < (1ll << 31), "ts_logprob_fwd: grid too large");
+  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < kMaxGrid && rows < (1ll << 32) / kCombineThreads * kCombineTokens,
+               "ts_logprob_fwd: grid too large");
   hipStream_t s = (hipStream_t)stream;
   { ts::TimedLaunch timed_("logprob.fwd_stats_kernel", s); TS_LAUNCH_TOKENS(dtype, width, fwd_stats_kernel, dim3((unsigned)(a.n_ttiles * a.n_vtiles)), dim3(kGemmThreads),
                      0, s, a); }
@@ -645,6 +646,7 @@ int ts_logprob_dlogits(const void* hidden, int64_t ld_hidden, const void* weight
   a.dl = (ts::bf16*)dlogits;
   a.ldl = ld_dlogits;
   TS_CHECK_ARG(a.vocab_pad <= ld_dlogits, "ts_logprob_dlogits: ld_dlogits below padded vocab");
+  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_vtiles < kMaxGrid, "ts_logprob_dlogits: grid too large");
   { ts::TimedLaunch timed_("logprob.dlogits_kernel", (hipStream_t)stream); TS_LAUNCH_TOKENS(dtype, width, dlogits_kernel, dim3((unsigned)(a.n_ttiles * a.n_vtiles)), dim3(kGemmThreads),
                      0, (hipStream_t)stream, a); }
   return ts::check_launch("ts_logprob_dlogits");
@@ -691,6 +693,8 @@ int grad_hidden_launch(const void* dlogits, int64_t ld_dlogits, const void* weig
   a.dh = (ts::bf16*)grad_hidden;
   a.ldd = ld_grad;
   a.part = a.ksplit > 1 ? (float*)workspace : wide ? (float*)grad_hidden : nullptr;
+  TS_CHECK_ARG((int64_t)a.n_ttiles * a.n_dtiles * a.ksplit < kMaxGrid && rows * dim < (1ll << 34),
+               "ts_logprob_grad_hidden: grid too large");
   if (a.ksplit > 1)
     TS_CHECK_ARG(workspace && workspace_bytes >= ts_logprob_grad_hidden_workspace(rows, dim, vocab) &&
                      ok16(workspace),
@@ -768,7 +772,7 @@ int ts_logprob_grad_weight_block(const void* dlogits, int64_t ld_dlogits, const 
   a.ldg = ld_accumulator;
   a.out = (ts::bf16*)grad_weight;
   a.ldo = ld_grad;
-  TS_CHECK_ARG((int64_t)a.n_vtiles * a.n_dtiles < (1ll << 31), "ts_logprob_grad_weight: grid too large");
+  TS_CHECK_ARG((int64_t)a.n_vtiles * a.n_dtiles < kMaxGrid, "ts_logprob_grad_weight: grid too large");
   {
     ts::TimedLaunch timed_("logprob.grad_weight_kernel", (hipStream_t)stream);
     TS_LAUNCH_E(dtype, grad_weight_kernel, dim3((unsigned)(a.n_vtiles * a.n_dtiles)), dim3(kGemmThreads), 0,
