@@ -18,7 +18,6 @@ keeps torch's forward for them.
 
 from __future__ import annotations
 
-import math
 import os
 
 import torch
@@ -37,8 +36,8 @@ def _validate(ids, weight, scale, padding_idx):
         raise ValueError(f"weight must be [V, D], got {tuple(weight.shape)}")
     if ids.dtype not in ID_DTYPES:
         raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
-    if not (isinstance(scale, (int, float)) and math.isfinite(scale)):
-        raise ValueError(f"scale must be a finite number, got {scale!r}")
+    if not (isinstance(scale, (int, float)) and abs(scale) <= torch.finfo(torch.float32).max):
+        raise ValueError(f"scale must be a finite number (in fp32, as it is used), got {scale!r}")
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} is outside the vocabulary [0, {weight.shape[0]})")
     if not ids.is_cuda or not weight.is_cuda:
