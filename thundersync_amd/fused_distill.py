@@ -74,6 +74,8 @@ from .fused_logprob import (
 from .operator_profiling import device_role, operator_range
 
 MAX_TOP = 1024  # teacher slots per row
+# Below it a logit over T, in fp32 octaves, has no digits left behind the point, and its exponential overflows
+MIN_TEMPERATURE = 1e-6
 TEACHER_DTYPES = (torch.bfloat16, torch.float16, torch.float32, torch.float64)
 
 
@@ -90,8 +92,8 @@ def _validate(hidden, weight, ids, logits, temperature):
         raise ValueError(f"1 to {MAX_TOP} teacher logits per row, got {ids.shape[1]}")
     if weight.shape[0] < 1 or hidden.shape[1] < 1:
         raise ValueError(f"an empty head: weight {tuple(weight.shape)}")
-    if not (isinstance(temperature, (int, float)) and 0 < temperature < math.inf):
-        raise ValueError(f"temperature must be a positive number, got {temperature!r}")
+    if not (isinstance(temperature, (int, float)) and MIN_TEMPERATURE <= temperature < math.inf):
+        raise ValueError(f"temperature must be a positive number of {MIN_TEMPERATURE} or more, got {temperature!r}")
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"teacher_ids must be int64 or int32, got {ids.dtype}")
     if logits.dtype not in TEACHER_DTYPES:
@@ -421,7 +423,7 @@ def fused_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch
 
     ``hidden`` ``[N, D]``, ``weight`` ``[V, D]``, ``teacher_ids`` (int64 or
     int32) and ``teacher_logits`` ``[N, K]``, K up to 1024.  Both softmaxes are
-    taken at ``temperature``; the loss is not multiplied by its square.
+    taken at ``temperature`` (1e-6 or more); the loss is not multiplied by its square.
     """
     _validate(hidden, weight, teacher_ids, teacher_logits, temperature)
     grad = torch.is_grad_enabled()
