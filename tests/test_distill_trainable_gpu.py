@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from thundersync_amd import fused_distill as module
 from thundersync_amd.fused_distill import fused_distill
 
 pytestmark = pytest.mark.gpu
@@ -36,14 +37,15 @@ def exact(h, w, ids, teacher, grad):
 @pytest.mark.parametrize("n, d, dtype", [
     (800, 64, BF16), (800, 64, FP16), (50, 64, BF16), (24, 64, FP16), (200, 64, FP32), (24, 64, FP32), (50, 64, FP64),
 ])
-def test_losses_that_wait_for_their_backward(cuda, n, d, dtype):
-    """Together they keep blocks of no more than the weight's size, and each has the same gradients, with a block kept
-    (one of 50 rows, two of 24, none of more than 64) or without."""
+def test_losses_that_wait_for_their_backward(cuda, n, d, dtype, monkeypatch):
+    """Together they keep blocks of no more than the bound (here the weight's size), and each has the same gradients,
+    with a block kept (one of 50 rows, two of 24, none of more than 64) or without."""
     print(f"distill waiting losses n={n} d={d} {dtype}", flush=True)
     v, k, calls = 20011, 5, 6
     h, w, ids, teacher, grad = inputs(cuda, n, d, v, k, dtype, n)
     grad = grad.to(dtype if dtype == FP64 else torch.float32)
-    want = torch.autograd.grad(fused_distill(h, w, ids, teacher), (h, w), grad)
+    want = torch.autograd.grad(fused_distill(h, w, ids, teacher), (h, w), grad)  # kept
+    monkeypatch.setattr(module, "KEPT_BYTES", w.numel() * dtype.itemsize)
     torch.cuda.synchronize()
     before = torch.cuda.memory_allocated()
     losses = [fused_distill(h, w, ids, teacher) for _ in range(calls)]
@@ -80,8 +82,8 @@ def test_every_tile_of_a_wide_head(cuda, n, d, dtype):
     """Losses, dh row by row, dw by tiles of 256 tokens, over a whole vocabulary and every token tile (320 among them,
     2305 rows in several blocks).  Each of the three roundings (an exponential, a block's entry, the result) is off by u
     of its value at most, and errors of entries of either sign add as the entries do: 3 u of a row's or tile's root mean
-    square; a tile left out is 1 of dw's and 4 % of dh's.  (The softmax's own entries: teachers name tokens whose row is zero.)  A loss:
-    2 (D / 16 + 20) 2^-24 sum |h w| <= 1e-5 of a logit and a slot's, a depth of 180 sums 2e-5, its own terms of at
+    square; a tile left out is 1 of dw's and 4 % of dh's.  (The softmax's own entries: teachers name tokens whose row is
+    zero.)  A loss: 2 (D / 16 + 20) 2^-24 sum |h w| <= 1e-5 of a logit and a slot's, a depth of 180 sums 2e-5, its own terms of at
     most 13 another 2e-5; the last, partial tile left out is 8e-4."""
     v, k = 151936, 7
     print(f"distill wide head n={n} d={d} {dtype}", flush=True)

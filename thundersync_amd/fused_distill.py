@@ -32,7 +32,7 @@ A block of rows (:func:`~thundersync_amd.fused_logprob.backward_block_rows` of
 * a trainable weight and one block of rows: the backward, which has the
   upstream gradient, wants the block that the forward stored.  It is kept where
   the blocks of all losses that wait for their backward then hold no more
-  than the weight does; otherwise the backward stores it again, by the same
+  than ``KEPT_BYTES``; otherwise the backward stores it again, by the same
   kernels and with the same bits (:class:`_KeptBlocks`).  Its 16-bit entries
   are rounded twice, as exponentials and with the row's factor: 2 bytes of
   memory an entry, where the logits that would be rounded once take 4;
@@ -76,6 +76,8 @@ from .operator_profiling import device_role, operator_range
 MAX_TOP = 1024  # teacher slots per row
 # Below it a logit over T, in fp32 octaves, has no digits left behind the point, and its exponential overflows
 MIN_TEMPERATURE = 1e-6
+# Blocks that wait for their backward, on a device: 2048 rows of a 16-bit vocabulary of 262144
+KEPT_BYTES = 1 << 30
 TEACHER_DTYPES = (torch.bfloat16, torch.float16, torch.float32, torch.float64)
 
 
@@ -144,19 +146,19 @@ def _live_rows(h, state):
 
 
 class _KeptBlocks:
-    """The blocks that losses keep until their backward, so that together they hold no more than a weight does (a
-    1999 x 151936 block is 0.6 GB, beside a weight of D 2048 as large: a batch scored in sixteen calls kept 9.7 GB).
-    Kept, a step of that size takes 3.85 ms; stored again in the backward 5.07."""
+    """The blocks that losses on a device keep until their backward, so that together they hold no more than
+    ``KEPT_BYTES`` (a batch scored in sixteen calls of 2000 rows of 151936 would keep 9.7 GB).  Kept, a step of
+    1999 rows of D 2048 takes 3.85 ms; stored again in the backward 5.07."""
 
     def __init__(self):
         self._lock, self._alive = threading.Lock(), []
 
-    def take(self, rows, ld, like, limit):
-        """An empty ``[rows, ld]`` block like ``like``, or None where it would take the blocks past ``limit`` bytes."""
+    def take(self, rows, ld, like):
+        """An empty ``[rows, ld]`` block like ``like``, or None where it would take the blocks past their bound."""
         with self._lock:
             self._alive = [r for r in self._alive if r() is not None]
             held = sum(t.nbytes for t in (r() for r in self._alive) if t is not None and t.device == like.device)
-            if held + rows * ld * like.element_size() > limit:
+            if held + rows * ld * like.element_size() > KEPT_BYTES:
                 return None
             block = torch.empty(rows, ld, dtype=like.dtype, device=like.device)
             self._alive.append(weakref.ref(block))  # lives as long as what autograd saves
@@ -251,7 +253,8 @@ class _Rows:
         return ws[: ws_bytes // 2]
 
     def stored_again(self, i, rows, block):
-        """``block`` and its tiles' references as a :meth:`forward` that kept them left them; what autograd saved stays."""
+        """``block`` and its tiles' references as a :meth:`forward` that kept them left them (what autograd saved
+        stays as it is)."""
         again = copy.copy(self)
         again.slot_z, again.lse, again.loss = (torch.empty_like(t) for t in (self.slot_z, self.lse, self.lse))
         return again.forward(i, rows, block)
@@ -317,7 +320,7 @@ def _forward(rows: _Rows, chunk, need_hidden, need_weight):
     frozen = need_hidden and not need_weight
     if n == 0:
         return (torch.empty(0, rows.d, dtype=rows.dtype, device=dev),) if frozen else ()
-    kept = _kept.take(n, rows.ld, rows.h, rows.w.nbytes) if need_weight and n <= block_rows else None
+    kept = _kept.take(n, rows.ld, rows.h) if need_weight and n <= block_rows else None
     if kept is None and not (rows.exact or frozen):
         rows.forward(0, n, None)
         return ()
