@@ -515,7 +515,7 @@ int ts_matmul_exact_ws(const void* a, int64_t a_m, int64_t a_k, const void* b, i
  * A row without a present slot has loss 0 and dlogits 0; an id of vocab or
  * more makes its row's loss NaN and takes no part in dlogits.
  * The slots' tokens, probabilities and logits (slot_id, slot_p, slot_z) are
- * [rows, pitch] with top <= pitch <= 1024; state is [rows].
+ * [rows, pitch] with top <= pitch <= 1024; state is [rows].  Fewer than 2^23 rows.
  * No counterpart in the reference, whose distillation scores sampled tokens
  * (opd/objectives.py:607-611).
  * ------------------------------------------------------------------------ */

@@ -20,7 +20,8 @@ part in its gradient), as a target of the fused logprob does;
 ``THUNDERSYNC_CHECK_TARGETS=1`` checks the present slots' ids first and raises.
 
 A block of rows (:func:`~thundersync_amd.fused_logprob.backward_block_rows` of
-``chunk``) has its ``[rows, V]`` block in the element type, one at a time:
+``chunk``) has its ``[rows, V]`` block in the element type, one at a time (two
+in a backward whose block was kept):
 
 * no gradient: the tiles' statistics alone, for all rows;
 * a frozen weight: the forward goes on, block by block, from the stored
