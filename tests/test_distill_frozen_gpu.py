@@ -62,3 +62,20 @@ def test_small_probabilities_count(cuda, dtype):
     want = exact(h, w, ids, teacher, grad, 1.0)
     bound = torch.finfo(dtype).eps / 2 * want.abs() + v / 16 * 2.0 ** -24 * 0.05 + 2.0 ** -25
     assert ((dh.double() - want).abs() <= bound).all(), ((dh.double() - want).abs() / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("size", [1.0, 40.0, 90.0])
+def test_gradients_stay_finite_at_the_lowest_temperature(cuda, size, dtype):
+    """Logits over T of 9e7 step by 8 octaves in fp32 and so come to lie some octaves above their reference: the stored
+    block has room for those."""
+    g = torch.Generator(device=cuda).manual_seed(0)
+    h = torch.randn(50, 64, generator=g, device=cuda)
+    h = (h / h.norm(dim=1, keepdim=True)).to(dtype).requires_grad_()
+    w = torch.randn(3000, 64, generator=g, device=cuda)
+    w = (size * w / w.norm(dim=1, keepdim=True)).to(dtype)
+    w[:50] = (size * h.detach()).to(dtype)  # a largest logit of `size` in every row
+    ids = torch.randint(0, 3000, (50, 5), generator=g, device=cuda)
+    loss = fused_distill(h, w, ids, torch.randn(50, 5, generator=g, device=cuda), temperature=1e-6)
+    (dh,) = torch.autograd.grad(loss, h, torch.full_like(loss, 1e-6))
+    assert loss.isfinite().all() and dh.isfinite().all()

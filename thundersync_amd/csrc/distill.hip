@@ -39,7 +39,9 @@ constexpr int kRowThreads = 512;  // of the kernels that give a row a work-group
 constexpr int64_t kMaxRows = (1ll << 32) / kRowThreads;  // a launch of 2^32 threads along an axis wraps
 constexpr int kRowWaves = 4;    // rows per work-group of the per-row kernels
 constexpr int kDead = 0, kLive = 1, kBadId = 2;  // row states
-constexpr int kHeadroom = 14;   // octaves of a frozen head's stored softmax above 1: below fp16's largest number
+// octaves of a frozen head's stored softmax above 1.  fp16's largest number leaves 5 more, for logits over T of up
+// to 1e8: in fp32 they step by 8 octaves and lie up to 4 above their tile's reference
+constexpr int kHeadroom = 10;
 
 template <typename T> __device__ __forceinline__ T wave_sum_of(T v) {
 #pragma unroll
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(64 * kLossTokens) void loss_kernel(const float* __r
 // Frozen head, after the forward: the stored exponentials of a row to one reference, the
 // softmax then being row_scale[1] times the block, and zero at the slots' tokens.  An entry
 // keeps its one rounding: it is multiplied by a power of two, and kHeadroom octaves above 1
-// leave fp16's smallest normal number 28 below the row's largest (unscaled, the softmax of
+// leave fp16's smallest normal number 24 below the row's largest (unscaled, the softmax of
 // 151936 equal logits is 6.6e-6 with four bits of it lost).  Bound as finish_kernel: 2048 x
 // 151936 in bf16 in 211 us, 5.9 TB/s.
 // ---------------------------------------------------------------------------
