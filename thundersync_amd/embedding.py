@@ -31,6 +31,13 @@ DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 ID_DTYPES = (torch.int64, torch.int32)
 
 
+def _on_one_device(ids, rows):
+    if not ids.is_cuda or not rows.is_cuda:
+        raise RuntimeError("thundersync_amd embedding runs on the GPU only; got a CPU tensor")
+    if ids.device != rows.device:
+        raise ValueError(f"ids on {ids.device} and rows on {rows.device}")
+
+
 def _validate(ids, weight, scale, padding_idx):
     if weight.dim() != 2 or weight.shape[1] < 1:
         raise ValueError(f"weight must be [V, D], got {tuple(weight.shape)}")
@@ -40,10 +47,7 @@ def _validate(ids, weight, scale, padding_idx):
         raise ValueError(f"scale must be a finite number (in fp32, as it is used), got {scale!r}")
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} is outside the vocabulary [0, {weight.shape[0]})")
-    if not ids.is_cuda or not weight.is_cuda:
-        raise RuntimeError("thundersync_amd embedding runs on the GPU only; got a CPU tensor")
-    if ids.device != weight.device:
-        raise ValueError(f"ids on {ids.device} and weight on {weight.device}")
+    _on_one_device(ids, weight)
     if weight.dtype not in DTYPES:
         raise TypeError(f"thundersync_amd embedding takes a bf16, fp16 or fp32 weight, got {weight.dtype}")
     if os.environ.get(CHECK_TARGETS_ENV, "0") not in ("", "0"):
@@ -57,22 +61,25 @@ def _unit_rows(t: torch.Tensor) -> torch.Tensor:
 
 def embedding_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
     """``scale * weight[ids]`` (ids of any shape), without autograd."""
+    _on_one_device(ids, weight)
     lib = _lib.require_library()
     flat = ids.reshape(-1).to(torch.int64).contiguous()
     w = weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
     v, d = w.shape
     out = torch.empty(*ids.shape, d, dtype=w.dtype, device=w.device)
-    _lib.check(
-        lib.ts_embedding_fwd(flat.data_ptr(), flat.numel(), w.data_ptr(), max(w.stride(0), d), v, d, float(scale),
-                             out.data_ptr(), _lib.dtype_code(w.dtype), _lib.stream_of(w)),
-        lambda: f"ts_embedding_fwd(tokens={flat.numel()}, vocab={v}, dim={d})",
-    )
+    with _lib.device_of(w):
+        _lib.check(
+            lib.ts_embedding_fwd(flat.data_ptr(), flat.numel(), w.data_ptr(), max(w.stride(0), d), v, d, float(scale),
+                                 out.data_ptr(), _lib.dtype_code(w.dtype), _lib.stream_of(w)),
+            lambda: f"ts_embedding_fwd(tokens={flat.numel()}, vocab={v}, dim={d})",
+        )
     return out
 
 
 def embedding_backward(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int, *, scale: float = 1.0,
                        padding_idx: int | None = None) -> torch.Tensor:
     """The table's gradient ``[vocab, D]`` for ``grad_out`` ``[*ids.shape, D]``."""
+    _on_one_device(ids, grad_out)
     lib = _lib.require_library()
     d = grad_out.shape[-1]
     flat = ids.reshape(-1).to(torch.int64).contiguous()
@@ -81,12 +88,13 @@ def embedding_backward(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int, *,
     grad = torch.empty(vocab, d, dtype=g.dtype, device=g.device)
     ws_bytes = int(lib.ts_embedding_bwd_workspace(n, d))
     ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=g.device)
-    _lib.check(
-        lib.ts_embedding_bwd(flat.data_ptr(), n, g.data_ptr(), g.stride(0), vocab, d,
-                             -1 if padding_idx is None else int(padding_idx), float(scale), grad.data_ptr(),
-                             ws.data_ptr(), ws_bytes, _lib.dtype_code(g.dtype), _lib.stream_of(g)),
-        lambda: f"ts_embedding_bwd(tokens={n}, vocab={vocab}, dim={d})",
-    )
+    with _lib.device_of(g):
+        _lib.check(
+            lib.ts_embedding_bwd(flat.data_ptr(), n, g.data_ptr(), g.stride(0), vocab, d,
+                                 -1 if padding_idx is None else int(padding_idx), float(scale), grad.data_ptr(),
+                                 ws.data_ptr(), ws_bytes, _lib.dtype_code(g.dtype), _lib.stream_of(g)),
+            lambda: f"ts_embedding_bwd(tokens={n}, vocab={vocab}, dim={d})",
+        )
     return grad
 
 
@@ -96,7 +104,7 @@ class _Embedding(torch.autograd.Function):
         ctx.save_for_backward(ids)
         ctx.save_for_forward(ids)
         ctx.vocab, ctx.dtype, ctx.scale, ctx.padding_idx = weight.shape[0], weight.dtype, scale, padding_idx
-        with _lib.device_of(weight), operator_range(
+        with operator_range(
                 "embedding_forward", role=device_role(weight.device), tokens=ids.numel(), hidden=weight.shape[1],
                 vocab=weight.shape[0], dtype=weight.dtype):
             return embedding_forward(ids, weight, scale)
@@ -105,7 +113,7 @@ class _Embedding(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
-        with _lib.device_of(grad), operator_range(
+        with operator_range(
                 "embedding_backward", role=device_role(grad.device), tokens=ids.numel(), hidden=grad.shape[-1],
                 vocab=ctx.vocab):
             gw = embedding_backward(ids, grad.to(ctx.dtype), ctx.vocab, scale=ctx.scale, padding_idx=ctx.padding_idx)
@@ -114,8 +122,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def jvp(ctx, ids_tangent, weight_tangent, *_):
         (ids,) = ctx.saved_tensors
-        with _lib.device_of(weight_tangent):
-            return embedding_forward(ids, weight_tangent, ctx.scale)
+        return embedding_forward(ids, weight_tangent, ctx.scale)
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
@@ -127,8 +134,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     """
     _validate(ids, weight, scale, padding_idx)
     if not (weight.requires_grad and torch.is_grad_enabled()) and forward_ad.unpack_dual(weight).tangent is None:
-        with _lib.device_of(weight):
-            return embedding_forward(ids, weight.detach(), float(scale))
+        return embedding_forward(ids, weight.detach(), float(scale))
     return _Embedding.apply(ids, weight, float(scale), padding_idx)
 
 
@@ -138,7 +144,7 @@ class HipEmbedding(torch.nn.Embedding):
 
     def forward(self, input):  # noqa: A002 - torch's name
         takes = (input.is_cuda and self.weight.is_cuda and input.dtype in ID_DTYPES and self.weight.dtype in DTYPES
-                 and input.device == self.weight.device and _lib.library() is not None)
+                 and input.device == self.weight.device and self.embedding_dim > 0 and _lib.library() is not None)
         if not takes:
             return super().forward(input)
         return embedding(input, self.weight, padding_idx=self.padding_idx)
