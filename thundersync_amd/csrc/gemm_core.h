@@ -83,6 +83,7 @@ struct Streamer {
   const bf16* base;  // row 0, k 0
   int64_t ld;
   int rows;          // valid rows from base (>= 1)
+  int width;         // of a stage that the last row holds: rows narrower than a stage end before it
   int K;
   int voff[kPerWave];  // byte offset of this lane's row and chunk within a stage, per u
   int kchunk;        // this lane's chunk start within a stage (elements)
@@ -90,15 +91,17 @@ struct Streamer {
     base = b;
     ld = ld_;
     rows = rows_;
+    width = (int)min((int64_t)TK, ld_);
     K = K_;
     kchunk = 8 * ((lane & 3) ^ (lane >> 4));
 #pragma unroll
     for (int u = 0; u < kPerWave; ++u)
       voff[u] = (int)(((16 * ((wave + kWaves * u) % kInstr) + (lane >> 2)) * ld + kchunk) * 2);
   }
-  // descriptor and this lane's chunk validity for K columns [k0, k0 + TK)
+  // descriptor and this lane's chunk validity for K columns [k0, k0 + TK).  (With TK in place of the width
+  // the rows behind the last one, where rows are narrower, were within range: 48 bytes past the operand.)
   __device__ __forceinline__ u32x4 descriptor(int k0) const {
-    return raw_descriptor(base + k0, (uint32_t)(((int64_t)(rows - 1) * ld + TK) * 2));
+    return raw_descriptor(base + k0, (uint32_t)(((int64_t)(rows - 1) * ld + width) * 2));
   }
   // instruction u of this wave's share of the stage into dst (wave-uniform);
   // a chunk past K reads nothing: zeros
