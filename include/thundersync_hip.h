@@ -640,6 +640,97 @@ int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab
               int64_t* tokens, float* logprobs, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Logits before sampling
+ * ------------------------------------------------------------------------ */
+
+/* out [rows, vocab] = logits [rows, vocab] (TS_F32, TS_F16 or TS_BF16) with, per
+ * token, in this order and in fp32, rounded once:
+ *   z / r where z > 0, else z * r, for tokens of the row's history (its first
+ *   `lengths` ids); minus f * count + p for tokens that occur count > 0 times in it
+ *   from `prompt_lengths` on; plus the row's biases of the token in their order; -inf
+ *   where the row's mask has a 0 (bit v & 31 of word v >> 5).
+ * lengths null: history_width; prompt_lengths null: 0.  Each of r, f, p is one value for
+ * all rows, or where its pointer is not null one per row (an r that is not above 0 counts
+ * as 1, a NaN f or p as 0).  ids (history and biases, of id_bytes 4 or 8) outside
+ * [0, vocab) are passed over.  allowed_rows: the row's mask, negative for none, one of
+ * `masks` and more gives a row of NaN; null: row i has mask i.  out may be logits.  No
+ * counterpart in the reference (its rollouts sample inside vLLM, rollout/engine.py). */
+int ts_adjust_logits(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, const void* history,
+                     int64_t ld_history, int64_t history_width, const int32_t* lengths, const int32_t* prompt_lengths,
+                     const float* repetition, float repetition_all, const float* frequency, float frequency_all,
+                     const float* presence, float presence_all, const void* bias_ids, int64_t ld_bias_ids,
+                     const float* bias, int64_t ld_bias, int64_t biases, const int32_t* allowed, int64_t ld_allowed,
+                     const int32_t* allowed_rows, int64_t masks, int id_bytes, void* out, int64_t ld_out, int dtype,
+                     void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged cache of keys and values (bf16 or fp16 rows, held in 16 or 8 bits)
+ * ------------------------------------------------------------------------ */
+
+/* Pages [pages][kv_heads][page_size][row] of keys and of values, page p at p *
+ * page_stride elements: in 16 bits elements of dtype; in 8 bits e4m3 codes, each
+ * times its scale (fp32, a power of two between 2^-118 and 2^120) a value of dtype, one
+ * scale for 16 tokens of a page and head, [pages][kv_heads][page_size / 16].  Rows hold
+ * head_dim elements (a multiple of 8) and zeros behind them. */
+typedef struct ts_paged_cache {
+  void* key;
+  void* value;
+  float* key_scale;    /* null in 16 bits */
+  float* value_scale;
+  int64_t key_page_stride;
+  int64_t value_page_stride;
+  int64_t pages;
+  int32_t page_size;   /* 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t row;         /* 64, 128, 192 or 256 */
+  int32_t bits;        /* 8 or 16 */
+  int32_t dtype;       /* TS_F16 or TS_BF16 */
+} ts_paged_cache;
+
+/* Sequences of a call: `lengths` their tokens in the cache, the call's own among them
+ * (0: none, a row of padding), page ids table[s * ld_table ..] of `width` pages, and the
+ * rows offsets[s] .. offsets[s + 1] of the call (null: row s alone).  Read on the device. */
+typedef struct ts_paged_batch {
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* offsets;
+  int64_t ld_table;
+  int64_t width;
+  int64_t seqs;
+} ts_paged_batch;
+
+/* Keys and values of `tokens` rows [kv_heads][head_dim] into the cache, at the last positions of
+ * their sequences, and query rows [heads][head_dim] into query_out (dense).  Where rotary_dim is
+ * not 0 (a multiple of 16), the first rotary_dim elements of query and key rows are rotated by row p
+ * of rotary [rotary_rows][rotary_dim] (cosines, then sines), p the position, or positions[row]; pairs
+ * are elements j and j + rotary_dim / 2, or 2 j and 2 j + 1 where interleaved; a p outside the table
+ * gives NaN.  In 8 bits the scale of a block of 16 tokens is the least that holds its new tokens, and not
+ * below the block's own where it holds older ones, which are written again by it.  Tokens past the page
+ * table or with a page id that is none go nowhere; query rows of no sequence are zero.  Sequences of one
+ * call may share pages that they read, not blocks of 16 tokens that they write. */
+int ts_paged_append(const ts_paged_cache* cache, const ts_paged_batch* batch, int64_t tokens, const void* query,
+                    int64_t query_token_stride, int64_t query_head_stride, int64_t heads, void* query_out,
+                    const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
+                    int64_t value_token_stride, int64_t value_head_stride, const float* rotary, int64_t rotary_rows,
+                    int64_t rotary_dim, int interleaved, const int32_t* positions, void* stream);
+
+/* The values that an 8-bit cache stands for, dense [pages][kv_heads][page_size][head_dim] of its dtype. */
+int ts_paged_values(const ts_paged_cache* cache, void* key_out, void* value_out, void* stream);
+
+/* Workspace bytes ts_paged_attention needs. */
+int64_t ts_paged_attention_workspace(const ts_paged_cache* cache, const ts_paged_batch* batch, int64_t tokens,
+                                     int64_t heads);
+
+/* out [tokens][heads][head_dim] (dense) = softmax(scale q k) v of each query row over the keys of KV head
+ * h / (heads / kv_heads) at its sequence's positions up to its own; zero for rows without keys, NaN for
+ * rows that see a key past the page table or on a page that is none.  Two calls in flight may not share a
+ * workspace. */
+int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch, int64_t tokens, const void* query,
+                       int64_t token_stride, int64_t head_stride, int64_t heads, float scale, void* out,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Merged-weight LoRA linear (bf16 or fp16 operands, fp32 accumulation)
  *
  * The caller has merged the adapters into the weight (W_eff = W + s B A,

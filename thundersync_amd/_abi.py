@@ -82,6 +82,26 @@ class AttnLayoutSizes(ctypes.Structure):
         "n_kv_work", "n_dq_work", "n_q_long", "n_kv_long", "n_dq_long", "ds_head")]
 
 
+class PagedCacheDesc(ctypes.Structure):
+    """ts_paged_cache"""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("key", "value", "key_scale", "value_scale")),
+        *((name, ctypes.c_int64) for name in ("key_page_stride", "value_page_stride", "pages")),
+        *((name, ctypes.c_int32) for name in ("page_size", "kv_heads", "head_dim", "row", "bits", "dtype")),
+    ]
+
+
+class PagedBatch(ctypes.Structure):
+    """ts_paged_batch"""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("table", "lengths", "offsets")),
+        *((name, ctypes.c_int64) for name in ("ld_table", "width", "seqs")),
+    ]
+
+
 assert SEG_DTYPE.itemsize == 24 and REF_DTYPE.itemsize == 8 and RUN_DTYPE.itemsize == 112
 assert ctypes.sizeof(AttnProblem) == 112 and ctypes.sizeof(AttnRows) == 24
 assert ctypes.sizeof(AttnLayoutDesc) == 72 and ctypes.sizeof(AttnLayoutSizes) == 128
+assert ctypes.sizeof(PagedCacheDesc) == 80 and ctypes.sizeof(PagedBatch) == 48

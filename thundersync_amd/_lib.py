@@ -24,7 +24,7 @@ import os
 import threading
 from pathlib import Path
 
-from ._abi import AttnLayoutDesc, AttnLayoutSizes, AttnProblem, AttnRows
+from ._abi import AttnLayoutDesc, AttnLayoutSizes, AttnProblem, AttnRows, PagedBatch, PagedCacheDesc
 
 HIP_ENV = "THUNDERSYNC_HIP"
 HIP_SETTINGS = ("require", "off", "auto")
@@ -37,6 +37,8 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _F = ctypes.c_float
 _D = ctypes.c_double
+_CACHE = ctypes.POINTER(PagedCacheDesc)
+_BATCH = ctypes.POINTER(PagedBatch)
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ts_hip_version": (ctypes.c_char_p, []),
     "ts_hip_last_error": (ctypes.c_char_p, []),
@@ -103,6 +105,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ts_sample_workspace": (_I64, [_I64, _I64, _INT]),
     "ts_sample": (
         _INT, [_P, _I64, _I64, _I64, _P, _INT, _P, _D, _P, _I64, _P, _D, _P, _D, _P, _P, _P, _I64, _INT, _P]),
+    "ts_adjust_logits": (
+        _INT,
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _F, _P, _F, _P, _F, _P, _I64, _P, _I64, _I64, _P, _I64, _P,
+         _I64, _INT, _P, _I64, _INT, _P],
+    ),
+    "ts_paged_append": (
+        _INT,
+        [_CACHE, _BATCH, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _INT, _P, _P],
+    ),
+    "ts_paged_values": (_INT, [_CACHE, _P, _P, _P]),
+    "ts_paged_attention_workspace": (_I64, [_CACHE, _BATCH, _I64, _I64]),
+    "ts_paged_attention": (_INT, [_CACHE, _BATCH, _I64, _P, _I64, _I64, _I64, _F, _P, _P, _I64, _P]),
     "ts_adjoint_reduce": (_INT, [ctypes.POINTER(_P), _INT, _P, _P, _I64, _INT, _P]),
     "ts_ledger_add": (_INT, [_P, _P, _I64, _INT, _INT, _P]),
     "ts_forest_build": (_INT, [_I64, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P]),
