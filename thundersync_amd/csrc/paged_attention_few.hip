@@ -1,0 +1,450 @@
+// Attention over a paged cache for sequences with few query rows: one token each, or a few.
+//
+// A work-group takes one item: up to 16 R query rows of one KV head (its tokens' heads of the group side by side, so
+// that keys and values are read once for all of them) over a slice of the keys.  Its four waves take 32-key steps in
+// turn, each with a running reference point, sum and accumulators of its own, and join them at the end; an item that is not
+// its sequence's only slice leaves partial rows for merge_kernel.
+//
+// A step of a wave:  S^T = K Q^T (16x16x32, keys as rows), so a lane holds 8 of the 32 scores of one query row, which
+// are, rounded, already the operand of O^T += V^T P^T: lane (g, r) has keys 4 g + i of both halves of query row r.  V^T
+// needs 8 keys of one element: a lane reads ROW / 16 elements of each of its 8 keys (a wave whole rows), and
+// pairs of keys are interleaved by byte permutes; codes become 16-bit values, times their scale, two to an instruction.
+// Nothing passes through LDS, and no wave waits for another before the end.
+//
+// Bound by HBM: a step's 32 ROW bytes of keys and as many of values against about 150 VALU instructions and 2 ROW / 8
+// matrix ones.
+#include "paged_attention.h"
+
+namespace ts {
+namespace paged {
+
+constexpr int kWaves = 4;
+constexpr float kSlack = 8.f;      // log2 units by which scores may pass the reference point before it moves
+constexpr float kSlackSum = 256.f;
+
+// N bytes at a multiple of four
+template <int N> struct Words {
+  uint32_t w[N / 4];
+};
+template <int N> __device__ __forceinline__ Words<N> load_words(const char* p) {
+  struct __attribute__((packed, aligned(4))) At { uint32_t w[N / 4]; };
+  const At x = *(const At*)p;
+  Words<N> y;
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) y.w[i] = x.w[i];
+  return y;
+}
+
+// A step's keys or values of one 16-token tile, as loaded.
+template <bool WIDE, int ROW> struct Tile {
+  static constexpr int kSize = WIDE ? 2 : 1;
+  static constexpr int kLoads = ROW * kSize / 64;  // 16-byte reads of a key's row by its four lanes
+  u32x4 k[kLoads];
+  Words<ROW / 16 * kSize> v[4];
+};
+
+// waves a SIMD: a step's loads and the accumulators are 3 ROW / 8 registers, of 16 bits 5 ROW / 8
+template <bool WIDE, int ROW, int R>
+constexpr int few_occupancy() {
+  if (ROW * R <= 64) return 4;
+  if (WIDE) return ROW * R <= 128 ? 3 : 2;
+  return ROW * R <= 128 ? 4 : ROW * R <= 192 ? 3 : 2;
+}
+
+template <typename T, bool WIDE, int ROW, int R>
+__global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void few_kernel(AttnArgs a) {
+  constexpr int NC = ROW / 32;  // k-steps of S
+  constexpr int NB = ROW / 16;  // elements of a value that a lane reads, and tiles of O
+  constexpr int kSize = WIDE ? 2 : 1;
+  using Part = float[16 * R][ROW + 4];
+  using Query = u32x4[NC][64];
+  constexpr int kBytes = 2 * sizeof(Part) > R * sizeof(Query) ? 2 * sizeof(Part) : R * sizeof(Query);
+  __shared__ __attribute__((aligned(16))) char s_space[kBytes];
+  Part* const s_part = (Part*)s_space;     // at the end
+  Query* const s_query = (Query*)s_space;  // until then
+  __shared__ float s_stat[kWaves][16 * R][2];
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Item it;
+  int past = 0;
+  if (!find_item<0>(a, 16 * R, (int)blockIdx.x, lane, it, past)) {
+    // rows behind the last sequence: 16 a work-group, zeros
+    if (a.batch.offsets) {
+      const int from = max(0, a.batch.offsets[a.batch.seqs]) + 16 * past;
+      const int row_bytes = a.heads * a.head_dim * 2;
+      for (int t = from; t < min(from + 16, a.batch.tokens); ++t)
+        for (int i = threadIdx.x; i < row_bytes / 16; i += 64 * kWaves)
+          *(u32x4*)(a.out + (int64_t)t * row_bytes + 16 * i) = u32x4{0, 0, 0, 0};
+    }
+    return;
+  }
+  const int first_row = it.tile * 16 * R;
+  const int len = it.seq.len, base = len - it.seq.n;  // position of the first new token
+  if (a.plan && threadIdx.x == 0 && it.head == 0 && it.tile == 0 && it.slice == 0)
+    a.plan[it.s] = Plan{it.part, it.slices, 16 * R, 0};
+
+  // Query rows as B operands: element 16 g + 8 (c & 1) of the 64 of c / 2 for codes, 32 c + 8 g in 16 bits, as the
+  // keys' elements lie in a lane's reads; the last key that each row sees.  The operands are the same in
+  // every wave and stay in LDS: their registers are worth more to loads in flight.
+  int limit[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    const int row = first_row + 16 * t + r;
+    const int token = row / a.group, head = it.head * a.group + row % a.group;
+    const bool there = row < it.rows;
+    limit[t] = there ? base + token : -1;
+    const char* p = a.query + ((int64_t)(it.seq.row0 + token) * a.token_stride + (int64_t)head * a.head_stride) * 2;
+    for (int c = wave; c < NC; c += kWaves) {
+      const int d = WIDE ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c & 1);
+      u32x4 v = u32x4{0, 0, 0, 0};
+      if (there && d < a.head_dim) v = *(const u32x4*)(p + 2 * d);
+      s_query[t][c][lane] = v;
+    }
+  }
+  const int low = max(-1, base + min(first_row / a.group, it.seq.n - 1));  // the least of the rows' limits
+
+  f32x4 acc[R][NB];
+  float m[R], l[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    m[t] = neg_inf();
+    l[t] = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t* table = a.batch.table + (int64_t)it.s * a.batch.ld_table;
+  const int page_mask = (1 << a.page_shift) - 1;
+  auto page_at = [&](int pos) -> int {  // of a 16-token tile; wave-uniform
+    const int at = pos >> a.page_shift;
+    if (pos >= it.end || at >= a.batch.width) return -1;
+    const int page = uniform_table(table)[at];
+    return page >= 0 && page < a.pages ? page : -1;
+  };
+  Tile<WIDE, ROW> tile[2];
+  float ks[2], vs[2];
+  int page[2];
+  const int key_lane = (r * ROW + (WIDE ? 8 : 16) * g) * kSize;
+  const int value_lane = (4 * g * ROW + NB * r) * kSize;
+  auto load_keys = [&](int pos) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = pos + 16 * h;
+      page[h] = page_at(at);
+      if (page[h] < 0) {
+        ks[h] = vs[h] = 1.f;
+        continue;
+      }
+      const int64_t line = ((int64_t)it.head << a.page_shift) + (at & page_mask);
+      const char* p = a.key + page[h] * a.key_page_stride + line * (ROW * kSize) + key_lane;
+#pragma unroll
+      for (int i = 0; i < Tile<WIDE, ROW>::kLoads; ++i) tile[h].k[i] = *(const u32x4*)(p + 64 * i);
+      if constexpr (!WIDE) {
+        const int64_t scale = (((int64_t)page[h] * a.kv_heads << a.page_shift) + line) >> 4;
+        ks[h] = uniform_table(a.key_scale)[scale];
+        vs[h] = uniform_table(a.value_scale)[scale];
+      }
+    }
+  };
+  auto load_values = [&](int pos) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = pos + 16 * h;
+      if (page[h] < 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tile[h].v[i] = Words<NB * kSize>{};
+        continue;
+      }
+      const int64_t line = ((int64_t)it.head << a.page_shift) + (at & page_mask);
+      const char* p = a.value + page[h] * a.value_page_stride + line * (ROW * kSize) + value_lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile[h].v[i] = load_words<NB * kSize>(p + i * ROW * kSize);
+    }
+  };
+
+  int pos = __builtin_amdgcn_readfirstlane(it.begin + 32 * wave);
+  if (pos < it.end) {
+    load_keys(pos);
+    load_values(pos);
+  }
+  __syncthreads();
+  // One step; `edge`: some row does not see some of its keys, or they are not there.
+  auto step = [&](auto edge_) __attribute__((always_inline)) {
+    constexpr bool edge = decltype(edge_)::value;
+    asm volatile("" ::: "memory");  // the query's operands are read again, not held over the loop
+    f32x4 sc[R][2];
+    bool ruined = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int t = 0; t < R; ++t) sc[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (page[h] < 0) {
+        ruined |= pos + 16 * h < it.end;
+        continue;
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        bf16x8 k;
+        if constexpr (WIDE) {
+          k = as_bf16x8(tile[h].k[c]);
+        } else {
+          const u32x4 x = tile[h].k[c / 2];
+          const uint32_t lo = x[2 * (c & 1)], hi = x[2 * (c & 1) + 1];
+          k = as_bf16x8(u32x4{widen2<T, false>(lo, ks[h]), widen2<T, true>(lo, ks[h]), widen2<T, false>(hi, ks[h]),
+                              widen2<T, true>(hi, ks[h])});
+        }
+#pragma unroll
+        for (int t = 0; t < R; ++t) sc[t][h] = mma16<T>(k, as_bf16x8(s_query[t][c][lane]), sc[t][h]);
+      }
+#pragma unroll
+      for (int t = 0; t < R; ++t) sc[t][h] *= a.scale;
+    }
+    const float vscale[2] = {WIDE ? 1.f : vs[0], WIDE ? 1.f : vs[1]};
+    const int pages[2] = {page[0], page[1]};
+    const int next = pos + 32 * kWaves;
+    if (next < it.end) load_keys(next);
+
+    if (ruined) {  // keys of a page that is none
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (pages[h] < 0)
+#pragma unroll
+          for (int t = 0; t < R; ++t) sc[t][h] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+    }
+    bf16x8 p[R];
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+      if constexpr (edge) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (pos + 16 * h + 4 * g + i > limit[t]) sc[t][h][i] = neg_inf();
+      }
+      float e[8], sum;
+      auto exponentials = [&]() __attribute__((always_inline)) {
+        const float ref = m[t] == neg_inf() ? 0.f : m[t];
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] = fast_exp2(sc[t][j >> 2][j & 3] - ref);
+          sum += e[j];
+        }
+      };
+      exponentials();
+      // They stand unless a score passes the reference point by more than kSlack, which shows in the sum.
+      if (__ballot((m[t] == neg_inf()) | (sum > kSlackSum))) {
+        float most = neg_inf();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, sc[t][j >> 2][j & 3]);
+        most = rows_max4(most);
+        const bool move = most > m[t] + kSlack || (m[t] == neg_inf() && most > m[t]);
+        const float alpha = move ? fast_exp2(m[t] - most) : 1.f;
+        m[t] = move ? most : m[t];
+        l[t] *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[t][b] *= alpha;
+        exponentials();
+      }
+      l[t] += sum;
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack2<T>(e[2 * j], e[2 * j + 1]);
+      p[t] = as_bf16x8(w);
+    }
+
+    // Values of keys behind the sequence are zeros.
+    if constexpr (edge) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool there = pos + 16 * h + 4 * g + i < len;
+#pragma unroll
+          for (int w = 0; w < NB * kSize / 4; ++w) tile[h].v[i].w[w] = there ? tile[h].v[i].w[w] : 0u;
+        }
+    }
+    auto value = [&](int b) -> u32x4 {  // element NB r + b of the lane's eight keys
+      u32x4 f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (WIDE) {
+            const uint32_t x = tile[h].v[2 * k].w[b / 2], y = tile[h].v[2 * k + 1].w[b / 2];
+            f[2 * h + k] = __builtin_amdgcn_perm(y, x, b & 1 ? 0x07060302u : 0x05040100u);
+          } else {
+            const uint32_t x = tile[h].v[2 * k].w[b / 4], y = tile[h].v[2 * k + 1].w[b / 4];
+            const uint32_t z = __builtin_amdgcn_perm(y, x, b & 2 ? 0x07030602u : 0x05010400u);
+            f[2 * h + k] = b & 1 ? widen2<T, true>(z, vscale[h]) : widen2<T, false>(z, vscale[h]);
+          }
+        }
+      return f;
+    };
+    if (!edge || it.seq.n == 1) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const bf16x8 v = as_bf16x8(value(b));
+#pragma unroll
+        for (int t = 0; t < R; ++t) acc[t][b] = mma16<T>(v, p[t], acc[t][b]);
+      }
+    } else {
+      // Rows differ in what they see, and a weight of 0 does not take a NaN out: values that are not finite are left out of
+      // the product, and a second one, of where they are with who sees them, ruins the elements of the rows that do.
+      constexpr uint32_t kTop = std::is_same_v<T, f16> ? 0x7c00u : 0x7f80u, kOne = std::is_same_v<T, f16> ? 0x3c00u : 0x3f80u;
+      auto split = [&](uint32_t x, uint32_t& fine, uint32_t& flag) __attribute__((always_inline)) {
+        const bool lo = (x & kTop) == kTop, hi = (x >> 16 & kTop) == kTop;
+        fine = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
+        flag = (lo ? kOne : 0u) | (hi ? kOne << 16 : 0u);
+      };
+      u32x4 seen[R];
+#pragma unroll
+      for (int t = 0; t < R; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = pos + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
+          seen[t][j] = (at <= limit[t] ? kOne : 0u) | (at + 1 <= limit[t] ? kOne << 16 : 0u);
+        }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const u32x4 f = value(b);
+        u32x4 fine, flag;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t x, y;
+          split(f[j], x, y);
+          fine[j] = x;
+          flag[j] = y;
+        }
+#pragma unroll
+        for (int t = 0; t < R; ++t) {
+          acc[t][b] = mma16<T>(as_bf16x8(fine), p[t], acc[t][b]);
+          const f32x4 n = mma16<T>(as_bf16x8(flag), as_bf16x8(seen[t]), f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n[i] > 0.f) acc[t][b][i] = __builtin_nanf("");
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (next < it.end) load_values(next);
+    pos = next;
+  };
+  while (pos < it.end && pos + 31 <= low) step(std::false_type{});
+  while (pos < it.end) step(std::true_type{});
+  __syncthreads();  // the query's operands have been read
+
+  // The waves' sums by one reference point: 2 and 3 into 0 and 1, 1 into 0.
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    l[t] = rows_sum4(l[t]);
+    if (g == 0) {
+      s_stat[wave][16 * t + r][0] = m[t];
+      s_stat[wave][16 * t + r][1] = l[t];
+    }
+  }
+  __syncthreads();
+  float ref[R], sum[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    float most = neg_inf();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_stat[w][16 * t + r][0]);
+    ref[t] = most;
+    const float by = most == neg_inf() ? 0.f : most;
+    sum[t] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum[t] += s_stat[w][16 * t + r][1] * fast_exp2(s_stat[w][16 * t + r][0] - by);
+    const float f = fast_exp2(m[t] - by);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[t][b] *= f;
+  }
+  auto put = [&](int to) {
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; b += 4)
+          *(f32x4*)&s_part[to][16 * t + r][NB * (4 * g + i) + b] =
+              f32x4{acc[t][b][i], acc[t][b + 1][i], acc[t][b + 2][i], acc[t][b + 3][i]};
+  };
+  auto add = [&](int from) {
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; b += 4) {
+          const f32x4 x = *(const f32x4*)&s_part[from][16 * t + r][NB * (4 * g + i) + b];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[t][b + j][i] += x[j];
+        }
+  };
+  if (wave >= 2) put(wave - 2);
+  __syncthreads();
+  if (wave < 2) add(wave);
+  __syncthreads();
+  if (wave == 1) put(0);
+  __syncthreads();
+  if (wave != 0) return;
+  add(0);
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    const int row = first_row + 16 * t + r;
+    if (row >= it.rows) continue;
+    if (it.slices > 1) {
+      const int64_t at = ((int64_t)it.part * a.kv_heads + it.head) * (16 * R) + 16 * t + r;
+      float* o = a.part[0] + at * ROW;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; b += 4)
+          *(f32x4*)(o + NB * (4 * g + i) + b) =
+              f32x4{acc[t][b][i], acc[t][b + 1][i], acc[t][b + 2][i], acc[t][b + 3][i]};
+      if (g == 0) {
+        a.stats[0][2 * at] = ref[t];
+        a.stats[0][2 * at + 1] = sum[t];
+      }
+      continue;
+    }
+    const float inv = sum[t] > 0.f ? 1.f / sum[t] : 0.f;
+    const int token = row / a.group, head = it.head * a.group + row % a.group;
+    char* o = a.out + (((int64_t)(it.seq.row0 + token) * a.heads + head) * a.head_dim) * 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int b = 0; b < NB; b += 4) {
+        const int d = NB * (4 * g + i) + b;
+        if (d < a.head_dim)
+          *(u32x2*)(o + 2 * d) = u32x2{pack2<T>(acc[t][b][i] * inv, acc[t][b + 1][i] * inv),
+                                       pack2<T>(acc[t][b + 2][i] * inv, acc[t][b + 3][i] * inv)};
+      }
+  }
+}
+
+template <typename T, bool WIDE, int ROW>
+void launch_rows(const AttnArgs& a, const Sizes& z, hipStream_t s) {
+  const dim3 grid((unsigned)(z.items[0] + (a.batch.offsets ? (a.batch.tokens + 15) / 16 : 0))), block(64 * kWaves);
+  ts::TimedLaunch timed_("paged.few_kernel", s);
+  if (z.rows[0] == 16) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 1>), grid, block, 0, s, a);
+  else if constexpr (!WIDE || ROW <= 128) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 2>), grid, block, 0, s, a);
+}
+
+template <typename T, bool WIDE>
+void launch_t(const AttnArgs& a, const Sizes& z, int row, hipStream_t s) {
+  switch (row) {
+    case 64: launch_rows<T, WIDE, 64>(a, z, s); break;
+    case 128: launch_rows<T, WIDE, 128>(a, z, s); break;
+    case 192: launch_rows<T, WIDE, 192>(a, z, s); break;
+    default: launch_rows<T, WIDE, 256>(a, z, s);
+  }
+}
+
+void launch_few(const AttnArgs& a, const Sizes& z, int dtype, bool wide, int row, hipStream_t s) {
+  if (dtype == kF16) wide ? launch_t<f16, true>(a, z, row, s) : launch_t<f16, false>(a, z, row, s);
+  else wide ? launch_t<bf16, true>(a, z, row, s) : launch_t<bf16, false>(a, z, row, s);
+}
+
+}  // namespace paged
+}  // namespace ts
