@@ -126,6 +126,15 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int tile_rows, int 
   return false;
 }
 
+// Two 16-bit values without those that are not finite, and ones in the place of these.
+template <typename T> constexpr uint32_t kOneOf = std::is_same_v<T, f16> ? 0x3c00u : 0x3f80u;
+template <typename T> __device__ __forceinline__ void split_finite(uint32_t x, uint32_t& fine, uint32_t& flag) {
+  constexpr uint32_t top = std::is_same_v<T, f16> ? 0x7c00u : 0x7f80u;
+  const bool lo = (x & top) == top, hi = (x >> 16 & top) == top;
+  fine = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
+  flag = (lo ? kOneOf<T> : 0u) | (hi ? kOneOf<T> << 16 : 0u);
+}
+
 // host side
 struct Sizes {
   int64_t items[2];  // at most, of each kernel (0: not launched)

@@ -62,7 +62,7 @@ constexpr int kFewRows = 32;
 Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens, int64_t heads) {
   Sizes z{};
   const int64_t group = heads / c.kv_heads, keys = b.width * c.page_size + 16;
-  const bool ragged = b.offsets != nullptr, chunks = false;
+  const bool ragged = b.offsets != nullptr, chunks = ragged && tokens * group > kFewRows;
   // 32 rows a tile in 16 bits would not fit the registers beside wide rows' loads
   z.rows[0] = (ragged || group > 16) && !(c.bits == 16 && c.row > 128) ? 32 : 16;
   z.rows[1] = 128;
@@ -70,7 +70,7 @@ Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens,
   z.target[1] = 512;
   const int64_t seqs = std::min(b.seqs, tokens);
   const int64_t tiles[2] = {
-      !ragged ? seqs * ((group + z.rows[0] - 1) / z.rows[0]) : tokens * group / z.rows[0] + seqs,
+      !ragged ? seqs * ((group + z.rows[0] - 1) / z.rows[0]) : seqs * (kFewRows / z.rows[0]),
       chunks ? tokens * group / z.rows[1] + std::min(seqs, tokens * group / (kFewRows + 1)) : 0};
   const int64_t least[2] = {kSliceLeast<0>, kSliceLeast<1>};
   int64_t plan = 0;

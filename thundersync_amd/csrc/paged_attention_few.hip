@@ -291,19 +291,13 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
     } else {
       // Rows differ in what they see, and a weight of 0 does not take a NaN out: values that are not finite are left out of
       // the product, and a second one, of where they are with who sees them, ruins the elements of the rows that do.
-      constexpr uint32_t kTop = std::is_same_v<T, f16> ? 0x7c00u : 0x7f80u, kOne = std::is_same_v<T, f16> ? 0x3c00u : 0x3f80u;
-      auto split = [&](uint32_t x, uint32_t& fine, uint32_t& flag) __attribute__((always_inline)) {
-        const bool lo = (x & kTop) == kTop, hi = (x >> 16 & kTop) == kTop;
-        fine = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
-        flag = (lo ? kOne : 0u) | (hi ? kOne << 16 : 0u);
-      };
       u32x4 seen[R];
 #pragma unroll
       for (int t = 0; t < R; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int at = pos + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
-          seen[t][j] = (at <= limit[t] ? kOne : 0u) | (at + 1 <= limit[t] ? kOne << 16 : 0u);
+          seen[t][j] = (at <= limit[t] ? kOneOf<T> : 0u) | (at + 1 <= limit[t] ? kOneOf<T> << 16 : 0u);
         }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
@@ -312,7 +306,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t x, y;
-          split(f[j], x, y);
+          split_finite<T>(f[j], x, y);
           fine[j] = x;
           flag[j] = y;
         }
@@ -424,7 +418,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
 }
 
 template <typename T, bool WIDE, int ROW>
-void launch_rows(const AttnArgs& a, const Sizes& z, hipStream_t s) {
+void launch_few_rows(const AttnArgs& a, const Sizes& z, hipStream_t s) {
   const dim3 grid((unsigned)(z.items[0] + (a.batch.offsets ? (a.batch.tokens + 15) / 16 : 0))), block(64 * kWaves);
   ts::TimedLaunch timed_("paged.few_kernel", s);
   if (z.rows[0] == 16) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 1>), grid, block, 0, s, a);
@@ -432,18 +426,18 @@ void launch_rows(const AttnArgs& a, const Sizes& z, hipStream_t s) {
 }
 
 template <typename T, bool WIDE>
-void launch_t(const AttnArgs& a, const Sizes& z, int row, hipStream_t s) {
+void launch_few_t(const AttnArgs& a, const Sizes& z, int row, hipStream_t s) {
   switch (row) {
-    case 64: launch_rows<T, WIDE, 64>(a, z, s); break;
-    case 128: launch_rows<T, WIDE, 128>(a, z, s); break;
-    case 192: launch_rows<T, WIDE, 192>(a, z, s); break;
-    default: launch_rows<T, WIDE, 256>(a, z, s);
+    case 64: launch_few_rows<T, WIDE, 64>(a, z, s); break;
+    case 128: launch_few_rows<T, WIDE, 128>(a, z, s); break;
+    case 192: launch_few_rows<T, WIDE, 192>(a, z, s); break;
+    default: launch_few_rows<T, WIDE, 256>(a, z, s);
   }
 }
 
 void launch_few(const AttnArgs& a, const Sizes& z, int dtype, bool wide, int row, hipStream_t s) {
-  if (dtype == kF16) wide ? launch_t<f16, true>(a, z, row, s) : launch_t<f16, false>(a, z, row, s);
-  else wide ? launch_t<bf16, true>(a, z, row, s) : launch_t<bf16, false>(a, z, row, s);
+  if (dtype == kF16) wide ? launch_few_t<f16, true>(a, z, row, s) : launch_few_t<f16, false>(a, z, row, s);
+  else wide ? launch_few_t<bf16, true>(a, z, row, s) : launch_few_t<bf16, false>(a, z, row, s);
 }
 
 }  // namespace paged
