@@ -145,12 +145,12 @@ __device__ __forceinline__ bool find_block(const Batch& b, int unit, int lane, i
       const int y = __shfl_up(upto, d, 64);
       if (lane >= d) upto += y;
     }
-    const int all = __shfl(upto, 63, 64);
+    const int all = __builtin_amdgcn_readlane(upto, 63);
     if (unit < before + all) {
       const uint64_t past = __ballot(before + upto > unit);
       const int at = __ffsll((unsigned long long)past) - 1;
       s = s0 + at;
-      const int skip = unit - before - (__shfl(upto, at, 64) - __shfl(count, at, 64));
+      const int skip = unit - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(count, at));
       q = seq_of(b, s);
       const int from = max(q.len - q.n, 0);
       const int block = (from >> 4) + skip;

@@ -11,8 +11,8 @@ namespace paged {
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
 
-// Where a sequence's partial rows lie, written by the work-group of its first item: slot (unit0 + tile * slices
-// + slice) * kv_heads + head of its kernel's, `rows` query rows a tile.
+// Where a sequence's partial rows lie, written by the work-group of its first item: slot (unit0 + slice * tiles
+// + tile) * kv_heads + head of its kernel's, `rows` query rows a tile.
 struct Plan {
   int32_t unit0, slices, rows, kernel;
 };
@@ -85,7 +85,9 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int tile_rows, int 
     }
   work = wave_sum(work);
   const float each = work * (float)a.kv_heads / (float)a.target[KERNEL];
-  const int slice = max(kSliceLeast<KERNEL>, (int)fminf(each / kSliceStep + 1.f, (float)(kMaxKeys / kSliceStep)) * kSliceStep);
+  // read from one lane, as what follows is: uniform to the compiler too, so that pages are looked up by scalar loads
+  const int slice = __builtin_amdgcn_readfirstlane(
+      max(kSliceLeast<KERNEL>, (int)fminf(each / kSliceStep + 1.f, (float)(kMaxKeys / kSliceStep)) * kSliceStep));
   const int unit = id / a.kv_heads;
   int before = 0, parts_before = 0;
   for (int s0 = 0; s0 < b.seqs; s0 += 64) {
@@ -98,7 +100,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int tile_rows, int 
     }
     const int upto = wave_prefix(count, lane) + before;
     const int parts = wave_prefix(slices > 1 ? count : 0, lane) + parts_before;
-    const int all = __shfl(upto, 63, 64);
+    const int all = __builtin_amdgcn_readlane(upto, 63);
     if (unit < all) {
       const int at = __ffsll((unsigned long long)__ballot(upto > unit)) - 1;
       it.s = __builtin_amdgcn_readfirstlane(s0 + at);
@@ -111,8 +113,9 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int tile_rows, int 
       const int of = __builtin_amdgcn_readlane(count, at);
       const int in = unit - (__builtin_amdgcn_readlane(upto, at) - of);
       it.part = __builtin_amdgcn_readlane(parts, at) - of + in;
-      it.tile = in / it.slices;
-      it.slice = in - it.tile * it.slices;
+      const int tiles = of / it.slices;  // of one slice side by side: they read the same keys
+      it.slice = in / tiles;
+      it.tile = in - it.slice * tiles;
       it.rows = it.seq.n * a.group;
       const int keys = keys_of(a, it.seq);
       it.begin = min(it.slice * slice, keys);
@@ -120,7 +123,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int tile_rows, int 
       return true;
     }
     before = all;
-    parts_before = __shfl(parts, 63, 64);
+    parts_before = __builtin_amdgcn_readlane(parts, 63);
   }
   past = id - before * a.kv_heads;
   return false;

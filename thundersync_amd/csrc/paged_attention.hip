@@ -27,8 +27,9 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
   if (plan.slices <= 1) return;
   const int head = h / a.group, row = (t - q.row0) * a.group + h % a.group, tile = row / plan.rows;
   const float *part = a.part[plan.kernel], *stats = a.stats[plan.kernel];
-  const int64_t step = (int64_t)a.kv_heads * plan.rows;
-  const int64_t at = ((int64_t)(plan.unit0 + tile * plan.slices) * a.kv_heads + head) * plan.rows + row % plan.rows;
+  const int tiles = (q.n * a.group + plan.rows - 1) / plan.rows;
+  const int64_t step = (int64_t)tiles * a.kv_heads * plan.rows;
+  const int64_t at = ((int64_t)(plan.unit0 + tile) * a.kv_heads + head) * plan.rows + row % plan.rows;
   float most = neg_inf();
   for (int p = lane; p < plan.slices; p += 64) most = fmaxf(most, stats[2 * (at + p * step)]);
   most = wave_max(most);
@@ -58,16 +59,19 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
 
 // Sequences of up to 32 query rows a KV head are the few kernel's.
 constexpr int kFewRows = 32;
+#ifndef TSC_TARGET
+#define TSC_TARGET 1024
+#endif
 
 Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens, int64_t heads) {
   Sizes z{};
   const int64_t group = heads / c.kv_heads, keys = b.width * c.page_size + 16;
   const bool ragged = b.offsets != nullptr, chunks = ragged && tokens * group > kFewRows;
-  // 32 rows a tile in 16 bits would not fit the registers beside wide rows' loads
-  z.rows[0] = (ragged || group > 16) && !(c.bits == 16 && c.row > 128) ? 32 : 16;
+  // 32 rows a tile would not fit the registers beside wide rows' loads
+  z.rows[0] = (ragged || group > 16) && c.row <= 128 ? 32 : 16;
   z.rows[1] = 128;
   z.target[0] = c.row * z.rows[0] <= 128 * 16 ? 2048 : 1024;
-  z.target[1] = 512;
+  z.target[1] = TSC_TARGET;
   const int64_t seqs = std::min(b.seqs, tokens);
   const int64_t tiles[2] = {
       !ragged ? seqs * ((group + z.rows[0] - 1) / z.rows[0]) : seqs * (kFewRows / z.rows[0]),

@@ -26,12 +26,18 @@ using attn::tr_read;
 
 constexpr int kTileRows = 128, kKeys = 32;
 constexpr float kSlack = 8.f, kSlackSum = 256.f;
+#ifndef TSC_OCC
+#define TSC_OCC 2
+#endif
+#ifndef TSC_OCC64
+#define TSC_OCC64 3
+#endif
 
 template <int ROW> constexpr int kBlocks = ROW <= 192 ? 2 : 1;  // 16-row query blocks a wave
 template <int ROW> constexpr int kChunkWaves = kTileRows / 16 / kBlocks<ROW>;
 
 template <typename T, bool WIDE, int ROW>
-__global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? 4 : ROW <= 128 ? 3 : 2)) void chunk_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW <= 128 ? TSC_OCC : 2)) void chunk_kernel(AttnArgs a) {
   constexpr int NQB = kBlocks<ROW>, kWaves = kChunkWaves<ROW>, kThreads = 64 * kWaves;
   constexpr int NC = ROW / 32, NB = ROW / 16;
   constexpr int kSize = WIDE ? 2 : 1;
@@ -181,47 +187,37 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? 4 : ROW <= 128 
           for (int i = 0; i < 4; ++i)
             if (pos + 16 * h + 4 * g + i > limit[t]) sc[h][t][i] = neg_inf();
     }
-    float e[NQB][8], sum[NQB];
-    auto exponentials = [&](int t) __attribute__((always_inline)) {
-      const float ref = m[t] == neg_inf() ? 0.f : m[t];
-      sum[t] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[t][j] = fast_exp2(fmaf(sc[j >> 2][t][j & 3], c, -ref));
-        sum[t] += e[t][j];
-      }
-    };
-    bool redo = false;
+    bf16x8 p[NQB];
 #pragma unroll
     for (int t = 0; t < NQB; ++t) {
-      exponentials(t);
-      redo |= (m[t] == neg_inf()) | (sum[t] > kSlackSum);
-    }
-    if (__ballot(redo)) {
+      float e[8], sum;
+      auto exponentials = [&]() __attribute__((always_inline)) {
+        const float ref = m[t] == neg_inf() ? 0.f : m[t];
+        sum = 0.f;
 #pragma unroll
-      for (int t = 0; t < NQB; ++t) {
+        for (int j = 0; j < 8; ++j) {
+          e[j] = fast_exp2(fmaf(sc[j >> 2][t][j & 3], c, -ref));
+          sum += e[j];
+        }
+      };
+      exponentials();
+      if (__ballot((m[t] == neg_inf()) | (sum > kSlackSum))) {
         float most = neg_inf();
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = fmaxf(most, sc[j >> 2][t][j & 3] * c);
         most = rows_max4(most);
         const bool move = most > m[t] + kSlack || (m[t] == neg_inf() && most > m[t]);
-        if (__ballot(move)) {
-          const float alpha = move ? fast_exp2(m[t] - most) : 1.f;
-          m[t] = move ? most : m[t];
-          l[t] *= alpha;
+        const float alpha = move ? fast_exp2(m[t] - most) : 1.f;
+        m[t] = move ? most : m[t];
+        l[t] *= alpha;
 #pragma unroll
-          for (int b = 0; b < NB; ++b) acc[b][t] *= alpha;
-        }
-        exponentials(t);
+        for (int b = 0; b < NB; ++b) acc[b][t] *= alpha;
+        exponentials();
       }
-    }
-    bf16x8 p[NQB];
-#pragma unroll
-    for (int t = 0; t < NQB; ++t) {
-      l[t] += sum[t];
+      l[t] += sum;
       u32x4 w;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack2<T>(e[t][2 * j], e[t][2 * j + 1]);
+      for (int j = 0; j < 4; ++j) w[j] = pack2<T>(e[2 * j], e[2 * j + 1]);
       p[t] = as_bf16x8(w);
     }
     __builtin_amdgcn_s_setprio(1);

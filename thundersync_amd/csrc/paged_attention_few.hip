@@ -121,49 +121,43 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
     const int page = uniform_table(table)[at];
     return page >= 0 && page < a.pages ? page : -1;
   };
+  // A page that is none is read as page 0, and its scores and values are not used.
   Tile<WIDE, ROW> tile[2];
-  float ks[2], vs[2];
-  int page[2];
-  const int key_lane = (r * ROW + (WIDE ? 8 : 16) * g) * kSize;
-  const int value_lane = (4 * g * ROW + NB * r) * kSize;
-  auto load_keys = [&](int pos) {
+  float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f;  // of the step whose keys have been asked for
+  int page0 = -1, page1 = -1;
+  const uint32_t key_lane = (r * ROW + (WIDE ? 8 : 16) * g) * kSize;
+  const uint32_t value_lane = (4 * g * ROW + NB * r) * kSize;
+  auto line_of = [&](int at) -> int64_t { return ((int64_t)it.head << a.page_shift) + (at & page_mask); };
+  auto load_tile_keys = [&](int at, int page, u32x4 (&k)[Tile<WIDE, ROW>::kLoads], float& key_scale, float& value_scale)
+                            __attribute__((always_inline)) {
+    const int id = max(page, 0);
+    const char* p = a.key + id * a.key_page_stride + line_of(at) * (ROW * kSize);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = pos + 16 * h;
-      page[h] = page_at(at);
-      if (page[h] < 0) {
-        ks[h] = vs[h] = 1.f;
-        continue;
-      }
-      const int64_t line = ((int64_t)it.head << a.page_shift) + (at & page_mask);
-      const char* p = a.key + page[h] * a.key_page_stride + line * (ROW * kSize) + key_lane;
-#pragma unroll
-      for (int i = 0; i < Tile<WIDE, ROW>::kLoads; ++i) tile[h].k[i] = *(const u32x4*)(p + 64 * i);
-      if constexpr (!WIDE) {
-        const int64_t scale = (((int64_t)page[h] * a.kv_heads << a.page_shift) + line) >> 4;
-        ks[h] = uniform_table(a.key_scale)[scale];
-        vs[h] = uniform_table(a.value_scale)[scale];
-      }
+    for (int i = 0; i < Tile<WIDE, ROW>::kLoads; ++i) k[i] = *(const u32x4*)(p + key_lane + 64 * i);
+    if constexpr (!WIDE) {
+      const int64_t scale = (((int64_t)id * a.kv_heads << a.page_shift) + line_of(at)) >> 4;
+      key_scale = uniform_table(a.key_scale)[scale];
+      value_scale = uniform_table(a.value_scale)[scale];
     }
   };
-  auto load_values = [&](int pos) {
+  auto load_keys = [&](int at) __attribute__((always_inline)) {
+    page0 = page_at(at);
+    page1 = page_at(at + 16);
+    load_tile_keys(at, page0, tile[0].k, ks0, vs0);
+    load_tile_keys(at + 16, page1, tile[1].k, ks1, vs1);
+  };
+  auto load_values = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int at = pos + 16 * h;
-      if (page[h] < 0) {
+      const char* p = a.value + max(h ? page1 : page0, 0) * a.value_page_stride + line_of(at + 16 * h) * (ROW * kSize);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tile[h].v[i] = Words<NB * kSize>{};
-        continue;
-      }
-      const int64_t line = ((int64_t)it.head << a.page_shift) + (at & page_mask);
-      const char* p = a.value + page[h] * a.value_page_stride + line * (ROW * kSize) + value_lane;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tile[h].v[i] = load_words<NB * kSize>(p + i * ROW * kSize);
+      for (int i = 0; i < 4; ++i) tile[h].v[i] = load_words<NB * kSize>(p + value_lane + i * ROW * kSize);
     }
   };
 
   int pos = __builtin_amdgcn_readfirstlane(it.begin + 32 * wave);
-  if (pos < it.end) {
+  const int whole = min(it.end, low + 1) - 31;  // steps before it are seen whole by every row
+  if (pos < whole) {
     load_keys(pos);
     load_values(pos);
   }
@@ -171,17 +165,19 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
   // One step; `edge`: some row does not see some of its keys, or they are not there.
   auto step = [&](auto edge_) __attribute__((always_inline)) {
     constexpr bool edge = decltype(edge_)::value;
+    if constexpr (edge) {  // few, and nothing is asked for ahead of them: the registers are worth more
+      load_keys(pos);
+      load_values(pos);
+    }
     asm volatile("" ::: "memory");  // the query's operands are read again, not held over the loop
     f32x4 sc[R][2];
-    bool ruined = false;
+    const bool ruined0 = page0 < 0 && pos < it.end, ruined1 = page1 < 0 && pos + 16 < it.end;
+    const float vscale0 = vs0, vscale1 = vs1;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int t = 0; t < R; ++t) sc[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (page[h] < 0) {
-        ruined |= pos + 16 * h < it.end;
-        continue;
-      }
+      const float key_scale = h ? ks1 : ks0;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         bf16x8 k;
@@ -190,8 +186,8 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
         } else {
           const u32x4 x = tile[h].k[c / 2];
           const uint32_t lo = x[2 * (c & 1)], hi = x[2 * (c & 1) + 1];
-          k = as_bf16x8(u32x4{widen2<T, false>(lo, ks[h]), widen2<T, true>(lo, ks[h]), widen2<T, false>(hi, ks[h]),
-                              widen2<T, true>(hi, ks[h])});
+          k = as_bf16x8(u32x4{widen2<T, false>(lo, key_scale), widen2<T, true>(lo, key_scale),
+                              widen2<T, false>(hi, key_scale), widen2<T, true>(hi, key_scale)});
         }
 #pragma unroll
         for (int t = 0; t < R; ++t) sc[t][h] = mma16<T>(k, as_bf16x8(s_query[t][c][lane]), sc[t][h]);
@@ -199,17 +195,15 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
 #pragma unroll
       for (int t = 0; t < R; ++t) sc[t][h] *= a.scale;
     }
-    const float vscale[2] = {WIDE ? 1.f : vs[0], WIDE ? 1.f : vs[1]};
-    const int pages[2] = {page[0], page[1]};
     const int next = pos + 32 * kWaves;
-    if (next < it.end) load_keys(next);
+    if (!edge && next < whole) load_keys(next);
 
-    if (ruined) {  // keys of a page that is none
+    if (ruined0 | ruined1) {  // keys of a page that is none
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (pages[h] < 0)
-#pragma unroll
-          for (int t = 0; t < R; ++t) sc[t][h] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+      for (int t = 0; t < R; ++t) {
+        if (ruined0) sc[t][0] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+        if (ruined1) sc[t][1] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+      }
     }
     bf16x8 p[R];
 #pragma unroll
@@ -276,7 +270,8 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
           } else {
             const uint32_t x = tile[h].v[2 * k].w[b / 4], y = tile[h].v[2 * k + 1].w[b / 4];
             const uint32_t z = __builtin_amdgcn_perm(y, x, b & 2 ? 0x07030602u : 0x05010400u);
-            f[2 * h + k] = b & 1 ? widen2<T, true>(z, vscale[h]) : widen2<T, false>(z, vscale[h]);
+            const float scale = h ? vscale1 : vscale0;
+            f[2 * h + k] = b & 1 ? widen2<T, true>(z, scale) : widen2<T, false>(z, scale);
           }
         }
       return f;
@@ -321,10 +316,10 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (next < it.end) load_values(next);
+    if (!edge && next < whole) load_values(next);
     pos = next;
   };
-  while (pos < it.end && pos + 31 <= low) step(std::false_type{});
+  while (pos < whole) step(std::false_type{});
   while (pos < it.end) step(std::true_type{});
   __syncthreads();  // the query's operands have been read
 
@@ -422,7 +417,7 @@ void launch_few_rows(const AttnArgs& a, const Sizes& z, hipStream_t s) {
   const dim3 grid((unsigned)(z.items[0] + (a.batch.offsets ? (a.batch.tokens + 15) / 16 : 0))), block(64 * kWaves);
   ts::TimedLaunch timed_("paged.few_kernel", s);
   if (z.rows[0] == 16) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 1>), grid, block, 0, s, a);
-  else if constexpr (!WIDE || ROW <= 128) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 2>), grid, block, 0, s, a);
+  else if constexpr (ROW <= 128) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 2>), grid, block, 0, s, a);
 }
 
 template <typename T, bool WIDE>
