@@ -30,19 +30,22 @@ struct AttnArgs {
   float scale;        // log2 units
   int32_t heads, kv_heads, group, head_dim, page_shift;
   int32_t few_rows;   // sequences of more query rows (tokens x group) are the chunk kernel's; 0: none are
-  int32_t target[2];  // items that a kernel's work is cut into, about
+  int32_t target[2];  // items that a kernel's work is cut into, at least
   Plan* plan;         // [seqs]
   float* part[2];     // of each kernel: [slots][rows][row] unnormalised sums
   float* stats[2];    // [slots][rows][2]: reference point (log2 units) and sum
 };
 
 // Items: (sequence, tile of ROWS query rows of a KV head, slice of its keys, KV head).  A slice is as long as cuts all
-// of a kernel's keys into about `target` of them, a multiple of kSliceStep and no shorter than kSliceLeast keys, so that
-// long and short sequences of a batch share the device evenly.  Lengths are known on the device alone:
+// of a kernel's keys into `target` of them, about what the device holds at once, or, where these are longer than
+// kSliceLong keys, into up to four times as many, so that a last round of them costs less; a multiple of kSliceStep and no
+// shorter than kSliceLeast, so that long and short sequences of a batch share the device evenly.  One sequence of 125000
+// keys, 8 KV heads: 59 us in 1024 items, 64 in 2048, 76 in 4096; 256 sequences of 256 to 16384: 835, 802 and 780.  Lengths are known on the device alone:
 // every wave works the plan out itself, 64 sequences at a time, and takes the item of its work-group.
-// Items number at most target + kv_heads * tiles; those of sequences with several slices, which leave partial rows, at
-// most 2 * target (each such sequence has at most twice its length in slices).
+// Items number at most kv_heads * (keys / slice + tiles); those of sequences with several slices, which leave partial
+// rows, at most twice kv_heads * keys / slice (each such sequence has at most twice its length in slices).
 constexpr int kSliceStep = 128;
+template <int KERNEL> constexpr int kSliceLong = KERNEL == 0 ? 4096 : 2048;
 template <int KERNEL> constexpr int kSliceLeast = KERNEL == 0 ? 256 : 512;
 
 struct Item {
@@ -84,7 +87,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int tile_rows, int 
       work += (float)keys_of(a, q) * (float)tiles_of<KERNEL>(a, q, tile_rows);
     }
   work = wave_sum(work);
-  const float each = work * (float)a.kv_heads / (float)a.target[KERNEL];
+  float each = work * (float)a.kv_heads / (float)a.target[KERNEL];
+  each = fmaxf(fminf(each, (float)kSliceLong<KERNEL>), each * 0.25f);
   // read from one lane, as what follows is: uniform to the compiler too, so that pages are looked up by scalar loads
   const int slice = __builtin_amdgcn_readfirstlane(
       max(kSliceLeast<KERNEL>, (int)fminf(each / kSliceStep + 1.f, (float)(kMaxKeys / kSliceStep)) * kSliceStep));

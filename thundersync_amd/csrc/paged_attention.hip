@@ -59,9 +59,6 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
 
 // Sequences of up to 32 query rows a KV head are the few kernel's.
 constexpr int kFewRows = 32;
-#ifndef TSC_TARGET
-#define TSC_TARGET 1024
-#endif
 
 Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens, int64_t heads) {
   Sizes z{};
@@ -70,18 +67,20 @@ Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens,
   // 32 rows a tile would not fit the registers beside wide rows' loads
   z.rows[0] = (ragged || group > 16) && c.row <= 128 ? 32 : 16;
   z.rows[1] = 128;
-  z.target[0] = c.row * z.rows[0] <= 128 * 16 ? 2048 : 1024;
-  z.target[1] = TSC_TARGET;
+  z.target[0] = c.row * z.rows[0] <= 128 * 16 ? 1024 : 512;
+  z.target[1] = 512;
   const int64_t seqs = std::min(b.seqs, tokens);
   const int64_t tiles[2] = {
       !ragged ? seqs * ((group + z.rows[0] - 1) / z.rows[0]) : seqs * (kFewRows / z.rows[0]),
       chunks ? tokens * group / z.rows[1] + std::min(seqs, tokens * group / (kFewRows + 1)) : 0};
-  const int64_t least[2] = {kSliceLeast<0>, kSliceLeast<1>};
+  const int64_t least[2] = {kSliceLeast<0>, kSliceLeast<1>}, longest[2] = {kSliceLong<0>, kSliceLong<1>};
   int64_t plan = 0;
   for (int k = 0; k < 2; ++k) {
     const int64_t most = c.kv_heads * tiles[k] * ((keys + least[k] - 1) / least[k]);
-    z.items[k] = std::min(most, z.target[k] + z.target[k] / 64 + c.kv_heads * (tiles[k] + 1));
-    z.slots[k] = keys <= least[k] ? 0 : std::min(most, 2 * (z.target[k] + z.target[k] / 64 + c.kv_heads));
+    // kv_heads * keys / slice, for any lengths (a rounded slice may be short of its length by 2^-20)
+    const int64_t cut = std::max(z.target[k], std::min(4 * z.target[k], c.kv_heads * tiles[k] * keys / longest[k])) * 65 / 64;
+    z.items[k] = std::min(most, cut + c.kv_heads * (tiles[k] + 1));
+    z.slots[k] = keys <= least[k] ? 0 : std::min(most, 2 * (cut + c.kv_heads));
     if (z.slots[k]) plan = (b.seqs * (int64_t)sizeof(Plan) + 255) / 256 * 256;
     z.bytes += z.slots[k] * z.rows[k] * (c.row + 2) * 4;
   }
@@ -120,7 +119,7 @@ int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch,
   // 2^24 work-groups of 256 threads wrap a launch; a slice of 2^30 keys has to be enough for `target` of them
   TS_CHECK_ARG(tokens * heads < (1ll << 24) && std::max(z.items[0], z.items[1]) + tokens / 16 < (1ll << 24) - 1 &&
                    batch->width * cache->page_size <= kMaxKeys &&
-                   (double)batch->width * cache->page_size * (double)(z.items[0] + z.items[1]) < 1e12,
+                   (double)batch->width * cache->page_size * (double)(z.items[0] + z.items[1]) < 1e11,
                "ts_paged_attention: %lld rows of %lld heads over %lld sequences of %lld pages: too large", (long long)tokens,
                (long long)heads, (long long)batch->seqs, (long long)batch->width);
   TS_CHECK_ARG(z.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bytes),
