@@ -11,10 +11,11 @@ namespace paged {
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
 
-// Where a sequence's partial rows lie, written by the work-group of its first item: slot (unit0 + slice * tiles
-// + tile) * kv_heads + head of its kernel's, `rows` query rows a tile.
+// Where a sequence's work lies in its kernel's, written by the work-group that begins it.
 struct Plan {
-  int32_t unit0, slices, rows, kernel;
+  int32_t start, blocks;  // of its first tile, and of each tile
+  int32_t per;            // blocks of a work-group
+  int32_t kernel;
 };
 constexpr int64_t kMaxKeys = 1 << 30;  // of a sequence
 
@@ -30,30 +31,67 @@ struct AttnArgs {
   float scale;        // log2 units
   int32_t heads, kv_heads, group, head_dim, page_shift;
   int32_t few_rows;   // sequences of more query rows (tokens x group) are the chunk kernel's; 0: none are
-  int32_t target[2];  // items that a kernel's work is cut into, at least
-  Plan* plan;         // [seqs]
+  int32_t jobs[2];    // work-groups of each KV head that a kernel's work is dealt to, at least
+  int32_t tile_rows[2];
+  Plan* plan;         // [seqs], or null where no tile can be cut
   float* part[2];     // of each kernel: [slots][rows][row] unnormalised sums
   float* stats[2];    // [slots][rows][2]: reference point (log2 units) and sum
 };
 
-// Items: (sequence, tile of ROWS query rows of a KV head, slice of its keys, KV head).  A slice is as long as cuts all
-// of a kernel's keys into `target` of them, about what the device holds at once, or, where these are longer than
-// kSliceLong keys, into up to four times as many, so that a last round of them costs less; a multiple of kSliceStep and no
-// shorter than kSliceLeast, so that long and short sequences of a batch share the device evenly.  One sequence of 125000
-// keys, 8 KV heads: 59 us in 1024 items, 64 in 2048, 76 in 4096; 256 sequences of 256 to 16384: 835, 802 and 780.  Lengths are known on the device alone:
-// every wave works the plan out itself, 64 sequences at a time, and takes the item of its work-group.
-// Items number at most kv_heads * (keys / slice + tiles); those of sequences with several slices, which leave partial
-// rows, at most twice kv_heads * keys / slice (each such sequence has at most twice its length in slices).
-constexpr int kSliceStep = 128;
-template <int KERNEL> constexpr int kSliceLong = KERNEL == 0 ? 4096 : 2048;
-template <int KERNEL> constexpr int kSliceLeast = KERNEL == 0 ? 256 : 512;
+// The kernel's only argument, read from its segment where it is used: over a loop of tiles its 50 words would not fit
+// the scalar registers beside the tile's own.
+__device__ __forceinline__ AttnArgs arguments() {
+  typedef const __attribute__((address_space(4))) uint32_t* Words;
+  Words p = (Words)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  uint32_t w[sizeof(AttnArgs) / 4];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(AttnArgs) / 4); ++i) w[i] = p[i];
+  AttnArgs a;
+  __builtin_memcpy(&a, w, sizeof(a));
+  // known to be global memory again: reads through pointers that may be any kind wait for LDS too
+  auto global = [](auto*& x) __attribute__((always_inline)) {
+    typedef std::remove_reference_t<decltype(*x)> E;
+    x = (E*)(__attribute__((address_space(1))) E*)(uint64_t)x;
+  };
+  global(a.batch.table);
+  global(a.batch.lengths);
+  global(a.batch.offsets);
+  global(a.query);
+  global(a.out);
+  global(a.key);
+  global(a.value);
+  global(a.key_scale);
+  global(a.value_scale);
+  global(a.plan);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    global(a.part[i]);
+    global(a.stats[i]);
+  }
+  return a;
+}
 
-struct Item {
-  Seq seq;
-  int s, head, tile, slice, slices, rows;
-  int unit, part;  // among all of the kernel's (tile, slice), and among those that leave partial rows
-  int begin, end;  // keys
-};
+// How a kernel's work is dealt out.  A tile (query rows of one KV head, of one sequence) is kTileCost blocks for its
+// start and end and one for each kBlockKeys keys; a KV head's tiles follow one another, and each of its work-groups
+// takes as many blocks in a row, ending tiles and beginning others on the way, so that all end together however lengths
+// differ.  A tile that a border cuts leaves partial rows: slot 2 j of work-group j where it began before, 2 j + 1 where it
+// ends behind.  Work-groups are as many as the device holds at once, or twice or four times as many where each still gets
+// kLong blocks, so that a slow one costs less, and fewer where they would get less than kLeast.  64 sequences of 100 to 6000
+// keys, 24/4 heads of 256: 100 us in slices of equal length a sequence, 88 dealt like this.
+//
+// Lengths are known on the device alone: every wave works the plan out itself, 64 sequences at a time.
+constexpr int kBlockKeys = 128, kTileCost = 1;
+template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 3 : 5;
+constexpr int kLong = 16;
+template <int KERNEL> constexpr int kFiner = KERNEL == 0 ? 4 : 2;  // a partial tile of the chunk kernel is 64 KB and more
+
+// waves a SIMD: a step's loads and the accumulators are 3 ROW / 8 registers, of 16 bits 5 ROW / 8
+__host__ __device__ constexpr int few_occupancy(bool wide, int row, int tiles) {
+  const int size = row * tiles;
+  return size <= 64 ? 4 : wide ? (size <= 128 ? 3 : 2) : size <= 128 ? 4 : size <= 192 ? 3 : 2;
+}
+__host__ __device__ constexpr int chunk_occupancy(int row) { return row <= 64 ? 4 : 2; }
 
 __device__ __forceinline__ int wave_prefix(int x, int lane) {
 #pragma unroll
@@ -64,74 +102,126 @@ __device__ __forceinline__ int wave_prefix(int x, int lane) {
   return x;
 }
 
-// Keys that a sequence's items go over: a key past the page table ruins the rows that see it, once.
+// Keys that a sequence's tiles go over: a key past the page table ruins the rows that see it, once.
 __device__ __forceinline__ int keys_of(const AttnArgs& a, const Seq& q) {
   return (int)min((int64_t)q.len, ((int64_t)a.batch.width << a.page_shift) + 16);
 }
-
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, const Seq& q) {
+  return kTileCost + (keys_of(a, q) + kBlockKeys - 1) / kBlockKeys;
+}
 template <int KERNEL>
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& q, int tile_rows) {
   const int64_t rows = (int64_t)q.n * a.group;
   const bool many = a.few_rows > 0 && rows > a.few_rows;
   return many == (KERNEL == 1) ? (int)((rows + tile_rows - 1) / tile_rows) : 0;
 }
-
-// The work-group's item; false if it has none, and `past` is then by how many it is past the last.
-template <int KERNEL>
-__device__ __forceinline__ bool find_item(const AttnArgs& a, int tile_rows, int id, int lane, Item& it, int& past) {
-  const Batch& b = a.batch;
-  float work = 0.f;  // keys of all tiles; a rounded sum is the same in every wave
-  for (int s0 = 0; s0 < b.seqs; s0 += 64)
-    if (s0 + lane < b.seqs) {
-      const Seq q = seq_of(b, s0 + lane);
-      work += (float)keys_of(a, q) * (float)tiles_of<KERNEL>(a, q, tile_rows);
-    }
-  work = wave_sum(work);
-  float each = work * (float)a.kv_heads / (float)a.target[KERNEL];
-  each = fmaxf(fminf(each, (float)kSliceLong<KERNEL>), each * 0.25f);
-  // read from one lane, as what follows is: uniform to the compiler too, so that pages are looked up by scalar loads
-  const int slice = __builtin_amdgcn_readfirstlane(
-      max(kSliceLeast<KERNEL>, (int)fminf(each / kSliceStep + 1.f, (float)(kMaxKeys / kSliceStep)) * kSliceStep));
-  const int unit = id / a.kv_heads;
-  int before = 0, parts_before = 0;
-  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
-    int slices = 0, count = 0;
-    Seq q{0, 0, 0};
-    if (s0 + lane < b.seqs) {
-      q = seq_of(b, s0 + lane);
-      slices = max(1, (keys_of(a, q) + slice - 1) / slice);
-      count = tiles_of<KERNEL>(a, q, tile_rows) * slices;
-    }
-    const int upto = wave_prefix(count, lane) + before;
-    const int parts = wave_prefix(slices > 1 ? count : 0, lane) + parts_before;
-    const int all = __builtin_amdgcn_readlane(upto, 63);
-    if (unit < all) {
-      const int at = __ffsll((unsigned long long)__ballot(upto > unit)) - 1;
-      it.s = __builtin_amdgcn_readfirstlane(s0 + at);
-      it.seq.len = __builtin_amdgcn_readlane(q.len, at);
-      it.seq.row0 = __builtin_amdgcn_readlane(q.row0, at);
-      it.seq.n = __builtin_amdgcn_readlane(q.n, at);
-      it.slices = __builtin_amdgcn_readlane(slices, at);
-      it.unit = unit;
-      it.head = id - unit * a.kv_heads;
-      const int of = __builtin_amdgcn_readlane(count, at);
-      const int in = unit - (__builtin_amdgcn_readlane(upto, at) - of);
-      it.part = __builtin_amdgcn_readlane(parts, at) - of + in;
-      const int tiles = of / it.slices;  // of one slice side by side: they read the same keys
-      it.slice = in / tiles;
-      it.tile = in - it.slice * tiles;
-      it.rows = it.seq.n * a.group;
-      const int keys = keys_of(a, it.seq);
-      it.begin = min(it.slice * slice, keys);
-      it.end = min(it.begin + slice, keys);
-      return true;
-    }
-    before = all;
-    parts_before = __builtin_amdgcn_readlane(parts, 63);
-  }
-  past = id - before * a.kv_heads;
-  return false;
+__host__ __device__ inline int64_t blocks_each(int64_t total, int64_t jobs, int least, int finer) {
+  int f = 1;
+  while (f < finer && total >= 2 * f * jobs * kLong) f *= 2;
+  const int64_t each = (total + f * jobs - 1) / (f * jobs);
+  return each > least ? each : least;
 }
+
+// A work-group's place in its kernel's work.  Everything is read from one lane, so that it is uniform to the compiler
+// too and pages are looked up by scalar loads.
+template <int KERNEL> struct Cursor {
+  Seq seq;
+  int s, tile, tiles, blocks;  // of the sequence
+  int from;                    // block of the tile
+  int left;                    // blocks of the work-group
+  int per, job, head;
+
+  // false if the work-group has none; `past` is then by how many it is past the last that has
+  __device__ __forceinline__ bool begin(const AttnArgs& a, int tile_rows, int id, int lane, int& past) {
+    const Batch& b = a.batch;
+    // the first 64 sequences are read once
+    Seq q{0, 0, 0};
+    int count = 0;
+    auto read = [&](int s0) __attribute__((always_inline)) {
+      count = 0;
+      if (s0 + lane < b.seqs) {
+        q = seq_of(b, s0 + lane);
+        count = tiles_of<KERNEL>(a, q, tile_rows) * blocks_of(a, q);
+      }
+    };
+    int total = 0;
+    for (int s0 = (b.seqs - 1) & ~63; s0 >= 0; s0 -= 64) {
+      read(s0);
+      total += count;
+    }
+    total = __builtin_amdgcn_readlane(wave_prefix(total, lane), 63);
+    per = (int)blocks_each(total, a.jobs[KERNEL], kLeast<KERNEL>, kFiner<KERNEL>);
+    job = id / a.kv_heads;
+    head = id - job * a.kv_heads;
+    const int used = (total + per - 1) / per;
+    past = id - used * a.kv_heads;
+    if (job >= used) return false;
+    const int start = job * per;
+    left = min(per, total - start);
+    int before = 0;
+    for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+      if (s0 > 0) read(s0);
+      const int upto = wave_prefix(count, lane) + before;
+      const int all = __builtin_amdgcn_readlane(upto, 63);
+      if (start < all) {
+        const int at = __ffsll((unsigned long long)__ballot(upto > start)) - 1;
+        const int in = start - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(count, at));
+        enter(a, tile_rows, s0, at, q);
+        tile = in / blocks;
+        from = in - tile * blocks;
+        return true;
+      }
+      before = all;
+    }
+    return false;
+  }
+  // Kept in LDS while a tile is computed, where scalar registers are short.
+  __device__ __forceinline__ void put(int* to) const {
+    if (threadIdx.x == 0) *(Cursor*)to = *this;
+  }
+  __device__ __forceinline__ void take(const int* from_) {
+    asm volatile("" ::: "memory");
+    int w[sizeof(Cursor) / 4];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Cursor) / 4); ++i) w[i] = __builtin_amdgcn_readfirstlane(from_[i]);
+    __builtin_memcpy(this, w, sizeof(Cursor));
+  }
+  // the sequence that lane `at` of a chunk of 64 has read
+  __device__ __forceinline__ void enter(const AttnArgs& a, int tile_rows, int s0, int at, const Seq& q) {
+    s = s0 + __builtin_amdgcn_readfirstlane(at);
+    seq.len = __builtin_amdgcn_readlane(q.len, at);
+    seq.row0 = __builtin_amdgcn_readlane(q.row0, at);
+    seq.n = __builtin_amdgcn_readlane(q.n, at);
+    tiles = tiles_of<KERNEL>(a, seq, tile_rows);
+    blocks = blocks_of(a, seq);
+    tile = from = 0;
+  }
+  // The keys of the tile that are the work-group's; whether it has all of it; else the slot of its partial rows.
+  __device__ __forceinline__ void piece(const AttnArgs& a, int& begin, int& end) const {
+    const int keys = keys_of(a, seq);
+    begin = min(keys, max(from - kTileCost, 0) * kBlockKeys);
+    end = min(keys, max(min(blocks, from + left) - kTileCost, 0) * kBlockKeys);
+  }
+  __device__ __forceinline__ bool whole() const { return from == 0 && left >= blocks; }
+  __device__ __forceinline__ int slot(int kv_heads) const { return (2 * job + (from == 0)) * kv_heads + head; }
+  // To the next tile; false at the work-group's end.
+  __device__ __forceinline__ bool next(const AttnArgs& a, int tile_rows, int lane) {
+    left -= min(blocks, from + left) - from;
+    if (left <= 0) return false;
+    from = 0;
+    if (++tile < tiles) return true;
+    for (int s0 = s + 1; s0 < a.batch.seqs; s0 += 64) {
+      Seq q{0, 0, 0};
+      if (s0 + lane < a.batch.seqs) q = seq_of(a.batch, s0 + lane);
+      const uint64_t which = __ballot(tiles_of<KERNEL>(a, q, tile_rows) > 0);
+      if (which) {
+        enter(a, tile_rows, s0, __ffsll((unsigned long long)which) - 1, q);
+        return true;
+      }
+    }
+    return false;
+  }
+};
 
 // Two 16-bit values without those that are not finite, and ones in the place of these.
 template <typename T> constexpr uint32_t kOneOf = std::is_same_v<T, f16> ? 0x3c00u : 0x3f80u;
@@ -144,10 +234,11 @@ template <typename T> __device__ __forceinline__ void split_finite(uint32_t x, u
 
 // host side
 struct Sizes {
-  int64_t items[2];  // at most, of each kernel (0: not launched)
-  int64_t slots[2];  // those that leave partial rows
-  int64_t rows[2];   // of a tile
-  int64_t target[2];
+  int64_t groups[2];  // work-groups of each kernel, at most (0: not launched)
+  int64_t slots[2];   // partial tiles, at most
+  int64_t rows[2];    // of a tile
+  int64_t jobs[2];
+  int64_t blocks[2];  // of a KV head, at most
   int64_t bytes;
 };
 Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens, int64_t heads);

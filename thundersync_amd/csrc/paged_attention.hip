@@ -11,50 +11,91 @@
 namespace ts {
 namespace paged {
 
-// o = sum_p acc_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over a row's slices, M the largest m: a work-group a row, its
-// waves every fourth slice, then the waves in order.
-template <typename T, int ROW>
-__global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
-  constexpr int N = ROW / 64;
-  __shared__ float s_acc[4][ROW], s_stat[4][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-  const int s = seq_of_row(a.batch, t);
-  if (s >= a.batch.seqs) return;
-  const Seq q = seq_of(a.batch, s);
-  if (t < q.row0 || t >= q.row0 + q.n) return;
-  const Plan plan = a.plan[s];
-  if (plan.slices <= 1) return;
-  const int head = h / a.group, row = (t - q.row0) * a.group + h % a.group, tile = row / plan.rows;
+// o = sum_p acc_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over a row's parts in order, M the largest m: WAVES waves a row,
+// each every WAVES-th part, then the waves in order.
+template <typename T, int ROW, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void merge_kernel(AttnArgs a) {
+  constexpr int N = ROW / 64, kRows = WAVES == 1 ? 4 : 1;
+  __shared__ float s_acc[WAVES][ROW], s_sum[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = (int)blockIdx.x * kRows + wave / WAVES;
+  const int t = id / a.heads, h = id - t * a.heads;
+  const int s = t < a.batch.tokens ? __builtin_amdgcn_readfirstlane(seq_of_row(a.batch, t)) : a.batch.seqs;
+  bool mine = s < a.batch.seqs;
+  Seq q{0, 0, 0};
+  if (mine) q = seq_of(a.batch, s);
+  mine = mine && t >= q.row0 && t < q.row0 + q.n;
+  Plan plan{0, 1, 1, 0};
+  if (mine) plan = a.plan[s];
+  const int rows = a.tile_rows[plan.kernel];
+  const int head = h / a.group, row = (t - q.row0) * a.group + h % a.group, tile = row / rows;
+  const int first = plan.start + tile * plan.blocks, job = first / plan.per;
+  const int parts = mine ? (first + plan.blocks - 1) / plan.per - job + 1 : 1;  // 1: written already
   const float *part = a.part[plan.kernel], *stats = a.stats[plan.kernel];
-  const int tiles = (q.n * a.group + plan.rows - 1) / plan.rows;
-  const int64_t step = (int64_t)tiles * a.kv_heads * plan.rows;
-  const int64_t at = ((int64_t)(plan.unit0 + tile) * a.kv_heads + head) * plan.rows + row % plan.rows;
-  float most = neg_inf();
-  for (int p = lane; p < plan.slices; p += 64) most = fmaxf(most, stats[2 * (at + p * step)]);
-  most = wave_max(most);
-  const float ref = most == neg_inf() ? 0.f : most;
+  // part 0 is slot 2 job + 1, part p > 0 slot 2 (job + p)
+  auto place = [&](int p) -> int64_t {
+    return ((int64_t)(2 * (job + p) + (p == 0)) * a.kv_heads + head) * rows + row % rows;
+  };
   float acc[N], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  if (parts > 1) {
+    float most = neg_inf();
+    for (int p = lane; p < parts; p += 64) most = fmaxf(most, stats[2 * place(p)]);
+    most = wave_max(most);
+    const float ref = most == neg_inf() ? 0.f : most;
 #pragma unroll 4
-  for (int p = wave; p < plan.slices; p += 4) {
-    const int64_t i0 = at + p * step;
-    const float w = fast_exp2(stats[2 * i0] - ref);
-    sum = fmaf(stats[2 * i0 + 1], w, sum);
-    const float* x = part + i0 * ROW + N * lane;
+    for (int p = wave % WAVES; p < parts; p += WAVES) {
+      const int64_t at = place(p);
+      const float m = stats[2 * at], l = stats[2 * at + 1];
+      const float w = fast_exp2(m - ref);
+      sum = fmaf(l, w, sum);
+      const float* x = part + at * ROW + N * lane;
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], w, acc[i]);
+      for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], w, acc[i]);
+    }
   }
+  T* out = (T*)a.out + ((int64_t)t * a.heads + h) * a.head_dim;
+  if constexpr (WAVES == 1) {
+    if (parts <= 1) return;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) s_acc[wave][N * lane + i] = acc[i];
-  if (lane == 0) s_stat[wave][0] = sum;
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= a.head_dim) return;
-  const float l = (s_stat[0][0] + s_stat[1][0]) + (s_stat[2][0] + s_stat[3][0]);
-  const float o = (s_acc[0][d] + s_acc[1][d]) + (s_acc[2][d] + s_acc[3][d]);
-  ((T*)a.out)[((int64_t)t * a.heads + h) * a.head_dim + d] = from_f<T>(o * (l > 0.f ? 1.f / l : 0.f));
+    for (int i = 0; i < N; ++i)
+      if (N * lane + i < a.head_dim) out[N * lane + i] = from_f<T>(acc[i] * inv);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s_acc[wave][N * lane + i] = acc[i];
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (parts <= 1 || d >= a.head_dim) return;
+    float l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      l += s_sum[w];
+      o += s_acc[w][d];
+    }
+    out[d] = from_f<T>(o * (l > 0.f ? 1.f / l : 0.f));
+  }
+}
+
+// Sixteen waves a row where rows are few and may have many parts, a wave a row where they are many.
+constexpr int64_t kManyRows = 1024;
+constexpr int kMergeWaves = 16;
+template <typename T, int ROW> void launch_merge(const AttnArgs& a, hipStream_t s) {
+  ts::TimedLaunch timed_("paged.merge_kernel", s);
+  const int64_t rows = (int64_t)a.batch.tokens * a.heads;
+  if (rows < kManyRows)
+    hipLaunchKernelGGL((merge_kernel<T, ROW, kMergeWaves>), dim3((unsigned)rows), dim3(64 * kMergeWaves), 0, s, a);
+  else hipLaunchKernelGGL((merge_kernel<T, ROW, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+}
+template <typename T> void launch_merge(const AttnArgs& a, int row, hipStream_t s) {
+  switch (row) {
+    case 64: launch_merge<T, 64>(a, s); break;
+    case 128: launch_merge<T, 128>(a, s); break;
+    case 192: launch_merge<T, 192>(a, s); break;
+    default: launch_merge<T, 256>(a, s);
+  }
 }
 
 // Sequences of up to 32 query rows a KV head are the few kernel's.
@@ -67,20 +108,24 @@ Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens,
   // 32 rows a tile would not fit the registers beside wide rows' loads
   z.rows[0] = (ragged || group > 16) && c.row <= 128 ? 32 : 16;
   z.rows[1] = 128;
-  z.target[0] = c.row * z.rows[0] <= 128 * 16 ? 1024 : 512;
-  z.target[1] = 512;
+  // work-groups of a KV head that the device's 256 CUs hold at once (four waves each, eight of chunks of 256-wide rows)
+  const int64_t held[2] = {256 * few_occupancy(c.bits == 16, c.row, (int)z.rows[0] / 16),
+                           256 * chunk_occupancy(c.row) / (c.row > 192 ? 2 : 1)};
+  for (int k = 0; k < 2; ++k) z.jobs[k] = std::max<int64_t>(1, held[k] / c.kv_heads);
   const int64_t seqs = std::min(b.seqs, tokens);
   const int64_t tiles[2] = {
       !ragged ? seqs * ((group + z.rows[0] - 1) / z.rows[0]) : seqs * (kFewRows / z.rows[0]),
       chunks ? tokens * group / z.rows[1] + std::min(seqs, tokens * group / (kFewRows + 1)) : 0};
-  const int64_t least[2] = {kSliceLeast<0>, kSliceLeast<1>}, longest[2] = {kSliceLong<0>, kSliceLong<1>};
   int64_t plan = 0;
   for (int k = 0; k < 2; ++k) {
-    const int64_t most = c.kv_heads * tiles[k] * ((keys + least[k] - 1) / least[k]);
-    // kv_heads * keys / slice, for any lengths (a rounded slice may be short of its length by 2^-20)
-    const int64_t cut = std::max(z.target[k], std::min(4 * z.target[k], c.kv_heads * tiles[k] * keys / longest[k])) * 65 / 64;
-    z.items[k] = std::min(most, cut + c.kv_heads * (tiles[k] + 1));
-    z.slots[k] = keys <= least[k] ? 0 : std::min(most, 2 * (cut + c.kv_heads));
+    z.blocks[k] = tiles[k] * (kTileCost + (keys + kBlockKeys - 1) / kBlockKeys);
+    // for any lengths: no more than `finer` times z.jobs, and than least blocks each leave
+    const int64_t least = k ? kLeast<1> : kLeast<0>, finer = k ? kFiner<1> : kFiner<0>;
+    int64_t f = 1;
+    while (f < finer && z.blocks[k] >= 2 * f * z.jobs[k] * kLong) f *= 2;
+    const int64_t jobs = std::min((z.blocks[k] + least - 1) / least, f * z.jobs[k]);
+    z.groups[k] = jobs * c.kv_heads;
+    z.slots[k] = jobs > 1 ? 2 * z.groups[k] : 0;
     if (z.slots[k]) plan = (b.seqs * (int64_t)sizeof(Plan) + 255) / 256 * 256;
     z.bytes += z.slots[k] * z.rows[k] * (c.row + 2) * 4;
   }
@@ -116,10 +161,9 @@ int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch,
   TS_CHECK_ARG((((uintptr_t)query | (uintptr_t)out) & 15) == 0 && (token_stride | head_stride) % 8 == 0,
                "ts_paged_attention: rows not 16-byte aligned");
   const Sizes z = sizes_of(*cache, *batch, tokens, heads);
-  // 2^24 work-groups of 256 threads wrap a launch; a slice of 2^30 keys has to be enough for `target` of them
-  TS_CHECK_ARG(tokens * heads < (1ll << 24) && std::max(z.items[0], z.items[1]) + tokens / 16 < (1ll << 24) - 1 &&
-                   batch->width * cache->page_size <= kMaxKeys &&
-                   (double)batch->width * cache->page_size * (double)(z.items[0] + z.items[1]) < 1e11,
+  // 2^24 work-groups of 256 threads wrap a launch; blocks are counted in 32 bits
+  TS_CHECK_ARG(tokens * heads < (1ll << 24) && std::max(z.groups[0], z.groups[1]) + tokens / 16 < (1ll << 23) &&
+                   batch->width * cache->page_size <= kMaxKeys && std::max(z.blocks[0], z.blocks[1]) < (1ll << 30),
                "ts_paged_attention: %lld rows of %lld heads over %lld sequences of %lld pages: too large", (long long)tokens,
                (long long)heads, (long long)batch->seqs, (long long)batch->width);
   TS_CHECK_ARG(z.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bytes),
@@ -143,7 +187,7 @@ int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch,
   a.group = (int32_t)(heads / cache->kv_heads);
   a.head_dim = cache->head_dim;
   a.page_shift = shift_of(cache->page_size);
-  a.few_rows = z.items[1] ? kFewRows : 0;
+  a.few_rows = z.groups[1] ? kFewRows : 0;
   char* at = (char*)workspace;
   const bool merges = z.slots[0] || z.slots[1];
   if (merges) {
@@ -151,23 +195,18 @@ int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch,
     at += (batch->seqs * (int64_t)sizeof(Plan) + 255) / 256 * 256;
   }
   for (int k = 0; k < 2; ++k) {
-    a.target[k] = (int32_t)z.target[k];
+    a.jobs[k] = (int32_t)z.jobs[k];
+    a.tile_rows[k] = (int32_t)z.rows[k];
     a.part[k] = (float*)at;
     a.stats[k] = a.part[k] + z.slots[k] * z.rows[k] * cache->row;
     at = (char*)(a.stats[k] + z.slots[k] * z.rows[k] * 2);
   }
   hipStream_t s = (hipStream_t)stream;
   launch_few(a, z, cache->dtype, cache->bits == 16, cache->row, s);
-  if (z.items[1]) launch_chunks(a, z, cache->dtype, cache->bits == 16, cache->row, s);
+  if (z.groups[1]) launch_chunks(a, z, cache->dtype, cache->bits == 16, cache->row, s);
   if (merges) {
-    ts::TimedLaunch timed_("paged.merge_kernel", s);
-    const dim3 grid((unsigned)(tokens * heads)), block(256);
-    switch (cache->row) {
-      case 64: TS_LAUNCH_E_T(cache->dtype, merge_kernel, 64, grid, block, 0, s, a); break;
-      case 128: TS_LAUNCH_E_T(cache->dtype, merge_kernel, 128, grid, block, 0, s, a); break;
-      case 192: TS_LAUNCH_E_T(cache->dtype, merge_kernel, 192, grid, block, 0, s, a); break;
-      default: TS_LAUNCH_E_T(cache->dtype, merge_kernel, 256, grid, block, 0, s, a);
-    }
+    if (cache->dtype == TS_F16) launch_merge<ts::f16>(a, cache->row, s);
+    else launch_merge<ts::bf16>(a, cache->row, s);
   }
   return ts::check_launch("ts_paged_attention");
 }

@@ -1,7 +1,7 @@
 // Attention over a paged cache for sequences with many query rows: chunks of a prompt.
 //
-// A work-group takes one item: 128 query rows of one KV head (its tokens' heads of the group side by side, 16 NQB
-// rows a wave) over a slice of the keys that they see.  Tiles of 32 keys and values go through registers, where
+// A work-group takes one tile after another: 128 query rows of one KV head (its tokens' heads of the group side by side, 16
+// NQB rows a wave) over its part of the keys that they see.  Tiles of 32 keys and values go through registers, where
 // codes become 16-bit values times their scale, once for all waves, into double-buffered swizzled LDS rows, one
 // barrier a tile; the next tile's reads are under way while a tile is computed.  As in the forward of packed attention,
 // S^T = K Q^T with Q^T in registers leaves 8 of a tile's 32 scores of a query row in a lane, which are, rounded, the
@@ -26,32 +26,36 @@ using attn::tr_read;
 
 constexpr int kTileRows = 128, kKeys = 32;
 constexpr float kSlack = 8.f, kSlackSum = 256.f;
-#ifndef TSC_OCC
-#define TSC_OCC 2
-#endif
-#ifndef TSC_OCC64
-#define TSC_OCC64 3
-#endif
 
 template <int ROW> constexpr int kBlocks = ROW <= 192 ? 2 : 1;  // 16-row query blocks a wave
 template <int ROW> constexpr int kChunkWaves = kTileRows / 16 / kBlocks<ROW>;
 
 template <typename T, bool WIDE, int ROW>
-__global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW <= 128 ? TSC_OCC : 2)) void chunk_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kChunkWaves<ROW>, (chunk_occupancy(ROW))) void chunk_kernel(AttnArgs) {
   constexpr int NQB = kBlocks<ROW>, kWaves = kChunkWaves<ROW>, kThreads = 64 * kWaves;
   constexpr int NC = ROW / 32, NB = ROW / 16;
   constexpr int kSize = WIDE ? 2 : 1;
   constexpr int kChunks = kKeys * ROW / 8 / kThreads;  // eight elements each, of a thread and tile
   __shared__ __attribute__((aligned(16))) bf16 s_k[2][kKeys * ROW];
   __shared__ __attribute__((aligned(16))) bf16 s_v[2][kKeys * ROW];
-  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int lane_id = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Item it;
+  __shared__ int s_cur[sizeof(Cursor<1>) / 4];
+  Cursor<1> cur;
+  AttnArgs a = arguments();
   int past;
-  if (!find_item<1>(a, kTileRows, (int)blockIdx.x, lane, it, past)) return;
-  const int first_row = it.tile * kTileRows, len = it.seq.len, base = len - it.seq.n;
-  if (a.plan && threadIdx.x == 0 && it.head == 0 && it.tile == 0 && it.slice == 0)
-    a.plan[it.s] = Plan{it.part, it.slices, kTileRows, 1};
+  if (!cur.begin(a, kTileRows, (int)blockIdx.x, lane_id, past)) return;
+  for (;;) {
+  a = arguments();
+  int lane = lane_id;
+  asm volatile("" : "+v"(lane));  // what follows from it is worked out again a tile, not held over the loop
+  const int g = lane >> 4, r = lane & 15;
+  const int first_row = cur.tile * kTileRows, rows = cur.seq.n * a.group, len = cur.seq.len, base = len - cur.seq.n;
+  cur.put(s_cur);
+  int begin, end;
+  cur.piece(a, begin, end);
+  if (a.plan && threadIdx.x == 0 && cur.head == 0 && cur.tile == 0 && cur.from == 0)
+    a.plan[cur.s] = Plan{cur.job * cur.per + (cur.per - cur.left), cur.blocks, cur.per, 1};
 
   const int wave_row = first_row + 16 * NQB * wave;
   bf16x8 q[NQB][NC];
@@ -59,10 +63,10 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
 #pragma unroll
   for (int t = 0; t < NQB; ++t) {
     const int row = wave_row + 16 * t + r;
-    const int token = row / a.group, head = it.head * a.group + row % a.group;
-    const bool there = row < it.rows;
+    const int token = row / a.group, head = cur.head * a.group + row % a.group;
+    const bool there = row < rows;
     limit[t] = there ? base + token : -1;
-    const char* p = a.query + ((int64_t)(it.seq.row0 + token) * a.token_stride + (int64_t)head * a.head_stride) * 2;
+    const char* p = a.query + ((int64_t)(cur.seq.row0 + token) * a.token_stride + (int64_t)head * a.head_stride) * 2;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       u32x4 v = u32x4{0, 0, 0, 0};
@@ -70,10 +74,9 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
       q[t][c] = as_bf16x8(v);
     }
   }
-  // the least and the greatest of the limits of the wave's rows, and the greatest of all
-  const int low = base + wave_row / a.group;
-  const int high = wave_row < it.rows ? base + min((wave_row + 16 * NQB - 1) / a.group, it.seq.n - 1) : -1;
-  const int stop = min(it.end, base + min((first_row + kTileRows - 1) / a.group, it.seq.n - 1) + 1);
+  // the greatest of the limits of the wave's rows, and of all
+  const int high = wave_row < rows ? base + min((wave_row + 16 * NQB - 1) / a.group, cur.seq.n - 1) : -1;
+  const int stop = min(end, base + min((first_row + kTileRows - 1) / a.group, cur.seq.n - 1) + 1);
 
   f32x4 acc[NB][NQB];
   float m[NQB], l[NQB];
@@ -87,11 +90,11 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
   int ro[kRowOffsets<ROW>], to[2 * kRowOffsets<ROW>];
   swizzled_offsets<ROW>(lane, ro, to);
 
-  const int32_t* table = a.batch.table + (int64_t)it.s * a.batch.ld_table;
+  const int32_t* table = a.batch.table + (int64_t)cur.s * a.batch.ld_table;
   const int page_mask = (1 << a.page_shift) - 1;
   auto page_at = [&](int pos) -> int {
     const int at = pos >> a.page_shift;
-    if (pos >= it.end || at >= a.batch.width) return -1;
+    if (pos >= end || at >= a.batch.width) return -1;
     const int page = uniform_table(table)[at];
     return page >= 0 && page < a.pages ? page : -1;
   };
@@ -111,11 +114,17 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
       rk[u] = rv[u] = Raw{};
       if constexpr (!WIDE) ks[u] = vs[u] = 1.f;
       if (id < 0) continue;
-      const int64_t line = ((int64_t)it.head << a.page_shift) + ((pos + (second ? 16 : 0)) & page_mask);
-      const int at = ((row & 15) * ROW + 8 * c) * kSize;
-      if (pos + row < len) {
-        rk[u] = *(const Raw*)(a.key + id * a.key_page_stride + line * (ROW * kSize) + at);
-        rv[u] = *(const Raw*)(a.value + id * a.value_page_stride + line * (ROW * kSize) + at);
+      const int64_t line = ((int64_t)cur.head << a.page_shift) + ((pos + (second ? 16 : 0)) & page_mask);
+      // rows behind the sequence are past the descriptors' ends, and read as zeros
+      const uint32_t bytes = min(16, len - (pos + (second ? 16 : 0))) * ROW * kSize, at = ((row & 15) * ROW + 8 * c) * kSize;
+      const rsrc_t k = make_rsrc(a.key + id * a.key_page_stride + line * (ROW * kSize), bytes);
+      const rsrc_t v = make_rsrc(a.value + id * a.value_page_stride + line * (ROW * kSize), bytes);
+      if constexpr (WIDE) {
+        rk[u] = __builtin_amdgcn_raw_buffer_load_b128(k, at, 0, 0);
+        rv[u] = __builtin_amdgcn_raw_buffer_load_b128(v, at, 0, 0);
+      } else {
+        rk[u] = __builtin_amdgcn_raw_buffer_load_b64(k, at, 0, 0);
+        rv[u] = __builtin_amdgcn_raw_buffer_load_b64(v, at, 0, 0);
       }
       if constexpr (!WIDE) {
         const int64_t scale = (((int64_t)id * a.kv_heads << a.page_shift) + line) >> 4;
@@ -174,7 +183,7 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
     if (page0 < 0 || page1 < 0) {  // keys of a page that is none
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if ((h ? page1 : page0) < 0 && pos + 16 * h < it.end)
+        if ((h ? page1 : page0) < 0 && pos + 16 * h < end)
 #pragma unroll
           for (int t = 0; t < NQB; ++t) sc[h][t] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
     }
@@ -274,34 +283,47 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
     __builtin_amdgcn_s_setprio(0);
   };
 
-  int pos = it.begin;
-  if (pos < stop) {
+  // Tiles that every row sees whole, each asked for while the one before is computed.
+  const int plain = min(stop, base + first_row / a.group + 1) - (kKeys - 1);  // such tiles begin before it
+  int pos = begin;
+  if (pos < plain) {
     load(pos);
     store(s_k[0], s_v[0]);
   }
   auto turn = [&](auto stage_) __attribute__((always_inline)) {
     constexpr int stage = decltype(stage_)::value;
     const int page0 = page[0], page1 = page[1], next = pos + kKeys;
-    if (next < stop) load(next);
+    if (next < plain) load(next);
     __syncthreads();  // the tile is in, and the other stage has been read
-    if (pos + kKeys - 1 <= low) compute(std::false_type{}, pos, s_k[stage], s_v[stage], page0, page1);
-    else if (pos <= high) compute(std::true_type{}, pos, s_k[stage], s_v[stage], page0, page1);
-    if (next < stop) store(s_k[stage ^ 1], s_v[stage ^ 1]);
+    compute(std::false_type{}, pos, s_k[stage], s_v[stage], page0, page1);
+    if (next < plain) store(s_k[stage ^ 1], s_v[stage ^ 1]);
     pos = next;
   };
-  while (pos < stop) {
+  while (pos < plain) {
     turn(std::integral_constant<int, 0>{});
-    if (pos >= stop) break;
+    if (pos >= plain) break;
     turn(std::integral_constant<int, 1>{});
   }
+  // The few at the diagonal, one by one: the registers are worth more.
+  for (; pos < stop; pos += kKeys) {
+    load(pos);
+    __syncthreads();
+    store(s_k[0], s_v[0]);
+    __syncthreads();
+    if (pos <= high) compute(std::true_type{}, pos, s_k[0], s_v[0], page[0], page[1]);
+  }
 
+  a = arguments();
+  cur.take(s_cur);
+  const bool all = cur.whole();
+  const int slot = cur.slot(a.kv_heads);
 #pragma unroll
   for (int t = 0; t < NQB; ++t) {
     const float sum = rows_sum4(l[t]);
     const int row = wave_row + 16 * t + r;
-    if (row >= it.rows) continue;
-    if (it.slices > 1) {
-      const int64_t at = ((int64_t)it.part * a.kv_heads + it.head) * kTileRows + row - first_row;
+    if (row >= rows) continue;
+    if (!all) {
+      const int64_t at = (int64_t)slot * kTileRows + row - first_row;
       float* o = a.part[1] + at * ROW + 4 * g;
 #pragma unroll
       for (int b = 0; b < NB; ++b) *(f32x4*)(o + 16 * b) = acc[b][t];
@@ -312,8 +334,8 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
       continue;
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    const int token = row / a.group, head = it.head * a.group + row % a.group;
-    char* o = a.out + (((int64_t)(it.seq.row0 + token) * a.heads + head) * a.head_dim + 4 * g) * 2;
+    const int token = row / a.group, head = cur.head * a.group + row % a.group;
+    char* o = a.out + (((int64_t)(cur.seq.row0 + token) * a.heads + head) * a.head_dim + 4 * g) * 2;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
       if (16 * b + 4 * g < a.head_dim) {
@@ -321,12 +343,15 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (ROW <= 64 ? TSC_OCC64 : ROW
         *(u32x2*)(o + 32 * b) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
       }
   }
+  if (!cur.next(a, kTileRows, lane_id)) return;
+  __syncthreads();  // the last keys and the cursor have been read
+  }
 }
 
 template <typename T, bool WIDE, int ROW>
 void launch_chunk_rows(const AttnArgs& a, const Sizes& z, hipStream_t s) {
   ts::TimedLaunch timed_("paged.chunk_kernel", s);
-  hipLaunchKernelGGL((chunk_kernel<T, WIDE, ROW>), dim3((unsigned)z.items[1]), dim3(64 * kChunkWaves<ROW>), 0, s, a);
+  hipLaunchKernelGGL((chunk_kernel<T, WIDE, ROW>), dim3((unsigned)z.groups[1]), dim3(64 * kChunkWaves<ROW>), 0, s, a);
 }
 
 template <typename T, bool WIDE>

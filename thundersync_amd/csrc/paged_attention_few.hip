@@ -1,9 +1,9 @@
 // Attention over a paged cache for sequences with few query rows: one token each, or a few.
 //
-// A work-group takes one item: up to 16 R query rows of one KV head (its tokens' heads of the group side by side, so
-// that keys and values are read once for all of them) over a slice of the keys.  Its four waves take 32-key steps in
-// turn, each with a running reference point, sum and accumulators of its own, and join them at the end; an item that is not
-// its sequence's only slice leaves partial rows for merge_kernel.
+// A work-group takes one tile after another: up to 16 R query rows of one KV head (its tokens' heads of the group side by
+// side, so that keys and values are read once for all of them) over its part of the keys.  Its four waves take 32-key steps in
+// turn, each with a running reference point, sum and accumulators of its own, and join them at the end; a tile that is not
+// all its own leaves partial rows for merge_kernel.
 //
 // A step of a wave:  S^T = K Q^T (16x16x32, keys as rows), so a lane holds 8 of the 32 scores of one query row, which
 // are, rounded, already the operand of O^T += V^T P^T: lane (g, r) has keys 4 g + i of both halves of query row r.  V^T
@@ -22,16 +22,30 @@ constexpr int kWaves = 4;
 constexpr float kSlack = 8.f;      // log2 units by which scores may pass the reference point before it moves
 constexpr float kSlackSum = 256.f;
 
-// N bytes at a multiple of four
+// N bytes of a lane, at a multiple of four from the descriptor's base and `more`, a constant.  Reads go through a descriptor of the 16 tokens: a
+// lane's place in them is one register for all of a kernel, where a pointer is two more for each read.
 template <int N> struct Words {
   uint32_t w[N / 4];
 };
-template <int N> __device__ __forceinline__ Words<N> load_words(const char* p) {
-  struct __attribute__((packed, aligned(4))) At { uint32_t w[N / 4]; };
-  const At x = *(const At*)p;
+template <int N> __device__ __forceinline__ Words<N> load_words(rsrc_t r, uint32_t at, int more) {
   Words<N> y;
+  if constexpr (N == 4) {
+    y.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, more, 0);
+  } else if constexpr (N == 8) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, at, more, 0);
+    __builtin_memcpy(y.w, &v, 8);
+  } else if constexpr (N == 12) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b96(r, at, more, 0);
+    __builtin_memcpy(y.w, &v, 12);
+  } else {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, at, more, 0);
+    __builtin_memcpy(y.w, &v, 16);
+    if constexpr (N > 16) {
+      const Words<N - 16> z = load_words<N - 16>(r, at, more + 16);
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) y.w[i] = x.w[i];
+      for (int i = 0; i < (N - 16) / 4; ++i) y.w[4 + i] = z.w[i];
+    }
+  }
   return y;
 }
 
@@ -43,16 +57,8 @@ template <bool WIDE, int ROW> struct Tile {
   Words<ROW / 16 * kSize> v[4];
 };
 
-// waves a SIMD: a step's loads and the accumulators are 3 ROW / 8 registers, of 16 bits 5 ROW / 8
-template <bool WIDE, int ROW, int R>
-constexpr int few_occupancy() {
-  if (ROW * R <= 64) return 4;
-  if (WIDE) return ROW * R <= 128 ? 3 : 2;
-  return ROW * R <= 128 ? 4 : ROW * R <= 192 ? 3 : 2;
-}
-
 template <typename T, bool WIDE, int ROW, int R>
-__global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void few_kernel(AttnArgs) {
   constexpr int NC = ROW / 32;  // k-steps of S
   constexpr int NB = ROW / 16;  // elements of a value that a lane reads, and tiles of O
   constexpr int kSize = WIDE ? 2 : 1;
@@ -63,11 +69,13 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
   Part* const s_part = (Part*)s_space;     // at the end
   Query* const s_query = (Query*)s_space;  // until then
   __shared__ float s_stat[kWaves][16 * R][2];
-  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int lane_id = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Item it;
+  __shared__ int s_at[sizeof(Cursor<0>) / 4];
+  Cursor<0> at;
+  AttnArgs a = arguments();
   int past = 0;
-  if (!find_item<0>(a, 16 * R, (int)blockIdx.x, lane, it, past)) {
+  if (!at.begin(a, 16 * R, (int)blockIdx.x, lane_id, past)) {
     // rows behind the last sequence: 16 a work-group, zeros
     if (a.batch.offsets) {
       const int from = max(0, a.batch.offsets[a.batch.seqs]) + 16 * past;
@@ -78,10 +86,19 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
     }
     return;
   }
-  const int first_row = it.tile * 16 * R;
-  const int len = it.seq.len, base = len - it.seq.n;  // position of the first new token
-  if (a.plan && threadIdx.x == 0 && it.head == 0 && it.tile == 0 && it.slice == 0)
-    a.plan[it.s] = Plan{it.part, it.slices, 16 * R, 0};
+  for (;;) {
+  a = arguments();
+  int lane = lane_id;
+  asm volatile("" : "+v"(lane));  // what follows from it is worked out again a tile, not held over the loop
+  const int g = lane >> 4, r = lane & 15;
+  const int first_row = at.tile * 16 * R;
+  const int rows = at.seq.n * a.group;
+  const int len = at.seq.len, base = len - at.seq.n;  // position of the first new token
+  at.put(s_at);
+  int begin, end;
+  at.piece(a, begin, end);
+  if (a.plan && threadIdx.x == 0 && at.head == 0 && at.tile == 0 && at.from == 0)
+    a.plan[at.s] = Plan{at.job * at.per + (at.per - at.left), at.blocks, at.per, 0};
 
   // Query rows as B operands: element 16 g + 8 (c & 1) of the 64 of c / 2 for codes, 32 c + 8 g in 16 bits, as the
   // keys' elements lie in a lane's reads; the last key that each row sees.  The operands are the same in
@@ -90,10 +107,10 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
 #pragma unroll
   for (int t = 0; t < R; ++t) {
     const int row = first_row + 16 * t + r;
-    const int token = row / a.group, head = it.head * a.group + row % a.group;
-    const bool there = row < it.rows;
+    const int token = row / a.group, head = at.head * a.group + row % a.group;
+    const bool there = row < rows;
     limit[t] = there ? base + token : -1;
-    const char* p = a.query + ((int64_t)(it.seq.row0 + token) * a.token_stride + (int64_t)head * a.head_stride) * 2;
+    const char* p = a.query + ((int64_t)(at.seq.row0 + token) * a.token_stride + (int64_t)head * a.head_stride) * 2;
     for (int c = wave; c < NC; c += kWaves) {
       const int d = WIDE ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c & 1);
       u32x4 v = u32x4{0, 0, 0, 0};
@@ -101,7 +118,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
       s_query[t][c][lane] = v;
     }
   }
-  const int low = max(-1, base + min(first_row / a.group, it.seq.n - 1));  // the least of the rows' limits
+  const int low = max(-1, base + min(first_row / a.group, at.seq.n - 1));  // the least of the rows' limits
 
   f32x4 acc[R][NB];
   float m[R], l[R];
@@ -113,12 +130,12 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
     for (int b = 0; b < NB; ++b) acc[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int32_t* table = a.batch.table + (int64_t)it.s * a.batch.ld_table;
+  const int32_t* table = a.batch.table + (int64_t)at.s * a.batch.ld_table;
   const int page_mask = (1 << a.page_shift) - 1;
   auto page_at = [&](int pos) -> int {  // of a 16-token tile; wave-uniform
-    const int at = pos >> a.page_shift;
-    if (pos >= it.end || at >= a.batch.width) return -1;
-    const int page = uniform_table(table)[at];
+    const int nth = pos >> a.page_shift;
+    if (pos >= end || nth >= a.batch.width) return -1;
+    const int page = uniform_table(table)[nth];
     return page >= 0 && page < a.pages ? page : -1;
   };
   // A page that is none is read as page 0, and its scores and values are not used.
@@ -127,38 +144,49 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
   int page0 = -1, page1 = -1;
   const uint32_t key_lane = (r * ROW + (WIDE ? 8 : 16) * g) * kSize;
   const uint32_t value_lane = (4 * g * ROW + NB * r) * kSize;
-  auto line_of = [&](int at) -> int64_t { return ((int64_t)it.head << a.page_shift) + (at & page_mask); };
-  auto load_tile_keys = [&](int at, int page, u32x4 (&k)[Tile<WIDE, ROW>::kLoads], float& key_scale, float& value_scale)
+  auto line_of = [&](int pos) -> int64_t { return ((int64_t)at.head << a.page_shift) + (pos & page_mask); };
+  auto load_tile_keys = [&](int pos, int page, u32x4 (&k)[Tile<WIDE, ROW>::kLoads], float& key_scale, float& value_scale)
                             __attribute__((always_inline)) {
     const int id = max(page, 0);
-    const char* p = a.key + id * a.key_page_stride + line_of(at) * (ROW * kSize);
+    const rsrc_t p = make_rsrc(a.key + id * a.key_page_stride + line_of(pos) * (ROW * kSize), 16 * ROW * kSize);
 #pragma unroll
-    for (int i = 0; i < Tile<WIDE, ROW>::kLoads; ++i) k[i] = *(const u32x4*)(p + key_lane + 64 * i);
+    for (int i = 0; i < Tile<WIDE, ROW>::kLoads; ++i) {
+      const Words<16> x = load_words<16>(p, key_lane, 64 * i);
+      k[i] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+    }
     if constexpr (!WIDE) {
-      const int64_t scale = (((int64_t)id * a.kv_heads << a.page_shift) + line_of(at)) >> 4;
+      const int64_t scale = (((int64_t)id * a.kv_heads << a.page_shift) + line_of(pos)) >> 4;
       key_scale = uniform_table(a.key_scale)[scale];
       value_scale = uniform_table(a.value_scale)[scale];
     }
   };
-  auto load_keys = [&](int at) __attribute__((always_inline)) {
-    page0 = page_at(at);
-    page1 = page_at(at + 16);
-    load_tile_keys(at, page0, tile[0].k, ks0, vs0);
-    load_tile_keys(at + 16, page1, tile[1].k, ks1, vs1);
+  int ahead0 = -1, ahead1 = -1;  // page ids of the step after, so that reads of keys wait for none
+  auto look = [&](int pos) __attribute__((always_inline)) {
+    ahead0 = page_at(pos);
+    ahead1 = page_at(pos + 16);
   };
-  auto load_values = [&](int at) __attribute__((always_inline)) {
+  auto load_keys = [&](int pos) __attribute__((always_inline)) {
+    page0 = ahead0;
+    page1 = ahead1;
+    load_tile_keys(pos, page0, tile[0].k, ks0, vs0);
+    load_tile_keys(pos + 16, page1, tile[1].k, ks1, vs1);
+  };
+  auto load_values = [&](int pos) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const char* p = a.value + max(h ? page1 : page0, 0) * a.value_page_stride + line_of(at + 16 * h) * (ROW * kSize);
+      const rsrc_t p = make_rsrc(a.value + max(h ? page1 : page0, 0) * a.value_page_stride +
+                                     line_of(pos + 16 * h) * (ROW * kSize), 16 * ROW * kSize);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tile[h].v[i] = load_words<NB * kSize>(p + value_lane + i * ROW * kSize);
+      for (int i = 0; i < 4; ++i) tile[h].v[i] = load_words<NB * kSize>(p, value_lane, i * ROW * kSize);
     }
   };
 
-  int pos = __builtin_amdgcn_readfirstlane(it.begin + 32 * wave);
-  const int whole = min(it.end, low + 1) - 31;  // steps before it are seen whole by every row
+  int pos = __builtin_amdgcn_readfirstlane(begin + 32 * wave);
+  const int whole = min(end, low + 1) - 31;  // steps before it are seen whole by every row
+  look(pos);
   if (pos < whole) {
     load_keys(pos);
+    look(pos + 32 * kWaves);
     load_values(pos);
   }
   __syncthreads();
@@ -166,12 +194,13 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
   auto step = [&](auto edge_) __attribute__((always_inline)) {
     constexpr bool edge = decltype(edge_)::value;
     if constexpr (edge) {  // few, and nothing is asked for ahead of them: the registers are worth more
+      look(pos);
       load_keys(pos);
       load_values(pos);
     }
     asm volatile("" ::: "memory");  // the query's operands are read again, not held over the loop
     f32x4 sc[R][2];
-    const bool ruined0 = page0 < 0 && pos < it.end, ruined1 = page1 < 0 && pos + 16 < it.end;
+    const bool ruined0 = page0 < 0 && pos < end, ruined1 = page1 < 0 && pos + 16 < end;
     const float vscale0 = vs0, vscale1 = vs1;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -196,7 +225,10 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
       for (int t = 0; t < R; ++t) sc[t][h] *= a.scale;
     }
     const int next = pos + 32 * kWaves;
-    if (!edge && next < whole) load_keys(next);
+    if (!edge && next < whole) {
+      load_keys(next);
+      look(next + 32 * kWaves);
+    }
 
     if (ruined0 | ruined1) {  // keys of a page that is none
 #pragma unroll
@@ -276,7 +308,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
         }
       return f;
     };
-    if (!edge || it.seq.n == 1) {
+    if (!edge || at.seq.n == 1) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const bf16x8 v = as_bf16x8(value(b));
@@ -291,8 +323,8 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
       for (int t = 0; t < R; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int at = pos + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
-          seen[t][j] = (at <= limit[t] ? kOneOf<T> : 0u) | (at + 1 <= limit[t] ? kOneOf<T> << 16 : 0u);
+          const int key = pos + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
+          seen[t][j] = (key <= limit[t] ? kOneOf<T> : 0u) | (key + 1 <= limit[t] ? kOneOf<T> << 16 : 0u);
         }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
@@ -320,9 +352,10 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
     pos = next;
   };
   while (pos < whole) step(std::false_type{});
-  while (pos < it.end) step(std::true_type{});
+  while (pos < end) step(std::true_type{});
   __syncthreads();  // the query's operands have been read
 
+  a = arguments();
   // The waves' sums by one reference point: 2 and 3 into 0 and 1, 1 into 0.
 #pragma unroll
   for (int t = 0; t < R; ++t) {
@@ -376,15 +409,19 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
   __syncthreads();
   if (wave == 1) put(0);
   __syncthreads();
-  if (wave != 0) return;
+  at.take(s_at);
+  if (wave == 0) {
   add(0);
+  const bool all = at.whole();
+  const int slot = at.slot(a.kv_heads);
+  const int first_row = at.tile * 16 * R, rows = at.seq.n * a.group;
 #pragma unroll
   for (int t = 0; t < R; ++t) {
     const int row = first_row + 16 * t + r;
-    if (row >= it.rows) continue;
-    if (it.slices > 1) {
-      const int64_t at = ((int64_t)it.part * a.kv_heads + it.head) * (16 * R) + 16 * t + r;
-      float* o = a.part[0] + at * ROW;
+    if (row >= rows) continue;
+    if (!all) {
+      const int64_t to = (int64_t)slot * (16 * R) + 16 * t + r;
+      float* o = a.part[0] + to * ROW;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -392,14 +429,14 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
           *(f32x4*)(o + NB * (4 * g + i) + b) =
               f32x4{acc[t][b][i], acc[t][b + 1][i], acc[t][b + 2][i], acc[t][b + 3][i]};
       if (g == 0) {
-        a.stats[0][2 * at] = ref[t];
-        a.stats[0][2 * at + 1] = sum[t];
+        a.stats[0][2 * to] = ref[t];
+        a.stats[0][2 * to + 1] = sum[t];
       }
       continue;
     }
     const float inv = sum[t] > 0.f ? 1.f / sum[t] : 0.f;
-    const int token = row / a.group, head = it.head * a.group + row % a.group;
-    char* o = a.out + (((int64_t)(it.seq.row0 + token) * a.heads + head) * a.head_dim) * 2;
+    const int token = row / a.group, head = at.head * a.group + row % a.group;
+    char* o = a.out + (((int64_t)(at.seq.row0 + token) * a.heads + head) * a.head_dim) * 2;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -410,11 +447,15 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy<WIDE, ROW, R>())) void 
                                        pack2<T>(acc[t][b + 2][i] * inv, acc[t][b + 3][i] * inv)};
       }
   }
+  }
+  if (!at.next(a, 16 * R, lane_id)) return;
+  __syncthreads();  // the next tile's operands go where the sums were
+  }
 }
 
 template <typename T, bool WIDE, int ROW>
 void launch_few_rows(const AttnArgs& a, const Sizes& z, hipStream_t s) {
-  const dim3 grid((unsigned)(z.items[0] + (a.batch.offsets ? (a.batch.tokens + 15) / 16 : 0))), block(64 * kWaves);
+  const dim3 grid((unsigned)(z.groups[0] + (a.batch.offsets ? (a.batch.tokens + 15) / 16 : 0))), block(64 * kWaves);
   ts::TimedLaunch timed_("paged.few_kernel", s);
   if (z.rows[0] == 16) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 1>), grid, block, 0, s, a);
   else if constexpr (ROW <= 128) hipLaunchKernelGGL((few_kernel<T, WIDE, ROW, 2>), grid, block, 0, s, a);
