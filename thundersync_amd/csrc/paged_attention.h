@@ -82,7 +82,7 @@ __device__ __forceinline__ AttnArgs arguments() {
 //
 // Lengths are known on the device alone: every wave works the plan out itself, 64 sequences at a time.
 constexpr int kBlockKeys = 128, kTileCost = 1;
-template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 3 : 5;
+template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 2 : 4;
 constexpr int kLong = 16;
 template <int KERNEL> constexpr int kFiner = KERNEL == 0 ? 4 : 2;  // a partial tile of the chunk kernel is 64 KB and more
 

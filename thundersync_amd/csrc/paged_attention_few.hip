@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   constexpr int kSize = WIDE ? 2 : 1;
   using Part = float[16 * R][ROW + 4];
   using Query = u32x4[NC][64];
-  constexpr int kBytes = 2 * sizeof(Part) > R * sizeof(Query) ? 2 * sizeof(Part) : R * sizeof(Query);
+  constexpr int kBytes = kWaves * sizeof(Part) > R * sizeof(Query) ? kWaves * sizeof(Part) : R * sizeof(Query);
   __shared__ __attribute__((aligned(16))) char s_space[kBytes];
   Part* const s_part = (Part*)s_space;     // at the end
   Query* const s_query = (Query*)s_space;  // until then
@@ -104,6 +104,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   // keys' elements lie in a lane's reads; the last key that each row sees.  The operands are the same in
   // every wave and stay in LDS: their registers are worth more to loads in flight.
   int limit[R];
+  u32x4 query[R][(NC + kWaves - 1) / kWaves];
 #pragma unroll
   for (int t = 0; t < R; ++t) {
     const int row = first_row + 16 * t + r;
@@ -111,11 +112,11 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
     const bool there = row < rows;
     limit[t] = there ? base + token : -1;
     const char* p = a.query + ((int64_t)(at.seq.row0 + token) * a.token_stride + (int64_t)head * a.head_stride) * 2;
-    for (int c = wave; c < NC; c += kWaves) {
-      const int d = WIDE ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c & 1);
-      u32x4 v = u32x4{0, 0, 0, 0};
-      if (there && d < a.head_dim) v = *(const u32x4*)(p + 2 * d);
-      s_query[t][c][lane] = v;
+#pragma unroll
+    for (int k = 0; k < (NC + kWaves - 1) / kWaves; ++k) {
+      const int c = wave + kWaves * k, d = WIDE ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c & 1);
+      query[t][k] = u32x4{0, 0, 0, 0};
+      if (there && d < a.head_dim) query[t][k] = *(const u32x4*)(p + 2 * d);
     }
   }
   const int low = max(-1, base + min(first_row / a.group, at.seq.n - 1));  // the least of the rows' limits
@@ -194,6 +195,11 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
     ahead0 = read_near(after(pos));
     ahead1 = read_near(after(pos) + 16);
   }
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int k = 0; k < (NC + kWaves - 1) / kWaves; ++k)
+      if (wave + kWaves * k < NC) s_query[t][wave + kWaves * k][lane] = query[t][k];
   __syncthreads();
   // One step; `edge`: some row does not see some of its keys, or they are not there.
   auto step = [&](auto edge_) __attribute__((always_inline)) {
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   __syncthreads();  // the query's operands have been read
 
   a = arguments();
-  // The waves' sums by one reference point: 2 and 3 into 0 and 1, 1 into 0.
+  // The waves' sums by one reference point: through LDS, and added there in the waves' order, a row in 16 threads.
 #pragma unroll
   for (int t = 0; t < R; ++t) {
     l[t] = rows_sum4(l[t]);
@@ -373,88 +379,55 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
       s_stat[wave][16 * t + r][0] = m[t];
       s_stat[wave][16 * t + r][1] = l[t];
     }
-  }
-  __syncthreads();
-  float ref[R], sum[R];
-#pragma unroll
-  for (int t = 0; t < R; ++t) {
-    float most = neg_inf();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_stat[w][16 * t + r][0]);
-    ref[t] = most;
-    const float by = most == neg_inf() ? 0.f : most;
-    sum[t] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum[t] += s_stat[w][16 * t + r][1] * fast_exp2(s_stat[w][16 * t + r][0] - by);
-    const float f = fast_exp2(m[t] - by);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[t][b] *= f;
-  }
-  auto put = [&](int to) {
-#pragma unroll
-    for (int t = 0; t < R; ++t)
+    if (first_row + 16 * t + r < rows)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int b = 0; b < NB; b += 4)
-          *(f32x4*)&s_part[to][16 * t + r][NB * (4 * g + i) + b] =
+          *(f32x4*)&s_part[wave][16 * t + r][NB * (4 * g + i) + b] =
               f32x4{acc[t][b][i], acc[t][b + 1][i], acc[t][b + 2][i], acc[t][b + 3][i]};
-  };
-  auto add = [&](int from) {
-#pragma unroll
-    for (int t = 0; t < R; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int b = 0; b < NB; b += 4) {
-          const f32x4 x = *(const f32x4*)&s_part[from][16 * t + r][NB * (4 * g + i) + b];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[t][b + j][i] += x[j];
-        }
-  };
-  if (wave >= 2) put(wave - 2);
-  __syncthreads();
-  if (wave < 2) add(wave);
-  __syncthreads();
-  if (wave == 1) put(0);
+  }
   __syncthreads();
   at.take(s_at);
-  if (wave == 0) {
-  add(0);
+  {
   const bool all = at.whole();
   const int slot = at.slot(a.kv_heads);
-  const int first_row = at.tile * 16 * R, rows = at.seq.n * a.group;
+  const int first_row = at.tile * 16 * R, here = min(16 * R, at.seq.n * a.group - first_row);
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  for (int in = tid >> 4; in < here; in += 4 * kWaves) {
+    float most = neg_inf();
 #pragma unroll
-  for (int t = 0; t < R; ++t) {
-    const int row = first_row + 16 * t + r;
-    if (row >= rows) continue;
-    if (!all) {
-      const int64_t to = (int64_t)slot * (16 * R) + 16 * t + r;
-      float* o = a.part[0] + to * ROW;
+    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_stat[w][in][0]);
+    const float by = most == neg_inf() ? 0.f : most;
+    float f[kWaves], sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int b = 0; b < NB; b += 4)
-          *(f32x4*)(o + NB * (4 * g + i) + b) =
-              f32x4{acc[t][b][i], acc[t][b + 1][i], acc[t][b + 2][i], acc[t][b + 3][i]};
-      if (g == 0) {
-        a.stats[0][2 * to] = ref[t];
-        a.stats[0][2 * to + 1] = sum[t];
-      }
-      continue;
+    for (int w = 0; w < kWaves; ++w) {
+      f[w] = fast_exp2(s_stat[w][in][0] - by);
+      sum = fmaf(s_stat[w][in][1], f[w], sum);
     }
-    const float inv = sum[t] > 0.f ? 1.f / sum[t] : 0.f;
-    const int token = row / a.group, head = at.head * a.group + row % a.group;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const int row = first_row + in, token = row / a.group, head = at.head * a.group + row % a.group;
     char* o = a.out + (((int64_t)(at.seq.row0 + token) * a.heads + head) * a.head_dim) * 2;
+    const int64_t to = (int64_t)slot * (16 * R) + in;
+    float* part = a.part[0] + to * ROW;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int k = 0; k < ROW / 64; ++k) {
+      const int d = 64 * k + 4 * (tid & 15);
+      f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int b = 0; b < NB; b += 4) {
-        const int d = NB * (4 * g + i) + b;
-        if (d < a.head_dim)
-          *(u32x2*)(o + 2 * d) = u32x2{pack2<T>(acc[t][b][i] * inv, acc[t][b + 1][i] * inv),
-                                       pack2<T>(acc[t][b + 2][i] * inv, acc[t][b + 3][i] * inv)};
+      for (int w = 0; w < kWaves; ++w) {
+        const f32x4 y = *(const f32x4*)&s_part[w][in][d];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fmaf(y[i], f[w], x[i]);
       }
+      if (!all) *(f32x4*)(part + d) = x;
+      else if (d < a.head_dim) *(u32x2*)(o + 2 * d) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
+    }
+    if (!all && (tid & 15) == 0) {
+      a.stats[0][2 * to] = most;
+      a.stats[0][2 * to + 1] = sum;
+    }
   }
   }
   if (!at.next(a, 16 * R, lane_id)) return;
