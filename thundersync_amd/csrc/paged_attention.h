@@ -33,6 +33,7 @@ struct AttnArgs {
   int32_t few_rows;   // sequences of more query rows (tokens x group) are the chunk kernel's; 0: none are
   int32_t jobs[2];    // work-groups of each KV head that a kernel's work is dealt to, at least
   int32_t tile_rows[2];
+  int64_t slots[2];
   Plan* plan;         // [seqs], or null where no tile can be cut
   float* part[2];     // of each kernel: [slots][rows][row] unnormalised sums
   float* stats[2];    // [slots][rows][2]: reference point (log2 units) and sum
@@ -83,7 +84,7 @@ __device__ __forceinline__ AttnArgs arguments() {
 // Lengths are known on the device alone: every wave works the plan out itself, 64 sequences at a time.
 constexpr int kBlockKeys = 128, kTileCost = 1;
 template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 2 : 4;
-constexpr int kLong = 16;
+constexpr int kLong = 8;
 template <int KERNEL> constexpr int kFiner = KERNEL == 0 ? 4 : 2;  // a partial tile of the chunk kernel is 64 KB and more
 
 // waves a SIMD: a step's loads and the accumulators are 3 ROW / 8 registers, of 16 bits 5 ROW / 8
@@ -122,6 +123,14 @@ __host__ __device__ inline int64_t blocks_each(int64_t total, int64_t jobs, int 
   return each > least ? each : least;
 }
 
+// A border less than kSnap blocks inside a tile moves to the nearer end of it: a tile that is cut costs a start, an end
+// and a partial tile more.
+constexpr int kSnap = 4;
+__device__ __forceinline__ int snapped(int border, int in_tile, int blocks) {
+  if (2 * in_tile <= blocks) return in_tile < kSnap ? border - in_tile : border;
+  return blocks - in_tile < kSnap ? border + blocks - in_tile : border;
+}
+
 // A work-group's place in its kernel's work.  Everything is read from one lane, so that it is uniform to the compiler
 // too and pages are looked up by scalar loads.
 template <int KERNEL> struct Cursor {
@@ -130,6 +139,7 @@ template <int KERNEL> struct Cursor {
   int from;                    // block of the tile
   int left;                    // blocks of the work-group
   int per, job, head;
+  int end;                     // of the work-group's blocks
 
   // false if the work-group has none; `past` is then by how many it is past the last that has
   __device__ __forceinline__ bool begin(const AttnArgs& a, int tile_rows, int id, int lane, int& past) {
@@ -156,24 +166,45 @@ template <int KERNEL> struct Cursor {
     const int used = (total + per - 1) / per;
     past = id - used * a.kv_heads;
     if (job >= used) return false;
-    const int start = job * per;
-    left = min(per, total - start);
-    int before = 0;
+    const int borders[2] = {job * per, min((job + 1) * per, total)};
+    int start = 0, stop = borders[1] == total ? total : 0, before = 0;
+    bool found = false;
     for (int s0 = 0; s0 < b.seqs; s0 += 64) {
       if (s0 > 0) read(s0);
       const int upto = wave_prefix(count, lane) + before;
       const int all = __builtin_amdgcn_readlane(upto, 63);
-      if (start < all) {
-        const int at = __ffsll((unsigned long long)__ballot(upto > start)) - 1;
-        const int in = start - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(count, at));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int border = borders[k];
+        if (border < before || border >= all) continue;
+        const int at = __ffsll((unsigned long long)__ballot(upto > border)) - 1;
+        const int size = __builtin_amdgcn_readlane(blocks_of(a, q), at);
+        const int in = border - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(count, at));
+        const int x = in - in / size * size, to = snapped(border, x, size);
+        if (k == 1) {
+          stop = to;
+          continue;
+        }
+        start = to;
         enter(a, tile_rows, s0, at, q);
         tile = in / blocks;
-        from = in - tile * blocks;
-        return true;
+        from = x + to - border;
+        found = true;
       }
+      if (found && stop > 0) break;
       before = all;
     }
-    return false;
+    end = stop;
+    left = stop - start;
+    if (!found || left <= 0) {
+      past = -1;  // nothing, but rows behind the last sequence are others'
+      return false;
+    }
+    if (from == blocks) {
+      from = 0;
+      if (++tile >= tiles && !skip(a, tile_rows, lane)) return false;
+    }
+    return true;
   }
   // Kept in LDS while a tile is computed, where scalar registers are short.
   __device__ __forceinline__ void put(int* to) const {
@@ -209,7 +240,10 @@ template <int KERNEL> struct Cursor {
     left -= min(blocks, from + left) - from;
     if (left <= 0) return false;
     from = 0;
-    if (++tile < tiles) return true;
+    return ++tile < tiles || skip(a, tile_rows, lane);
+  }
+  // To the next sequence that has tiles.
+  __device__ __forceinline__ bool skip(const AttnArgs& a, int tile_rows, int lane) {
     for (int s0 = s + 1; s0 < a.batch.seqs; s0 += 64) {
       Seq q{0, 0, 0};
       if (s0 + lane < a.batch.seqs) q = seq_of(a.batch, s0 + lane);

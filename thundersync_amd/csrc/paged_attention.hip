@@ -27,14 +27,21 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void merge_kernel(At
   mine = mine && t >= q.row0 && t < q.row0 + q.n;
   Plan plan{0, 1, 1, 0};
   if (mine) plan = a.plan[s];
+  // a plan that no work-group wrote (lengths or offsets changed under the call) reads nothing out of the workspace
+  mine = mine && plan.per > 0 && plan.blocks > 0 && plan.start >= 0 && (plan.kernel & ~1) == 0;
+  if (!mine) plan = Plan{0, 1, 1, 0};
   const int rows = a.tile_rows[plan.kernel];
   const int head = h / a.group, row = (t - q.row0) * a.group + h % a.group, tile = row / rows;
-  const int first = plan.start + tile * plan.blocks, job = first / plan.per;
-  const int parts = mine ? (first + plan.blocks - 1) / plan.per - job + 1 : 1;  // 1: written already
+  // the work-group that begins the tile: the last whose border lies before it or has moved to its start; those that begin
+  // inside, from `inner` on: their borders have not moved
+  const int first = plan.start + tile * plan.blocks, last = first + plan.blocks;
+  const int owner = (first + min(kSnap - 1, plan.blocks / 2)) / plan.per;
+  const int inner = (first + kSnap + plan.per - 1) / plan.per;
+  int parts = mine ? 1 + max(0, (last - kSnap) / plan.per - inner + 1) : 1;  // 1: written already
+  if (((int64_t)max(owner, inner + parts - 2) + 1) * 2 * a.kv_heads > a.slots[plan.kernel]) parts = 1;
   const float *part = a.part[plan.kernel], *stats = a.stats[plan.kernel];
-  // part 0 is slot 2 job + 1, part p > 0 slot 2 (job + p)
   auto place = [&](int p) -> int64_t {
-    return ((int64_t)(2 * (job + p) + (p == 0)) * a.kv_heads + head) * rows + row % rows;
+    return ((int64_t)(p == 0 ? 2 * owner + 1 : 2 * (inner + p - 1)) * a.kv_heads + head) * rows + row % rows;
   };
   float acc[N], sum = 0.f;
 #pragma unroll
@@ -197,6 +204,7 @@ int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch,
   for (int k = 0; k < 2; ++k) {
     a.jobs[k] = (int32_t)z.jobs[k];
     a.tile_rows[k] = (int32_t)z.rows[k];
+    a.slots[k] = z.slots[k];
     a.part[k] = (float*)at;
     a.stats[k] = a.part[k] + z.slots[k] * z.rows[k] * cache->row;
     at = (char*)(a.stats[k] + z.slots[k] * z.rows[k] * 2);

@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (chunk_occupancy(ROW))) void
   int begin, end;
   cur.piece(a, begin, end);
   if (a.plan && threadIdx.x == 0 && cur.head == 0 && cur.tile == 0 && cur.from == 0)
-    a.plan[cur.s] = Plan{cur.job * cur.per + (cur.per - cur.left), cur.blocks, cur.per, 1};
+    a.plan[cur.s] = Plan{cur.end - cur.left, cur.blocks, cur.per, 1};
 
   const int wave_row = first_row + 16 * NQB * wave;
   bf16x8 q[NQB][NC];

@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   int past = 0;
   if (!at.begin(a, 16 * R, (int)blockIdx.x, lane_id, past)) {
     // rows behind the last sequence: 16 a work-group, zeros
-    if (a.batch.offsets) {
+    if (a.batch.offsets && past >= 0) {
       const int from = max(0, a.batch.offsets[a.batch.seqs]) + 16 * past;
       const int row_bytes = a.heads * a.head_dim * 2;
       for (int t = from; t < min(from + 16, a.batch.tokens); ++t)
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   int begin, end;
   at.piece(a, begin, end);
   if (a.plan && threadIdx.x == 0 && at.head == 0 && at.tile == 0 && at.from == 0)
-    a.plan[at.s] = Plan{at.job * at.per + (at.per - at.left), at.blocks, at.per, 0};
+    a.plan[at.s] = Plan{at.end - at.left, at.blocks, at.per, 0};
 
   // Query rows as B operands: element 16 g + 8 (c & 1) of the 64 of c / 2 for codes, 32 c + 8 g in 16 bits, as the
   // keys' elements lie in a lane's reads; the last key that each row sees.  The operands are the same in
