@@ -81,7 +81,7 @@ __device__ __forceinline__ AttnArgs arguments() {
 // kLong blocks, so that a slow one costs less, and fewer where they would get less than kLeast.  64 sequences of 100 to 6000
 // keys, 24/4 heads of 256: 100 us in slices of equal length a sequence, 88 dealt like this.
 //
-// Lengths are known on the device alone: every wave works the plan out itself, 64 sequences at a time.
+// Lengths are known on the device alone: every work-group works its part out itself, 64 sequences at a time.
 constexpr int kBlockKeys = 128, kTileCost = 1;
 template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 2 : 4;
 constexpr int kLong = 8;
@@ -108,7 +108,7 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, const Seq& q) {
   return (int)min((int64_t)q.len, ((int64_t)a.batch.width << a.page_shift) + 16);
 }
 __device__ __forceinline__ int blocks_of(const AttnArgs& a, const Seq& q) {
-  return kTileCost + (keys_of(a, q) + kBlockKeys - 1) / kBlockKeys;
+  return kTileCost + (int)((uint32_t)(keys_of(a, q) + kBlockKeys - 1) / kBlockKeys);
 }
 template <int KERNEL>
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& q, int tile_rows) {
@@ -116,11 +116,10 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& q, int til
   const bool many = a.few_rows > 0 && rows > a.few_rows;
   return many == (KERNEL == 1) ? (int)((rows + tile_rows - 1) / tile_rows) : 0;
 }
-__host__ __device__ inline int64_t blocks_each(int64_t total, int64_t jobs, int least, int finer) {
+__device__ __forceinline__ int blocks_each(int total, int jobs, int least, int finer) {
   int f = 1;
   while (f < finer && total >= 2 * f * jobs * kLong) f *= 2;
-  const int64_t each = (total + f * jobs - 1) / (f * jobs);
-  return each > least ? each : least;
+  return max((int)((uint32_t)(total + f * jobs - 1) / (uint32_t)(f * jobs)), least);
 }
 
 // A border less than kSnap blocks inside a tile moves to the nearer end of it: a tile that is cut costs a start, an end
@@ -160,10 +159,10 @@ template <int KERNEL> struct Cursor {
       total += count;
     }
     total = __builtin_amdgcn_readlane(wave_prefix(total, lane), 63);
-    per = (int)blocks_each(total, a.jobs[KERNEL], kLeast<KERNEL>, kFiner<KERNEL>);
-    job = id / a.kv_heads;
+    per = blocks_each(total, a.jobs[KERNEL], kLeast<KERNEL>, kFiner<KERNEL>);
+    job = (uint32_t)id / (uint32_t)a.kv_heads;
     head = id - job * a.kv_heads;
-    const int used = (total + per - 1) / per;
+    const int used = (uint32_t)(total + per - 1) / (uint32_t)per;
     past = id - used * a.kv_heads;
     if (job >= used) return false;
     const int borders[2] = {job * per, min((job + 1) * per, total)};
@@ -180,14 +179,14 @@ template <int KERNEL> struct Cursor {
         const int at = __ffsll((unsigned long long)__ballot(upto > border)) - 1;
         const int size = __builtin_amdgcn_readlane(blocks_of(a, q), at);
         const int in = border - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(count, at));
-        const int x = in - in / size * size, to = snapped(border, x, size);
+        const int nth = (uint32_t)in / (uint32_t)size, x = in - nth * size, to = snapped(border, x, size);
         if (k == 1) {
           stop = to;
           continue;
         }
         start = to;
         enter(a, tile_rows, s0, at, q);
-        tile = in / blocks;
+        tile = nth;
         from = x + to - border;
         found = true;
       }
@@ -206,16 +205,27 @@ template <int KERNEL> struct Cursor {
     }
     return true;
   }
-  // Kept in LDS while a tile is computed, where scalar registers are short.
-  __device__ __forceinline__ void put(int* to) const {
-    if (threadIdx.x == 0) *(Cursor*)to = *this;
+  // One wave finds the work-group's place and the next tile, the others read it in LDS: all of them at it took 6 us a tile.
+  // It is also kept there while a tile is computed, where scalar registers are short.
+  struct Kept {
+    int word[12 + 4];
+  };
+  __device__ __forceinline__ void put(Kept& to, bool some, int past) const {
+    static_assert(sizeof(Cursor) <= sizeof(int) * 14, "a cursor and two words");
+    if (threadIdx.x == 0) {
+      __builtin_memcpy(to.word, this, sizeof(Cursor));
+      to.word[14] = some;
+      to.word[15] = past;
+    }
   }
-  __device__ __forceinline__ void take(const int* from_) {
+  __device__ __forceinline__ bool take(const Kept& kept, int* past = nullptr) {
     asm volatile("" ::: "memory");
     int w[sizeof(Cursor) / 4];
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(Cursor) / 4); ++i) w[i] = __builtin_amdgcn_readfirstlane(from_[i]);
+    for (int i = 0; i < (int)(sizeof(Cursor) / 4); ++i) w[i] = __builtin_amdgcn_readfirstlane(kept.word[i]);
     __builtin_memcpy(this, w, sizeof(Cursor));
+    if (past) *past = __builtin_amdgcn_readfirstlane(kept.word[15]);
+    return __builtin_amdgcn_readfirstlane(kept.word[14]) != 0;
   }
   // the sequence that lane `at` of a chunk of 64 has read
   __device__ __forceinline__ void enter(const AttnArgs& a, int tile_rows, int s0, int at, const Seq& q) {

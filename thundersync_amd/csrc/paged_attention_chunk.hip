@@ -40,18 +40,23 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (chunk_occupancy(ROW))) void
   __shared__ __attribute__((aligned(16))) bf16 s_v[2][kKeys * ROW];
   const int lane_id = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  __shared__ int s_cur[sizeof(Cursor<1>) / 4];
-  Cursor<1> cur;
+  __shared__ Cursor<1>::Kept s_cur[2];
+  Cursor<1> cur{};
   AttnArgs a = arguments();
-  int past;
-  if (!cur.begin(a, kTileRows, (int)blockIdx.x, lane_id, past)) return;
+  int turn_of = 0;
+  if (wave == 0) {
+    int past;
+    const bool some = cur.begin(a, kTileRows, (int)blockIdx.x, lane_id, past);
+    cur.put(s_cur[0], some, 0);
+  }
+  __syncthreads();
+  if (!cur.take(s_cur[0])) return;
   for (;;) {
   a = arguments();
   int lane = lane_id;
   asm volatile("" : "+v"(lane));  // what follows from it is worked out again a tile, not held over the loop
   const int g = lane >> 4, r = lane & 15;
   const int first_row = cur.tile * kTileRows, rows = cur.seq.n * a.group, len = cur.seq.len, base = len - cur.seq.n;
-  cur.put(s_cur);
   int begin, end;
   cur.piece(a, begin, end);
   if (a.plan && threadIdx.x == 0 && cur.head == 0 && cur.tile == 0 && cur.from == 0)
@@ -314,7 +319,7 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (chunk_occupancy(ROW))) void
   }
 
   a = arguments();
-  cur.take(s_cur);
+  cur.take(s_cur[turn_of]);
   const bool all = cur.whole();
   const int slot = cur.slot(a.kv_heads);
 #pragma unroll
@@ -343,8 +348,13 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (chunk_occupancy(ROW))) void
         *(u32x2*)(o + 32 * b) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
       }
   }
-  if (!cur.next(a, kTileRows, lane_id)) return;
-  __syncthreads();  // the last keys and the cursor have been read
+  turn_of ^= 1;
+  if (wave == 0) {
+    const bool more = cur.next(a, kTileRows, lane_id);
+    cur.put(s_cur[turn_of], more, 0);
+  }
+  __syncthreads();  // the next tile is known, and the last keys have been read
+  if (!cur.take(s_cur[turn_of])) return;
   }
 }
 

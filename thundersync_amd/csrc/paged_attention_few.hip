@@ -71,11 +71,16 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   __shared__ float s_stat[kWaves][16 * R][2];
   const int lane_id = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  __shared__ int s_at[sizeof(Cursor<0>) / 4];
-  Cursor<0> at;
+  __shared__ Cursor<0>::Kept s_at[2];
+  Cursor<0> at{};
   AttnArgs a = arguments();
-  int past = 0;
-  if (!at.begin(a, 16 * R, (int)blockIdx.x, lane_id, past)) {
+  int past = 0, turn = 0;
+  if (wave == 0) {
+    const bool some = at.begin(a, 16 * R, (int)blockIdx.x, lane_id, past);
+    at.put(s_at[0], some, past);
+  }
+  __syncthreads();
+  if (!at.take(s_at[0], &past)) {
     // rows behind the last sequence: 16 a work-group, zeros
     if (a.batch.offsets && past >= 0) {
       const int from = max(0, a.batch.offsets[a.batch.seqs]) + 16 * past;
@@ -94,7 +99,6 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   const int first_row = at.tile * 16 * R;
   const int rows = at.seq.n * a.group;
   const int len = at.seq.len, base = len - at.seq.n;  // position of the first new token
-  at.put(s_at);
   int begin, end;
   at.piece(a, begin, end);
   if (a.plan && threadIdx.x == 0 && at.head == 0 && at.tile == 0 && at.from == 0)
@@ -388,7 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
               f32x4{acc[t][b][i], acc[t][b + 1][i], acc[t][b + 2][i], acc[t][b + 3][i]};
   }
   __syncthreads();
-  at.take(s_at);
+  at.take(s_at[turn]);
   {
   const bool all = at.whole();
   const int slot = at.slot(a.kv_heads);
@@ -430,8 +434,13 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
     }
   }
   }
-  if (!at.next(a, 16 * R, lane_id)) return;
-  __syncthreads();  // the next tile's operands go where the sums were
+  turn ^= 1;
+  if (wave == 0) {
+    const bool more = at.next(a, 16 * R, lane_id);
+    at.put(s_at[turn], more, 0);
+  }
+  __syncthreads();  // the next tile is known, and its operands go where the sums were
+  if (!at.take(s_at[turn])) return;
   }
 }
 
