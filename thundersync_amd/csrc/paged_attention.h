@@ -82,8 +82,8 @@ __device__ __forceinline__ AttnArgs arguments() {
 // keys, 24/4 heads of 256: 100 us in slices of equal length a sequence, 88 dealt like this.
 //
 // Lengths are known on the device alone: every work-group works its part out itself, 64 sequences at a time.
-constexpr int kBlockKeys = 128, kTileCost = 1;
-template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 2 : 4;
+constexpr int kBlockKeys = 128, kTileCost = 3;
+template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 4 : 5;
 constexpr int kLong = 8;
 template <int KERNEL> constexpr int kFiner = KERNEL == 0 ? 4 : 2;  // a partial tile of the chunk kernel is 64 KB and more
 

@@ -155,10 +155,11 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   const uint32_t key_lane = (r * ROW + (WIDE ? 8 : 16) * g) * kSize;
   const uint32_t value_lane = (4 * g * ROW + NB * r) * kSize;
   auto line_of = [&](int pos) -> int64_t { return ((int64_t)at.head << a.page_shift) + (pos & page_mask); };
-  auto load_tile_keys = [&](int pos, int page, u32x4 (&k)[Tile<WIDE, ROW>::kLoads], float& key_scale, float& value_scale)
+  auto load_tile_keys = [&](int pos, bool there, int page, u32x4 (&k)[Tile<WIDE, ROW>::kLoads], float& key_scale, float& value_scale)
                             __attribute__((always_inline)) {
     const int id = max(page, 0);
-    const rsrc_t p = make_rsrc(a.key + id * a.key_page_stride + line_of(pos) * (ROW * kSize), 16 * ROW * kSize);
+    const rsrc_t p = make_rsrc(a.key + id * a.key_page_stride + line_of(pos) * (ROW * kSize),
+                               there ? 16 * ROW * kSize : 0);
 #pragma unroll
     for (int i = 0; i < Tile<WIDE, ROW>::kLoads; ++i) {
       const Words<16> x = load_words<16>(p, key_lane, 64 * i);
@@ -170,15 +171,16 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
       value_scale = uniform_table(a.value_scale)[scale];
     }
   };
-  auto load_keys = [&](int pos) __attribute__((always_inline)) {  // of the pages that page0 and page1 say
-    load_tile_keys(pos, page0, tile[0].k, ks0, vs0);
-    load_tile_keys(pos + 16, page1, tile[1].k, ks1, vs1);
+  // of the pages that page0 and page1 say; a step that is not there reads nothing
+  auto load_keys = [&](int pos, bool there) __attribute__((always_inline)) {
+    load_tile_keys(pos, there, page0, tile[0].k, ks0, vs0);
+    load_tile_keys(pos + 16, there, page1, tile[1].k, ks1, vs1);
   };
-  auto load_values = [&](int pos) __attribute__((always_inline)) {
+  auto load_values = [&](int pos, bool there) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const rsrc_t p = make_rsrc(a.value + max(h ? page1 : page0, 0) * a.value_page_stride +
-                                     line_of(pos + 16 * h) * (ROW * kSize), 16 * ROW * kSize);
+                                     line_of(pos + 16 * h) * (ROW * kSize), there ? 16 * ROW * kSize : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) tile[h].v[i] = load_words<NB * kSize>(p, value_lane, i * ROW * kSize);
     }
@@ -186,18 +188,18 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
 
   int pos = __builtin_amdgcn_readfirstlane(begin + 32 * wave);
   // Steps before `whole` are seen whole by every row.  Their reads run a step ahead, their page ids two, and
-  // unconditionally: the last ones ask for their own again (out of the cache), so that every wait counts exactly what was
-  // asked for since.  256 sequences of 256 to 16384 keys: 812 us with the last ones skipped.
+  // unconditionally, so that every wait counts exactly what was asked for since; past the last one the descriptors are
+  // empty, and nothing is read.  256 sequences of 256 to 16384 keys: 812 us where the last reads were skipped.
   const int whole = min(end, low + 1) - 31;
-  auto after = [&](int pos) { return pos + 32 * kWaves < whole ? pos + 32 * kWaves : pos; };
+  constexpr int kStride = 32 * kWaves;
   int ahead0 = -1, ahead1 = -1;
   if (pos < whole) {
     page0 = page_near(pos, read_near(pos));
     page1 = page_near(pos + 16, read_near(pos + 16));
-    load_keys(pos);
-    load_values(pos);
-    ahead0 = read_near(after(pos));
-    ahead1 = read_near(after(pos) + 16);
+    load_keys(pos, true);
+    load_values(pos, true);
+    ahead0 = read_near(pos + kStride);
+    ahead1 = read_near(pos + kStride + 16);
   }
 #pragma unroll
   for (int t = 0; t < R; ++t)
@@ -211,8 +213,8 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
     if constexpr (edge) {  // few, and nothing is asked for ahead of them: the registers are worth more
       page0 = page_at(pos);
       page1 = page_at(pos + 16);
-      load_keys(pos);
-      load_values(pos);
+      load_keys(pos, true);
+      load_values(pos, true);
     }
     asm volatile("" ::: "memory");  // the query's operands are read again, not held over the loop
     f32x4 sc[R][2];
@@ -240,13 +242,13 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
 #pragma unroll
       for (int t = 0; t < R; ++t) sc[t][h] *= a.scale;
     }
-    const int next = pos + 32 * kWaves;
+    const int next = pos + kStride;
     if constexpr (!edge) {
-      page0 = page_near(after(pos), ahead0);
-      page1 = page_near(after(pos) + 16, ahead1);
-      load_keys(after(pos));
-      ahead0 = read_near(after(after(pos)));
-      ahead1 = read_near(after(after(pos)) + 16);
+      page0 = page_near(next, ahead0);
+      page1 = page_near(next + 16, ahead1);
+      load_keys(next, next < whole);
+      ahead0 = read_near(next + kStride);
+      ahead1 = read_near(next + kStride + 16);
     }
 
     if (ruined0 | ruined1) {  // keys of a page that is none
@@ -367,7 +369,7 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if constexpr (!edge) load_values(after(pos));
+    if constexpr (!edge) load_values(next, next < whole);
     pos = next;
   };
   while (pos < whole) step(std::false_type{});
