@@ -77,20 +77,19 @@ __device__ __forceinline__ AttnArgs arguments() {
 // start and end and one for each kBlockKeys keys; a KV head's tiles follow one another, and each of its work-groups
 // takes as many blocks in a row, ending tiles and beginning others on the way, so that all end together however lengths
 // differ.  A tile that a border cuts leaves partial rows: slot 2 j of work-group j where it began before, 2 j + 1 where it
-// ends behind.  Work-groups are as many as the device holds at once, or twice or four times as many where each still gets
-// kLong blocks, so that a slow one costs less, and fewer where they would get less than kLeast.  64 sequences of 100 to 6000
-// keys, 24/4 heads of 256: 100 us in slices of equal length a sequence, 88 dealt like this.
+// ends behind.  Work-groups are as many as the device holds at once, and fewer where they would get less than kLeast
+// blocks.  64 sequences of 100 to 6000 keys, 24/4 heads of 256: 100 us in slices of equal length a sequence, 88 dealt like
+// this; 128 of 8192, 32/8 heads of 128: 370 us, 411 dealt to four times as many.
 //
 // Lengths are known on the device alone: every work-group works its part out itself, 64 sequences at a time.
 constexpr int kBlockKeys = 128, kTileCost = 3;
 template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 4 : 5;
-constexpr int kLong = 8;
-template <int KERNEL> constexpr int kFiner = KERNEL == 0 ? 4 : 2;  // a partial tile of the chunk kernel is 64 KB and more
-
-// waves a SIMD: a step's loads and the accumulators are 3 ROW / 8 registers, of 16 bits 5 ROW / 8
+// Waves a SIMD: a step's loads and the accumulators are 3 ROW / 8 registers, of 16 bits 5 ROW / 8, and one wave fewer
+// with nothing spilled is faster (rows of 128: 256 sequences of 256 to 16384 keys 752 us at three, 796 at four; 16 bits, 64
+// of 100 to 6000: 151 us at two, 161 at three).
 __host__ __device__ constexpr int few_occupancy(bool wide, int row, int tiles) {
   const int size = row * tiles;
-  return size <= 64 ? 4 : wide ? (size <= 128 ? 3 : 2) : size <= 128 ? 4 : size <= 192 ? 3 : 2;
+  return size <= 64 ? 3 : wide ? 2 : size <= 128 ? 3 : 2;
 }
 __host__ __device__ constexpr int chunk_occupancy(int row) { return row <= 64 ? 4 : 2; }
 
@@ -116,12 +115,6 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& q, int til
   const bool many = a.few_rows > 0 && rows > a.few_rows;
   return many == (KERNEL == 1) ? (int)((rows + tile_rows - 1) / tile_rows) : 0;
 }
-__device__ __forceinline__ int blocks_each(int total, int jobs, int least, int finer) {
-  int f = 1;
-  while (f < finer && total >= 2 * f * jobs * kLong) f *= 2;
-  return max((int)((uint32_t)(total + f * jobs - 1) / (uint32_t)(f * jobs)), least);
-}
-
 // A border less than kSnap blocks inside a tile moves to the nearer end of it: a tile that is cut costs a start, an end
 // and a partial tile more.
 constexpr int kSnap = 4;
@@ -159,7 +152,7 @@ template <int KERNEL> struct Cursor {
       total += count;
     }
     total = __builtin_amdgcn_readlane(wave_prefix(total, lane), 63);
-    per = blocks_each(total, a.jobs[KERNEL], kLeast<KERNEL>, kFiner<KERNEL>);
+    per = max((int)((uint32_t)(total + a.jobs[KERNEL] - 1) / (uint32_t)a.jobs[KERNEL]), kLeast<KERNEL>);
     job = (uint32_t)id / (uint32_t)a.kv_heads;
     head = id - job * a.kv_heads;
     const int used = (uint32_t)(total + per - 1) / (uint32_t)per;

@@ -126,11 +126,8 @@ Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens,
   int64_t plan = 0;
   for (int k = 0; k < 2; ++k) {
     z.blocks[k] = tiles[k] * (kTileCost + (keys + kBlockKeys - 1) / kBlockKeys);
-    // for any lengths: no more than `finer` times z.jobs, and than least blocks each leave
-    const int64_t least = k ? kLeast<1> : kLeast<0>, finer = k ? kFiner<1> : kFiner<0>;
-    int64_t f = 1;
-    while (f < finer && z.blocks[k] >= 2 * f * z.jobs[k] * kLong) f *= 2;
-    const int64_t jobs = std::min((z.blocks[k] + least - 1) / least, f * z.jobs[k]);
+    const int64_t least = k ? kLeast<1> : kLeast<0>;
+    const int64_t jobs = std::min((z.blocks[k] + least - 1) / least, z.jobs[k]);
     z.groups[k] = jobs * c.kv_heads;
     z.slots[k] = jobs > 1 ? 2 * z.groups[k] : 0;
     if (z.slots[k]) plan = (b.seqs * (int64_t)sizeof(Plan) + 255) / 256 * 256;
