@@ -25,7 +25,7 @@ from .operator_profiling import device_role, operator_range
 from .sampling import DTYPES, MAX_VOCAB
 
 ID_DTYPES = (torch.int64, torch.int32)
-MAX_BIASES = 1 << 16
+MAX_BIASES = 1024
 
 
 def _penalty(name: str, value, logits: torch.Tensor):
