@@ -185,6 +185,8 @@ def test_the_c_entries_refuse_rows():
         args = list(good)
         args[at] = value
         assert lib.ts_paged_attention(*args) == 1 and words in lib.ts_hip_last_error().decode(), (at, value)
+    good[0] = desc(pages=0)
+    assert lib.ts_paged_attention(*good) == 1 and "without pages" in lib.ts_hip_last_error().decode()
     many = batch(offsets=4096)
     assert lib.ts_paged_attention(desc(), many, (1 << 31) - 1, p, 1 << 18, 64, 4096, 0.1, p, p, 1 << 62, None) == 1
     assert "too large" in lib.ts_hip_last_error().decode()

@@ -183,13 +183,14 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(Args a) {
         for (int k = 0; k < 4; ++k) x[k] = k == d ? value : x[k];
       }
     }
-    if (bad) x = Quad{1, 1, 1, 1} * (sizeof(T) == 4 ? 0x7fc00000u : __builtin_bit_cast(R, from_f<T>(__builtin_nanf(""))) * 0x10001u);
+    if (bad) x = Quad{1, 1, 1, 1} * (__builtin_bit_cast(R, from_f<T>(__builtin_nanf(""))) * (sizeof(T) == 4 ? 1u : 0x10001u));
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (sizeof(T) == 4) {
         x[k] = bits[j] >> k & 1 ? x[k] : none;
       } else {
-        const uint32_t low = bits[j] >> 2 * k & 1 ? x[k] & 0xffff : none, high = bits[j] >> (2 * k + 1) & 1 ? x[k] >> 16 : none;
+        const uint32_t low = bits[j] >> 2 * k & 1 ? x[k] & 0xffff : none;
+        const uint32_t high = bits[j] >> (2 * k + 1) & 1 ? x[k] >> 16 : none;
         x[k] = low | high << 16;
       }
     }

@@ -78,14 +78,14 @@ __device__ __forceinline__ AttnArgs arguments() {
 // takes as many blocks in a row, ending tiles and beginning others on the way, so that all end together however lengths
 // differ.  A tile that a border cuts leaves partial rows: slot 2 j of work-group j where it began before, 2 j + 1 where it
 // ends behind.  Work-groups are as many as the device holds at once, and fewer where they would get less than kLeast
-// blocks.  64 sequences of 100 to 6000 keys, 24/4 heads of 256: 100 us in slices of equal length a sequence, 88 dealt like
-// this; 128 of 8192, 32/8 heads of 128: 370 us, 411 dealt to four times as many.
+// blocks.  64 sequences of 100 to 6000 keys, 24/4 heads of 256, five rows each: 132 us in slices of equal length a sequence,
+// 114 dealt like this; 128 of 8192, 32/8 heads of 128: 370 us, 411 dealt to four times as many.
 //
 // Lengths are known on the device alone: every work-group works its part out itself, 64 sequences at a time.
 constexpr int kBlockKeys = 128, kTileCost = 3;
 template <int KERNEL> constexpr int kLeast = KERNEL == 0 ? 4 : 5;
 // Waves a SIMD: a step's loads and the accumulators are 3 ROW / 8 registers, of 16 bits 5 ROW / 8, and one wave fewer
-// with nothing spilled is faster (rows of 128: 256 sequences of 256 to 16384 keys 752 us at three, 796 at four; 16 bits, 64
+// with nothing spilled is faster (rows of 128: 256 sequences of 256 to 16384 keys 737 us at three, 796 at four; 16 bits, 64
 // of 100 to 6000: 151 us at two, 161 at three).
 __host__ __device__ constexpr int few_occupancy(bool wide, int row, int tiles) {
   const int size = row * tiles;
@@ -198,8 +198,8 @@ template <int KERNEL> struct Cursor {
     }
     return true;
   }
-  // One wave finds the work-group's place and the next tile, the others read it in LDS: all of them at it took 6 us a tile.
-  // It is also kept there while a tile is computed, where scalar registers are short.
+  // One wave finds the work-group's place and the next tile and the others read it in LDS, where it is also kept while a
+  // tile is computed, for scalar registers are short.
   struct Kept {
     int word[12 + 4];
   };
