@@ -174,3 +174,57 @@ def test_captured(cuda):
         graph.replay()
         want = call()
         assert torch.equal(out, want)
+
+
+def dense(z, history, lengths, prompts, repetition, frequency, presence, bias_ids, bias, allowed):
+    """(want, bound) in 64 bits, over whole rows at once."""
+    b, v = z.shape
+    x, spots = z.double(), torch.arange(history.shape[1], device=z.device)[None]
+    fine = (spots < lengths[:, None]) & (history >= 0) & (history < v)
+    ids = history.long().masked_fill(~fine, 0)
+    zeros = torch.zeros(b, v, dtype=torch.float64, device=z.device)
+    seen = zeros.scatter_add(1, ids, fine.double()) > 0
+    counts = zeros.scatter_add(1, ids, (fine & (spots >= prompts[:, None])).double())
+    x = torch.where(seen, torch.where(x > 0, x / repetition, x * repetition), x)
+    x = x - frequency * counts - presence * (counts > 0)
+    there = (bias_ids >= 0) & (bias_ids < v)
+    at, size = bias_ids.long().masked_fill(~there, 0), bias.double() * there
+    x = x.scatter_add(1, at, size)
+    size = zeros.scatter_add(1, at, size.abs() * max(1, bias.shape[1]))  # each of a token's biases may round the sum
+    bound = ref.bound(z, x, frequency, presence, counts, size, z.dtype)
+    return x.masked_fill(~allowed, -math.inf), bound
+
+
+@pytest.mark.parametrize("dtype, rows, vocab, width, biases", [
+    (torch.bfloat16, 131, 33001, 40, 0),        # long slices, rows that begin at odd places
+    (torch.bfloat16, 131, 33001, 5000, 1024),   # lists that a thread does not hold at once, the most biases
+    (torch.float16, 67, 65537, 16383, 3),       # the longest history that 16 bits count
+    (torch.float16, 67, 65537, 16384, 700),     # and one more
+    (torch.bfloat16, 1, 65537, 16384, 700),
+    (torch.float32, 131, 33001, 5000, 1024),
+])
+def test_long_rows(cuda, dtype, rows, vocab, width, biases):
+    g = torch.Generator(device=cuda).manual_seed(rows + vocab)
+    draw = lambda high, *shape: torch.randint(-1, high, shape, generator=g, device=cuda)  # noqa: E731
+    z = torch.randn(rows, vocab, generator=g, device=cuda).to(dtype)
+    history = draw(vocab + 1, rows, width)
+    history[:, ::3] = vocab - 1  # one token again and again
+    history[0] = 5
+    lengths = draw(width + 1, rows).to(torch.int32)
+    lengths[0] = width
+    prompts = draw(width + 1, rows).to(torch.int32)
+    prompts[0] = 0
+    ids, bias = draw(vocab + 1, rows, biases), torch.randn(rows, biases, generator=g, device=cuda)
+    ids[:, 1::2] = 7
+    allowed = torch.rand(rows, vocab, generator=g, device=cuda) < 0.7
+    allowed[:, [5, 7, vocab - 1]] = True
+    options = (1.25, 2.0 ** -10, 0.5)
+    got = adjust_logits(z, history=history, lengths=lengths, prompt_lengths=prompts, repetition=options[0],
+                        frequency=options[1], presence=options[2], bias_ids=ids, bias=bias, allowed=pack_allowed(allowed))
+    want, bound = dense(z, history, lengths, prompts, *options, ids, bias, allowed)
+    assert excess(got, want.cpu(), bound.cpu()) <= 0
+    again = z.clone()
+    adjust_logits(again, history=history.to(torch.int32), lengths=lengths, prompt_lengths=prompts, repetition=options[0],
+                  frequency=options[1], presence=options[2], bias_ids=ids.to(torch.int32), bias=bias,
+                  allowed=pack_allowed(allowed), out=again)
+    assert torch.equal(again, got)
