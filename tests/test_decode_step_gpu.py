@@ -166,3 +166,25 @@ def test_checked_batches(cuda, monkeypatch):
             paged_attention(x, cache, t, n, 1.0, offsets=off)
     with pytest.raises(ValueError, match="one block"):
         append_tokens(cache, int32([[0, 1], [1, 3]], cuda), int32([17, 3], cuda), x, x)
+
+
+def test_availability(cuda, monkeypatch):
+    from thundersync_amd import _lib, dispatch
+
+    for dtype in (BF, torch.float16):
+        for dim in (64, 72, 128, 256):
+            assert dispatch.hip_paged_available(torch.zeros(2, 4, dim, device=cuda, dtype=dtype))
+        assert dispatch.hip_adjust_logits_available(torch.zeros(2, 70, device=cuda, dtype=dtype))
+    assert dispatch.hip_adjust_logits_available(torch.zeros(2, 1, device=cuda))
+    for query in (torch.zeros(2, 4, 64, device=cuda), torch.zeros(2, 4, 64, dtype=BF),
+                  torch.zeros(2, 4, 60, device=cuda, dtype=BF), torch.zeros(2, 4, 264, device=cuda, dtype=BF)):
+        assert not dispatch.hip_paged_available(query)
+    assert not dispatch.hip_adjust_logits_available(torch.zeros(2, 64))
+    monkeypatch.setenv("THUNDERSYNC_HIP", "off")
+    _lib.reset()
+    try:
+        assert not dispatch.hip_paged_available(torch.zeros(2, 4, 64, device=cuda, dtype=BF))
+        assert not dispatch.hip_adjust_logits_available(torch.zeros(2, 64, device=cuda))
+    finally:
+        monkeypatch.undo()
+        _lib.reset()

@@ -5,7 +5,8 @@ The integration point of the reference's attention dispatch
 
 * :func:`hip_attention_available` / :func:`hip_logprob_available` /
   :func:`hip_distill_available` / :func:`hip_embedding_available` /
-  :func:`hip_sampling_available` answer for one call's tensors.  Under ``THUNDERSYNC_HIP=off`` (or ``auto`` without a
+  :func:`hip_sampling_available` / :func:`hip_paged_available` /
+  :func:`hip_adjust_logits_available` answer for one call's tensors.  Under ``THUNDERSYNC_HIP=off`` (or ``auto`` without a
   loadable library) the answer is no; under ``require`` a library that cannot
   load raises at every call (``_lib.library``), and a loaded one is used
   without a trial, so that a kernel that cannot run on the device fails at
@@ -125,6 +126,32 @@ def sampling_trial(device: torch.device, dtype: torch.dtype, vocab: int) -> None
             raise RuntimeError("HIP sampling trial drew other tokens")
 
 
+def paged_trial(device: torch.device, dtype: torch.dtype, row: int) -> None:
+    """A token of two KV heads stored in caches of 8 and 16 bits, and the attention that sees it alone: its value."""
+    from .paged import PagedCache, append_tokens, paged_attention
+
+    ones = torch.ones(1, 2, row, device=device, dtype=dtype)
+    batch = (torch.zeros(1, 1, device=device, dtype=torch.int32), torch.ones(1, device=device, dtype=torch.int32))
+    for bits in (8, 16):
+        cache = PagedCache.empty(1, 16, 2, row, dtype=dtype, bits=bits, device=device)
+        append_tokens(cache, *batch, ones, 3 * ones)
+        if not bool((paged_attention(ones, cache, *batch, 1.0) == 3).all()):
+            raise RuntimeError("HIP paged attention trial read another value")
+
+
+def adjust_logits_trial(device: torch.device, dtype: torch.dtype, vocab: int) -> None:
+    """One row: a penalty on its first token, a bias on the same, nothing allowed but it."""
+    from .logits import adjust_logits
+
+    token = torch.zeros(1, 1, device=device, dtype=torch.int64)
+    allowed = torch.zeros(1, (vocab + 31) // 32, device=device, dtype=torch.int32)
+    allowed[0, 0] = 1
+    z = adjust_logits(torch.full((1, vocab), 4.0, device=device, dtype=dtype), history=token, repetition=2.0,
+                      presence=1.0, bias_ids=token, bias=token.float() + 3.0, allowed=allowed)
+    if float(z[0, 0]) != 4.0 or not bool((z[0, 1:] == -torch.inf).all()):
+        raise RuntimeError("HIP logits trial gave other values")
+
+
 def _available(like: torch.Tensor, kernel: str, key: int, trial,
                dtypes=(torch.bfloat16, torch.float16)) -> bool:
     if not like.is_cuda or like.dtype not in dtypes:
@@ -167,4 +194,21 @@ def hip_embedding_available(weight: torch.Tensor) -> bool:
 def hip_sampling_available(logits: torch.Tensor) -> bool:
     """Whether these logits may take the HIP sampling (bf16, fp16 and fp32)."""
     return _available(logits, "hip_sampling", int(logits.shape[-1]), sampling_trial,
+                      (torch.bfloat16, torch.float16, torch.float32))
+
+
+def hip_paged_available(query: torch.Tensor) -> bool:
+    """Whether this query ``[tokens, heads, head_dim]`` may take the HIP paged cache and its attention (bf16 and fp16,
+    head dims up to 256 that are multiples of eight)."""
+    from .paged import stored_row
+
+    if query.shape[-1] % 8 or not 8 <= query.shape[-1] <= 256:
+        return False
+    row = stored_row(int(query.shape[-1]))
+    return _available(query, "hip_paged", row, paged_trial)
+
+
+def hip_adjust_logits_available(logits: torch.Tensor) -> bool:
+    """Whether these logits may take the HIP adjustment (bf16, fp16 and fp32)."""
+    return _available(logits, "hip_adjust_logits", int(logits.shape[-1]), adjust_logits_trial,
                       (torch.bfloat16, torch.float16, torch.float32))
