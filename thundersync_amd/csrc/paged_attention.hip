@@ -11,16 +11,18 @@
 namespace ts {
 namespace paged {
 
-// o = sum_p acc_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over a row's parts in order, M the largest m: WAVES waves a row,
-// each every WAVES-th part, then the waves in order.
-template <typename T, int ROW, int WAVES>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void merge_kernel(AttnArgs a) {
-  constexpr int N = ROW / 64, kRows = WAVES == 1 ? 4 : 1;
-  __shared__ float s_acc[WAVES][ROW], s_sum[WAVES];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int id = (int)blockIdx.x * kRows + wave / WAVES;
-  const int t = id / a.heads, h = id - t * a.heads;
-  const int s = t < a.batch.tokens ? __builtin_amdgcn_readfirstlane(seq_of_row(a.batch, t)) : a.batch.seqs;
+// Where the partial rows of one row (token t, query head h) lie: part p at place(p).  parts is 1 where there is nothing to
+// join: the row has been written.
+struct Parts {
+  const float *part, *stats;
+  int owner, inner, parts, rows, at;  // at: the row of its tile, of its KV head
+  int kv_heads, head;
+
+  __device__ __forceinline__ int64_t place(int p) const {
+    return ((int64_t)(p == 0 ? 2 * owner + 1 : 2 * (inner + p - 1)) * kv_heads + head) * rows + at;
+  }
+};
+__device__ __forceinline__ Parts parts_of(const AttnArgs& a, int t, int h, int s) {
   bool mine = s < a.batch.seqs;
   Seq q{0, 0, 0};
   if (mine) q = seq_of(a.batch, s);
@@ -30,71 +32,121 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void merge_kernel(At
   // a plan that no work-group wrote (lengths or offsets changed under the call) reads nothing out of the workspace
   mine = mine && plan.per > 0 && plan.blocks > 0 && plan.start >= 0 && (plan.kernel & ~1) == 0;
   if (!mine) plan = Plan{0, 1, 1, 0};
-  const int rows = a.tile_rows[plan.kernel];
-  const int head = h / a.group, row = (t - q.row0) * a.group + h % a.group, tile = row / rows;
+  Parts y;
+  y.rows = plan.kernel ? a.tile_rows[1] : a.tile_rows[0];
+  y.kv_heads = a.kv_heads;
+  y.head = h / a.group;
+  const int row = (t - q.row0) * a.group + h % a.group, tile = row / y.rows;
+  y.at = row - tile * y.rows;
   // the work-group that begins the tile: the last whose border lies before it or has moved to its start; those that begin
   // inside, from `inner` on: their borders have not moved
   const int first = plan.start + tile * plan.blocks, last = first + plan.blocks;
-  const int owner = (first + min(kSnap - 1, plan.blocks / 2)) / plan.per;
-  const int inner = (first + kSnap + plan.per - 1) / plan.per;
-  int parts = mine ? 1 + max(0, (last - kSnap) / plan.per - inner + 1) : 1;  // 1: written already
-  if (((int64_t)max(owner, inner + parts - 2) + 1) * 2 * a.kv_heads > a.slots[plan.kernel]) parts = 1;
-  const float *part = a.part[plan.kernel], *stats = a.stats[plan.kernel];
-  auto place = [&](int p) -> int64_t {
-    return ((int64_t)(p == 0 ? 2 * owner + 1 : 2 * (inner + p - 1)) * a.kv_heads + head) * rows + row % rows;
-  };
+  y.owner = (first + min(kSnap - 1, plan.blocks / 2)) / plan.per;
+  y.inner = (first + kSnap + plan.per - 1) / plan.per;
+  y.parts = mine ? 1 + max(0, (last - kSnap) / plan.per - y.inner + 1) : 1;
+  const int64_t slots = plan.kernel ? a.slots[1] : a.slots[0];
+  if (min(y.owner, y.inner) < 0 || ((int64_t)max(y.owner, y.inner + y.parts - 2) + 1) * 2 * a.kv_heads > slots) y.parts = 1;
+  y.part = plan.kernel ? a.part[1] : a.part[0];
+  y.stats = plan.kernel ? a.stats[1] : a.stats[0];
+  return y;
+}
+
+// o = sum_p acc_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over a row's parts in order, M the largest m.
+//
+// Few rows: WAVES waves a row, each every WAVES-th part, then the waves in order.
+template <typename T, int ROW, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttnArgs a) {
+  constexpr int N = ROW / 64;
+  __shared__ float s_acc[WAVES][ROW], s_sum[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = (int)blockIdx.x / a.heads, h = (int)blockIdx.x - t * a.heads;
+  const Parts y = parts_of(a, t, h, __builtin_amdgcn_readfirstlane(seq_of_row(a.batch, t)));
+  if (y.parts <= 1) return;
   float acc[N], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  if (parts > 1) {
-    float most = neg_inf();
-    for (int p = lane; p < parts; p += 64) most = fmaxf(most, stats[2 * place(p)]);
-    most = wave_max(most);
-    const float ref = most == neg_inf() ? 0.f : most;
+  float most = neg_inf();
+  for (int p = lane; p < y.parts; p += 64) most = fmaxf(most, y.stats[2 * y.place(p)]);
+  most = wave_max(most);
+  const float ref = most == neg_inf() ? 0.f : most;
 #pragma unroll 4
-    for (int p = wave % WAVES; p < parts; p += WAVES) {
-      const int64_t at = place(p);
-      const float m = stats[2 * at], l = stats[2 * at + 1];
-      const float w = fast_exp2(m - ref);
-      sum = fmaf(l, w, sum);
-      const float* x = part + at * ROW + N * lane;
+  for (int p = wave; p < y.parts; p += WAVES) {
+    const int64_t at = y.place(p);
+    const float w = fast_exp2(y.stats[2 * at] - ref);
+    sum = fmaf(y.stats[2 * at + 1], w, sum);
+    const float* x = y.part + at * ROW + N * lane;
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], w, acc[i]);
+    for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], w, acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) s_acc[wave][N * lane + i] = acc[i];
+  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= a.head_dim) return;
+  float l = 0.f, o = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    l += s_sum[w];
+    o += s_acc[w][d];
+  }
+  ((T*)a.out)[((int64_t)t * a.heads + h) * a.head_dim + d] = from_f<T>(o * (l > 0.f ? 1.f / l : 0.f));
+}
+
+// Many rows: 16 lanes a row.
+constexpr int kMergeLanes = 16, kMergeThreads = 256;
+template <typename T, int ROW>
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
+  constexpr int N = ROW / kMergeLanes;
+  const int lane = threadIdx.x % kMergeLanes;
+  const int id = ((int)blockIdx.x * kMergeThreads + (int)threadIdx.x) / kMergeLanes;
+  const int t = (uint32_t)id / (uint32_t)a.heads, h = id - t * a.heads;
+  const Parts y = parts_of(a, t, h, t < a.batch.tokens ? seq_of_row(a.batch, t) : a.batch.seqs);
+  const int parts = y.parts > 1 ? y.parts : 0;
+  float most = neg_inf();
+  for (int p = lane; p < parts; p += kMergeLanes) most = fmaxf(most, y.stats[2 * y.place(p)]);
+#pragma unroll
+  for (int d = 1; d < kMergeLanes; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+  if (parts == 0) return;
+  const float ref = most == neg_inf() ? 0.f : most;
+  f32x4 acc[N / 4];
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int p = 0; p < parts; ++p) {
+    const int64_t at = y.place(p);
+    const float w = fast_exp2(y.stats[2 * at] - ref);
+    sum = fmaf(y.stats[2 * at + 1], w, sum);
+    const f32x4* x = (const f32x4*)(y.part + at * ROW + N * lane);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const f32x4 v = x[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][k] = fmaf(v[k], w, acc[i][k]);
     }
   }
-  T* out = (T*)a.out + ((int64_t)t * a.heads + h) * a.head_dim;
-  if constexpr (WAVES == 1) {
-    if (parts <= 1) return;
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  T* out = (T*)a.out + ((int64_t)t * a.heads + h) * a.head_dim + N * lane;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (N * lane + i < a.head_dim) out[N * lane + i] = from_f<T>(acc[i] * inv);
-  } else {
+  for (int i = 0; i < N / 4; ++i) {
+    if (N * lane + 4 * i >= a.head_dim) continue;
+    T v[4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) s_acc[wave][N * lane + i] = acc[i];
-    if (lane == 0) s_sum[wave] = sum;
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (parts <= 1 || d >= a.head_dim) return;
-    float l = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      l += s_sum[w];
-      o += s_acc[w][d];
-    }
-    out[d] = from_f<T>(o * (l > 0.f ? 1.f / l : 0.f));
+    for (int k = 0; k < 4; ++k) v[k] = from_f<T>(acc[i][k] * inv);
+    __builtin_memcpy(__builtin_assume_aligned(out + 4 * i, 8), v, 8);
   }
 }
 
-// Sixteen waves a row where rows are few and may have many parts, a wave a row where they are many: 32 rows of 123 parts
-// 8.4 us (four waves 9.8), 768 of a few parts 6.2 (sixteen waves 8.7), 65536 of three 36 (four waves 90).
+// Sixteen waves a row where rows are few and may have many parts, 16 lanes where they are many: 32 rows of 123 parts 7.7 us
+// (four waves 9.8), 768 of a few parts 6.2 (sixteen waves 8.7), 65536 of three 17.5, 4.9 TB/s (a wave a row 39).
 constexpr int64_t kFewMerged = 64, kManyMerged = 2048;
 template <typename T, int ROW> void launch_merge(const AttnArgs& a, hipStream_t s) {
   ts::TimedLaunch timed_("paged.merge_kernel", s);
   const int64_t rows = (int64_t)a.batch.tokens * a.heads;
   if (rows <= kFewMerged) hipLaunchKernelGGL((merge_kernel<T, ROW, 16>), dim3((unsigned)rows), dim3(1024), 0, s, a);
   else if (rows < kManyMerged) hipLaunchKernelGGL((merge_kernel<T, ROW, 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((merge_kernel<T, ROW, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((merge_kernel<T, ROW>), dim3((unsigned)((rows + 15) / 16)), dim3(kMergeThreads), 0, s, a);
 }
 template <typename T> void launch_merge(const AttnArgs& a, int row, hipStream_t s) {
   switch (row) {
