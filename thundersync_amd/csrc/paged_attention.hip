@@ -226,6 +226,10 @@ int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch,
                "ts_paged_attention: workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)z.bytes);
   AttnArgs a{};
   a.batch = batch_of(*batch, tokens);
+  if (batch->width == 0) {  // a table that may be read, though none of it is used
+    a.batch.table = batch->lengths;
+    a.batch.ld_table = 0;
+  }
   a.query = (const char*)query;
   a.token_stride = token_stride;
   a.head_stride = head_stride;
