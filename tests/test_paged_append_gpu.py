@@ -184,6 +184,19 @@ def test_rows_that_go_nowhere(cuda, bits):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
+def test_rows_before_the_first_sequence(cuda, bits):
+    cache = PagedCache.empty(3, 16, 1, 64, bits=bits, device=cuda)
+    x = torch.randn(9, 1, 64, generator=torch.Generator().manual_seed(1)).to(BF).to(cuda)
+    q = append_tokens(cache, int32([[1], [2]], cuda), int32([10, 4], cuda), x, x, query=x, offsets=int32([3, 5, 8], cuda))
+    assert q[:3].abs().max() == 0 and q[8].abs().max() == 0 and torch.equal(q[3:8], x[3:8])
+    key = cache.values()[0].float()
+    got = key.abs().amax(dim=(1, 3)) > 0  # [page, token]
+    want = torch.zeros(3, 16, dtype=torch.bool)
+    want[1, 8:10] = want[2, 1:4] = True
+    assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
 def test_numbers_that_are_none(cuda, bits):
     """NaN stays NaN; an infinity is NaN as a code, and neither moves the block's scale; positions past the table are NaN."""
     cache = PagedCache.empty(1, 16, 1, 64, bits=bits, device=cuda)

@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Args a) {
   int pos = -1, page = -1;
   if (s < a.batch.seqs) {
     const Seq q = seq_of(a.batch, s);
-    pos = q.len - q.n + (t - q.row0);
+    if (t >= q.row0 && t < q.row0 + q.n) pos = q.len - q.n + (t - q.row0);  // else a row before the first sequence
     if (WIDE && pos >= 0) page = page_of(a.batch, s, pos, a.page_shift, a.pages);
   }
   const int slot = pos & ((1 << a.page_shift) - 1);
