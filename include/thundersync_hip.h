@@ -723,7 +723,7 @@ int64_t ts_paged_attention_workspace(const ts_paged_cache* cache, const ts_paged
                                      int64_t heads);
 
 /* out [tokens][heads][head_dim] (dense) = softmax(scale q k) v of each query row over the keys of KV head
- * h / (heads / kv_heads) at its sequence's positions up to its own; zero for rows without keys, NaN for
+ * h / (heads / kv_heads) at its sequence's positions up to its own; zero for rows without keys or sequence, NaN for
  * rows that see a key past the page table or on a page that is none.  Two calls in flight may not share a
  * workspace. */
 int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch, int64_t tokens, const void* query,

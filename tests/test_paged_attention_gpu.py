@@ -186,6 +186,20 @@ def test_rows_of_no_sequence(cuda):
         assert excess(got, want, bound) <= 0
 
 
+@pytest.mark.parametrize("n", [2, 50])
+@pytest.mark.parametrize("skipped", [1, 40])
+def test_rows_before_the_first_sequence(cuda, n, skipped):
+    g = torch.Generator().manual_seed(16)
+    cache, table, dense = random_cache(g, [60, 70], page=16, heads=1, dim=64, dtype=BF, bits=8, device=cuda)
+    q = torch.randn(skipped + n + 5, 2, 64, generator=g).to(BF)
+    out = paged_attention(q.to(cuda), cache, table, int32([60, 70], cuda), 0.1,
+                          offsets=int32([skipped, skipped + n, skipped + n + 1], cuda)).double().cpu()
+    want, bound = torch.zeros_like(out), torch.zeros_like(out)
+    for s, rows in enumerate((slice(skipped, skipped + n), slice(skipped + n, skipped + n + 1))):
+        want[rows], bound[rows] = ref.attention(q[rows], *dense[s], 0.1, BF)
+    assert excess(out, want, bound) <= 0
+
+
 def test_shared_pages(cuda):
     """Sequences that begin with the same pages."""
     g = torch.Generator().manual_seed(7)

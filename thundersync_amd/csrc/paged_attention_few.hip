@@ -83,13 +83,16 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
   }
   __syncthreads();
   if (!at.take(s_at[0], &past)) {
-    // rows behind the last sequence: 16 a work-group, zeros
+    // rows before the first sequence and behind the last: 16 a work-group, zeros
     if (a.batch.offsets && past >= 0) {
-      const int from = max(0, a.batch.offsets[a.batch.seqs]) + 16 * past;
-      const int row_bytes = a.heads * a.head_dim * 2;
-      for (int t = from; t < min(from + 16, a.batch.tokens); ++t)
+      const int before = min(max(0, a.batch.offsets[0]), a.batch.tokens);
+      const int behind = min(max(before, a.batch.offsets[a.batch.seqs]), a.batch.tokens);
+      const int none = before + a.batch.tokens - behind, row_bytes = a.heads * a.head_dim * 2;
+      for (int k = 16 * past; k < min(16 * past + 16, none); ++k) {
+        const int t = k < before ? k : behind + k - before;
         for (int i = threadIdx.x; i < row_bytes / 16; i += 64 * kWaves)
           *(u32x4*)(a.out + (int64_t)t * row_bytes + 16 * i) = u32x4{0, 0, 0, 0};
+      }
     }
     return;
   }
@@ -157,7 +160,8 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
     const uint32_t key_lane = (r * ROW + (WIDE ? 8 : 16) * g) * kSize;
     const uint32_t value_lane = (4 * g * ROW + NB * r) * kSize;
     auto line_of = [&](int pos) -> int64_t { return ((int64_t)at.head << a.page_shift) + (pos & page_mask); };
-    auto load_tile_keys = [&](int pos, bool there, int page, u32x4 (&k)[Tile<WIDE, ROW>::kLoads], float& key_scale, float& value_scale)
+    auto load_tile_keys = [&](int pos, bool there, int page, u32x4 (&k)[Tile<WIDE, ROW>::kLoads], float& key_scale,
+                              float& value_scale)
                               __attribute__((always_inline)) {
       const int id = max(page, 0);
       const rsrc_t p = make_rsrc(a.key + id * a.key_page_stride + line_of(pos) * (ROW * kSize),
@@ -398,45 +402,46 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
     __syncthreads();
     at.take(s_at[turn]);
     {
-    const bool all = at.whole();
-    const int slot = at.slot(a.kv_heads);
-    const int first_row = at.tile * 16 * R, here = min(16 * R, at.seq.n * a.group - first_row);
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    for (int in = tid >> 4; in < here; in += 4 * kWaves) {
-      float most = neg_inf();
+      const bool all = at.whole();
+      const int slot = at.slot(a.kv_heads);
+      const int first_row = at.tile * 16 * R, here = min(16 * R, at.seq.n * a.group - first_row);
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));
+      for (int in = tid >> 4; in < here; in += 4 * kWaves) {
+        float most = neg_inf();
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_stat[w][in][0]);
-      const float by = most == neg_inf() ? 0.f : most;
-      float f[kWaves], sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        f[w] = fast_exp2(s_stat[w][in][0] - by);
-        sum = fmaf(s_stat[w][in][1], f[w], sum);
-      }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      const int row = first_row + in, token = row / a.group, head = at.head * a.group + row % a.group;
-      char* o = a.out + (((int64_t)(at.seq.row0 + token) * a.heads + head) * a.head_dim) * 2;
-      const int64_t to = (int64_t)slot * (16 * R) + in;
-      float* part = a.part[0] + to * ROW;
-#pragma unroll
-      for (int k = 0; k < ROW / 64; ++k) {
-        const int d = 64 * k + 4 * (tid & 15);
-        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_stat[w][in][0]);
+        const float by = most == neg_inf() ? 0.f : most;
+        float f[kWaves], sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const f32x4 y = *(const f32x4*)&s_part[w][in][d];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = fmaf(y[i], f[w], x[i]);
+          f[w] = fast_exp2(s_stat[w][in][0] - by);
+          sum = fmaf(s_stat[w][in][1], f[w], sum);
         }
-        if (!all) *(f32x4*)(part + d) = x;
-        else if (d < a.head_dim) *(u32x2*)(o + 2 * d) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const int row = first_row + in, token = row / a.group, head = at.head * a.group + row % a.group;
+        char* o = a.out + (((int64_t)(at.seq.row0 + token) * a.heads + head) * a.head_dim) * 2;
+        const int64_t to = (int64_t)slot * (16 * R) + in;
+        float* part = a.part[0] + to * ROW;
+#pragma unroll
+        for (int k = 0; k < ROW / 64; ++k) {
+          const int d = 64 * k + 4 * (tid & 15);
+          f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) {
+            const f32x4 y = *(const f32x4*)&s_part[w][in][d];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = fmaf(y[i], f[w], x[i]);
+          }
+          if (!all) *(f32x4*)(part + d) = x;
+          else if (d < a.head_dim)
+            *(u32x2*)(o + 2 * d) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
+        }
+        if (!all && (tid & 15) == 0) {
+          a.stats[0][2 * to] = most;
+          a.stats[0][2 * to + 1] = sum;
+        }
       }
-      if (!all && (tid & 15) == 0) {
-        a.stats[0][2 * to] = most;
-        a.stats[0][2 * to + 1] = sum;
-      }
-    }
     }
     turn ^= 1;
     if (wave == 0) {

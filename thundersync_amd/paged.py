@@ -14,7 +14,8 @@ captured graph replays with new values: ``page_table`` ``[B, W]`` (int32 page
 ids, a sequence's pages in order), ``lengths`` ``[B]`` (int32, tokens of each
 sequence with the call's own; 0 for a row of padding) and ``offsets``
 ``[B + 1]`` (int32, the rows of the call that are each sequence's; None: one
-each).  A call's new tokens are the last of their sequence: token ``i`` of
+each; rows before the first and behind the last are no sequence's, and zero in
+what comes out).  A call's new tokens are the last of their sequence: token ``i`` of
 ``n`` has position ``length - n + i`` and sees the keys up to its own.
 
 Held in 8 bits, keys and values are e4m3 codes times a scale for each 16 tokens
