@@ -182,10 +182,10 @@ def _rows(name: str, x: torch.Tensor, cache: PagedCache) -> torch.Tensor:
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires grad, and there are no gradients through a paged cache: detach it, or call "
                            "under torch.no_grad()")
-    x = x.detach()
-    if x.stride(2) == 1 and (x.stride(0) | x.stride(1)) % 8 == 0 and x.data_ptr() % 16 == 0:
+    a, b, c = x.stride()
+    if c == 1 and (a | b) % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
-    return x.clone(memory_format=torch.contiguous_format)
+    return x.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _batch(cache, page_table, lengths, offsets, tokens, like, writes=False) -> tuple[PagedBatch, list]:
@@ -199,15 +199,16 @@ def _batch(cache, page_table, lengths, offsets, tokens, like, writes=False) -> t
             raise ValueError(f"without offsets each sequence has one row: {tokens} rows for {b} sequences")
     elif offsets.shape != (b + 1,):
         raise ValueError(f"offsets must be [B + 1] = [{b + 1}], got {tuple(offsets.shape)}")
+    device = like.device
     for name, x in (("page_table", page_table), ("lengths", lengths), ("offsets", offsets)):
         if x is None:
             continue
         if x.dtype != torch.int32:
             raise TypeError(f"{name} must be int32, got {x.dtype}")
-        if x.device != like.device:
-            raise ValueError(f"{name} on {x.device} and rows on {like.device}")
-    if cache.device != like.device:
-        raise ValueError(f"cache on {cache.device} and rows on {like.device}")
+        if x.device != device:
+            raise ValueError(f"{name} on {x.device} and rows on {device}")
+    if cache.device != device:
+        raise ValueError(f"cache on {cache.device} and rows on {device}")
     _on_the_gpu(like)
     table = page_table if w <= 1 or page_table.stride(1) == 1 else page_table.contiguous()
     lengths = lengths.contiguous()
