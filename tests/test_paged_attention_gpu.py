@@ -169,6 +169,21 @@ def test_bad_pages_give_nan(cuda, counts, bits):
     assert bool(got[3][sees < 75].isfinite().all())
 
 
+@pytest.mark.parametrize("counts", [None, [2, 3], [60, 40]])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_tables_of_no_pages(cuda, counts, bits):
+    """Every key is past the table."""
+    cache = PagedCache.empty(2, 16, 1, 64, bits=bits, device=cuda)
+    n = sum(counts) if counts else 2
+    table = torch.empty(2, 0, dtype=torch.int32, device=cuda)
+    q = torch.ones(n, 2, 64, device=cuda, dtype=BF)
+    out = paged_attention(q, cache, table, int32(counts or [1, 1], cuda), 0.1,
+                          offsets=offsets_of(counts, cuda) if counts else None)
+    assert bool(out.isnan().all())
+    out = paged_attention(q, cache, table, int32([0, 0], cuda), 0.1, offsets=offsets_of(counts, cuda) if counts else None)
+    assert bool((out == 0).all())
+
+
 def test_rows_of_no_sequence(cuda):
     """Rows behind the last sequence, rows of sequences without keys, more new tokens than keys: zeros."""
     g = torch.Generator().manual_seed(6)
@@ -240,3 +255,38 @@ def test_pages_past_two_to_the_31_bytes(cuda):
     dense = [x.double().transpose(1, 2).reshape(-1, heads, dim)[:700] for x in kv]
     want, bound = ref.attention(q, *dense, 0.1, BF)
     assert excess(out, want, bound) <= 0
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_captured_with_other_batches(cuda, bits):
+    """A captured call reads lengths, offsets and pages anew at each replay: few rows and chunks, cut tiles and whole ones."""
+    g = torch.Generator().manual_seed(17)
+    cache, table, dense = random_cache(g, [2500, 300, 40, 900], page=32, heads=2, dim=128, dtype=BF, bits=bits, device=cuda)
+    q = torch.randn(120, 4, 128, generator=g).to(BF).to(cuda)
+    batches = [([2500, 300, 40, 900], [100, 5, 10, 5]), ([2400, 300, 1, 0], [1, 1, 1, 0]), ([30, 299, 40, 77], [20, 60, 40, 0]),
+               ([2500, 300, 40, 900], [2, 3, 2, 113])]
+    pages, lengths, offsets = table.clone(), int32(batches[0][0], cuda), offsets_of(batches[0][1], cuda)
+    call = lambda: paged_attention(q, cache, pages, lengths, 0.1, offsets=offsets)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for n, counts in batches + batches[::-1]:
+        lengths.copy_(int32(n, cuda))
+        offsets.copy_(offsets_of(counts, cuda))
+        out.fill_(7.0)
+        graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        want, bound = torch.zeros(out.shape, dtype=torch.float64), torch.zeros(out.shape, dtype=torch.float64)
+        at = 0
+        for s, (length, count) in enumerate(zip(n, counts)):
+            rows = slice(at, at + count)
+            want[rows], bound[rows] = ref.attention(q[rows].cpu(), *(x[:length] for x in dense[s]), 0.1, BF)
+            at += count
+        assert excess(out, want, bound) <= 0
