@@ -1,0 +1,37 @@
+"""A decoding step's operators over inputs at the edge of what they take: mixed id types, masks without rows, scales of blocks
+that hold nothing, values at the lower end of fp16."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import logits as ref_logits
+from oracle import paged as ref
+from tests.paged_cases import excess, int32, offsets_of, random_cache
+from tests.test_paged_attention_gpu import check
+from thundersync_amd.logits import adjust_logits, pack_allowed
+from thundersync_amd.paged import PagedCache, append_tokens, paged_attention, rotary_table
+
+pytestmark = pytest.mark.gpu
+BF, FP = torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("history_ids, bias_ids", [(torch.int32, torch.int64), (torch.int64, torch.int32),
+                                                   (torch.int64, torch.int64)])
+def test_ids_past_32_bits_are_passed_over(cuda, history_ids, bias_ids):
+    """Each list in its own type: an id of 64 bits that 32 would cut to a token is none."""
+    vocab = 40
+    far = [2 ** 32 + 5, -2 ** 63, -2 ** 32 + 6, 2 ** 31, 2 ** 63 - 1, 2 ** 32]
+    near = [3, -1, vocab, vocab - 1, -2 ** 31, 2 ** 31 - 1]
+    history = torch.tensor([near, near[::-1]] if history_ids == torch.int32 else [near, far]).to(history_ids)
+    ids = torch.tensor([near, near] if bias_ids == torch.int32 else [far, near]).to(bias_ids)
+    bias = torch.arange(1.0, 13.0).view(2, 6)
+    z = torch.linspace(-2, 2, 2 * vocab).view(2, vocab)
+    out = adjust_logits(z.to(cuda), history=history.to(cuda), presence=0.5, bias_ids=ids.to(cuda), bias=bias.to(cuda))
+    want = torch.stack([ref_logits.adjust(z[i], history[i].tolist(), presence=0.5, bias_ids=ids[i].tolist(), bias=bias[i])
+                        for i in range(2)])
+    # a presence penalty and up to one bias of 12 on logits of up to 2: two roundings of less than 16
+    assert excess(out, want, torch.full_like(want, 2 * 16 * 2.0 ** -24)) <= 0

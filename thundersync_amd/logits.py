@@ -156,7 +156,9 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
         prompt_lengths = None if prompt_lengths is None else prompt_lengths.contiguous()
     if biases:
         ids = bias_ids.dtype if history is None else ids
-        bias_ids, bias = _unit_rows(bias_ids.to(ids)), _unit_rows(bias)
+        if bias_ids.dtype != ids:  # one type for both lists: an id outside the vocabulary stays outside in 32 bits
+            bias_ids = bias_ids.clamp(-1, v).to(ids)
+        bias_ids, bias = _unit_rows(bias_ids), _unit_rows(bias)
     if allowed is not None:
         allowed = _unit_rows(allowed)
         allowed_rows = None if allowed_rows is None else allowed_rows.contiguous()
