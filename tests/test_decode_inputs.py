@@ -1,0 +1,27 @@
+"""Inputs of a decoding step's operators that need no GPU: what is refused, what a check of the batch lets pass."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from tests.paged_cases import int32
+from thundersync_amd import _lib, paged
+from thundersync_amd.logits import adjust_logits, pack_allowed
+from thundersync_amd.paged import PagedCache, append_tokens, paged_attention
+
+BF = torch.bfloat16
+
+
+def test_an_output_of_one_column_has_rows_of_its_own():
+    """One column, whose rows are one element: a kernel would write past it."""
+    z = torch.zeros(3, 1)
+    for out in (torch.empty(1, 1).expand(3, 1), torch.empty(1).expand(3)[:, None]):
+        with pytest.raises(ValueError, match="out must have rows of their own"):
+            adjust_logits(z, out=out)
+    for out in (torch.empty(3, 1), torch.empty(3, 8)[:, 2:3], torch.empty(1, 3).t()):
+        with pytest.raises(RuntimeError, match="on the GPU only"):
+            adjust_logits(z, out=out)

@@ -139,7 +139,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device):
         raise ValueError(f"out must be like logits, {tuple(logits.shape)} {logits.dtype} on {logits.device}, got "
                          f"{tuple(out.shape)} {out.dtype} on {out.device}")
-    if out is not None and v > 1 and (out.stride(1) != 1 or (b > 1 and out.stride(0) < v)):
+    if out is not None and ((v > 1 and out.stride(1) != 1) or (b > 1 and out.stride(0) < v)):
         raise ValueError(f"out must have rows of their own, got strides {out.stride()}")
     if out is not None and _overlaps(out, logits):
         raise ValueError("out overlaps logits without being logits")
