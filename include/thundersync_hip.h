@@ -653,7 +653,7 @@ int ts_sample(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab
  * all rows, or where its pointer is not null one per row (an r that is not above 0 counts
  * as 1, a NaN f or p as 0).  ids (history and biases, of id_bytes 4 or 8) outside
  * [0, vocab) are passed over.  allowed_rows: the row's mask, negative for none, one of
- * `masks` and more gives a row of NaN; null: row i has mask i.  out may be logits.  No
+ * `masks` (0 of them where allowed is null) and more gives a row of NaN; null: row i has mask i.  out may be logits.  No
  * counterpart in the reference (its rollouts sample inside vLLM, rollout/engine.py). */
 int ts_adjust_logits(const void* logits, int64_t ld_logits, int64_t rows, int64_t vocab, const void* history,
                      int64_t ld_history, int64_t history_width, const int32_t* lengths, const int32_t* prompt_lengths,

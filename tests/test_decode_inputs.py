@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import ctypes
 
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -25,3 +27,10 @@ def test_an_output_of_one_column_has_rows_of_its_own():
     for out in (torch.empty(3, 1), torch.empty(3, 8)[:, 2:3], torch.empty(1, 3).t()):
         with pytest.raises(RuntimeError, match="on the GPU only"):
             adjust_logits(z, out=out)
+
+
+def test_the_c_entry_refuses_masks_that_are_not_there():
+    lib, p = _lib.require_library(), ctypes.c_void_p(4096)
+    args = [p, 70, 3, 70, None, 0, 0, None, None, None, 1.0, None, 0.0, None, 0.0, None, 0, None, 0, 0, None, 0, p, 2, 8, p, 70,
+            0, None]
+    assert lib.ts_adjust_logits(*args) == 1 and "null pointer" in lib.ts_hip_last_error().decode()

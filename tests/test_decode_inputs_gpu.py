@@ -35,3 +35,16 @@ def test_ids_past_32_bits_are_passed_over(cuda, history_ids, bias_ids):
                         for i in range(2)])
     # a presence penalty and up to one bias of 12 on logits of up to 2: two roundings of less than 16
     assert excess(out, want, torch.full_like(want, 2 * 16 * 2.0 ** -24)) <= 0
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, torch.float32])
+def test_rows_of_a_mask_without_rows(cuda, dtype):
+    """No mask at all, and rows that name one: NaN, as past the last of several; rows that name none are as they were."""
+    z = torch.randn(4, 70, generator=torch.Generator().manual_seed(0)).to(dtype).to(cuda)
+    rows = int32([0, -1, 3, -5], cuda)
+    empty = torch.empty(0, 3, dtype=torch.int32, device=cuda)
+    out = adjust_logits(z, allowed=empty, allowed_rows=rows)
+    assert bool(out[[0, 2]].isnan().all()) and torch.equal(out[[1, 3]], z[[1, 3]])
+    out = adjust_logits(z, history=torch.zeros(4, 1, dtype=torch.int64, device=cuda), presence=1.0, allowed=empty,
+                        allowed_rows=rows)
+    assert bool(out[[0, 2]].isnan().all()) and torch.equal(out[[1, 3], 1:], z[[1, 3], 1:])

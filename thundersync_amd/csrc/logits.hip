@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(Args a) {
   }
   const uint8_t* mask = nullptr;
   bool bad = false;
-  if (a.allowed) {
+  if (a.allowed || a.allowed_rows) {  // rows may name a mask where there is none
     const int64_t at = a.allowed_rows ? a.allowed_rows[row] : row;
     bad = at >= a.masks;
     if (at >= 0 && !bad) mask = (const uint8_t*)(a.allowed + at * a.ld_allowed);
@@ -257,7 +257,8 @@ int ts_adjust_logits(const void* logits, int64_t ld_logits, int64_t rows, int64_
                    (presence || presence_all == presence_all),
                "ts_adjust_logits: a penalty that is no number, or a repetition not above 0");
   if (rows == 0) return TS_OK;
-  TS_CHECK_ARG(logits && out && (biases == 0 || (bias_ids && bias)), "ts_adjust_logits: null pointer");
+  TS_CHECK_ARG(logits && out && (biases == 0 || (bias_ids && bias)) && (allowed || !allowed_rows || masks == 0),
+               "ts_adjust_logits: null pointer");
   Args a{};
   a.logits = (const char*)logits;
   a.out = (char*)out;
