@@ -48,3 +48,37 @@ def test_rows_of_a_mask_without_rows(cuda, dtype):
     out = adjust_logits(z, history=torch.zeros(4, 1, dtype=torch.int64, device=cuda), presence=1.0, allowed=empty,
                         allowed_rows=rows)
     assert bool(out[[0, 2]].isnan().all()) and torch.equal(out[[1, 3], 1:], z[[1, 3], 1:])
+
+
+def with_stale_scales(cache, table, lengths):
+    """The cache behind one more page, its first; that page's scales and those of blocks without tokens are NaN."""
+    page, table = cache.page_size, table + 1
+    first = lambda x, fill: torch.cat([torch.full_like(x[:1].float(), fill).to(x.dtype), x])  # noqa: E731
+    held = torch.zeros(cache.pages + 1, 1, page // 16, dtype=torch.bool, device=table.device)
+    for s, n in enumerate(lengths):
+        for block in range(-(-n // 16)):
+            held[int(table[s, block * 16 // page]), 0, block * 16 % page // 16] = True
+    scales = [torch.where(held, first(x, math.nan), math.nan).contiguous() for x in (cache.key_scale, cache.value_scale)]
+    codes = [first(x.view(torch.uint8), 0x7F).view(cache.key.dtype) for x in (cache.key, cache.value)]
+    return PagedCache(*codes, *scales, dtype=cache.dtype, head_dim=cache.head_dim), table
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("counts", [None, [1] * 9, [1, 2, 3, 4, 1, 5, 2, 1, 3], [1, 15, 16, 3, 33, 40, 1, 60, 70]])
+def test_scales_of_blocks_that_hold_nothing(cuda, dtype, page, counts):
+    """Whatever the first page's scales and those behind a sequence's end hold, no row has part of it."""
+    g = torch.Generator().manual_seed(11)
+    lengths = [1, 15, 16, 17, 33, 48, 65, 144, 200]
+    cache, table, dense = random_cache(g, lengths, page=page, heads=2, dim=64, dtype=dtype, bits=8, device=cuda)
+    cache, table = with_stale_scales(cache, table, lengths)
+    n = [1] * len(lengths) if counts is None else counts
+    q = torch.randn(sum(n), 4, 64, generator=g).to(dtype)
+    out = paged_attention(q.to(cuda), cache, table, int32(lengths, cuda), 0.1,
+                          offsets=None if counts is None else offsets_of(counts, cuda))
+    at = 0
+    for s, c in enumerate(n):
+        want, bound = ref.attention(q[at:at + c], *dense[s], 0.1, dtype)
+        over = excess(out[at:at + c], want, bound)
+        assert over <= 0, (s, lengths[s], c, over)
+        at += c

@@ -225,7 +225,8 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
       asm volatile("" ::: "memory");  // the query's operands are read again, not held over the loop
       f32x4 sc[R][2];
       const bool ruined0 = page0 < 0 && pos < end, ruined1 = page1 < 0 && pos + 16 < end;
-      const float vscale0 = vs0, vscale1 = vs1;
+      // the scale of a half behind the end is whatever its place holds, and a code of 0 times a NaN is one
+      const float vscale0 = vs0, vscale1 = edge && pos + 16 >= end ? 1.f : vs1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
