@@ -82,3 +82,18 @@ def test_scales_of_blocks_that_hold_nothing(cuda, dtype, page, counts):
         over = excess(out[at:at + c], want, bound)
         assert over <= 0, (s, lengths[s], c, over)
         at += c
+
+
+def test_checked_batches_with_rows_of_no_sequence(cuda, monkeypatch):
+    """The check of a batch lets pass what the module describes: rows outside the sequences, padding with rows of its own."""
+    monkeypatch.setenv("THUNDERSYNC_CHECK_TARGETS", "1")
+    x = torch.ones(9, 1, 64, dtype=BF, device=cuda)
+    table, lengths, offsets = int32([[0, 1], [2, 3], [9, 9]], cuda), int32([17, 3, 0], cuda), int32([2, 4, 5, 7], cuda)
+    cache = PagedCache.empty(4, 16, 1, 64, device=cuda)
+    q = append_tokens(cache, table, lengths, x, x, query=x, offsets=offsets)
+    out = paged_attention(x, cache, table, lengths, 1.0, offsets=offsets)
+    for rows in (q, out):
+        assert not bool(rows[[0, 1, 5, 6, 7, 8]].any()) and bool((rows[2:5] != 0).all())
+    for bad in ([-1, 4, 5, 7], [2, 4, 3, 7], [2, 4, 5, 10]):
+        with pytest.raises(ValueError, match="offsets"):
+            paged_attention(x, cache, table, lengths, 1.0, offsets=int32(bad, cuda))

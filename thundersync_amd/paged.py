@@ -222,11 +222,9 @@ def _batch(cache, page_table, lengths, offsets, tokens, like, writes=False) -> t
 def _check_batch(cache, table, lengths, offsets, tokens, writes):
     b, w = table.shape
     n = torch.ones_like(lengths) if offsets is None else offsets[1:] - offsets[:-1]
-    if offsets is not None and (int(offsets[0]) != 0 or int(offsets[-1]) != tokens or bool((n < 0).any())):
-        raise ValueError(f"offsets must rise from 0 to the {tokens} rows")
+    if offsets is not None and (int(offsets[0]) < 0 or int(offsets[-1]) > tokens or bool((n < 0).any())):
+        raise ValueError(f"offsets must be rising places among the {tokens} rows")
     bad = (lengths < 0) | (lengths > w * cache.page_size) | ((lengths > 0) & (lengths < n))
-    if offsets is not None:
-        bad |= (lengths == 0) & (n > 0)
     used = torch.arange(w, device=table.device) < (lengths[:, None] + cache.page_size - 1) // cache.page_size
     bad |= (used & ((table < 0) | (table >= cache.pages))).any(dim=1)
     if bool(bad.any()):
