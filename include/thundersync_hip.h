@@ -669,7 +669,7 @@ int ts_adjust_logits(const void* logits, int64_t ld_logits, int64_t rows, int64_
 
 /* Pages [pages][kv_heads][page_size][row] of keys and of values, page p at p *
  * page_stride elements: in 16 bits elements of dtype; in 8 bits e4m3 codes, each
- * times its scale (fp32, a power of two between 2^-118 and 2^120) a value of dtype, one
+ * times its scale (fp32, a power of two from 2^-118, in fp16 2^-15, to 2^120) a value of dtype, one
  * scale for 16 tokens of a page and head, [pages][kv_heads][page_size / 16].  Rows hold
  * head_dim elements (a multiple of 8) and zeros behind them. */
 typedef struct ts_paged_cache {

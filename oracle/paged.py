@@ -12,15 +12,16 @@ import torch
 E4M3_MAX = 448.0
 BLOCK = 16
 MIN_EXPONENT, MAX_EXPONENT = -118, 120
+MIN_EXPONENT_FP16 = -15  # steps of codes below the normal ones are 2^-9 of the scale, of fp16 2^-24
 
 
-def exponent_for(most: float) -> int:
+def exponent_for(most: float, dtype: torch.dtype = torch.bfloat16) -> int:
     """The smallest e of those allowed with most <= 448 * 2^e."""
     e = MIN_EXPONENT
     if most > 0:
         m, x = math.frexp(most)  # most = m 2^x, 448 = 0.875 * 2^9
         e = x - 9 if m <= 0.875 else x - 8
-    return max(MIN_EXPONENT, min(MAX_EXPONENT, e))
+    return max(MIN_EXPONENT_FP16 if dtype == torch.float16 else MIN_EXPONENT, min(MAX_EXPONENT, e))
 
 
 def code_limit(e: int, dtype: torch.dtype) -> float:
@@ -39,7 +40,7 @@ def encode(x: torch.Tensor, e: int, dtype: torch.dtype) -> torch.Tensor:
 def append_block(old: torch.Tensor, old_exponent: int, new: torch.Tensor, first: int, dtype: torch.dtype):
     """A block's values [16, D] and exponent after `new` [n, D] came to slots first .. first + n - 1."""
     finite = torch.where(new.double().isfinite(), new.double(), 0.0)
-    e = exponent_for(float(finite.abs().max()) if finite.numel() else 0.0)
+    e = exponent_for(float(finite.abs().max()) if finite.numel() else 0.0, dtype)
     if first > 0:
         e = max(e, old_exponent)
     values = old.clone()

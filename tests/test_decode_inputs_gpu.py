@@ -84,6 +84,29 @@ def test_scales_of_blocks_that_hold_nothing(cuda, dtype, page, counts):
         at += c
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("loud", [2.0 ** -8, 2.0 ** -12, 2.0 ** -15, 2.0 ** -20])
+def test_small_fp16_values_are_codes_of_fp16_values(cuda, loud, interleaved):
+    """What a code stands for is a value of the type also where rotated keys lie below its smallest steps."""
+    g = torch.Generator().manual_seed(12)
+    cache = PagedCache.empty(4, 16, 2, 64, dtype=FP, bits=8, device=cuda)
+    table, angles = int32([[2, 0, 3]], cuda), rotary_table(64, 64, device=cuda)
+    key, value = (loud * torch.randn(40, 2, 64, generator=g) for _ in range(2))
+    key, value = key.to(FP), value.to(FP)
+    append_tokens(cache, table, int32([40], cuda), key.to(cuda), value.to(cuda), offsets=int32([0, 40], cuda),
+                  rotary=angles, interleaved=interleaved)
+    rows = ref.rotate(key, angles.cpu(), torch.arange(40), interleaved), value.double()
+    for codes, scale, got, want in zip((cache.key, cache.value), (cache.key_scale, cache.value_scale), cache.values(), rows):
+        scale = scale.double().cpu().repeat_interleave(16, dim=-1)[..., None]
+        stands = codes.double().cpu() * scale
+        assert torch.equal(stands, got.double().cpu())
+        ids = table[0].long().cpu()
+        flat = lambda x: x[ids].transpose(1, 2).flatten(0, 1)[:40]  # noqa: E731
+        # half a step of a code, normal or below, and fp32's roundings of the rotation (three of up to twice the largest)
+        bound = want.abs() * 2.0 ** -4 + flat(scale) * 2.0 ** -10 + 6 * 2.0 ** -24 * want.abs().amax(dim=-1, keepdim=True)
+        assert excess(flat(got), want, bound) <= 0
+
+
 def test_checked_batches_with_rows_of_no_sequence(cuda, monkeypatch):
     """The check of a batch lets pass what the module describes: rows outside the sequences, padding with rows of its own."""
     monkeypatch.setenv("THUNDERSYNC_CHECK_TARGETS", "1")

@@ -69,16 +69,18 @@ __device__ __forceinline__ int page_of(const Batch& b, int s, int pos, int page_
 }
 
 // Scales are powers of two within these exponents, so that code * scale and value / scale are
-// exact in fp32.
+// exact in fp32, and code * scale in the element type: codes below the normal ones have steps of 2^-9 of the
+// scale, fp16 has steps of 2^-24 (values of the type lose nothing by it: they have no smaller steps to keep).
 constexpr int kMinExponent = -118, kMaxExponent = 120;
+template <typename T> constexpr int kLeastExponent = std::is_same_v<T, f16> ? -15 : kMinExponent;
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127; }
 
 // The smallest exponent e with most <= 448 * 2^e (448 = 1.75 * 2^8: e4m3's largest value).
-__device__ __forceinline__ int exponent_for(float most) {
+template <typename T> __device__ __forceinline__ int exponent_for(float most) {
   const uint32_t u = __float_as_uint(most);
   const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return max(kMinExponent, min(kMaxExponent, e));
+  return max(kLeastExponent<T>, min(kMaxExponent, e));
 }
 
 // The largest code of a block: below the top of the element type all of e4m3, at it the largest

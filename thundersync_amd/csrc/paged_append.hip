@@ -6,7 +6,7 @@
 //     or (x_{2j}, x_{2j+1}) where interleaved
 //   query rows are rotated into an output of their own, key rows into the cache; value rows go there as they are
 //   8 bits: one scale 2^e, the smallest with most <= 448 * 2^e over the new tokens of a block of 16 tokens and
-//   head, no smaller than before where the block holds older tokens; these are then written by the new scale (a
+//   head (in fp16 not below 2^-15), no smaller than before where the block holds older tokens; these are then written by the new scale (a
 //   power of two, so that only e4m3's subnormal codes can lose bits).
 //
 // Bound by HBM where tokens are many (each row is read and written once) and by latency where they
@@ -218,7 +218,7 @@ __device__ __forceinline__ void append_block(const Args& a, int unit, int lane) 
   }
   most = wave_max(most);
   const int old = held ? exponent_of(*scale) : kMinExponent;
-  const int e = max(old, exponent_for(most));
+  const int e = max(old, exponent_for<T>(most));
   if (held && e > old) {
     // the older tokens by the new scale
     const float ratio = two_to(max(old - e, -126));

@@ -19,7 +19,8 @@ what comes out).  A call's new tokens are the last of their sequence: token ``i`
 ``n`` has position ``length - n + i`` and sees the keys up to its own.
 
 Held in 8 bits, keys and values are e4m3 codes times a scale for each 16 tokens
-of a page and head.  Scales are powers of two: a value is ``code * scale``
+of a page and head.  Scales are powers of two, in an fp16 cache from 2^-15 on,
+so that codes have no smaller steps than fp16: a value is ``code * scale``
 exactly, in bf16 and fp16 too, attention over the codes is attention over those
 values, and a block whose scale grows keeps its older codes' values (but for
 bits that pass below e4m3's range).  The rounding to a code is the only one.
