@@ -64,7 +64,8 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scale
     """(out, bound) of the last n = len(query) tokens of a sequence: query [n, H, D], key and value [L, Hkv, D].
 
     The bound counts: weights rounded to `dtype` and the result (half a step each), what fp32 loses of a score (D products
-    summed, the scale, the exponential) and of sums over L keys, and fp16 weights below its smallest number.
+    summed, the scale, the exponential) and of sums over L keys, and fp16 weights below its normal numbers: these are rounded
+    with the largest at 2^7, by half of 2^-24.
     """
     n, heads, d = query.shape
     length, hkv, _ = key.shape
@@ -86,5 +87,5 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scale
         loss = (d + 8) * 2.0 ** -24 * score + (length + 16) * 2.0 ** -24 + 2.0 ** -21
         bound[:, h] = size * (half + 2 * loss) + out[:, h].abs() * half
         if dtype == torch.float16:
-            bound[:, h] += length * 2.0 ** -25 * seen.abs().amax(dim=1) + 2.0 ** -25
+            bound[:, h] += length * 2.0 ** -32 * seen.abs().amax(dim=1) + 2.0 ** -25
     return out, bound

@@ -107,6 +107,30 @@ def test_small_fp16_values_are_codes_of_fp16_values(cuda, loud, interleaved):
         assert excess(flat(got), want, bound) <= 0
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("counts, length", [(None, 30001), ([3], 30001), ([33], 30001), (None, 400), ([1], 400), ([3], 400),
+                                            ([33], 400)])
+def test_many_small_fp16_weights(cuda, counts, length, bits):
+    """One key of score 17.5 before others of 0: each of these has a weight of 2^-25.2, together they are 30000 times that."""
+    n = counts[0] if counts else 1
+    row = torch.zeros(length, 1, 8, dtype=FP)
+    key, value = row.clone(), row.clone() + 1.0
+    key[3, 0, 0], value[3, 0, :4] = 7.0, 0.0
+    cache = PagedCache.empty(length // 256 + 1, 256, 1, 8, dtype=FP, bits=bits, device=cuda)
+    table = torch.arange(cache.pages, dtype=torch.int32, device=cuda)[None]
+    lengths = int32([length], cuda)
+    append_tokens(cache, table, lengths, key.to(cuda), value.to(cuda), offsets=int32([0, length], cuda))
+    q = torch.zeros(n, 1, 8, dtype=FP)
+    q[:, 0, 0] = 2.5
+    out = paged_attention(q.to(cuda), cache, table, lengths, 1.0, offsets=None if counts is None else offsets_of(counts, cuda))
+    others = (length - n + torch.arange(n, dtype=torch.float64)) * math.exp(-17.5)
+    want = torch.ones(n, 1, 8, dtype=torch.float64)
+    want[:, 0, :4] = (others / (1 + others))[:, None]
+    # the result's half a step, the weights' (each within 2^-32 of the largest), fp32 sums of 30000
+    bound = want * 2.0 ** -11 + length * 2.0 ** -32 + want * (length + 100) * 2.0 ** -24 + 2.0 ** -25
+    assert excess(out, want, bound) <= 0
+
+
 def test_checked_batches_with_rows_of_no_sequence(cuda, monkeypatch):
     """The check of a batch lets pass what the module describes: rows outside the sequences, padding with rows of its own."""
     monkeypatch.setenv("THUNDERSYNC_CHECK_TARGETS", "1")

@@ -260,6 +260,15 @@ template <int KERNEL> struct Cursor {
   }
 };
 
+// Weights are rounded to the element type for the product with the values, half a step each, as in packed attention: in fp32
+// there is no matrix instruction of this rate.  That is 1.4e-3 of an output's size in bf16 and 1.4e-4 in fp16, beside 1.7e-3
+// and 2.1e-4 of the output's own rounding.  Their sum is of the unrounded ones, in fp32.  A row's reference point is its
+// largest score when it last moved, in fp16 kLift below it: weights go up to 2^(kLift + kSlack), below 65504, and half of
+// fp16's smallest number is 2^-32 of the largest, not 2^-25, which many small weights beside a large one would be lost to.
+constexpr float kSlack = 8.f;  // log2 units by which scores may pass the largest before the reference point moves
+template <typename T> constexpr float kLift = std::is_same_v<T, f16> ? 7.f : 0.f;
+template <typename T> constexpr float kSlackSum = std::is_same_v<T, f16> ? 32768.f : 256.f;  // 2^(kLift + kSlack)
+
 // Two 16-bit values without those that are not finite, and ones in the place of these.
 template <typename T> constexpr uint32_t kOneOf = std::is_same_v<T, f16> ? 0x3c00u : 0x3f80u;
 template <typename T> __device__ __forceinline__ void split_finite(uint32_t x, uint32_t& fine, uint32_t& flag) {

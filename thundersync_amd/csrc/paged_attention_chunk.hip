@@ -27,7 +27,6 @@ using attn::to_of;
 using attn::tr_read;
 
 constexpr int kTileRows = 128, kKeys = 32;
-constexpr float kSlack = 8.f, kSlackSum = 256.f;
 
 template <int ROW> constexpr int kBlocks = ROW <= 192 ? 2 : 1;  // 16-row query blocks a wave
 template <int ROW> constexpr int kChunkWaves = kTileRows / 16 / kBlocks<ROW>;
@@ -216,14 +215,14 @@ __global__ __launch_bounds__(64 * kChunkWaves<ROW>, (chunk_occupancy(ROW))) void
           }
         };
         exponentials();
-        if (__ballot((m[t] == neg_inf()) | (sum > kSlackSum))) {
+        if (__ballot((m[t] == neg_inf()) | (sum > kSlackSum<T>))) {
           float most = neg_inf();
 #pragma unroll
           for (int j = 0; j < 8; ++j) most = fmaxf(most, sc[j >> 2][t][j & 3] * c);
           most = rows_max4(most);
-          const bool move = most > m[t] + kSlack || (m[t] == neg_inf() && most > m[t]);
-          const float alpha = move ? fast_exp2(m[t] - most) : 1.f;
-          m[t] = move ? most : m[t];
+          const bool move = most > m[t] + (kSlack + kLift<T>) || (m[t] == neg_inf() && most > m[t]);
+          const float to = move ? most - kLift<T> : m[t], alpha = move ? fast_exp2(m[t] - to) : 1.f;
+          m[t] = to;
           l[t] *= alpha;
 #pragma unroll
           for (int b = 0; b < NB; ++b) acc[b][t] *= alpha;

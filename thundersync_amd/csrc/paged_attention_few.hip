@@ -20,8 +20,6 @@ namespace ts {
 namespace paged {
 
 constexpr int kWaves = 4;
-constexpr float kSlack = 8.f;      // log2 units by which scores may pass the reference point before it moves
-constexpr float kSlackSum = 256.f;
 
 // N bytes of a lane, at a multiple of four from the descriptor's base and `more`, a constant.  Reads go through a
 // descriptor of the 16 tokens: a lane's place in them is one register for all of a kernel, where a pointer is two more
@@ -287,14 +285,14 @@ __global__ __launch_bounds__(64 * kWaves, (few_occupancy(WIDE, ROW, R))) void fe
         };
         exponentials();
         // They stand unless a score passes the reference point by more than kSlack, which shows in the sum.
-        if (__ballot((m[t] == neg_inf()) | (sum > kSlackSum))) {
+        if (__ballot((m[t] == neg_inf()) | (sum > kSlackSum<T>))) {
           float most = neg_inf();
 #pragma unroll
           for (int j = 0; j < 8; ++j) most = fmaxf(most, sc[t][j >> 2][j & 3]);
           most = rows_max4(most);
-          const bool move = most > m[t] + kSlack || (m[t] == neg_inf() && most > m[t]);
-          const float alpha = move ? fast_exp2(m[t] - most) : 1.f;
-          m[t] = move ? most : m[t];
+          const bool move = most > m[t] + (kSlack + kLift<T>) || (m[t] == neg_inf() && most > m[t]);
+          const float to = move ? most - kLift<T> : m[t], alpha = move ? fast_exp2(m[t] - to) : 1.f;
+          m[t] = to;
           l[t] *= alpha;
 #pragma unroll
           for (int b = 0; b < NB; ++b) acc[t][b] *= alpha;
