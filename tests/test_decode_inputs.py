@@ -34,3 +34,39 @@ def test_the_c_entry_refuses_masks_that_are_not_there():
     args = [p, 70, 3, 70, None, 0, 0, None, None, None, 1.0, None, 0.0, None, 0.0, None, 0, None, 0, 0, None, 0, p, 2, 8, p, 70,
             0, None]
     assert lib.ts_adjust_logits(*args) == 1 and "null pointer" in lib.ts_hip_last_error().decode()
+
+
+def append(**change):
+    x = torch.zeros(3, 2, 64, dtype=BF)
+    return append_tokens(**{"cache": PagedCache.empty(4, 16, 2, 64, device="cpu"), "lengths": int32([1] * 3, "cpu"),
+                            "page_table": torch.zeros(3, 2, dtype=torch.int32), "key": x, "value": x} | change)
+
+
+def attend(**change):
+    return paged_attention(**{"query": torch.zeros(3, 4, 64, dtype=BF), "cache": PagedCache.empty(4, 16, 2, 64, device="cpu"),
+                              "page_table": torch.zeros(3, 2, dtype=torch.int32), "lengths": int32([1] * 3, "cpu"),
+                              "scale": 0.1} | change)
+
+
+def adjust(**change):
+    return adjust_logits(**{"logits": torch.zeros(3, 70), "history": torch.zeros(3, 5, dtype=torch.int64)} | change)
+
+
+ROWS = [(append, "key", (3, 2, 64), BF), (append, "value", (3, 2, 64), BF), (append, "query", (3, 4, 64), BF),
+        (attend, "query", (3, 4, 64), BF), (adjust, "logits", (3, 70), torch.float32)]
+
+
+@pytest.mark.parametrize("call, name, shape, dtype", ROWS)
+def test_tangents_are_refused(call, name, shape, dtype):
+    """A tangent would be lost without a word; torch.no_grad() does not switch it off, as in torch."""
+    x = torch.zeros(shape, dtype=dtype)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match=f"{name} ha(s|ve) a forward-mode tangent"):
+            call(**{name: dual})
+        with torch.no_grad(), pytest.raises(RuntimeError, match=f"{name} ha(s|ve) a forward-mode tangent"):
+            call(**{name: dual})
+        with pytest.raises(RuntimeError, match="on the GPU only"):
+            call(**{name: dual.detach()})
+    with pytest.raises(RuntimeError, match="on the GPU only"):
+        call(**{name: x})

@@ -11,7 +11,7 @@ For each row and token, in this order, in fp32 and rounded once:
 4. ``-inf`` for tokens that the row's mask does not allow.
 
 A row whose mask allows nothing becomes all ``-inf``, for which the sampler draws
-token -1.  No gradients, and GPU only: other dtypes and CPU tensors raise.
+token -1.  No gradients or tangents, and GPU only: other dtypes and CPU tensors raise.
 """
 
 from __future__ import annotations
@@ -19,6 +19,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .operator_profiling import device_role, operator_range
@@ -100,6 +101,8 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
         raise TypeError(f"thundersync_amd takes bf16, fp16 or fp32 logits, got {logits.dtype}")
     if logits.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("logits require grad, and adjust_logits has none: detach them, or call under torch.no_grad()")
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise RuntimeError("logits have a forward-mode tangent, and adjust_logits has none: detach them")
     penalties = [_penalty(*x, logits) for x in (("repetition", repetition), ("frequency", frequency),
                                                 ("presence", presence))]
     if history is None:

@@ -29,8 +29,8 @@ Bad input found on the device: a token past the page table, or whose page id is
 no page of the cache, is stored nowhere, and attention rows that see such a key
 are NaN; ``THUNDERSYNC_CHECK_TARGETS=1`` checks the batch first and raises.  A
 block of 16 tokens that a call writes belongs to one sequence (sequences may
-share pages that they only read).  There are no gradients through a cache, and
-no host path: other dtypes and CPU tensors raise.
+share pages that they only read).  There are no gradients and no tangents through a cache,
+and no host path: other dtypes and CPU tensors raise.
 """
 
 from __future__ import annotations
@@ -40,6 +40,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._abi import PagedBatch, PagedCacheDesc
@@ -183,6 +184,8 @@ def _rows(name: str, x: torch.Tensor, cache: PagedCache) -> torch.Tensor:
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires grad, and there are no gradients through a paged cache: detach it, or call "
                            "under torch.no_grad()")
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError(f"{name} has a forward-mode tangent, and there are none through a paged cache: detach it")
     a, b, c = x.stride()
     if c == 1 and (a | b) % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
