@@ -70,3 +70,20 @@ def test_tangents_are_refused(call, name, shape, dtype):
             call(**{name: dual.detach()})
     with pytest.raises(RuntimeError, match="on the GPU only"):
         call(**{name: x})
+
+
+@pytest.mark.parametrize("call, name, shape", [(append, "rotary", (9, 32)), (adjust, "bias", (3, 2)), (adjust, "repetition", (3,)),
+                                               (adjust, "frequency", (3,)), (adjust, "presence", (3,)), (adjust, "out", (3, 70))])
+def test_gradients_of_other_inputs_are_refused(call, name, shape):
+    """Of a table, biases, penalties, an output: what would be dropped is refused as it is for rows and logits."""
+    x = torch.ones(shape)
+    more = {"bias_ids": torch.zeros(3, 2, dtype=torch.int64)} if name == "bias" else {}
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match=f"{name} requires grad"):
+        call(**{name: leaf}, **more)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="on the GPU only"):
+        call(**{name: leaf}, **more)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match=f"{name} has a forward-mode tangent"):
+        call(**{name: forward_ad.make_dual(x, x)}, **more)
+    with pytest.raises(RuntimeError, match="on the GPU only"):
+        call(**{name: x}, **more)

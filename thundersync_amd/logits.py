@@ -29,6 +29,16 @@ ID_DTYPES = (torch.int64, torch.int32)
 MAX_BIASES = 1024
 
 
+def _no_gradients(name: str, x: torch.Tensor):
+    many = name == "logits"
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} require{'s'[many:]} grad, and adjust_logits has none: detach {'them' if many else 'it'}, or "
+                           "call under torch.no_grad()")
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError(f"{name} {'have' if many else 'has'} a forward-mode tangent, and adjust_logits has none: detach "
+                           f"{'them' if many else 'it'}")
+
+
 def _penalty(name: str, value, logits: torch.Tensor):
     """``(tensor or None, number)`` of a penalty given per row or once."""
     if not isinstance(value, torch.Tensor):
@@ -38,6 +48,7 @@ def _penalty(name: str, value, logits: torch.Tensor):
             raise ValueError(f"repetition must be above 0, got {value!r}")
         return None, float(value)
     _per_row(name, value, logits, (torch.float32,))
+    _no_gradients(name, value)
     return value.contiguous(), 0.0
 
 
@@ -99,10 +110,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
         raise ValueError(f"a vocabulary of at most {MAX_VOCAB}, got {v}")
     if logits.dtype not in DTYPES:
         raise TypeError(f"thundersync_amd takes bf16, fp16 or fp32 logits, got {logits.dtype}")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("logits require grad, and adjust_logits has none: detach them, or call under torch.no_grad()")
-    if forward_ad.unpack_dual(logits).tangent is not None:
-        raise RuntimeError("logits have a forward-mode tangent, and adjust_logits has none: detach them")
+    _no_gradients("logits", logits)
     penalties = [_penalty(*x, logits) for x in (("repetition", repetition), ("frequency", frequency),
                                                 ("presence", presence))]
     if history is None:
@@ -121,6 +129,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     if bias is not None:
         _per_row("bias_ids", bias_ids, logits, ID_DTYPES, width=True)
         _per_row("bias", bias, logits, (torch.float32,), width=True)
+        _no_gradients("bias", bias)
         if bias.shape != bias_ids.shape or bias.shape[1] > MAX_BIASES:
             raise ValueError(f"bias must have the shape of bias_ids, of at most {MAX_BIASES} a row, got "
                              f"{tuple(bias.shape)} and {tuple(bias_ids.shape)}")
@@ -142,6 +151,8 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device):
         raise ValueError(f"out must be like logits, {tuple(logits.shape)} {logits.dtype} on {logits.device}, got "
                          f"{tuple(out.shape)} {out.dtype} on {out.device}")
+    if out is not None:
+        _no_gradients("out", out)
     if out is not None and ((v > 1 and out.stride(1) != 1) or (b > 1 and out.stride(0) < v)):
         raise ValueError(f"out must have rows of their own, got strides {out.stride()}")
     if out is not None and _overlaps(out, logits):

@@ -175,17 +175,21 @@ def _on_the_gpu(*tensors):
         raise RuntimeError("thundersync_amd's paged cache runs on the GPU only; got a CPU tensor")
 
 
+def _no_gradients(name: str, x: torch.Tensor):
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires grad, and there are no gradients through a paged cache: detach it, or call "
+                           "under torch.no_grad()")
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError(f"{name} has a forward-mode tangent, and there are none through a paged cache: detach it")
+
+
 def _rows(name: str, x: torch.Tensor, cache: PagedCache) -> torch.Tensor:
     """``x`` ``[T, heads, head_dim]`` with dense, 16-byte aligned rows."""
     if x.dim() != 3 or x.shape[2] != cache.head_dim:
         raise ValueError(f"{name} must be [T, heads, {cache.head_dim}], got {tuple(x.shape)}")
     if x.dtype != cache.dtype:
         raise TypeError(f"{name} must be {cache.dtype} as the cache, got {x.dtype}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} requires grad, and there are no gradients through a paged cache: detach it, or call "
-                           "under torch.no_grad()")
-    if forward_ad.unpack_dual(x).tangent is not None:
-        raise RuntimeError(f"{name} has a forward-mode tangent, and there are none through a paged cache: detach it")
+    _no_gradients(name, x)
     a, b, c = x.stride()
     if c == 1 and (a | b) % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
@@ -277,6 +281,7 @@ def append_tokens(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Te
                              f"{tuple(rotary.shape)}")
         if rotary.dtype != torch.float32:
             raise TypeError(f"rotary must be fp32, got {rotary.dtype}")
+        _no_gradients("rotary", rotary)
         rotary = rotary.detach().contiguous()
         rotary = rotary if rotary.data_ptr() % 16 == 0 else rotary.clone()
         r = rotary.shape[1]
