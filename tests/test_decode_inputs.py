@@ -87,3 +87,16 @@ def test_gradients_of_other_inputs_are_refused(call, name, shape):
         call(**{name: forward_ad.make_dual(x, x)}, **more)
     with pytest.raises(RuntimeError, match="on the GPU only"):
         call(**{name: x}, **more)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_what_a_cache_was_made_of_is_not_set_anew(bits):
+    """The kernels would go on with the tensors, sizes and types that they were given."""
+    cache, other = (PagedCache.empty(4, 16, 2, 64, bits=bits, device="cpu") for _ in range(2))
+    was = {name: getattr(cache, name) for name in sorted(PagedCache._GIVEN)}
+    for name in was:
+        with pytest.raises(AttributeError, match=f"{name} of a PagedCache"):
+            setattr(cache, name, getattr(other, name))
+        assert getattr(cache, name) is was[name]
+    cache.owner = "a rollout"  # a program's own
+    assert cache.owner == "a rollout" and cache._desc.key == cache.key.data_ptr()

@@ -72,7 +72,12 @@ class PagedCache:
     16]`` (8 bits).  Both are used in place; a page's ``[kv_heads, page_size,
     row]`` lies densely.  ``row`` is one of 64, 128, 192 and 256; a smaller
     ``head_dim`` (a multiple of 8) leaves zeros behind it, as :meth:`empty` does.
+    The kernels are given what was checked here, so none of it can be set anew:
+    other tensors are another cache.
     """
+
+    _GIVEN = frozenset(("key", "value", "key_scale", "value_scale", "bits", "pages", "kv_heads", "page_size", "row",
+                        "head_dim", "dtype"))
 
     def __init__(self, key: torch.Tensor, value: torch.Tensor, key_scale: torch.Tensor | None = None,
                  value_scale: torch.Tensor | None = None, *, dtype: torch.dtype | None = None,
@@ -125,6 +130,11 @@ class PagedCache:
             key.stride(0) if pages > 1 else stride, value.stride(0) if pages > 1 else stride, pages, page_size, heads,
             head_dim, row, self.bits, _lib.dtype_code(dtype))
         self._ref = ctypes.byref(self._desc)
+
+    def __setattr__(self, name, value):
+        if name in self._GIVEN and "_ref" in self.__dict__:
+            raise AttributeError(f"{name} of a PagedCache is what its kernels were given; make another over other tensors")
+        super().__setattr__(name, value)
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, *, dtype: torch.dtype = torch.bfloat16,
