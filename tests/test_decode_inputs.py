@@ -100,3 +100,14 @@ def test_what_a_cache_was_made_of_is_not_set_anew(bits):
         assert getattr(cache, name) is was[name]
     cache.owner = "a rollout"  # a program's own
     assert cache.owner == "a rollout" and cache._desc.key == cache.key.data_ptr()
+
+
+@pytest.mark.parametrize("rows, vocab", [(1, 70), (3, 1), (1, 1)])
+def test_an_output_that_is_the_logits_by_other_strides(rows, vocab):
+    """A single row or column is the same whatever stride the tensor gives it."""
+    x = torch.zeros(500)
+    z = x.as_strided((rows, vocab), (80 if rows == 1 else 5, 1))
+    out = x.as_strided((rows, vocab), (200 if rows == 1 else 5, 1 if vocab > 1 else 3))
+    assert z.stride() != out.stride()
+    with pytest.raises(RuntimeError, match="on the GPU only"):
+        adjust_logits(z, out=out)

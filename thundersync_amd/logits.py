@@ -67,7 +67,8 @@ def _unit_rows(x: torch.Tensor) -> torch.Tensor:
 
 def _overlaps(out: torch.Tensor, logits: torch.Tensor) -> bool:
     """Whether the two share memory in another way than as the same rows."""
-    if out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride():
+    if out.data_ptr() == logits.data_ptr() and all(n == 1 or s == t for n, s, t in zip(
+            out.shape, out.stride(), logits.stride())):
         return False
     span = lambda x: (x.data_ptr(), x.data_ptr() + x.element_size() * (  # noqa: E731
         1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))))
