@@ -111,3 +111,14 @@ def test_an_output_that_is_the_logits_by_other_strides(rows, vocab):
     assert z.stride() != out.stride()
     with pytest.raises(RuntimeError, match="on the GPU only"):
         adjust_logits(z, out=out)
+
+
+@pytest.mark.parametrize("rows, vocab", [(0, 40), (1, 1), (3, 31), (2, 32), (2, 33), (5, 1001), (64, 64)])
+def test_packed_masks(rows, vocab):
+    """Masks of any width, of no rows, seen as columns."""
+    mask = torch.rand(rows, vocab, generator=torch.Generator().manual_seed(rows)) < 0.5
+    for given in (mask, mask.t().contiguous().t()):
+        bits = pack_allowed(given)
+        assert bits.dtype == torch.int32 and bits.shape == (rows, -(-vocab // 32)) and bits.is_contiguous()
+        back = ((bits[..., None] >> torch.arange(32, dtype=torch.int32)) & 1).flatten(1).bool()
+        assert torch.equal(back[:, :vocab], mask) and not bool(back[:, vocab:].any())

@@ -131,6 +131,21 @@ def test_many_small_fp16_weights(cuda, counts, length, bits):
     assert excess(out, want, bound) <= 0
 
 
+def test_packing_a_mask_takes_little_memory(cuda):
+    """The bits of a mask, of any width, in a few bytes a token."""
+    g = torch.Generator(device=cuda).manual_seed(0)
+    for rows, vocab in ((1, 1), (3, 31), (2, 64), (5, 1001), (200, 151936)):
+        mask = torch.rand(rows, vocab, generator=g, device=cuda) < 0.5
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        bits = pack_allowed(mask)
+        used = torch.cuda.max_memory_allocated() - before
+        assert bits.dtype == torch.int32 and bits.shape == (rows, -(-vocab // 32))
+        back = (bits[..., None] >> torch.arange(32, device=cuda, dtype=torch.int32)) & 1
+        assert torch.equal(back.flatten(1)[:, :vocab].bool(), mask) and not bool(back.flatten(1)[:, vocab:].any())
+        assert used <= 3 * mask.numel() + 65536, used / mask.numel()
+
+
 def test_checked_batches_with_rows_of_no_sequence(cuda, monkeypatch):
     """The check of a batch lets pass what the module describes: rows outside the sequences, padding with rows of its own."""
     monkeypatch.setenv("THUNDERSYNC_CHECK_TARGETS", "1")

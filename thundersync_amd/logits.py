@@ -80,9 +80,12 @@ def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
     """The bits that ``allowed`` of :func:`adjust_logits` takes, ``[M, ceil(V / 32)]`` int32, of a bool mask ``[M, V]``."""
     if allowed.dim() != 2 or allowed.dtype != torch.bool:
         raise ValueError(f"a bool mask [M, V], got {allowed.dtype} {tuple(allowed.shape)}")
-    bits = torch.nn.functional.pad(allowed, (0, -allowed.shape[1] % 32)).unflatten(1, (-1, 32)).to(torch.int64)
-    words = (bits << torch.arange(32, device=allowed.device)).sum(dim=-1)
-    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    # byte by byte of the words (of which the lowest comes first), a bit of all of them at a time
+    bits = torch.nn.functional.pad(allowed, (0, -allowed.shape[1] % 32)).view(torch.uint8).unflatten(1, (-1, 8))
+    packed = bits[..., 0].clone(memory_format=torch.contiguous_format)
+    for i in range(1, 8):
+        packed |= bits[..., i] << i
+    return packed.view(torch.int32)
 
 
 def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
