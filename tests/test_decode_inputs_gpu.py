@@ -131,6 +131,20 @@ def test_many_small_fp16_weights(cuda, counts, length, bits):
     assert excess(out, want, bound) <= 0
 
 
+@pytest.mark.parametrize("kv_heads", [1, 4])
+@pytest.mark.parametrize("kind", ["one", "few", "mixed"])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_more_than_64_long_sequences(cuda, kv_heads, kind, bits):
+    """The search for a work-group's borders goes over several 64s of sequences whose tiles are cut."""
+    g = torch.Generator().manual_seed(13)
+    lengths = torch.randint(600, 3001, (131,), generator=g).tolist()
+    counts = None if kind == "one" else torch.randint(0, 4, (131,), generator=g).tolist()
+    if kind == "mixed":
+        for s in (0, 63, 64, 100, 130):
+            counts[s] = 40
+    check(cuda, lengths, counts, heads=2 * kv_heads, kv_heads=kv_heads, dim=64, page=64, bits=bits, seed=13)
+
+
 def test_packing_a_mask_takes_little_memory(cuda):
     """The bits of a mask, of any width, in a few bytes a token."""
     g = torch.Generator(device=cuda).manual_seed(0)
