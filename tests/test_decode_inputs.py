@@ -4,14 +4,12 @@ from __future__ import annotations
 
 import ctypes
 
-import ctypes
-
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from tests.paged_cases import int32
-from thundersync_amd import _lib, paged
+from thundersync_amd import _lib
 from thundersync_amd.logits import adjust_logits, pack_allowed
 from thundersync_amd.paged import PagedCache, append_tokens, paged_attention
 

@@ -164,7 +164,7 @@ Sizes sizes_of(const ts_paged_cache& c, const ts_paged_batch& b, int64_t tokens,
   Sizes z{};
   const int64_t group = heads / c.kv_heads, keys = b.width * c.page_size + 16;
   const bool ragged = b.offsets != nullptr, chunks = ragged && tokens * group > kFewRows;
-  // 32 rows a tile would not fit the registers beside wide rows' loads
+  // 32 rows a tile would not fit the registers beside wide rows' loads: their sequences of more than 16 rows are read twice
   z.rows[0] = (ragged || group > 16) && c.row <= 128 ? 32 : 16;
   z.rows[1] = 128;
   // work-groups of a KV head that the device's 256 CUs hold at once (four waves each, eight of chunks of 256-wide rows)

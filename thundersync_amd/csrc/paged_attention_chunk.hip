@@ -8,9 +8,10 @@
 // operand of O^T += V^T P^T, and V^T comes from transposed LDS reads; the reference point of a row moves only
 // when a score passes it by 8 (log2 units).  Only tiles at a wave's diagonal are masked.
 //
-// Bound by the matrix instructions and the exponentials, and by the LDS reads and the barrier between them: four sequences'
-// chunks of 512 tokens after 1024 to 15872 keys, 32/8 heads of 128, take 370 us, 790 TFLOP/s (page ids a tile ahead and
-// reads without a branch: 375 without).
+// Bound by the conversion, LDS reads and barrier of every 32 keys beside the products, which keep the matrix cores 30 % busy:
+// four sequences' chunks of 512 tokens after 4757 to 14925 keys, 32/8 heads of 128, take 427 us in 8 bits, 770 TFLOP/s, and
+// 397 in 16, 830.  Page ids a tile ahead and reads without a branch: 370 us over three batches, 375 without.  Tiles are dealt
+// as if they saw all keys of their sequence, so whole prompts are slower: one of 8192 tokens 490 TFLOP/s.
 #include "attention_impl.h"
 #include "paged_attention.h"
 

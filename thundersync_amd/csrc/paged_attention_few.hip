@@ -12,8 +12,10 @@
 // Nothing passes through LDS, and no wave waits for another before the end.
 //
 // Bound by HBM: a step's 32 ROW bytes of keys and as many of values against about 150 VALU instructions and 2 ROW / 8
-// matrix ones.  256 sequences of 256 to 16384 keys, 32/8 heads of 128 in 8 bits, take 700 to 740 us, 6.1 TB/s; one of 125000
-// 53, 4.9 TB/s; 64 of 256 to 4096 in 16 bits 111, 5.2 TB/s; 24/4 heads of 256, two waves a SIMD, 4.6 TB/s.
+// matrix ones.  256 sequences of 256 to 16384 keys, 32/8 heads of 128 in 8 bits, take 700 to 750 us, 5.9 TB/s; one of 125000
+// 53, 4.8 TB/s; 64 of 256 to 4096 in 16 bits 102 to 124, 5.0 TB/s.  64 of 100 to 6000, one to five rows, 24/4 heads of 256:
+// 103 us, 6.3 TB/s of what is read; wide rows have 16 a tile, so sequences of 17 to 32 query rows are read twice, and 4.1
+// TB/s is what reading them once would be.
 #include "paged_attention.h"
 
 namespace ts {

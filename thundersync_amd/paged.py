@@ -328,7 +328,9 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, page_table: torch.Te
 
     Query head ``h`` reads KV head ``h // (heads // kv_heads)``.  Keys that a row does not see
     (those of tokens behind it, and what lies behind a sequence's end in its last
-    page) have no part in it whatever they hold.  A row without keys is zero.
+    page) have no part in it whatever they hold.  A row without keys is zero.  Scores, weights and sums
+    are fp32; for the product with the values a weight is rounded to the query's type.  A call takes
+    fewer than 2^24 rows (tokens times heads).
     """
     q = _rows("query", query, cache)
     t, heads, _ = q.shape
