@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -10,6 +11,7 @@ from torch.autograd import forward_ad
 
 from tests.paged_cases import int32
 from thundersync_amd import _lib
+from thundersync_amd._abi import PagedBatch, PagedCacheDesc
 from thundersync_amd.logits import adjust_logits, pack_allowed
 from thundersync_amd.paged import PagedCache, append_tokens, paged_attention
 
@@ -120,3 +122,16 @@ def test_packed_masks(rows, vocab):
         assert bits.dtype == torch.int32 and bits.shape == (rows, -(-vocab // 32)) and bits.is_contiguous()
         back = ((bits[..., None] >> torch.arange(32, dtype=torch.int32)) & 1).flatten(1).bool()
         assert torch.equal(back[:, :vocab], mask) and not bool(back[:, vocab:].any())
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.5e38, math.inf, math.nan])
+def test_scales_that_pass_fp32_in_log2_units_are_refused(scale):
+    """They are infinite where the kernels use them, and every row would be NaN."""
+    lib, p = _lib.require_library(), ctypes.c_void_p(4096)
+    cache = ctypes.byref(PagedCacheDesc(4096, 4096, None, None, 2048, 2048, 4, 16, 2, 64, 64, 16, _lib.TS_BF16))
+    batch = ctypes.byref(PagedBatch(4096, 4096, None, 2, 2, 3))
+    # a workspace too small for any batch: the call ends at the host's checks whatever the scale
+    assert lib.ts_paged_attention(cache, batch, 3, p, 256, 64, 4, scale, p, p, 0, None) == 1
+    assert "scale" in lib.ts_hip_last_error().decode()
+    assert lib.ts_paged_attention(cache, batch, 3, p, 256, 64, 4, 2e38, p, p, 0, None) == 1
+    assert "workspace of 0 bytes" in lib.ts_hip_last_error().decode()

@@ -211,7 +211,7 @@ int ts_paged_attention(const ts_paged_cache* cache, const ts_paged_batch* batch,
   if (int e = check_batch(batch, tokens, "ts_paged_attention")) return e;
   TS_CHECK_ARG(heads >= 1 && heads <= (1 << 16) && heads % cache->kv_heads == 0, "ts_paged_attention: %lld heads over %d",
                (long long)heads, cache->kv_heads);
-  TS_CHECK_ARG(__builtin_isfinite(scale), "ts_paged_attention: scale %g", (double)scale);
+  TS_CHECK_ARG(__builtin_isfinite(scale * kLog2e), "ts_paged_attention: scale %g", (double)scale);
   if (tokens == 0) return TS_OK;
   TS_CHECK_ARG(query && out && cache->pages > 0, "ts_paged_attention: null pointer, or a cache without pages");
   TS_CHECK_ARG((((uintptr_t)query | (uintptr_t)out) & 15) == 0 && (token_stride | head_stride) % 8 == 0,
