@@ -107,6 +107,33 @@ def test_small_fp16_values_are_codes_of_fp16_values(cuda, loud, interleaved):
         assert excess(flat(got), want, bound) <= 0
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotated_keys_next_to_a_border_between_codes(cuda, dtype, interleaved):
+    """Tables chosen so that half of the rotated elements lie within a rounding of a border: the code is that of the
+    rotation rounded once to fp32, not of products that were rounded before."""
+    g = torch.Generator().manual_seed(14)
+    n, half = 400, 32
+    sign = lambda *shape: 1.0 - 2.0 * torch.randint(0, 2, shape, generator=g)  # noqa: E731
+    u, v = ((sign(n, half) * (0.5 + 0.5 * torch.rand(n, half, generator=g))).to(dtype) for _ in range(2))
+    cos = 2 * torch.rand(n, half, generator=g) - 1
+    # e4m3's borders below 1.5, for the scale 2^-6 that an element of 7 gives
+    border = sign(n, half) * (8 + torch.randint(0, 8, (n, half), generator=g) + 0.5) * 2.0 ** -torch.randint(
+        4, 6, (n, half), generator=g)
+    sin = ((u.double() * cos.double() - border) / v.double()).float()
+    key = torch.zeros(n, 1, 128, dtype=dtype)
+    pair = (slice(0, 64, 2), slice(1, 64, 2)) if interleaved else (slice(0, half), slice(half, 64))
+    key[:, 0, pair[0]], key[:, 0, pair[1]], key[:, 0, 100] = u, v, 7.0
+    table = torch.cat([cos, sin], dim=1)
+    cache = PagedCache.empty(25, 16, 1, 128, dtype=dtype, bits=8, device=cuda)
+    append_tokens(cache, torch.arange(25, dtype=torch.int32, device=cuda)[None], int32([n], cuda), key.to(cuda), key.to(cuda),
+                  offsets=int32([0, n], cuda), rotary=table.to(cuda), interleaved=interleaved)
+    assert bool((cache.key_scale == 2.0 ** -6).all())
+    want = ref.encode(ref.rotate(key, table, torch.arange(n), interleaved), -6, dtype)
+    got = cache.values()[0].double().cpu().transpose(1, 2).flatten(0, 1)
+    assert torch.equal(got, want), (got != want).sum()
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 @pytest.mark.parametrize("counts, length", [(None, 30001), ([3], 30001), ([33], 30001), (None, 400), ([1], 400), ([3], 400),
                                             ([33], 400)])

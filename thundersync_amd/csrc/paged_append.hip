@@ -11,7 +11,7 @@
 //
 // Bound by HBM where tokens are many (each row is read and written once) and by latency where they
 // are few.  One launch: its first work-groups take the blocks of an 8-bit cache, the others rows.  16 prompts of 1024
-// tokens, 32 + 2 * 8 heads of 128, 8 bits: 85 us for 370 MB, 4.4 TB/s; a token for each of 64 sequences: 7 us.
+// tokens, 32 + 2 * 8 heads of 128, 8 bits: 87 us for 370 MB, 4.3 TB/s; a token for each of 64 sequences: 7 us.
 #include <algorithm>
 
 #include "paged.h"
@@ -101,24 +101,31 @@ __device__ __forceinline__ void angles(const Args& a, int pos, int j, float (&c)
   }
 }
 
+// a c + b s rounded once: what the products and their sum lose is added at the end.  Of the 33.5 million keys of 16 prompts of
+// 1024 tokens none goes to another code than in 64 bits; 3 to 8 did where a product was rounded before (87 us, then 85).
+__device__ __forceinline__ float rounded_once(float a, float c, float b, float s) {
+#pragma clang fp contract(off)
+  const float p = a * c, q = b * s, sum = p + q, second = sum - p;
+  const float lost = ((p - (sum - second)) + (q - second)) + (__builtin_fmaf(a, c, -p) + __builtin_fmaf(b, s, -q));
+  return fabsf(sum) < __builtin_huge_valf() ? sum + lost : sum;
+}
+template <bool ONCE>
 __device__ __forceinline__ void rotate(const Args& a, float (&x)[8], float (&y)[8], const float (&c)[8],
                                        const float (&s)[8]) {
+  auto turn = [](float& u, float& v, float cos, float sin) __attribute__((always_inline)) {
+    const float p = u, q = v;
+    u = ONCE ? rounded_once(p, cos, q, -sin) : p * cos - q * sin;
+    v = ONCE ? rounded_once(q, cos, p, sin) : q * cos + p * sin;
+  };
   if (a.interleaved) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float u = x[2 * i], v = x[2 * i + 1], p = y[2 * i], q = y[2 * i + 1];
-      x[2 * i] = u * c[i] - v * s[i];
-      x[2 * i + 1] = v * c[i] + u * s[i];
-      y[2 * i] = p * c[4 + i] - q * s[4 + i];
-      y[2 * i + 1] = q * c[4 + i] + p * s[4 + i];
+      turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
+      turn(y[2 * i], y[2 * i + 1], c[4 + i], s[4 + i]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float u = x[i], v = y[i];
-      x[i] = u * c[i] - v * s[i];
-      y[i] = v * c[i] + u * s[i];
-    }
+    for (int i = 0; i < 8; ++i) turn(x[i], y[i], c[i], s[i]);
   }
 }
 
@@ -206,7 +213,8 @@ __device__ __forceinline__ void append_block(const Args& a, int unit, int lane) 
     if (!is_value && 16 * j < a.rotary_dim) {
       float c[8], sn[8];
       angles(a, a.positions ? a.positions[row] : first + t, j, c, sn);
-      rotate(a, x[k][0], x[k][1], c, sn);
+      // a key on the other side of a border between codes is off by up to 1/8 of its size
+      rotate<true>(a, x[k][0], x[k][1], c, sn);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -320,7 +328,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Args a) {
         float x[8], y[8];
         load8((const T*)&v0[k], x);
         load8((const T*)&v1[k], y);
-        rotate(a, x, y, c, sn);
+        rotate<false>(a, x, y, c, sn);
         store8((T*)&v0[k], x);
         store8((T*)&v1[k], y);
       }
